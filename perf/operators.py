@@ -205,7 +205,7 @@ def prepare(case, seed):
         s["q"] = _normal(seed, 1, (len(lens), hq, d), dt)
         if own:
             from turbopi_b200 import ops
-            s["workspace"] = ops.paged_attention_workspace(len(lens), hq, hk, d, DEV)
+            s["workspace"] = ops.paged_attention_workspace(hq, hk, d, DEV)
         return s
     qkv = _normal(seed, 1, (sum(lens), hq + 2 * hk, d), dt)
     s["q"], s["k"], s["v"] = qkv.split([hq, hk, hk], 1)
