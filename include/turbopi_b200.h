@@ -83,7 +83,7 @@ const char* tpb200_status_string(int status);
 /* last non-OK status produced on this host thread by a void-returning entry point (and clears it) */
 int tpb200_last_error(void);
 /* code recorded by a kernel whose bounded wait ran out on the current device (or 401: a prompt token outside the embedding
- * table, see TPB200_FLAG_STRICT_TOKENS), 0 if none; synchronises the device.  `clear` != 0 resets the word.
+ * table, see TPB200_FLAG_STRICT_TOKENS; or 501: a length, position or page id outside a paged cache), 0 if none; synchronises the device.  `clear` != 0 resets the word.
  * Recovery: a kernel that gave up may have left its split-K counters non-zero.  After a non-zero code
  * every workspace that was passed to a GEMM / GEMV / attention launch since the last check must be set
  * to zero again (cudaMemsetAsync) before it is reused; results of the failed launch are undefined. */
@@ -415,6 +415,60 @@ typedef struct {
     int cluster_ctas, head_dim_parts, tmem_columns, smem_bytes;
 } tpb200_attention_launch_info;
 int tpb200_attention_describe(int n_rows, int n_keys, int head_dim, int groups, int fused_quant, tpb200_attention_launch_info* info);
+
+/* ---------------------------------------------------------------------------------------------
+ * A cache of pages that many sequences share (one layer of it).  Key and value pages lie apart, with the same strides (in
+ * elements, multiples of 8): row r of head h of page p starts at p * page_stride + r * row_stride + h * head_stride.  Position j of
+ * sequence s is row j % page_size of page table[s * table_stride + j / page_size].  bf16 or fp16; head_dim a multiple of 8, <= 256.
+ * table and lengths are read on the device, so a captured call follows them.  What they must not hold is checked
+ * there: a page id outside the pool, a position outside the table or a length beyond table_width * page_size is skipped, and
+ * tpb200_device_error() reports 501.  table_width * page_size < 2^31.
+ * ------------------------------------------------------------------------------------------- */
+typedef struct {
+    void* k_pages; void* v_pages;
+    long long page_stride; long long row_stride; long long head_stride;
+    int num_pages; int page_size; int kv_heads; int head_dim; int dtype;
+    const int* table; long long table_stride; int table_width;
+    const int* lengths; int seqs;
+} tpb200_paged_cache;
+
+/* Attention of one new token per sequence on the cache: out[s] = softmax(scale * q[s] K^T) V over the first lengths[s] positions
+ * (the new token's own key among them); query heads [h * g, (h + 1) * g) read key head h, g = q_heads / kv_heads; fp32 sums,
+ * outputs rounded once.  A sequence of length 0 gives zeros.  q / out: element strides of a sequence and of a head, multiples of 8.
+ * The lengths' sum is cut into equal pieces over the GPU whatever the single lengths; items that cross a cut are joined by a second
+ * small kernel through `workspace` (no initialisation needed; its size depends on the heads only). */
+typedef struct {
+    tpb200_paged_cache cache;
+    const void* q; void* out;
+    long long q_stride[2]; long long o_stride[2];
+    int q_heads;
+    float scale;
+    void* workspace; size_t workspace_bytes;
+    int flags;
+} tpb200_paged_attention_args;
+size_t tpb200_paged_attention_workspace_size(int q_heads, int kv_heads, int head_dim);
+int tpb200_paged_attention(const tpb200_paged_attention_args* args, tpb200_stream_t stream);
+
+/* New tokens into the cache.  Sequence s brings the tokens [cu[s], cu[s + 1]); its last one goes to position lengths[s] - 1, so
+ * lengths are those after the call.  Tokens behind cu[seqs] are left alone.  With cos / sin ([rope_positions, head_dim / 2], rows
+ * contiguous, fp32, fp16 or bf16) the keys, and the queries where given, are rotated at their positions in rotate-half form:
+ *   y[d] = x[d] cos[d] - x[d + D/2] sin[d],  y[d + D/2] = x[d + D/2] cos[d] + x[d] sin[d]
+ * in fp32, rounded once (modeling_gemma.py:132-197); q_out may be q.  A token without a place (501) writes nothing. */
+typedef struct {
+    tpb200_paged_cache cache;
+    const void* k; const void* v; const void* q; void* q_out;
+    long long k_stride[2]; long long v_stride[2]; long long q_stride[2]; long long o_stride[2];
+    const int* cu; int tokens; int q_heads;
+    const void* cos; const void* sin; int rope_dtype; int rope_positions;
+    int flags;
+} tpb200_paged_append_args;
+int tpb200_paged_append(const tpb200_paged_append_args* args, tpb200_stream_t stream);
+
+/* Pages copied within their pool, in each of `slabs` slabs (a layer's keys or values: num_pages pages of page_bytes bytes, slab_bytes
+ * apart): page dst[i] <- page src[i].  src / dst are HOST arrays, read before the call returns.  TPB200_ERR_SHAPE for an index
+ * outside the pool, a page that is written twice, or one that is both read and written. */
+int tpb200_copy_pages(void* pages, long long slab_bytes, int slabs, long long page_bytes, int num_pages, const int* src, const int* dst,
+                      int count, int flags, tpb200_stream_t stream);
 
 /* ---------------------------------------------------------------------------------------------
  * Row-wise glue between two linears, fused with the activation quantiser of the tensor-core GEMM:

@@ -1,0 +1,91 @@
+"""What the calls on a paged cache refuse, before anything is launched: the C entry points with pointers they never follow, and
+the Python calls on tensors that claim to be on a GPU."""
+import ctypes
+
+import pytest
+import torch
+
+from turbopi_b200 import _lib, ops
+from turbopi_b200._lib import TurboPiError
+
+NULL, SHAPE, ALIGN, ENUM, WORKSPACE = -1, -2, -3, -4, -6
+Two = ctypes.c_longlong * 2
+
+
+def _cache(**kw):
+    base = dict(k_pages=1024, v_pages=4096, page_stride=16 * 256, row_stride=256, head_stride=256, num_pages=8, page_size=16, kv_heads=1,
+                head_dim=256, dtype=_lib.BF16, table=64, table_stride=4, table_width=4, lengths=64, seqs=2)
+    return _lib.PagedCacheView(**{**base, **kw})
+
+
+BAD_CACHE = [(dict(k_pages=0), NULL), (dict(v_pages=0), NULL), (dict(table=0), NULL), (dict(lengths=0), NULL), (dict(k_pages=8), ALIGN),
+             (dict(page_stride=4097), ALIGN), (dict(row_stride=4), ALIGN), (dict(head_stride=-8), SHAPE), (dict(num_pages=0), SHAPE),
+             (dict(page_size=0), SHAPE), (dict(head_dim=12), SHAPE), (dict(head_dim=264), SHAPE), (dict(head_dim=0), SHAPE),
+             (dict(dtype=_lib.F32), ENUM), (dict(table_width=0), SHAPE), (dict(seqs=-1), SHAPE),
+             (dict(page_size=1 << 16, table_width=1 << 15), SHAPE)]
+
+
+@pytest.mark.parametrize("change,status", BAD_CACHE)
+def test_views_of_a_cache(change, status):
+    lib = _lib.load()
+    attention = _lib.PagedAttentionArgs(cache=_cache(**change), q=64, out=64, q_stride=Two(2048, 256), o_stride=Two(2048, 256), q_heads=8,
+                                        scale=1.0, workspace=256, workspace_bytes=1 << 30)
+    append = _lib.PagedAppendArgs(cache=_cache(**change), k=64, v=64, k_stride=Two(256, 256), v_stride=Two(256, 256), cu=64, tokens=3)
+    assert lib.tpb200_paged_attention(attention, None) == status
+    assert lib.tpb200_paged_append(append, None) == status
+
+
+@pytest.mark.parametrize("change,status", [(dict(q=0), NULL), (dict(out=0), NULL), (dict(q=8), ALIGN), (dict(q_stride=Two(2044, 256)), ALIGN),
+                                           (dict(q_heads=0), SHAPE), (dict(flags=4), ENUM)])
+def test_attention_arguments(change, status):
+    base = dict(cache=_cache(), q=64, out=64, q_stride=Two(2048, 256), o_stride=Two(2048, 256), q_heads=8, scale=1.0, workspace=256,
+                workspace_bytes=1 << 30)
+    assert _lib.load().tpb200_paged_attention(_lib.PagedAttentionArgs(**{**base, **change}), None) == status
+
+
+def test_attention_heads_must_divide():
+    args = _lib.PagedAttentionArgs(cache=_cache(kv_heads=3), q=64, out=64, q_heads=8, scale=1.0)
+    assert _lib.load().tpb200_paged_attention(args, None) == SHAPE
+
+
+@pytest.mark.parametrize("change,status", [(dict(k=0), NULL), (dict(cu=0), NULL), (dict(v=4), ALIGN), (dict(tokens=-1), SHAPE),
+                                           (dict(cos=64), NULL), (dict(cos=64, sin=64), SHAPE), (dict(cos=64, sin=8, rope_positions=4), ALIGN),
+                                           (dict(cos=64, sin=64, rope_positions=4, rope_dtype=9), ENUM),
+                                           (dict(q=64, q_out=64, q_heads=8), SHAPE),
+                                           (dict(q=64, q_heads=8, cos=64, sin=64, rope_positions=4), NULL),
+                                           (dict(k_stride=Two(4, 256)), ALIGN), (dict(flags=2), ENUM)])
+def test_append_arguments(change, status):
+    base = dict(cache=_cache(), k=64, v=64, k_stride=Two(256, 256), v_stride=Two(256, 256), cu=64, tokens=3)
+    assert _lib.load().tpb200_paged_append(_lib.PagedAppendArgs(**{**base, **change}), None) == status
+
+
+def _copy(src, dst, pages=1024, slab=8 * 4096, slabs=4, page=4096, count=8, flags=0):
+    a, b = ((ctypes.c_int * len(x))(*x) for x in (src, dst))
+    return _lib.load().tpb200_copy_pages(pages, slab, slabs, page, count, a, b, len(src), flags, None)
+
+
+@pytest.mark.parametrize("src,dst", [([0], [8]), ([8], [0]), ([-1], [0]), ([0], [-1]), ([0, 1], [2, 2]), ([0, 1], [1, 2]), ([3], [3]),
+                                     ([0, 1, 2], [5, 6, 0])])
+def test_copies_that_would_depend_on_their_order(src, dst):
+    assert _copy(src, dst) == SHAPE
+
+
+def test_copy_arguments():
+    assert _copy([0], [1], pages=0) == NULL
+    assert _copy([0], [1], pages=1028) == ALIGN
+    assert _copy([0], [1], page=4100) == ALIGN
+    assert _copy([0], [1], slab=4096) == SHAPE
+    assert _copy([0], [1], slabs=0) == SHAPE
+    assert _copy([0], [1], flags=8) == ENUM
+    assert _copy([], []) == 0
+
+
+def test_cpu_tensors_are_refused():
+    k = torch.zeros(2, 16, 1, 64, dtype=torch.bfloat16)
+    table, lengths = torch.zeros(1, 2, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(TurboPiError, match="CUDA"):
+        ops.paged_attention(torch.zeros(1, 1, 64, dtype=torch.bfloat16), k, k, table, lengths, 1.0)
+    with pytest.raises(TurboPiError, match="CUDA"):
+        ops.paged_append(k[:, 0], k[:, 0], k, k, table, lengths, lengths)
+    with pytest.raises(TurboPiError, match="CUDA"):
+        ops.copy_pages(k, [0], [1])

@@ -102,6 +102,26 @@ class AttentionArgs(ctypes.Structure):
                 ("quant_sf", c_void_p), ("quant_pitch", c_int), ("quant_piece_rows", c_int)]
 
 
+class PagedCacheView(ctypes.Structure):
+    _fields_ = [("k_pages", c_void_p), ("v_pages", c_void_p),
+                ("page_stride", c_longlong), ("row_stride", c_longlong), ("head_stride", c_longlong),
+                ("num_pages", c_int), ("page_size", c_int), ("kv_heads", c_int), ("head_dim", c_int), ("dtype", c_int),
+                ("table", c_void_p), ("table_stride", c_longlong), ("table_width", c_int), ("lengths", c_void_p), ("seqs", c_int)]
+
+
+class PagedAttentionArgs(ctypes.Structure):
+    _fields_ = [("cache", PagedCacheView), ("q", c_void_p), ("out", c_void_p), ("q_stride", c_longlong * 2),
+                ("o_stride", c_longlong * 2), ("q_heads", c_int), ("scale", c_float), ("workspace", c_void_p),
+                ("workspace_bytes", c_size_t), ("flags", c_int)]
+
+
+class PagedAppendArgs(ctypes.Structure):
+    _fields_ = [("cache", PagedCacheView), ("k", c_void_p), ("v", c_void_p), ("q", c_void_p), ("q_out", c_void_p),
+                ("k_stride", c_longlong * 2), ("v_stride", c_longlong * 2), ("q_stride", c_longlong * 2),
+                ("o_stride", c_longlong * 2), ("cu", c_void_p), ("tokens", c_int), ("q_heads", c_int), ("cos", c_void_p),
+                ("sin", c_void_p), ("rope_dtype", c_int), ("rope_positions", c_int), ("flags", c_int)]
+
+
 class ActTc(ctypes.Structure):
     _fields_ = [("x", c_void_p), ("ldx", c_int), ("K", c_int), ("x_image", c_void_p), ("x_row_scale", c_void_p)]
 
@@ -162,6 +182,11 @@ SIGNATURES = {
     "tpb200_attention_workspace_size": (c_size_t, [c_int, c_int, c_int, c_int]),
     "tpb200_attention_describe": (c_int, [c_int, c_int, c_int, c_int, c_int, ctypes.POINTER(AttentionLaunchInfo)]),
     "tpb200_attention": (c_int, [ctypes.POINTER(AttentionArgs), c_void_p]),
+    "tpb200_paged_attention_workspace_size": (c_size_t, [c_int, c_int, c_int]),
+    "tpb200_paged_attention": (c_int, [ctypes.POINTER(PagedAttentionArgs), c_void_p]),
+    "tpb200_paged_append": (c_int, [ctypes.POINTER(PagedAppendArgs), c_void_p]),
+    "tpb200_copy_pages": (c_int, [c_void_p, c_longlong, c_int, c_longlong, c_int, ctypes.POINTER(c_int), ctypes.POINTER(c_int),
+                                  c_int, c_int, c_void_p]),
     "tpb200_w4a16_gemm": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_int,
                                   c_int, c_int, c_int, c_float, c_float, c_int, c_void_p]),
     "tpb200_row_transform_quantize": (c_int, [ctypes.POINTER(RowOpArgs), c_void_p]),

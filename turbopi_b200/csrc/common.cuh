@@ -32,6 +32,8 @@ enum DeviceErrorCode : int {
     kErrGemmSplitTimeout = 205,
     kErrAttnBarrierTimeout = 301,
     kErrTokenOutOfRange = 401,
+    kErrPagedIndex = 501,
+    kErrPackedBarrierTimeout = 601,
 };
 
 __device__ __forceinline__ void record_error(int code) { atomicCAS(&g_device_error, 0, code); }

@@ -693,6 +693,154 @@ def attention(q, k, v, out, scale, key_bias=None, workspace=None, quant=None, ro
     return out if nd == 4 or out is None else out[None, None]      # the [1, 1, rows, D] view of a 2-D call
 
 
+# ------------------------------------------------------------------------------------- a cache of pages
+_HALF = {torch.bfloat16: BF16, torch.float16: F16}
+
+
+def _paged_view(what, k_pages, v_pages, table, lengths):
+    """The checks and the C view of one layer of a paged cache: pages [P, page, heads, D] (any strides that both share, unit last),
+    table int32 [S, W], lengths int32 [S]."""
+    _cuda(k_pages, v_pages, table, lengths)
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype or k_pages.dtype not in _HALF:
+        raise TurboPiError(f"{what}: key and value pages must be bf16 or fp16 [pages, page, heads, D] of one shape")
+    if k_pages.stride() != v_pages.stride() or k_pages.stride(3) != 1:
+        raise TurboPiError(f"{what}: key and value pages must have the same strides and a contiguous last dimension")
+    if table.dim() != 2 or lengths.dim() != 1 or table.dtype != torch.int32 or lengths.dtype != torch.int32:
+        raise TurboPiError(f"{what}: table must be int32 [sequences, pages], lengths int32 [sequences]")
+    S, W = table.shape
+    if lengths.numel() != S or (S > 1 and lengths.stride(0) != 1) or (W > 1 and table.stride(1) != 1):
+        raise TurboPiError(f"{what}: one contiguous length per row of the table, rows contiguous")
+    _one_device(what, k_pages, v_pages, table, lengths)
+    P, page, H, D = k_pages.shape
+    return _lib.PagedCacheView(_ptr(k_pages), _ptr(v_pages), k_pages.stride(0), k_pages.stride(1), k_pages.stride(2), P, page, H, D,
+                               _HALF[k_pages.dtype], _ptr(table), table.stride(0), W, _ptr(lengths), S)
+
+
+def _one_device(what, first, *others):
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise TurboPiError(f"{what}: tensors on different devices")
+
+
+def _rows_of_heads(what, name, t, tokens, heads, D, dtype):
+    if t.dim() != 3 or tuple(t.shape) != (tokens, heads, D) or t.dtype != dtype or t.stride(2) != 1:
+        raise TurboPiError(f"{what}: {name} must be {dtype} [{tokens}, {heads}, {D}] with a contiguous last dimension")
+
+
+def _strides(t):
+    return _Two(t.stride(0), t.stride(1))
+
+
+def paged_attention_workspace(q_heads, kv_heads, head_dim, device):
+    """Scratch for `paged_attention`, whatever the number of sequences and their lengths; needs no initialisation.  Calls that
+    may overlap need one each."""
+    with torch.cuda.device(device):
+        n = int(_lib.load().tpb200_paged_attention_workspace_size(int(q_heads), int(kv_heads), int(head_dim)))
+    if n == 0:
+        raise TurboPiError("paged_attention: unsupported heads")
+    return torch.empty(n, dtype=torch.uint8, device=device)
+
+
+def paged_attention(q, k_pages, v_pages, table, lengths, scale, out=None, workspace=None):
+    """out[s] = softmax(scale * q[s] K^T) V for one new token of each sequence on a cache of pages; returns out.
+    q / out [S, Hq, D]; pages [P, page, Hk, D] (one layer; Hq a multiple of Hk, consecutive query heads share a key head); table
+    int32 [S, W]: position j of sequence s is row j % page of page table[s, j // page]; lengths int32 [S], the new token among them.
+    bf16 or fp16.  A sequence of length 0 gives zeros.  table and lengths are read on the device: a captured call follows
+    them, and what they must not hold is reported by tpb200_device_error()."""
+    view = _paged_view("paged_attention", k_pages, v_pages, table, lengths)
+    _cuda(q, out, workspace)
+    if q.dim() != 3:
+        raise TurboPiError("paged_attention: q must be [sequences, heads, D]")
+    Hq = q.shape[1]
+    _rows_of_heads("paged_attention", "q", q, view.seqs, Hq, view.head_dim, k_pages.dtype)
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    else:
+        _rows_of_heads("paged_attention", "out", out, view.seqs, Hq, view.head_dim, k_pages.dtype)
+    if Hq < 1 or Hq % view.kv_heads:
+        raise TurboPiError(f"paged_attention: {Hq} query heads on {view.kv_heads} key heads")
+    if view.seqs == 0:
+        return out
+    if workspace is None:
+        workspace = paged_attention_workspace(Hq, view.kv_heads, view.head_dim, q.device)
+    _one_device("paged_attention", k_pages, q, out, workspace)
+    args = _lib.PagedAttentionArgs(cache=view, q=_ptr(q), out=_ptr(out), q_stride=_strides(q), o_stride=_strides(out), q_heads=Hq,
+                                   scale=float(scale), workspace=_ptr(workspace),
+                                   workspace_bytes=workspace.numel() * workspace.element_size(), flags=_flags.value)
+    _lib.check(_run(q, _lib.load().tpb200_paged_attention, args), "tpb200_paged_attention")
+    return out
+
+
+def paged_append(k, v, k_pages, v_pages, table, cu, lengths, q=None, cos=None, sin=None, q_out=None):
+    """Writes new tokens' keys and values into their pages; returns the rotated queries (None without q).
+    k / v [T, Hk, D], q [T, Hq, D]: the sequences' tokens one behind the other, sequence s at [cu[s], cu[s + 1]) (cu int32 [S + 1]);
+    its last token goes to position lengths[s] - 1.  Tokens behind cu[S] are left alone, in q_out too.
+    cos / sin [positions, D / 2] (fp32, fp16 or bf16): keys and queries are rotated (rotate-half, in fp32, rounded once); q_out
+    may be q."""
+    view = _paged_view("paged_append", k_pages, v_pages, table, lengths)
+    _cuda(k, v, cu, q, cos, sin, q_out)
+    D, H, dtype = view.head_dim, view.kv_heads, k_pages.dtype
+    if k.dim() != 3:
+        raise TurboPiError("paged_append: k must be [tokens, heads, D]")
+    T = k.shape[0]
+    _rows_of_heads("paged_append", "k", k, T, H, D, dtype)
+    _rows_of_heads("paged_append", "v", v, T, H, D, dtype)
+    if cu.dtype != torch.int32 or cu.dim() != 1 or cu.numel() != view.seqs + 1 or not cu.is_contiguous():
+        raise TurboPiError("paged_append: cu must be contiguous int32 [sequences + 1]")
+    if (cos is None) != (sin is None) or (q is not None and cos is None) or (q is None and q_out is not None):
+        raise TurboPiError("paged_append: cos and sin go together, q with them, q_out with q")
+    if cos is not None and (cos.dim() != 2 or cos.shape != sin.shape or cos.shape[1] != D // 2 or cos.dtype != sin.dtype
+                            or cos.dtype not in _DTYPES or not cos.is_contiguous() or not sin.is_contiguous()):
+        raise TurboPiError(f"paged_append: cos and sin must be contiguous [positions, {D // 2}] of one floating type")
+    if q is not None:
+        if q.dim() != 3:
+            raise TurboPiError("paged_append: q must be [tokens, heads, D]")
+        _rows_of_heads("paged_append", "q", q, T, q.shape[1], D, dtype)
+        if q_out is None:
+            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        else:
+            _rows_of_heads("paged_append", "q_out", q_out, T, q.shape[1], D, dtype)
+    _one_device("paged_append", k_pages, k, v, cu, q, cos, sin, q_out)
+    args = _lib.PagedAppendArgs(cache=view, k=_ptr(k), v=_ptr(v), q=_ptr(q), q_out=_ptr(q_out), k_stride=_strides(k),
+                                v_stride=_strides(v), q_stride=_strides(q) if q is not None else _Two(0, 0),
+                                o_stride=_strides(q_out) if q is not None else _Two(0, 0), cu=_ptr(cu), tokens=T,
+                                q_heads=q.shape[1] if q is not None else 0, cos=_ptr(cos), sin=_ptr(sin),
+                                rope_dtype=_dt(cos) if cos is not None else F32,
+                                rope_positions=cos.shape[0] if cos is not None else 0, flags=_flags.value)
+    _lib.check(_run(k, _lib.load().tpb200_paged_append, args), "tpb200_paged_append")
+    return q_out
+
+
+def copy_pages(pages, src, dst):
+    """pages[..., dst[i], :, :, :] = pages[..., src[i], :, :, :] for every i, in one pass over the moved bytes.
+    pages: contiguous [..., P, page, heads, D] of any type (PagedCache holds [layers, 2, P, page, heads, D]).  src / dst: sequences of
+    ints or integer tensors on the CPU; an index outside the pool, a page written twice or a page both read and written is
+    refused.  The lists are read before the call returns."""
+    _cuda(pages)
+    if pages.dim() < 4 or not pages.is_contiguous():
+        raise TurboPiError("copy_pages: pages must be contiguous [..., pages, page, heads, D]")
+    lists = []
+    for x in (src, dst):
+        if torch.is_tensor(x):
+            if x.is_cuda or x.is_floating_point() or x.dim() != 1:
+                raise TurboPiError("copy_pages: src and dst are sequences of ints or 1-D integer tensors on the CPU")
+            x = x.tolist()
+        lists.append(x)
+    n = len(lists[0])
+    if len(lists[1]) != n:
+        raise TurboPiError("copy_pages: src and dst differ in length")
+    P = pages.shape[-4]
+    slab = pages.stride(-4) * P * pages.element_size()
+    if n == 0 or pages.numel() == 0:
+        if n:
+            raise TurboPiError("copy_pages: the pool is empty")
+        return
+    arrays = [(ctypes.c_int * n)(*x) for x in lists]
+    st = _run(pages, _lib.load().tpb200_copy_pages, _ptr(pages), slab, pages.numel() * pages.element_size() // slab,
+              slab // P, P, arrays[0], arrays[1], n, _flags.value)
+    _lib.check(st, "tpb200_copy_pages")
+
+
 # ------------------------------------------------------------------------------------- tensor-core GEMV
 class TcGemv:
     """NVFP4 weight-only GEMV(s) for M <= 16 tokens on the tensor cores.  Built once from a list of
