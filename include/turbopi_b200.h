@@ -417,6 +417,24 @@ typedef struct {
 int tpb200_attention_describe(int n_rows, int n_keys, int head_dim, int groups, int fused_quant, tpb200_attention_launch_info* info);
 
 /* ---------------------------------------------------------------------------------------------
+ * Attention over prompts packed one behind the other.  Sequence s has the queries [cu[s], cu[s + 1]) and the keys
+ * [cu_keys[s], cu_keys[s + 1]) (cu_keys NULL: the same offsets); out = softmax(scale * Q K^T) V per sequence and head.  causal != 0: query i of
+ * n sees the keys up to i + (m - n) of m, so queries may stand behind keys that were there before them.  A query without
+ * keys gives zeros.  Query heads [h * g, (h + 1) * g) read key head h.  q / out [q_tokens, q_heads, head_dim], k / v
+ * [k_tokens, kv_heads, head_dim] with element strides of a token and a head, multiples of 8 that do not overlap; bf16 or fp16;
+ * head_dim a multiple of 8, <= 256.  Tokens behind cu[seqs] are left alone.  The offsets are read on the device (a captured call
+ * follows them); ones outside the tensors are clamped to them.
+ * ------------------------------------------------------------------------------------------- */
+typedef struct {
+    const void* q; const void* k; const void* v; void* out;
+    long long q_stride[2]; long long k_stride[2]; long long v_stride[2]; long long o_stride[2];
+    const int* cu; const int* cu_keys;
+    int seqs; int q_tokens; int k_tokens; int q_heads; int kv_heads; int head_dim; int dtype;
+    float scale; int causal; int flags;
+} tpb200_packed_attention_args;
+int tpb200_packed_attention(const tpb200_packed_attention_args* args, tpb200_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------------
  * A cache of pages that many sequences share (one layer of it).  Key and value pages lie apart, with the same strides (in
  * elements, multiples of 8): row r of head h of page p starts at p * page_stride + r * row_stride + h * head_stride.  Position j of
  * sequence s is row j % page_size of page table[s * table_stride + j / page_size].  bf16 or fp16; head_dim a multiple of 8, <= 256.

@@ -89,3 +89,20 @@ def test_cpu_tensors_are_refused():
         ops.paged_append(k[:, 0], k[:, 0], k, k, table, lengths, lengths)
     with pytest.raises(TurboPiError, match="CUDA"):
         ops.copy_pages(k, [0], [1])
+
+
+@pytest.mark.parametrize("change,status", [(dict(q=0), NULL), (dict(v=0), NULL), (dict(cu=0), NULL), (dict(out=0), NULL), (dict(k=8), ALIGN),
+                                           (dict(q_stride=Two(1020, 256)), ALIGN), (dict(k_stride=Two(0, 256)), SHAPE),
+                                           (dict(head_dim=260), SHAPE), (dict(head_dim=4), SHAPE), (dict(q_heads=3), SHAPE),
+                                           (dict(kv_heads=0), SHAPE), (dict(dtype=_lib.F32), ENUM), (dict(flags=2), ENUM),
+                                           (dict(seqs=-1), SHAPE)])
+def test_packed_attention_arguments(change, status):
+    base = dict(q=64, k=64, v=64, out=64, q_stride=Two(1024, 256), k_stride=Two(512, 256), v_stride=Two(512, 256), o_stride=Two(1024, 256),
+                cu=64, seqs=1, q_tokens=9, k_tokens=9, q_heads=4, kv_heads=2, head_dim=256, dtype=_lib.BF16, scale=1.0, causal=1)
+    assert _lib.load().tpb200_packed_attention(_lib.PackedAttentionArgs(**{**base, **change}), None) == status
+
+
+def test_packed_attention_refuses_cpu_tensors():
+    q = torch.zeros(4, 2, 64, dtype=torch.bfloat16)
+    with pytest.raises(TurboPiError, match="CUDA"):
+        ops.packed_attention(q, q, q, torch.zeros(2, dtype=torch.int32), 1.0)

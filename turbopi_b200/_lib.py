@@ -122,6 +122,13 @@ class PagedAppendArgs(ctypes.Structure):
                 ("sin", c_void_p), ("rope_dtype", c_int), ("rope_positions", c_int), ("flags", c_int)]
 
 
+class PackedAttentionArgs(ctypes.Structure):
+    _fields_ = [("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("out", c_void_p), ("q_stride", c_longlong * 2),
+                ("k_stride", c_longlong * 2), ("v_stride", c_longlong * 2), ("o_stride", c_longlong * 2), ("cu", c_void_p),
+                ("cu_keys", c_void_p), ("seqs", c_int), ("q_tokens", c_int), ("k_tokens", c_int), ("q_heads", c_int),
+                ("kv_heads", c_int), ("head_dim", c_int), ("dtype", c_int), ("scale", c_float), ("causal", c_int), ("flags", c_int)]
+
+
 class ActTc(ctypes.Structure):
     _fields_ = [("x", c_void_p), ("ldx", c_int), ("K", c_int), ("x_image", c_void_p), ("x_row_scale", c_void_p)]
 
@@ -182,6 +189,7 @@ SIGNATURES = {
     "tpb200_attention_workspace_size": (c_size_t, [c_int, c_int, c_int, c_int]),
     "tpb200_attention_describe": (c_int, [c_int, c_int, c_int, c_int, c_int, ctypes.POINTER(AttentionLaunchInfo)]),
     "tpb200_attention": (c_int, [ctypes.POINTER(AttentionArgs), c_void_p]),
+    "tpb200_packed_attention": (c_int, [ctypes.POINTER(PackedAttentionArgs), c_void_p]),
     "tpb200_paged_attention_workspace_size": (c_size_t, [c_int, c_int, c_int]),
     "tpb200_paged_attention": (c_int, [ctypes.POINTER(PagedAttentionArgs), c_void_p]),
     "tpb200_paged_append": (c_int, [ctypes.POINTER(PagedAppendArgs), c_void_p]),

@@ -1,0 +1,673 @@
+// Attention over whole prompts, packed one behind the other: softmax(scale Q K^T) V per sequence, causal or not, with
+// grouped heads, queries behind keys that are already there, bf16 or fp16, on tcgen05.mma kind::f16.
+//
+// One pass over the keys per tile of 128 query rows, with the running reference m of a softmax:
+//     S = Q K_j^T,  P = 2^(scale2 S - m),  O += P V_j,  l += rowsum P,      out = O / l
+// m is raised (and O, l scaled by 2^(m_old - m_new)) only when a row's maximum passes m by 8: P stays below 2^8, which costs no
+// relative precision in either type, and after the first tiles O is hardly ever touched between its products.
+//
+// A row of a tile is a (token, head) pair: `pack` query heads of one key head, the largest power of two in the group, side by side,
+// so that short prompts fill tiles and the heads of a group read their keys once.
+//
+// Roles (384 threads, one CTA an SM): warp 0 requests tiles of K and V by TMA into a ring of units, warp 1 issues the products, two
+// groups of four warps do the softmax, a thread per row, with registers moved over to them from the others (setmaxnreg).
+// The products are a line of events e; event e computes S into tensor-memory buffer e & 1, group e & 1 turns it into P in the same
+// columns, the product with V reads P from there:
+//   head sizes up to 128  two tiles of 128 rows per CTA, one per group: event e is key tile e / 2 of row tile e & 1; each unit of K
+//                         and V is read by both, which halves what comes through L2 (a row tile of its own would need 64 KB per
+//                         1024 cycles of products, twice what an SM gets);
+//   above                 one row tile (its O alone is 256 columns), the groups take alternate key tiles and hand m on through
+//                         shared memory.
+// While one group works the other's products run.
+//
+// What may stand in masked places does not matter: scores are selected, not biased.  Rows of V behind a sequence's end are zeroed in
+// shared memory, and in tiles that hold masked pairs V is searched for infinities and NaN (weight 0 times those would be NaN): they are
+// taken out and added to the rows that do see them at the end.
+#include <algorithm>
+#include <atomic>
+#include <type_traits>
+
+#include "paged.cuh"
+#include "tcgen05.cuh"
+
+namespace tpb {
+namespace {
+
+constexpr int kTile = 128;               // rows of a query tile, keys of a key tile
+constexpr int kBlockBytes = kTile * 128; // 128 rows x 64 columns of 16 bits
+constexpr int kThreadsPacked = 384;
+constexpr uint32_t kTmemCols = 512, kColO = 256;
+constexpr long long kWait = 200000000LL; // about 0.1 s: the bound of each wait
+constexpr float kRaise = 8.0f;
+constexpr int kBadTiles = 4;             // key tiles with masked pairs at most: 256 rows on the diagonal and the sequence's end
+
+struct PackedParams {
+    CUtensorMap q, k, v;
+    uint16_t* out;
+    const uint16_t* v_rows;
+    long long o_stride[2], v_stride[2];
+    const int *cu, *cu_keys;
+    int seqs, q_tokens, k_tokens;
+    int head_dim;
+    int pack, pack_shift, head_groups;   // query heads of a tile; tiles' worth of heads
+    int groups_per_kv;                   // head groups that share a key head
+    float scale2;                        // |scale| log2 e
+    uint32_t idesc_s, idesc_o;
+    int causal;
+};
+
+template <int DP>
+struct Layout {
+    static constexpr bool kTwo = DP <= 128;
+    static constexpr int kRowTiles = kTwo ? 2 : 1;
+    static constexpr int kBlocks = DP / 64;                        // 64-column blocks of a row
+    static constexpr int kUnitBlocks = DP < 128 ? 1 : 2;           // a unit: 128 keys x up to 128 columns
+    static constexpr int kHalves = kBlocks / kUnitBlocks;          // units of a tile
+    static constexpr int kUnitBytes = kUnitBlocks * kBlockBytes;
+    static constexpr int kUnits = DP < 128 ? 8 : 4;
+    static constexpr int kQBytes = kRowTiles * kBlocks * kBlockBytes;
+};
+
+struct PackedControl {
+    uint64_t q_full;
+    uint64_t full[8], empty[8];
+    uint64_t s_ready[2], p_ready[2], o_done[2];
+    uint64_t ref_ready[2][4];            // one row tile: the reference of event e, by quarter of the rows
+    uint32_t tmem_base;
+    int failed;
+    int seq, tile, q0, nq, k0, nk;       // the CTA's work
+    int bad_any;
+    uint32_t bad[kBadTiles][4];          // keys of masked tiles with infinities or NaN in V, from the first masked tile on
+    float ref[kTile];
+    float part_l[2][kTile], part_m[2][kTile];
+};
+
+template <int DP>
+constexpr int packed_smem() {
+    return Layout<DP>::kQBytes + Layout<DP>::kUnits * Layout<DP>::kUnitBytes + static_cast<int>(sizeof(PackedControl)) + 1024;
+}
+
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a),
+        "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d), "r"(a),
+        "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int c0, int c1, int c2, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+            smem_u32(dst)),
+        "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(smem_u32(bar))
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};\n" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_done() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Pairs of floats in one instruction
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpair(uint64_t p, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity) {
+    return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, kWait));
+}
+
+// The keys a query row sees: [0, limit)
+__device__ __forceinline__ int row_limit(const PackedParams& P, int nq, int nk, int token) {
+    if (token >= nq) return 0;
+    return P.causal ? max(0, min(nk, nk - nq + token + 1)) : nk;
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreadsPacked, 1) packed_attention_kernel(const __grid_constant__ PackedParams P) {
+    using L = Layout<DP>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* sQ = smem;
+    uint8_t* ring = smem + L::kQBytes;
+    PackedControl* ctl = reinterpret_cast<PackedControl*>(ring + L::kUnits * L::kUnitBytes);
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    const int head_group = blockIdx.x % P.head_groups;
+    constexpr int kRowsCta = L::kRowTiles * kTile;
+    const int tokens_cta = kRowsCta >> P.pack_shift;
+
+    pdl_wait_prior_grids();              // the offsets may come from the previous kernel too
+    if (warp == 0) {
+        // which tile of which sequence: tiles are dealt from the last one back, so that within a sequence the long rows come first
+        const int want = static_cast<int>(gridDim.x / P.head_groups - 1 - blockIdx.x / P.head_groups);
+        int before = 0, found = -1, tile = 0;
+        for (int s0 = 0; s0 < P.seqs; s0 += 32) {
+            const int s = s0 + lane;
+            int n = 0;
+            if (s < P.seqs) {
+                const int a = min(max(P.cu[s], 0), P.q_tokens), b = min(max(P.cu[s + 1], a), P.q_tokens);
+                n = (b - a + tokens_cta - 1) / tokens_cta;
+            }
+            int upto = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += y;
+            }
+            const uint32_t hit = __ballot_sync(0xffffffffu, want >= before + upto - n && want < before + upto);
+            if (hit != 0) {
+                const int at = __ffs(hit) - 1;
+                found = s0 + at;
+                tile = want - before - __shfl_sync(0xffffffffu, upto - n, at);
+                break;
+            }
+            before += __shfl_sync(0xffffffffu, upto, 31);
+        }
+        if (lane == 0) {
+            ctl->seq = found;
+            ctl->tile = tile;
+            if (found >= 0) {
+                const int a = min(max(P.cu[found], 0), P.q_tokens);
+                ctl->q0 = a;
+                ctl->nq = min(max(P.cu[found + 1], a), P.q_tokens) - a;
+                const int ka = min(max(P.cu_keys[found], 0), P.k_tokens);
+                ctl->k0 = ka;
+                ctl->nk = min(max(P.cu_keys[found + 1], ka), P.k_tokens) - ka;
+            }
+        }
+    }
+    if (threadIdx.x == 32) {
+        mbar_init(&ctl->q_full, 1);
+        for (int i = 0; i < L::kUnits; ++i) {
+            mbar_init(&ctl->full[i], 1);
+            mbar_init(&ctl->empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&ctl->s_ready[i], 1);
+            mbar_init(&ctl->p_ready[i], 4);
+            mbar_init(&ctl->o_done[i], 1);
+            for (int w = 0; w < 4; ++w) mbar_init(&ctl->ref_ready[i][w], 1);
+        }
+        fence_mbar_init();
+        ctl->failed = 0;
+        ctl->bad_any = 0;
+        for (int i = 0; i < kBadTiles * 4; ++i) ctl->bad[i >> 2][i & 3] = 0;
+        tc::prefetch_tensormap(&P.q);
+        if (P.k_tokens > 0) {
+            tc::prefetch_tensormap(&P.k);
+            tc::prefetch_tensormap(&P.v);
+        }
+    }
+    __syncthreads();
+    if (ctl->seq < 0) {
+        pdl_launch_dependents();
+        return;
+    }
+    if (warp == 2) {
+        tc::tmem_alloc(&ctl->tmem_base, kTmemCols);
+        tc::tmem_relinquish();
+    }
+    tc::fence_before_thread_sync();
+    __syncthreads();
+    tc::fence_after_thread_sync();
+    pdl_launch_dependents();
+    const uint32_t tmem = ctl->tmem_base;
+    const int nq = ctl->nq, nk = ctl->nk, q0 = ctl->q0, k0 = ctl->k0;
+    const int token0 = ctl->tile * tokens_cta;
+    const int tokens_tile = kTile >> P.pack_shift;
+    // key tiles of each row tile: up to the last row's limit; the second row tile of a CTA never has fewer than the first
+    int tiles[2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+        const int first = token0 + x * tokens_tile, last = min(first + tokens_tile, nq) - 1;
+        tiles[x] = (x < L::kRowTiles && last >= first) ? (row_limit(P, nq, nk, last) + kTile - 1) / kTile : 0;
+    }
+    if (!L::kTwo) tiles[1] = 0;
+    const int n_tiles = max(tiles[0], tiles[1]);
+    const int events = L::kTwo ? 2 * n_tiles : n_tiles;
+    // the order of the line of events: which are computed, and where the tiles of K and V stand in the ring
+    auto active = [&](int e) { return L::kTwo ? (e >> 1) < tiles[e & 1] : true; };
+    auto key_tile = [&](int e) { return L::kTwo ? e >> 1 : e; };
+    auto last_use = [&](int e) { return !L::kTwo || (e & 1) == 1 || tiles[1] == 0; };
+    auto k_unit = [&](int j) { return L::kHalves * (L::kTwo ? 2 * j : (j < 2 ? j : 2 * j - 1)); };
+    auto v_unit = [&](int j) { return L::kHalves * (L::kTwo ? 2 * j + 1 : (j == n_tiles - 1 ? 2 * j + 1 : 2 * j + 2)); };
+
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        if (warp == 0 && n_tiles > 0) {
+            // -------------------------------------------------------- producer
+            const int kv_head = head_group / P.groups_per_kv;
+            if (tc::elect_one()) {
+                bool ok = true;
+                mbar_expect_tx(&ctl->q_full, (tiles[1] > 0 ? 2 : 1) * L::kBlocks * kBlockBytes);
+                for (int x = 0; x < (tiles[1] > 0 ? 2 : 1); ++x) {
+                    for (int b = 0; b < L::kBlocks; ++b) {
+                        tma_load_3d(sQ + (x * L::kBlocks + b) * kBlockBytes, &P.q, b * 64, head_group << P.pack_shift,
+                                    q0 + token0 + x * tokens_tile, &ctl->q_full);
+                    }
+                }
+                int u = 0;
+                auto request = [&](const CUtensorMap* map, int j) {
+                    for (int h = 0; h < L::kHalves; ++h, ++u) {
+                        const int slot = u % L::kUnits;
+                        if (!mbar_wait_bounded(&ctl->empty[slot], ((u / L::kUnits) & 1) ^ 1, kWait)) return false;
+                        mbar_expect_tx(&ctl->full[slot], L::kUnitBytes);
+                        for (int b = 0; b < L::kUnitBlocks; ++b) {
+                            tma_load_3d(ring + slot * L::kUnitBytes + b * kBlockBytes, map, (h * L::kUnitBlocks + b) * 64, kv_head,
+                                        k0 + j * kTile, &ctl->full[slot]);
+                        }
+                    }
+                    return true;
+                };
+                if (L::kTwo) {
+                    for (int j = 0; j < n_tiles && ok; ++j) ok = request(&P.k, j) && request(&P.v, j);
+                } else {
+                    ok = request(&P.k, 0);
+                    for (int j = 1; j < n_tiles && ok; ++j) ok = request(&P.k, j) && (j < 1 || request(&P.v, j - 1));
+                    ok = ok && request(&P.v, n_tiles - 1);
+                }
+                if (!ok) {
+                    record_error(kErrPackedBarrierTimeout);
+                    ctl->failed = 1;
+                }
+            }
+            __syncwarp();
+        } else if (warp == 1 && n_tiles > 0) {
+            // -------------------------------------------------------- products
+            const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+            const uint32_t q16 = (smem_u32(sQ) & 0x3FFFFu) >> 4, r16 = (smem_u32(ring) & 0x3FFFFu) >> 4;
+            const int ksteps = (P.head_dim + 15) >> 4;
+            constexpr uint32_t kDescHiMnSw128 = (1024u >> 4) | (1u << 14) | (static_cast<uint32_t>(tc::kSwizzle128B) << 29);
+            constexpr uint32_t kLboField = (static_cast<uint32_t>(kBlockBytes) >> 4) << 16;
+            bool ok = wait_warp(&ctl->q_full, 0);
+            auto scores = [&](int e) {
+                const int u0 = k_unit(key_tile(e));
+                const uint32_t qa = q16 + (L::kTwo ? (e & 1) * (L::kBlocks * kBlockBytes >> 4) : 0);
+#pragma unroll
+                for (int h = 0; h < L::kHalves; ++h) {
+                    const int slot = (u0 + h) % L::kUnits;
+                    if (!wait_warp(&ctl->full[slot], ((u0 + h) / L::kUnits) & 1)) return false;
+                    tc::fence_after_thread_sync();
+                    if (tc::elect_one()) {
+                        const uint32_t ka = r16 + (slot * L::kUnitBytes >> 4);
+                        const int steps = min(ksteps - h * L::kUnitBlocks * 4, L::kUnitBlocks * 4);
+                        for (int kk = 0; kk < steps; ++kk) {
+                            const uint32_t off = static_cast<uint32_t>((kk >> 2) * kBlockBytes + (kk & 3) * 32) >> 4;
+                            mma_ss(tm + (e & 1) * kTile, tc::desc_from_words(qa + h * (L::kUnitBytes >> 4) + off, tc::kDescHiKmajorSw128),
+                                   tc::desc_from_words(ka + off, tc::kDescHiKmajorSw128), P.idesc_s, (h | kk) > 0 ? 1u : 0u);
+                        }
+                        if (last_use(e)) tc::commit(&ctl->empty[slot]);
+                        if (h == L::kHalves - 1) tc::commit(&ctl->s_ready[e & 1]);
+                    }
+                    __syncwarp();
+                }
+                return true;
+            };
+            auto values = [&](int e) {
+                if (!wait_warp(&ctl->p_ready[e & 1], (e >> 1) & 1)) return false;
+                const int j = key_tile(e), u0 = v_unit(j);
+#pragma unroll
+                for (int h = 0; h < L::kHalves; ++h) {
+                    const int slot = (u0 + h) % L::kUnits;
+                    if (!wait_warp(&ctl->full[slot], ((u0 + h) / L::kUnits) & 1)) return false;
+                    tc::fence_after_thread_sync();
+                    if (tc::elect_one()) {
+                        const uint32_t va = r16 + (slot * L::kUnitBytes >> 4);
+                        const uint32_t d = tm + kColO + (L::kTwo ? (e & 1) * DP : h * 128);
+                        for (int kk = 0; kk < kTile / 16; ++kk) {
+                            mma_ts(d, tm + (e & 1) * kTile + kk * 8, tc::desc_from_words((va + (kk * 2048 >> 4)) | kLboField, kDescHiMnSw128),
+                                   P.idesc_o, (j | kk) > 0 ? 1u : 0u);
+                        }
+                        if (last_use(e)) tc::commit(&ctl->empty[slot]);
+                        if (h == L::kHalves - 1) tc::commit(&ctl->o_done[e & 1]);
+                    }
+                    __syncwarp();
+                }
+                return true;
+            };
+            if (ok && active(0)) ok = scores(0);
+            if (ok && events > 1 && active(1)) ok = scores(1);
+            for (int e = 0; e < events && ok; ++e) {
+                if (!active(e)) continue;
+                ok = values(e);
+                if (ok && e + 2 < events && active(e + 2)) ok = scores(e + 2);
+            }
+            if (!ok && lane == 0) {
+                record_error(kErrPackedBarrierTimeout);
+                ctl->failed = 1;
+            }
+        }
+    } else {
+        // ------------------------------------------------------------ softmax: group x, thread = row of a tile
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        const int x = (warp >> 2) - 1;
+        const int quarter = warp & 3, row = quarter * 32 + lane;
+        const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+        const uint32_t s_at = lanes + x * kTile, o_at = lanes + kColO + (L::kTwo ? x * DP : 0);
+        const int my_tile = L::kTwo ? x : 0;
+        const int token = token0 + my_tile * tokens_tile + (row >> P.pack_shift);
+        const int limit = row_limit(P, nq, nk, token);
+        const int lowest = row_limit(P, nq, nk, token0 + my_tile * tokens_tile);     // of the tile's rows that exist
+        const int first_masked = row_limit(P, nq, nk, token0) / kTile;               // of the CTA: where `bad` begins
+        float ref = -INFINITY, l = 0.0f;
+        float l_ref = -INFINITY;         // the reference that l is relative to (one row tile: the groups share ref)
+        bool ok = true;
+        for (int e = x; e < events; e += 2) {
+            if (!active(e)) break;
+            const int j = key_tile(e);
+            if (!wait_warp(&ctl->s_ready[x], (e >> 1) & 1)) { ok = false; break; }
+            tc::fence_after_thread_sync();
+            uint32_t s[kTile];
+#pragma unroll
+            for (int c = 0; c < kTile / 32; ++c) tc::tmem_ld_32x32b_x32(s_at + c * 32, *reinterpret_cast<uint32_t(*)[32]>(s + c * 32));
+            tc::tmem_ld_wait();
+            const bool masked = (j + 1) * kTile > lowest;
+            if (masked) {
+                const int lim = limit - j * kTile;
+#pragma unroll
+                for (int i = 0; i < kTile; ++i) s[i] = i < lim ? s[i] : 0xff800000u;
+            }
+            float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int i = 0; i < kTile; i += 4) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c) top[c] = fmaxf(top[c], __uint_as_float(s[i + c]));
+            }
+            const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * P.scale2;
+            if (!L::kTwo && e > 0) {     // the reference after the event before, from the other group
+                if (!wait_warp(&ctl->ref_ready[x ^ 1][quarter], ((e - 1) >> 1) & 1)) { ok = false; break; }
+                ref = ctl->ref[row];
+            }
+            const bool raise = high > ref + kRaise || (ref == -INFINITY && high > ref);
+            const float now = raise ? high : ref;
+            if (!L::kTwo) {
+                ctl->ref[row] = now;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&ctl->ref_ready[x][quarter]);
+            }
+            const int before = L::kTwo ? e - 2 : e - 1;                    // the last product into this O
+            if (__any_sync(0xffffffffu, raise) && before >= 0) {
+                if (!wait_warp(&ctl->o_done[before & 1], (before >> 1) & 1)) { ok = false; break; }
+                tc::fence_after_thread_sync();
+                const float f = raise ? ex2(ref - now) : 1.0f;
+                for (int c = 0; c < DP; c += 32) {
+                    uint32_t o[32];
+                    tc::tmem_ld_32x32b_x32(o_at + c, o);
+                    tc::tmem_ld_wait();
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                    tmem_st_x32(o_at + c, o);
+                }
+                tmem_st_done();
+            }
+            ref = now;
+            const float base = ref == -INFINITY ? 0.0f : ref;
+            if (l_ref != ref) {
+                l *= ex2(l_ref - base);
+                l_ref = ref;
+            }
+            // P = 2^(scale2 S - m), its row sum, rounded pairs into the columns S was in
+            const uint64_t scale = pair(P.scale2, P.scale2), minus = pair(-base, -base);
+            uint64_t sum[2] = {pair(0.0f, 0.0f), pair(0.0f, 0.0f)};
+            uint32_t p[kTile / 2];
+#pragma unroll
+            for (int i = 0; i < kTile / 2; ++i) {
+                float a, b;
+                unpair(fma2(pair(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), scale, minus), a, b);
+                a = ex2(a);
+                b = ex2(b);
+                sum[i & 1] = add2(sum[i & 1], pair(a, b));
+                p[i] = Half16<T>::pack(a, b);
+            }
+            tmem_st_x32(s_at, p);
+            tmem_st_x32(s_at + 32, p + 32);
+            float a, b;
+            unpair(add2(sum[0], sum[1]), a, b);
+            l += a + b;
+            // V of a tile with masked pairs: rows behind the sequence's end to zero, infinities and NaN out of the product
+            if (masked && (!L::kTwo || x == 0 || j >= tiles[0])) {
+                const int u0 = v_unit(j);
+                const bool there = j * kTile + row < nk;
+                bool bad = false;
+                for (int h = 0; h < L::kHalves && ok; ++h) {
+                    const int slot = (u0 + h) % L::kUnits;
+                    if (!wait_warp(&ctl->full[slot], ((u0 + h) / L::kUnits) & 1)) { ok = false; break; }
+                    for (int b2 = 0; b2 < L::kUnitBlocks; ++b2) {
+                        uint4* at = reinterpret_cast<uint4*>(ring + slot * L::kUnitBytes + b2 * kBlockBytes + row * 128);
+                        if (!there) {
+#pragma unroll
+                            for (int c = 0; c < 8; ++c) at[c] = make_uint4(0, 0, 0, 0);
+                            continue;
+                        }
+#pragma unroll
+                        for (int c = 0; c < 8; ++c) {
+                            uint4 v = at[c ^ (row & 7)];
+                            uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+                            bool here = false;
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                constexpr uint32_t kExp = std::is_same<T, __nv_bfloat16>::value ? 0x7f80u : 0x7c00u;
+                                if ((w[i] & kExp) == kExp) { w[i] &= 0xffff0000u; here = true; }
+                                if ((w[i] & (kExp << 16)) == (kExp << 16)) { w[i] &= 0xffffu; here = true; }
+                            }
+                            if (here) {
+                                at[c ^ (row & 7)] = v;
+                                bad = true;
+                            }
+                        }
+                    }
+                }
+                if (!ok) break;
+                const uint32_t word = __ballot_sync(0xffffffffu, bad);
+                if (lane == 0 && word != 0) {
+                    ctl->bad[min(j - first_masked, kBadTiles - 1)][quarter] = word;
+                    ctl->bad_any = 1;
+                }
+                fence_proxy_async_smem();
+            }
+            tmem_st_done();
+            tc::fence_before_thread_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&ctl->p_ready[x]);
+        }
+        // ------------------------------------------------------------ O / l -> the rows
+        if (!L::kTwo) {
+            ctl->part_l[x][row] = l;
+            ctl->part_m[x][row] = l_ref;
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            const float m = fmaxf(ctl->part_m[0][row], ctl->part_m[1][row]), base = m == -INFINITY ? 0.0f : m;
+            l = ctl->part_l[0][row] * ex2(ctl->part_m[0][row] - base) + ctl->part_l[1][row] * ex2(ctl->part_m[1][row] - base);
+        }
+        const int mine = L::kTwo ? tiles[x] : tiles[0];
+        if (ok && mine > 0) {
+            const int last = L::kTwo ? 2 * (mine - 1) + x : mine - 1;
+            if (!wait_warp(&ctl->o_done[last & 1], (last >> 1) & 1)) ok = false;
+            tc::fence_after_thread_sync();
+        }
+        if (!ok && lane == 0) {
+            record_error(kErrPackedBarrierTimeout);
+            ctl->failed = 1;
+        }
+        if (ok && (L::kTwo || x == 0 || DP > 128)) {
+            const float inv = mine > 0 ? 1.0f / l : 0.0f;
+            const int head = (head_group << P.pack_shift) + (row & (P.pack - 1));
+            uint16_t* to = P.out + static_cast<long long>(q0 + token) * P.o_stride[0] + head * P.o_stride[1];
+            const int c_lo = L::kTwo ? 0 : x * (DP / 2), c_hi = L::kTwo ? DP : c_lo + DP / 2;
+            const bool any_bad = mine > 0 && ctl->bad_any != 0;
+            for (int c = c_lo; c < c_hi; c += 32) {
+                uint32_t o[32];
+                if (mine > 0) {
+                    tc::tmem_ld_32x32b_x32(o_at + c, o);
+                    tc::tmem_ld_wait();
+                }
+                if (token >= nq) continue;
+                if (any_bad) {           // what was taken out of V, for the rows that see it
+                    for (int i = 0; i < kBadTiles * kTile; ++i) {
+                        const int key = (first_masked + i / kTile) * kTile + i % kTile;
+                        if (!((ctl->bad[i >> 7][(i >> 5) & 3] >> (i & 31)) & 1) || key >= limit) continue;
+                        const uint16_t* from = P.v_rows + static_cast<long long>(k0 + key) * P.v_stride[0] +
+                                               head_group / P.groups_per_kv * P.v_stride[1];
+#pragma unroll
+                        for (int n = 0; n < 32; ++n) {
+                            if (c + n >= P.head_dim) continue;
+                            const uint32_t w = from[c + n];
+                            const float v = Half16<T>::unpack(w).x;
+                            if (!(fabsf(v) < INFINITY)) o[n] = __float_as_uint(__uint_as_float(o[n]) + v);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < 32; n += 8) {
+                    if (c + n >= P.head_dim) continue;
+                    uint32_t w[4] = {0, 0, 0, 0};
+                    if (limit > 0) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            w[i] = Half16<T>::pack(__uint_as_float(o[n + 2 * i]) * inv, __uint_as_float(o[n + 2 * i + 1]) * inv);
+                        }
+                    }
+                    *reinterpret_cast<uint4*>(to + c + n) = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            }
+        }
+        tc::fence_before_thread_sync();
+    }
+    __syncthreads();
+    if (ctl->failed) {                   // copies may still be on their way into this CTA's shared memory
+        const long long start = clock64();
+        while (clock64() - start < 2000000) {}
+        __syncthreads();
+    }
+    tc::fence_after_thread_sync();
+    if (warp == 2) tc::tmem_dealloc(tmem, kTmemCols);
+}
+
+template <typename T, int DP>
+int launch_packed(const PackedParams& P, unsigned blocks, int flags, cudaStream_t stream) {
+    constexpr int smem = packed_smem<DP>();
+    static_assert(smem <= 227 * 1024, "shared memory of a CTA");
+    static std::atomic<uint64_t> configured{0};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    const uint64_t bit = 1ull << (dev & 63);
+    if (!(configured.load(std::memory_order_relaxed) & bit)) {
+        if (cudaFuncSetAttribute(packed_attention_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
+            return TPB200_ERR_CUDA;
+        }
+        configured.fetch_or(bit, std::memory_order_relaxed);
+    }
+    cudaLaunchAttribute attr;
+    const cudaLaunchConfig_t cfg = paged_config(blocks, kThreadsPacked, smem, flags, &attr, stream);
+    return cudaLaunchKernelEx(&cfg, packed_attention_kernel<T, DP>, P) == cudaSuccess ? TPB200_OK : TPB200_ERR_CUDA;
+}
+
+// [tokens][heads][head_dim] with element strides, boxes of 64 columns x `heads` x `rows` tokens
+bool rows_map(CUtensorMap* map, const void* base, int head_dim, int heads, long long head_stride, int tokens, long long token_stride,
+              int box_heads, int box_tokens) {
+    const uint64_t dims[3] = {static_cast<uint64_t>(head_dim), static_cast<uint64_t>(heads), static_cast<uint64_t>(tokens)};
+    const uint64_t strides[2] = {static_cast<uint64_t>(heads > 1 ? head_stride : head_dim) * 2,
+                                 static_cast<uint64_t>(tokens > 1 ? token_stride : static_cast<long long>(head_dim) * heads) * 2};
+    const uint32_t box[3] = {64, static_cast<uint32_t>(box_heads), static_cast<uint32_t>(box_tokens)};
+    return make_tensor_map_bf16_nd_sw128(map, base, 3, dims, strides, box);
+}
+
+}  // namespace
+
+int device_error_packed_attention(int clear) { return read_device_error(clear); }
+
+}  // namespace tpb
+
+extern "C" int tpb200_packed_attention(const tpb200_packed_attention_args* a, tpb200_stream_t stream) {
+    using namespace tpb;
+    TPB_REQUIRE(a != nullptr, TPB200_ERR_NULL);
+    TPB_REQUIRE((a->flags & ~TPB200_FLAG_PDL) == 0, TPB200_ERR_ENUM);
+    TPB_REQUIRE(a->dtype == TPB200_BF16 || a->dtype == TPB200_F16, TPB200_ERR_ENUM);
+    TPB_REQUIRE(a->seqs >= 0 && a->q_tokens >= 0 && a->k_tokens >= 0, TPB200_ERR_SHAPE);
+    TPB_REQUIRE(a->q_heads >= 1 && a->kv_heads >= 1 && a->q_heads % a->kv_heads == 0, TPB200_ERR_SHAPE);
+    TPB_REQUIRE(a->head_dim >= 8 && a->head_dim <= 256 && a->head_dim % 8 == 0, TPB200_ERR_SHAPE);
+    if (a->seqs == 0 || a->q_tokens == 0) return TPB200_OK;
+    TPB_REQUIRE(a->q && a->out && a->cu && (a->k_tokens == 0 || (a->k && a->v)), TPB200_ERR_NULL);
+    TPB_REQUIRE(tpb_aligned16(a->q) && tpb_aligned16(a->k) && tpb_aligned16(a->v) && tpb_aligned16(a->out), TPB200_ERR_ALIGN);
+    PackedParams P = {};
+    for (int i = 0; i < 2; ++i) {
+        TPB_REQUIRE(a->q_stride[i] % 8 == 0 && a->k_stride[i] % 8 == 0 && a->v_stride[i] % 8 == 0 && a->o_stride[i] % 8 == 0,
+                    TPB200_ERR_ALIGN);
+        const int qn = i == 0 ? a->q_tokens : a->q_heads, kn = i == 0 ? a->k_tokens : a->kv_heads;
+        TPB_REQUIRE((qn <= 1 || (a->q_stride[i] >= a->head_dim && a->o_stride[i] >= a->head_dim)) &&
+                        (kn <= 1 || (a->k_stride[i] >= a->head_dim && a->v_stride[i] >= a->head_dim)),
+                    TPB200_ERR_SHAPE);
+        P.o_stride[i] = a->o_stride[i];
+        P.v_stride[i] = a->v_stride[i];
+    }
+    const int group = a->q_heads / a->kv_heads;
+    int pack = 1;
+    while (group % (2 * pack) == 0 && pack < 16) pack *= 2;
+    for (int p = pack; p > 1; p /= 2) ++P.pack_shift;
+    P.pack = pack;
+    P.head_groups = a->q_heads / pack;
+    P.groups_per_kv = group / pack;
+    P.seqs = a->seqs;
+    P.q_tokens = a->q_tokens;
+    P.k_tokens = a->k_tokens;
+    P.head_dim = a->head_dim;
+    P.cu = a->cu;
+    P.cu_keys = a->cu_keys != nullptr ? a->cu_keys : a->cu;
+    P.out = static_cast<uint16_t*>(a->out);
+    P.v_rows = static_cast<const uint16_t*>(a->v);
+    P.causal = a->causal != 0;
+    // the sign of the scale goes into the product (operand A negated), its size into the exponent; none at all would lose the mask
+    P.scale2 = fmaxf(fabsf(a->scale) * 1.4426950408889634f, 1.1754944e-38f);
+    const int DP = a->head_dim <= 64 ? 64 : (a->head_dim <= 128 ? 128 : 256);
+    const bool bf = a->dtype == TPB200_BF16;
+    // instruction descriptor: fp32 sums, A and B bf16 (1) or fp16 (0), [13] negate A, [16] B MN-major, N >> 3 at 17, M >> 4 at 24
+    const uint32_t types = (1u << 4) | (bf ? (1u << 7) | (1u << 10) : 0u) | ((128u >> 4) << 24);
+    P.idesc_s = types | (a->scale < 0.0f ? 1u << 13 : 0u) | ((128u >> 3) << 17);
+    P.idesc_o = types | (1u << 16) | (static_cast<uint32_t>(std::min(DP, 128) >> 3) << 17);
+    const int rows_tokens = kTile / pack;
+    if (!rows_map(&P.q, a->q, a->head_dim, a->q_heads, a->q_stride[1], a->q_tokens, a->q_stride[0], pack, rows_tokens)) return TPB200_ERR_SHAPE;
+    if (a->k_tokens > 0) {
+        if (!rows_map(&P.k, a->k, a->head_dim, a->kv_heads, a->k_stride[1], a->k_tokens, a->k_stride[0], 1, kTile) ||
+            !rows_map(&P.v, a->v, a->head_dim, a->kv_heads, a->v_stride[1], a->k_tokens, a->v_stride[0], 1, kTile)) {
+            return TPB200_ERR_SHAPE;
+        }
+    }
+    // no more tiles than whole ones and a ragged one per sequence
+    const int tokens_cta = rows_tokens * (DP <= 128 ? 2 : 1);
+    const long long tiles = static_cast<long long>(a->q_tokens) / tokens_cta + std::min(a->seqs, a->q_tokens);
+    const long long blocks = tiles * P.head_groups;
+    TPB_REQUIRE(blocks <= 0x7fffffff, TPB200_ERR_SHAPE);
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    const unsigned n = static_cast<unsigned>(blocks);
+    if (DP == 64) return bf ? launch_packed<__nv_bfloat16, 64>(P, n, a->flags, s) : launch_packed<__half, 64>(P, n, a->flags, s);
+    if (DP == 128) return bf ? launch_packed<__nv_bfloat16, 128>(P, n, a->flags, s) : launch_packed<__half, 128>(P, n, a->flags, s);
+    return bf ? launch_packed<__nv_bfloat16, 256>(P, n, a->flags, s) : launch_packed<__half, 256>(P, n, a->flags, s);
+}

@@ -171,6 +171,7 @@ int device_error_w4_gemm(int clear);
 int device_error_pi05_inputs(int clear);
 int device_error_paged_cache(int clear);
 int device_error_paged_attention(int clear);
+int device_error_packed_attention(int clear);
 
 }  // namespace tpb
 
@@ -204,7 +205,7 @@ int tpb200_device_error(int clear) {
                                      tpb::device_error_nvfp4_gemm, tpb::device_error_gemv_tc,
                                      tpb::device_error_attention, tpb::device_error_w4_gemm,
                                      tpb::device_error_pi05_inputs, tpb::device_error_paged_cache,
-                                     tpb::device_error_paged_attention};
+                                     tpb::device_error_paged_attention, tpb::device_error_packed_attention};
     int first = 0;
     for (auto r : readers) {
         const int v = r(clear);

@@ -731,6 +731,39 @@ def _strides(t):
     return _Two(t.stride(0), t.stride(1))
 
 
+def packed_attention(q, k, v, cu, scale, out=None, causal=True, cu_keys=None):
+    """out = softmax(scale * q k^T) v for prompts packed one behind the other; returns out.
+    q / out [T, Hq, D], k / v [Tk, Hk, D] (views such as columns of a fused projection are fine; Hq a multiple of Hk, consecutive
+    query heads share a key head), bf16 or fp16.  cu int32 [S + 1]: sequence s has the tokens [cu[s], cu[s + 1]).  cu_keys: the
+    same for the keys where a sequence has more (or fewer) of them; causal then means that the last query sees every key:
+    query i of n sees the keys up to i + (m - n) of m.  A query without keys gives zeros; tokens behind cu[S] are left alone.  The
+    offsets are read on the device: a captured call follows them; ones outside the tensors are clamped."""
+    _cuda(q, k, v, cu, out, cu_keys)
+    if q.dim() != 3 or k.dim() != 3 or q.dtype not in _HALF:
+        raise TurboPiError("packed_attention: bf16 or fp16 q [tokens, heads, D] and k, v [tokens, heads, D]")
+    T, Hq, D = q.shape
+    Tk, Hk, _ = k.shape
+    _rows_of_heads("packed_attention", "q", q, T, Hq, D, q.dtype)
+    _rows_of_heads("packed_attention", "k", k, Tk, Hk, D, q.dtype)
+    _rows_of_heads("packed_attention", "v", v, Tk, Hk, D, q.dtype)
+    if out is None:
+        out = torch.empty((T, Hq, D), dtype=q.dtype, device=q.device)
+    else:
+        _rows_of_heads("packed_attention", "out", out, T, Hq, D, q.dtype)
+    for t in (cu, cu_keys):
+        if t is not None and (t.dtype != torch.int32 or t.dim() != 1 or t.numel() != cu.numel() or not t.is_contiguous()):
+            raise TurboPiError("packed_attention: cu and cu_keys must be contiguous int32 [sequences + 1]")
+    if cu.numel() < 1 or (cu_keys is None and Tk != T):
+        raise TurboPiError("packed_attention: keys of another number than the queries need cu_keys, cu an entry more than sequences")
+    _one_device("packed_attention", q, k, v, cu, out, cu_keys)
+    args = _lib.PackedAttentionArgs(q=_ptr(q), k=_ptr(k), v=_ptr(v), out=_ptr(out), q_stride=_strides(q), k_stride=_strides(k),
+                                    v_stride=_strides(v), o_stride=_strides(out), cu=_ptr(cu), cu_keys=_ptr(cu_keys),
+                                    seqs=cu.numel() - 1, q_tokens=T, k_tokens=Tk, q_heads=Hq, kv_heads=Hk, head_dim=D,
+                                    dtype=_HALF[q.dtype], scale=float(scale), causal=int(bool(causal)), flags=_flags.value)
+    _lib.check(_run(q, _lib.load().tpb200_packed_attention, args), "tpb200_packed_attention")
+    return out
+
+
 def paged_attention_workspace(q_heads, kv_heads, head_dim, device):
     """Scratch for `paged_attention`, whatever the number of sequences and their lengths; needs no initialisation.  Calls that
     may overlap need one each."""
