@@ -202,7 +202,8 @@ def test_what_the_table_must_not_hold_is_reported(cuda_device):
     n[1] = table.shape[1] * 16 + 1
     out = ops.paged_attention(q, k, v, table, n, 0.1)
     assert lib.tpb200_device_error(1) == 501
-    assert torch.equal(out[0], want[0])
+    # all lengths decide where the work is cut, and so the order of a sequence's sums: right within the bound, not bit by bit
+    _check(out[:1], q[:1], k, v, rows[:1], lens[:1], 0.1)
     n[1] = -3                                                    # no keys
     assert bool((ops.paged_attention(q, k, v, table, n, 0.1)[1] == 0).all())
     assert lib.tpb200_device_error(1) == 0
