@@ -221,7 +221,9 @@ _native = None
 
 # the entry points csrc/calls.cpp calls, in the order of its Entries
 _NATIVE_ENTRIES = ("tpb200_w4_gemm", "tpb200_w4a16_gemv", "tpb200_w4a16_gemm", "tpb200_attention", "quantizeActivationToFP8",
-                   "tpb200_last_error", "tpb200_nvfp4_tiled_a_bytes", "tpb200_nvfp4_quantize_act_tiled", "tpb200_nvfp4_gemm_ex")
+                   "tpb200_last_error", "tpb200_nvfp4_tiled_a_bytes", "tpb200_nvfp4_quantize_act_tiled", "tpb200_nvfp4_gemm_ex",
+                   "tpb200_packed_attention", "tpb200_paged_attention_workspace_size", "tpb200_paged_attention", "tpb200_paged_append",
+                   "tpb200_copy_pages")
 
 
 def calls_path():

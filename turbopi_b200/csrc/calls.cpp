@@ -24,6 +24,11 @@ struct Entries {
     decltype(&tpb200_nvfp4_tiled_a_bytes) tiled_a_bytes;
     decltype(&tpb200_nvfp4_quantize_act_tiled) quantize_act_tiled;
     decltype(&tpb200_nvfp4_gemm_ex) gemm_ex;
+    decltype(&tpb200_packed_attention) packed_attention;
+    decltype(&tpb200_paged_attention_workspace_size) paged_workspace;
+    decltype(&tpb200_paged_attention) paged_attention;
+    decltype(&tpb200_paged_append) paged_append;
+    decltype(&tpb200_copy_pages) copy_pages;
 } g;
 
 using OptTensor = std::optional<at::Tensor>;
@@ -251,6 +256,193 @@ py::object nvfp4_linear(const at::Tensor& x, const at::Tensor& w, int64_t N, dou
     return done(st, y);
 }
 
+// ------------------------------------------------------------------------------------------------ a cache of pages
+bool half(const at::Tensor& t) { return t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf; }
+
+// [tokens, heads, D] of one type and device with a contiguous last dimension
+bool rows(const at::Tensor& t, int dev, int64_t tokens, int64_t heads, int64_t D, at::ScalarType type) {
+    return on(t, dev) && t.dim() == 3 && t.size(0) == tokens && t.size(1) == heads && t.size(2) == D && t.scalar_type() == type && t.stride(2) == 1;
+}
+bool offsets(const at::Tensor& t, int dev, int64_t n) {
+    return on(t, dev) && t.dim() == 1 && t.numel() == n && t.scalar_type() == at::kInt && t.is_contiguous();
+}
+void strides(const at::Tensor& t, long long (&to)[2]) {
+    to[0] = t.stride(0);
+    to[1] = t.stride(1);
+}
+
+bool paged(const at::Tensor& k, const at::Tensor& v, const at::Tensor& table, const at::Tensor& lengths, int dev, tpb200_paged_cache& c) {
+    if (!on(k, dev) || !on(v, dev) || !on(table, dev) || !on(lengths, dev) || k.dim() != 4 || !half(k) || v.scalar_type() != k.scalar_type() ||
+        v.sizes() != k.sizes() || v.strides() != k.strides() || k.stride(3) != 1 || table.dim() != 2 || table.scalar_type() != at::kInt ||
+        lengths.dim() != 1 || lengths.scalar_type() != at::kInt || lengths.numel() != table.size(0) || !lengths.is_contiguous() ||
+        (table.size(1) > 1 && table.stride(1) != 1)) {
+        return false;
+    }
+    c.k_pages = k.data_ptr();
+    c.v_pages = v.data_ptr();
+    c.page_stride = k.stride(0);
+    c.row_stride = k.stride(1);
+    c.head_stride = k.stride(2);
+    c.num_pages = static_cast<int>(k.size(0));
+    c.page_size = static_cast<int>(k.size(1));
+    c.kv_heads = static_cast<int>(k.size(2));
+    c.head_dim = static_cast<int>(k.size(3));
+    c.dtype = code_of(k.scalar_type());
+    c.table = static_cast<const int*>(table.data_ptr());
+    c.table_stride = table.stride(0);
+    c.table_width = static_cast<int>(table.size(1));
+    c.lengths = static_cast<const int*>(lengths.data_ptr());
+    c.seqs = static_cast<int>(table.size(0));
+    return true;
+}
+
+// ops.paged_attention
+py::object paged_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& table, const at::Tensor& lengths,
+                           double scale, const OptTensor& out, const OptTensor& workspace, int flags) {
+    const int dev = here(q);
+    tpb200_paged_attention_args a = {};
+    if (dev < 0 || !paged(k, v, table, lengths, dev, a.cache) || q.dim() != 3 || a.cache.seqs < 1 || a.cache.kv_heads < 1) return py::none();
+    const int64_t H = q.size(1);
+    if (!rows(q, dev, a.cache.seqs, H, a.cache.head_dim, k.scalar_type()) || !on(workspace, dev) || H < 1 || H % a.cache.kv_heads != 0 ||
+        (out.has_value() && !rows(*out, dev, a.cache.seqs, H, a.cache.head_dim, k.scalar_type()))) {
+        return py::none();
+    }
+    at::Tensor ws;
+    if (workspace.has_value()) ws = *workspace;
+    else {
+        const size_t n = g.paged_workspace(static_cast<int>(H), a.cache.kv_heads, a.cache.head_dim);
+        if (n == 0) return py::none();
+        ws = at::empty({static_cast<int64_t>(n)}, q.options().dtype(at::kByte));
+    }
+    const at::Tensor y = out.has_value() ? *out : at::empty(q.sizes(), q.options());
+    a.q = q.data_ptr();
+    a.out = y.data_ptr();
+    strides(q, a.q_stride);
+    strides(y, a.o_stride);
+    a.q_heads = static_cast<int>(H);
+    a.scale = static_cast<float>(scale);
+    a.workspace = ws.data_ptr();
+    a.workspace_bytes = ws.nbytes();
+    a.flags = flags;
+    const tpb200_stream_t s = stream_of(dev);
+    return done(launch([&] { return g.paged_attention(&a, s); }), y);
+}
+
+// ops.paged_append; True where there are no queries to give back
+py::object paged_append(const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_pages, const at::Tensor& v_pages, const at::Tensor& table,
+                        const at::Tensor& cu, const at::Tensor& lengths, const OptTensor& q, const OptTensor& cos, const OptTensor& sin,
+                        const OptTensor& q_out, int flags) {
+    const int dev = here(k);
+    tpb200_paged_append_args a = {};
+    if (dev < 0 || !paged(k_pages, v_pages, table, lengths, dev, a.cache) || k.dim() != 3) return py::none();
+    const int64_t T = k.size(0), D = a.cache.head_dim;
+    const auto type = k_pages.scalar_type();
+    if (!rows(k, dev, T, a.cache.kv_heads, D, type) || !rows(v, dev, T, a.cache.kv_heads, D, type) || !offsets(cu, dev, a.cache.seqs + 1) ||
+        cos.has_value() != sin.has_value() || (q.has_value() && !cos.has_value()) || (!q.has_value() && q_out.has_value())) {
+        return py::none();
+    }
+    if (cos.has_value()) {
+        if (!on(*cos, dev) || !on(*sin, dev) || cos->dim() != 2 || cos->sizes() != sin->sizes() || cos->size(1) != D / 2 ||
+            cos->scalar_type() != sin->scalar_type() || code_of(cos->scalar_type()) < 0 || !cos->is_contiguous() || !sin->is_contiguous()) {
+            return py::none();
+        }
+        a.cos = cos->data_ptr();
+        a.sin = sin->data_ptr();
+        a.rope_dtype = code_of(cos->scalar_type());
+        a.rope_positions = static_cast<int>(cos->size(0));
+    }
+    at::Tensor y;
+    if (q.has_value()) {
+        if (q->dim() != 3 || !rows(*q, dev, T, q->size(1), D, type) || (q_out.has_value() && !rows(*q_out, dev, T, q->size(1), D, type))) {
+            return py::none();
+        }
+        y = q_out.has_value() ? *q_out : at::empty(q->sizes(), q->options());
+        a.q = q->data_ptr();
+        a.q_out = y.data_ptr();
+        a.q_heads = static_cast<int>(q->size(1));
+        strides(*q, a.q_stride);
+        strides(y, a.o_stride);
+    }
+    a.k = k.data_ptr();
+    a.v = v.data_ptr();
+    strides(k, a.k_stride);
+    strides(v, a.v_stride);
+    a.cu = static_cast<const int*>(cu.data_ptr());
+    a.tokens = static_cast<int>(T);
+    a.flags = flags;
+    const tpb200_stream_t s = stream_of(dev);
+    const int st = launch([&] { return g.paged_append(&a, s); });
+    if (st != 0) return py::int_(st);
+    return q.has_value() ? py::cast(y) : py::object(py::bool_(true));
+}
+
+// ops.packed_attention
+py::object packed_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& cu, double scale,
+                            const OptTensor& out, bool causal, const OptTensor& cu_keys, int flags) {
+    const int dev = here(q);
+    if (dev < 0 || q.dim() != 3 || k.dim() != 3 || !half(q)) return py::none();
+    const int64_t T = q.size(0), H = q.size(1), D = q.size(2), Tk = k.size(0), Hk = k.size(1);
+    const auto type = q.scalar_type();
+    if (!rows(q, dev, T, H, D, type) || !rows(k, dev, Tk, Hk, D, type) || !rows(v, dev, Tk, Hk, D, type) || cu.numel() < 1 ||
+        !offsets(cu, dev, cu.numel()) || (cu_keys.has_value() ? !offsets(*cu_keys, dev, cu.numel()) : Tk != T) ||
+        (out.has_value() && !rows(*out, dev, T, H, D, type))) {
+        return py::none();
+    }
+    const at::Tensor y = out.has_value() ? *out : at::empty({T, H, D}, q.options());
+    tpb200_packed_attention_args a = {};
+    a.q = q.data_ptr();
+    a.k = k.data_ptr();
+    a.v = v.data_ptr();
+    a.out = y.data_ptr();
+    strides(q, a.q_stride);
+    strides(k, a.k_stride);
+    strides(v, a.v_stride);
+    strides(y, a.o_stride);
+    a.cu = static_cast<const int*>(cu.data_ptr());
+    a.cu_keys = static_cast<const int*>(ptr(cu_keys));
+    a.seqs = static_cast<int>(cu.numel() - 1);
+    a.q_tokens = static_cast<int>(T);
+    a.k_tokens = static_cast<int>(Tk);
+    a.q_heads = static_cast<int>(H);
+    a.kv_heads = static_cast<int>(Hk);
+    a.head_dim = static_cast<int>(D);
+    a.dtype = code_of(type);
+    a.scale = static_cast<float>(scale);
+    a.causal = causal;
+    a.flags = flags;
+    const tpb200_stream_t s = stream_of(dev);
+    return done(launch([&] { return g.packed_attention(&a, s); }), y);
+}
+
+// ops.copy_pages on lists of ints; True when done
+py::object copy_pages(const at::Tensor& pages, const py::object& src, const py::object& dst, int flags) {
+    const int dev = here(pages);
+    if (dev < 0 || pages.dim() < 4 || !pages.is_contiguous() || pages.numel() == 0 || !PyList_CheckExact(src.ptr()) ||
+        !PyList_CheckExact(dst.ptr()) || PyList_GET_SIZE(src.ptr()) != PyList_GET_SIZE(dst.ptr()) || PyList_GET_SIZE(src.ptr()) > 0x7fffffff) {
+        return py::none();
+    }
+    const Py_ssize_t n = PyList_GET_SIZE(src.ptr());
+    std::vector<int> ids(2 * n);
+    for (int side = 0; side < 2; ++side) {
+        PyObject* list = side == 0 ? src.ptr() : dst.ptr();
+        for (Py_ssize_t i = 0; i < n; ++i) {
+            PyObject* x = PyList_GET_ITEM(list, i);
+            int overflow = 0;
+            const long id = PyLong_CheckExact(x) ? PyLong_AsLongAndOverflow(x, &overflow) : -1;
+            if (overflow != 0 || id < 0 || id > 0x7fffffff) return py::none();       // refused by the Python form
+            ids[side * n + i] = static_cast<int>(id);
+        }
+    }
+    const int64_t P = pages.size(-4), page_bytes = pages.stride(-4) * pages.element_size(), slab = page_bytes * P;
+    void* base = pages.data_ptr();
+    const tpb200_stream_t s = stream_of(dev);
+    const int st = launch([&] {
+        return g.copy_pages(base, slab, static_cast<int>(pages.nbytes() / slab), page_bytes, static_cast<int>(P), ids.data(), ids.data() + n,
+                            static_cast<int>(n), flags, s);
+    });
+    return st == 0 ? py::object(py::bool_(true)) : py::int_(st);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_calls, m) {
@@ -261,4 +453,8 @@ PYBIND11_MODULE(_calls, m) {
     m.def("attention", &attention);
     m.def("quantize_fp8", &quantize_fp8);
     m.def("nvfp4_linear", &nvfp4_linear);
+    m.def("packed_attention", &packed_attention);
+    m.def("paged_attention", &paged_attention);
+    m.def("paged_append", &paged_append);
+    m.def("copy_pages", &copy_pages);
 }

@@ -738,6 +738,9 @@ def packed_attention(q, k, v, cu, scale, out=None, causal=True, cu_keys=None):
     same for the keys where a sequence has more (or fewer) of them; causal then means that the last query sees every key:
     query i of n sees the keys up to i + (m - n) of m.  A query without keys gives zeros; tokens behind cu[S] are left alone.  The
     offsets are read on the device: a captured call follows them; ones outside the tensors are clamped."""
+    done = (_lib._native or _lib.native()).packed_attention(q, k, v, cu, scale, out, bool(causal), cu_keys, _flags.value)
+    if done is not None:
+        return _result(done, "tpb200_packed_attention")
     _cuda(q, k, v, cu, out, cu_keys)
     if q.dim() != 3 or k.dim() != 3 or q.dtype not in _HALF:
         raise TurboPiError("packed_attention: bf16 or fp16 q [tokens, heads, D] and k, v [tokens, heads, D]")
@@ -780,6 +783,9 @@ def paged_attention(q, k_pages, v_pages, table, lengths, scale, out=None, worksp
     int32 [S, W]: position j of sequence s is row j % page of page table[s, j // page]; lengths int32 [S], the new token among them.
     bf16 or fp16.  A sequence of length 0 gives zeros.  table and lengths are read on the device: a captured call follows
     them, and what they must not hold is reported by tpb200_device_error()."""
+    done = (_lib._native or _lib.native()).paged_attention(q, k_pages, v_pages, table, lengths, scale, out, workspace, _flags.value)
+    if done is not None:
+        return _result(done, "tpb200_paged_attention")
     view = _paged_view("paged_attention", k_pages, v_pages, table, lengths)
     _cuda(q, out, workspace)
     if q.dim() != 3:
@@ -810,6 +816,10 @@ def paged_append(k, v, k_pages, v_pages, table, cu, lengths, q=None, cos=None, s
     its last token goes to position lengths[s] - 1.  Tokens behind cu[S] are left alone, in q_out too.
     cos / sin [positions, D / 2] (fp32, fp16 or bf16): keys and queries are rotated (rotate-half, in fp32, rounded once); q_out
     may be q."""
+    done = (_lib._native or _lib.native()).paged_append(k, v, k_pages, v_pages, table, cu, lengths, q, cos, sin, q_out, _flags.value)
+    if done is not None:
+        done = _result(done, "tpb200_paged_append")
+        return None if q is None else done
     view = _paged_view("paged_append", k_pages, v_pages, table, lengths)
     _cuda(k, v, cu, q, cos, sin, q_out)
     D, H, dtype = view.head_dim, view.kv_heads, k_pages.dtype
@@ -849,6 +859,10 @@ def copy_pages(pages, src, dst):
     pages: contiguous [..., P, page, heads, D] of any type (PagedCache holds [layers, 2, P, page, heads, D]).  src / dst: sequences of
     ints or integer tensors on the CPU; an index outside the pool, a page written twice or a page both read and written is
     refused.  The lists are read before the call returns."""
+    done = (_lib._native or _lib.native()).copy_pages(pages, src, dst, _flags.value)
+    if done is not None:
+        _result(done, "tpb200_copy_pages")
+        return
     _cuda(pages)
     if pages.dim() < 4 or not pages.is_contiguous():
         raise TurboPiError("copy_pages: pages must be contiguous [..., pages, page, heads, D]")
