@@ -9,8 +9,9 @@
 // A row of a tile is a (token, head) pair: `pack` query heads of one key head, the largest power of two in the group, side by side,
 // so that short prompts fill tiles and the heads of a group read their keys once.
 //
-// Roles (384 threads, one CTA an SM): warp 0 requests tiles of K and V by TMA into a ring of units, warp 1 issues the products, two
-// groups of four warps do the softmax, a thread per row, with registers moved over to them from the others (setmaxnreg).
+// Roles (384 threads, one CTA an SM): warp 0 requests tiles of K and V by TMA into a ring of units, warp 1 issues the products, warps
+// 2 and 3 look tiles with masked pairs over, two groups of four warps do the softmax, a thread per row, with registers moved over to
+// them from the others (setmaxnreg).
 // The products are a line of events e; event e computes S into tensor-memory buffer e & 1, group e & 1 turns it into P in the same
 // columns, the product with V reads P from there:
 //   head sizes up to 128  two tiles of 128 rows per CTA, one per group: event e is key tile e / 2 of row tile e & 1; each unit of K
@@ -19,6 +20,9 @@
 //   above                 one row tile (its O alone is 256 columns), the groups take alternate key tiles and hand m on through
 //                         shared memory.
 // While one group works the other's products run.
+//
+// The exponentials are what is left to speed up once the products are fed: 16 a cycle on an SM, 1024 cycles for a tile of 128 x 128, as
+// many as its products take at head size 128.  A quarter of them is therefore computed on the FMA pipes (exp2_pair).
 //
 // What may stand in masked places does not matter: scores are selected, not biased.  Rows of V behind a sequence's end are zeroed in
 // shared memory, and in tiles that hold masked pairs V is searched for infinities and NaN (weight 0 times those would be NaN): they are
@@ -73,6 +77,7 @@ struct PackedControl {
     uint64_t full[8], empty[8];
     uint64_t s_ready[2], p_ready[2], o_done[2];
     uint64_t ref_ready[2][4];            // one row tile: the reference of event e, by quarter of the rows
+    uint64_t v_landed[kBadTiles];        // V of a tile with masked pairs, which is looked over before its units count as full
     uint32_t tmem_base;
     int failed;
     int seq, tile, q0, nq, k0, nk;       // the CTA's work
@@ -117,6 +122,23 @@ __device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t* r) {
         "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
 }
+__device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};\n" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+// Waits for the loads into r, which nothing may read before: the operands keep the compiler from moving a use up
+__device__ __forceinline__ void tmem_ld_wait_for(uint32_t* r) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                   "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                   "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+                 :
+                 : "memory");
+}
 __device__ __forceinline__ void tmem_st_done() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -140,6 +162,50 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     uint64_t r;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
+}
+
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {        // NaN stays NaN
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+// 2^x of a pair for x <= 8 without the special-function unit, after Cody and Waite: x = n + f with n the nearest integer (it falls out
+// of adding 1.5 * 2^23), |f| <= 1/2, 2^f by the polynomial of least relative error (Remez exchange), times 2^n assembled as a float.
+// Degree 3 is off by 7.5e-5 at most, a fiftieth of bf16's half step; degree 4, for fp16, by 2.7e-6.  x below -126 gives
+// 2^-126: such a weight is nothing beside the row's largest.
+template <typename T>
+__device__ __forceinline__ uint64_t exp2_pair(uint64_t x) {
+    float a, b;
+    unpair(x, a, b);
+    x = pair(max_nan(a, -126.0f), max_nan(b, -126.0f));
+    constexpr float kShift = 12582912.0f;
+    const uint64_t t = add2(x, pair(kShift, kShift)), n = add2(t, pair(-kShift, -kShift));
+    const uint64_t f = fma2(n, pair(-1.0f, -1.0f), x);
+    uint64_t p;
+    auto c = [](float v) { return pair(v, v); };
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        p = fma2(c(0.0551716685f), f, c(0.242611125f));
+        p = fma2(p, f, c(0.693260968f));
+        p = fma2(p, f, c(0.999928057f));
+    } else {
+        p = fma2(c(0.00957010221f), f, c(0.0559178591f));
+        p = fma2(p, f, c(0.240247443f));
+        p = fma2(p, f, c(0.693121791f));
+        p = fma2(p, f, c(0.999999285f));
+    }
+    unpair(t, a, b);
+    return mul2(p, pair(__uint_as_float((__float_as_uint(a) << 23) + 0x3f800000u), __uint_as_float((__float_as_uint(b) << 23) + 0x3f800000u)));
 }
 
 __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity) {
@@ -217,6 +283,7 @@ __global__ void __launch_bounds__(kThreadsPacked, 1) packed_attention_kernel(con
             mbar_init(&ctl->o_done[i], 1);
             for (int w = 0; w < 4; ++w) mbar_init(&ctl->ref_ready[i][w], 1);
         }
+        for (int i = 0; i < kBadTiles; ++i) mbar_init(&ctl->v_landed[i], L::kHalves);
         fence_mbar_init();
         ctl->failed = 0;
         ctl->bad_any = 0;
@@ -253,6 +320,7 @@ __global__ void __launch_bounds__(kThreadsPacked, 1) packed_attention_kernel(con
     }
     if (!L::kTwo) tiles[1] = 0;
     const int n_tiles = max(tiles[0], tiles[1]);
+    const int first_masked = row_limit(P, nq, nk, token0) / kTile;       // key tiles from here on hold masked pairs: kBadTiles at most
     const int events = L::kTwo ? 2 * n_tiles : n_tiles;
     // the order of the line of events: which are computed, and where the tiles of K and V stand in the ring
     auto active = [&](int e) { return L::kTwo ? (e >> 1) < tiles[e & 1] : true; };
@@ -276,24 +344,25 @@ __global__ void __launch_bounds__(kThreadsPacked, 1) packed_attention_kernel(con
                     }
                 }
                 int u = 0;
-                auto request = [&](const CUtensorMap* map, int j) {
+                auto request = [&](const CUtensorMap* map, int j, bool values = false) {
                     for (int h = 0; h < L::kHalves; ++h, ++u) {
                         const int slot = u % L::kUnits;
                         if (!mbar_wait_bounded(&ctl->empty[slot], ((u / L::kUnits) & 1) ^ 1, kWait)) return false;
-                        mbar_expect_tx(&ctl->full[slot], L::kUnitBytes);
+                        uint64_t* bar = values && j >= first_masked ? &ctl->v_landed[j - first_masked] : &ctl->full[slot];
+                        mbar_expect_tx(bar, L::kUnitBytes);
                         for (int b = 0; b < L::kUnitBlocks; ++b) {
                             tma_load_3d(ring + slot * L::kUnitBytes + b * kBlockBytes, map, (h * L::kUnitBlocks + b) * 64, kv_head,
-                                        k0 + j * kTile, &ctl->full[slot]);
+                                        k0 + j * kTile, bar);
                         }
                     }
                     return true;
                 };
                 if (L::kTwo) {
-                    for (int j = 0; j < n_tiles && ok; ++j) ok = request(&P.k, j) && request(&P.v, j);
+                    for (int j = 0; j < n_tiles && ok; ++j) ok = request(&P.k, j) && request(&P.v, j, true);
                 } else {
                     ok = request(&P.k, 0);
-                    for (int j = 1; j < n_tiles && ok; ++j) ok = request(&P.k, j) && (j < 1 || request(&P.v, j - 1));
-                    ok = ok && request(&P.v, n_tiles - 1);
+                    for (int j = 1; j < n_tiles && ok; ++j) ok = request(&P.k, j) && request(&P.v, j - 1, true);
+                    ok = ok && request(&P.v, n_tiles - 1, true);
                 }
                 if (!ok) {
                     record_error(kErrPackedBarrierTimeout);
@@ -365,6 +434,59 @@ __global__ void __launch_bounds__(kThreadsPacked, 1) packed_attention_kernel(con
                 record_error(kErrPackedBarrierTimeout);
                 ctl->failed = 1;
             }
+        } else if (warp >= 2) {
+            // -------------------------------------------------------- V of tiles with masked pairs
+            // Rows behind the sequence's end to zero, infinities and NaN out of the product.  x * 0 summed up is NaN if there is one.
+            for (int j = first_masked; j < n_tiles; ++j) {
+                const int u0 = v_unit(j);
+                bool ok = wait_warp(&ctl->v_landed[j - first_masked], 0);
+                for (int r = (warp - 2) * 32 + lane; r < kTile && ok; r += 64) {
+                    const bool there = j * kTile + r < nk;
+                    bool bad = false;
+                    for (int h = 0; h < L::kHalves; ++h) {
+                        for (int b = 0; b < L::kUnitBlocks; ++b) {
+                            uint4* at = reinterpret_cast<uint4*>(ring + (u0 + h) % L::kUnits * L::kUnitBytes + b * kBlockBytes + r * 128);
+                            uint4 v[8];
+                            uint32_t sum = 0;
+#pragma unroll
+                            for (int c = 0; c < 8; ++c) v[c] = at[c ^ (r & 7)];
+#pragma unroll
+                            for (int c = 0; c < 8; ++c) {
+                                sum = Half16<T>::add_zeros(v[c].x, sum);
+                                sum = Half16<T>::add_zeros(v[c].y, sum);
+                                sum = Half16<T>::add_zeros(v[c].z, sum);
+                                sum = Half16<T>::add_zeros(v[c].w, sum);
+                            }
+                            if (!there) {
+#pragma unroll
+                                for (int c = 0; c < 8; ++c) at[c] = make_uint4(0, 0, 0, 0);
+                            } else if ((sum & 0x7fff7fffu) != 0) {
+                                bad = true;
+                                uint16_t* x = reinterpret_cast<uint16_t*>(at);
+                                constexpr uint16_t kExp = std::is_same<T, __nv_bfloat16>::value ? 0x7f80 : 0x7c00;
+                                for (int i = 0; i < 64; ++i) {
+                                    if ((x[i] & kExp) == kExp) x[i] = 0;
+                                }
+                            }
+                        }
+                    }
+                    const uint32_t word = __ballot_sync(0xffffffffu, bad);
+                    if (lane == 0 && word != 0) {
+                        ctl->bad[j - first_masked][r >> 5] = word;
+                        ctl->bad_any = 1;
+                    }
+                }
+                fence_proxy_async_smem();
+                asm volatile("bar.sync 2, 64;" ::: "memory");
+                if (!ok) {               // the units stay empty: the products' wait runs out too
+                    if (lane == 0) {
+                        record_error(kErrPackedBarrierTimeout);
+                        ctl->failed = 1;
+                    }
+                    break;
+                }
+                if (warp == 2 && lane < L::kHalves) mbar_arrive(&ctl->full[(u0 + lane) % L::kUnits]);
+            }
         }
     } else {
         // ------------------------------------------------------------ softmax: group x, thread = row of a tile
@@ -377,7 +499,6 @@ __global__ void __launch_bounds__(kThreadsPacked, 1) packed_attention_kernel(con
         const int token = token0 + my_tile * tokens_tile + (row >> P.pack_shift);
         const int limit = row_limit(P, nq, nk, token);
         const int lowest = row_limit(P, nq, nk, token0 + my_tile * tokens_tile);     // of the tile's rows that exist
-        const int first_masked = row_limit(P, nq, nk, token0) / kTile;               // of the CTA: where `bad` begins
         float ref = -INFINITY, l = 0.0f;
         float l_ref = -INFINITY;         // the reference that l is relative to (one row tile: the groups share ref)
         bool ok = true;
@@ -386,23 +507,23 @@ __global__ void __launch_bounds__(kThreadsPacked, 1) packed_attention_kernel(con
             const int j = key_tile(e);
             if (!wait_warp(&ctl->s_ready[x], (e >> 1) & 1)) { ok = false; break; }
             tc::fence_after_thread_sync();
-            uint32_t s[kTile];
-#pragma unroll
-            for (int c = 0; c < kTile / 32; ++c) tc::tmem_ld_32x32b_x32(s_at + c * 32, *reinterpret_cast<uint32_t(*)[32]>(s + c * 32));
-            tc::tmem_ld_wait();
             const bool masked = (j + 1) * kTile > lowest;
-            if (masked) {
-                const int lim = limit - j * kTile;
+            const int lim = limit - j * kTile;
+            uint32_t s[kTile];
+            float top[2] = {-INFINITY, -INFINITY};
+            tc::tmem_ld_32x32b_x32(s_at, *reinterpret_cast<uint32_t(*)[32]>(s));
 #pragma unroll
-                for (int i = 0; i < kTile; ++i) s[i] = i < lim ? s[i] : 0xff800000u;
+            for (int c = 0; c < kTile; c += 32) {        // the next 32 columns on their way while the maximum of these is taken
+                tmem_ld_wait_for(s + c);
+                if (c + 32 < kTile) tc::tmem_ld_32x32b_x32(s_at + c + 32, *reinterpret_cast<uint32_t(*)[32]>(s + (c + 32) % kTile));
+                if (masked) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) s[c + i] = c + i < lim ? s[c + i] : 0xff800000u;
+                }
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) top[(i >> 1) & 1] = max3(top[(i >> 1) & 1], __uint_as_float(s[c + i]), __uint_as_float(s[c + i + 1]));
             }
-            float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-            for (int i = 0; i < kTile; i += 4) {
-#pragma unroll
-                for (int c = 0; c < 4; ++c) top[c] = fmaxf(top[c], __uint_as_float(s[i + c]));
-            }
-            const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * P.scale2;
+            const float high = fmaxf(top[0], top[1]) * P.scale2;
             if (!L::kTwo && e > 0) {     // the reference after the event before, from the other group
                 if (!wait_warp(&ctl->ref_ready[x ^ 1][quarter], ((e - 1) >> 1) & 1)) { ok = false; break; }
                 ref = ctl->ref[row];
@@ -438,62 +559,35 @@ __global__ void __launch_bounds__(kThreadsPacked, 1) packed_attention_kernel(con
             // P = 2^(scale2 S - m), its row sum, rounded pairs into the columns S was in
             const uint64_t scale = pair(P.scale2, P.scale2), minus = pair(-base, -base);
             uint64_t sum[2] = {pair(0.0f, 0.0f), pair(0.0f, 0.0f)};
-            uint32_t p[kTile / 2];
+            auto weights = [&](auto poly) {
 #pragma unroll
-            for (int i = 0; i < kTile / 2; ++i) {
-                float a, b;
-                unpair(fma2(pair(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), scale, minus), a, b);
-                a = ex2(a);
-                b = ex2(b);
-                sum[i & 1] = add2(sum[i & 1], pair(a, b));
-                p[i] = Half16<T>::pack(a, b);
-            }
-            tmem_st_x32(s_at, p);
-            tmem_st_x32(s_at + 32, p + 32);
+                for (int c = 0; c < kTile / 2; c += 16) {
+                    uint32_t p[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        uint64_t w = fma2(pair(__uint_as_float(s[2 * (c + i)]), __uint_as_float(s[2 * (c + i) + 1])), scale, minus);
+                        float a, b;
+                        if (decltype(poly)::value && i % 4 == 3) {
+                            w = exp2_pair<T>(w);
+                            unpair(w, a, b);
+                        } else {
+                            unpair(w, a, b);
+                            a = ex2(a);
+                            b = ex2(b);
+                            w = pair(a, b);
+                        }
+                        sum[i & 1] = add2(sum[i & 1], w);
+                        p[i] = Half16<T>::pack(a, b);
+                    }
+                    tmem_st_x16(s_at + c, p);
+                }
+            };
+            // masked scores are -inf and have to become zeros; with one row tile the products take twice the exponentials' time
+            if (masked || !L::kTwo) weights(std::false_type{});
+            else weights(std::true_type{});
             float a, b;
             unpair(add2(sum[0], sum[1]), a, b);
             l += a + b;
-            // V of a tile with masked pairs: rows behind the sequence's end to zero, infinities and NaN out of the product
-            if (masked && (!L::kTwo || x == 0 || j >= tiles[0])) {
-                const int u0 = v_unit(j);
-                const bool there = j * kTile + row < nk;
-                bool bad = false;
-                for (int h = 0; h < L::kHalves && ok; ++h) {
-                    const int slot = (u0 + h) % L::kUnits;
-                    if (!wait_warp(&ctl->full[slot], ((u0 + h) / L::kUnits) & 1)) { ok = false; break; }
-                    for (int b2 = 0; b2 < L::kUnitBlocks; ++b2) {
-                        uint4* at = reinterpret_cast<uint4*>(ring + slot * L::kUnitBytes + b2 * kBlockBytes + row * 128);
-                        if (!there) {
-#pragma unroll
-                            for (int c = 0; c < 8; ++c) at[c] = make_uint4(0, 0, 0, 0);
-                            continue;
-                        }
-#pragma unroll
-                        for (int c = 0; c < 8; ++c) {
-                            uint4 v = at[c ^ (row & 7)];
-                            uint32_t* w = reinterpret_cast<uint32_t*>(&v);
-                            bool here = false;
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                constexpr uint32_t kExp = std::is_same<T, __nv_bfloat16>::value ? 0x7f80u : 0x7c00u;
-                                if ((w[i] & kExp) == kExp) { w[i] &= 0xffff0000u; here = true; }
-                                if ((w[i] & (kExp << 16)) == (kExp << 16)) { w[i] &= 0xffffu; here = true; }
-                            }
-                            if (here) {
-                                at[c ^ (row & 7)] = v;
-                                bad = true;
-                            }
-                        }
-                    }
-                }
-                if (!ok) break;
-                const uint32_t word = __ballot_sync(0xffffffffu, bad);
-                if (lane == 0 && word != 0) {
-                    ctl->bad[min(j - first_masked, kBadTiles - 1)][quarter] = word;
-                    ctl->bad_any = 1;
-                }
-                fence_proxy_async_smem();
-            }
             tmem_st_done();
             tc::fence_before_thread_sync();
             __syncwarp();
@@ -519,18 +613,18 @@ __global__ void __launch_bounds__(kThreadsPacked, 1) packed_attention_kernel(con
         }
         if (ok && (L::kTwo || x == 0 || DP > 128)) {
             const float inv = mine > 0 ? 1.0f / l : 0.0f;
-            const int head = (head_group << P.pack_shift) + (row & (P.pack - 1));
-            uint16_t* to = P.out + static_cast<long long>(q0 + token) * P.o_stride[0] + head * P.o_stride[1];
-            const int c_lo = L::kTwo ? 0 : x * (DP / 2), c_hi = L::kTwo ? DP : c_lo + DP / 2;
+            // through shared memory where Q was (its products are done), each warp its own rows, so that whole rows leave together
+            constexpr int kCols = L::kTwo ? DP : DP / 2, kChunks = kCols / 8, kRowsIter = 32 / kChunks;
+            const int c_lo = L::kTwo ? 0 : x * kCols;
+            uint8_t* stage = sQ + (x * 4 + quarter) * 32 * kCols * 2;
             const bool any_bad = mine > 0 && ctl->bad_any != 0;
-            for (int c = c_lo; c < c_hi; c += 32) {
+            for (int c = 0; c < kCols; c += 32) {
                 uint32_t o[32];
                 if (mine > 0) {
-                    tc::tmem_ld_32x32b_x32(o_at + c, o);
+                    tc::tmem_ld_32x32b_x32(o_at + c_lo + c, o);
                     tc::tmem_ld_wait();
                 }
-                if (token >= nq) continue;
-                if (any_bad) {           // what was taken out of V, for the rows that see it
+                if (any_bad && token < nq) {             // what was taken out of V, for the rows that see it
                     for (int i = 0; i < kBadTiles * kTile; ++i) {
                         const int key = (first_masked + i / kTile) * kTile + i % kTile;
                         if (!((ctl->bad[i >> 7][(i >> 5) & 3] >> (i & 31)) & 1) || key >= limit) continue;
@@ -538,8 +632,8 @@ __global__ void __launch_bounds__(kThreadsPacked, 1) packed_attention_kernel(con
                                                head_group / P.groups_per_kv * P.v_stride[1];
 #pragma unroll
                         for (int n = 0; n < 32; ++n) {
-                            if (c + n >= P.head_dim) continue;
-                            const uint32_t w = from[c + n];
+                            if (c_lo + c + n >= P.head_dim) continue;
+                            const uint32_t w = from[c_lo + c + n];
                             const float v = Half16<T>::unpack(w).x;
                             if (!(fabsf(v) < INFINITY)) o[n] = __float_as_uint(__uint_as_float(o[n]) + v);
                         }
@@ -547,7 +641,6 @@ __global__ void __launch_bounds__(kThreadsPacked, 1) packed_attention_kernel(con
                 }
 #pragma unroll
                 for (int n = 0; n < 32; n += 8) {
-                    if (c + n >= P.head_dim) continue;
                     uint32_t w[4] = {0, 0, 0, 0};
                     if (limit > 0) {
 #pragma unroll
@@ -555,8 +648,18 @@ __global__ void __launch_bounds__(kThreadsPacked, 1) packed_attention_kernel(con
                             w[i] = Half16<T>::pack(__uint_as_float(o[n + 2 * i]) * inv, __uint_as_float(o[n + 2 * i + 1]) * inv);
                         }
                     }
-                    *reinterpret_cast<uint4*>(to + c + n) = make_uint4(w[0], w[1], w[2], w[3]);
+                    *reinterpret_cast<uint4*>(stage + lane * (kCols * 2) + ((((c + n) >> 3) ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
                 }
+            }
+            __syncwarp();
+            const int chunk = lane % kChunks;
+#pragma unroll
+            for (int r0 = 0; r0 < 32; r0 += kRowsIter) {
+                const int r = r0 + lane / kChunks, t = token0 + my_tile * tokens_tile + ((quarter * 32 + r) >> P.pack_shift);
+                if (t >= nq || c_lo + chunk * 8 >= P.head_dim) continue;
+                const int head = (head_group << P.pack_shift) + ((quarter * 32 + r) & (P.pack - 1));
+                const uint4 v = *reinterpret_cast<const uint4*>(stage + r * (kCols * 2) + ((chunk ^ (r & 7)) << 4));
+                *reinterpret_cast<uint4*>(P.out + static_cast<long long>(q0 + t) * P.o_stride[0] + head * P.o_stride[1] + c_lo + chunk * 8) = v;
             }
         }
         tc::fence_before_thread_sync();

@@ -17,12 +17,23 @@ struct Half16<__nv_bfloat16> {
         const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
         return *reinterpret_cast<const uint32_t*>(&h);
     }
+    // x * 0 + sum: NaN from the first infinity or NaN on
+    static __device__ __forceinline__ uint32_t add_zeros(uint32_t x, uint32_t sum) {
+        const __nv_bfloat162 h = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&x), __nv_bfloat162(__float2bfloat16_rn(0.0f), __float2bfloat16_rn(0.0f)),
+                                         *reinterpret_cast<const __nv_bfloat162*>(&sum));
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
 };
 template <>
 struct Half16<__half> {
     static __device__ __forceinline__ float2 unpack(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
     static __device__ __forceinline__ uint32_t pack(float a, float b) {
         const __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    static __device__ __forceinline__ uint32_t add_zeros(uint32_t x, uint32_t sum) {
+        const __half2 h = __hfma2(*reinterpret_cast<const __half2*>(&x), __half2(__float2half_rn(0.0f), __float2half_rn(0.0f)),
+                                  *reinterpret_cast<const __half2*>(&sum));
         return *reinterpret_cast<const uint32_t*>(&h);
     }
 };
