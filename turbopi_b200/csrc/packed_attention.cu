@@ -75,7 +75,7 @@ struct Layout {
 struct PackedControl {
     uint64_t q_full;
     uint64_t full[8], empty[8];
-    uint64_t s_ready[2], p_ready[2], o_done[2];
+    uint64_t s_ready[2], p_ready[2][2], o_done[2];       // p_ready: by half of the tile's keys
     uint64_t ref_ready[2][4];            // one row tile: the reference of event e, by quarter of the rows
     uint64_t v_landed[kBadTiles];        // V of a tile with masked pairs, which is looked over before its units count as full
     uint32_t tmem_base;
@@ -279,7 +279,7 @@ __global__ void __launch_bounds__(kThreadsPacked, 1) packed_attention_kernel(con
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&ctl->s_ready[i], 1);
-            mbar_init(&ctl->p_ready[i], 4);
+            for (int h = 0; h < 2; ++h) mbar_init(&ctl->p_ready[i][h], 4);
             mbar_init(&ctl->o_done[i], 1);
             for (int w = 0; w < 4; ++w) mbar_init(&ctl->ref_ready[i][w], 1);
         }
@@ -401,25 +401,30 @@ __global__ void __launch_bounds__(kThreadsPacked, 1) packed_attention_kernel(con
                 }
                 return true;
             };
+            // the first half of the keys' weights is multiplied while the second is computed
             auto values = [&](int e) {
-                if (!wait_warp(&ctl->p_ready[e & 1], (e >> 1) & 1)) return false;
                 const int j = key_tile(e), u0 = v_unit(j);
 #pragma unroll
-                for (int h = 0; h < L::kHalves; ++h) {
-                    const int slot = (u0 + h) % L::kUnits;
-                    if (!wait_warp(&ctl->full[slot], ((u0 + h) / L::kUnits) & 1)) return false;
-                    tc::fence_after_thread_sync();
-                    if (tc::elect_one()) {
-                        const uint32_t va = r16 + (slot * L::kUnitBytes >> 4);
-                        const uint32_t d = tm + kColO + (L::kTwo ? (e & 1) * DP : h * 128);
-                        for (int kk = 0; kk < kTile / 16; ++kk) {
-                            mma_ts(d, tm + (e & 1) * kTile + kk * 8, tc::desc_from_words((va + (kk * 2048 >> 4)) | kLboField, kDescHiMnSw128),
-                                   P.idesc_o, (j | kk) > 0 ? 1u : 0u);
+                for (int part = 0; part < 2; ++part) {
+                    if (!wait_warp(&ctl->p_ready[e & 1][part], (e >> 1) & 1)) return false;
+#pragma unroll
+                    for (int h = 0; h < L::kHalves; ++h) {
+                        const int slot = (u0 + h) % L::kUnits;
+                        if (part == 0 && !wait_warp(&ctl->full[slot], ((u0 + h) / L::kUnits) & 1)) return false;
+                        tc::fence_after_thread_sync();
+                        if (tc::elect_one()) {
+                            const uint32_t va = r16 + (slot * L::kUnitBytes >> 4);
+                            const uint32_t d = tm + kColO + (L::kTwo ? (e & 1) * DP : h * 128);
+#pragma unroll
+                            for (int kk = part * 4; kk < part * 4 + 4; ++kk) {
+                                mma_ts(d, tm + (e & 1) * kTile + kk * 8, tc::desc_from_words((va + (kk * 2048 >> 4)) | kLboField, kDescHiMnSw128),
+                                       P.idesc_o, (j | kk) > 0 ? 1u : 0u);
+                            }
+                            if (part == 1 && last_use(e)) tc::commit(&ctl->empty[slot]);
+                            if (part == 1 && h == L::kHalves - 1) tc::commit(&ctl->o_done[e & 1]);
                         }
-                        if (last_use(e)) tc::commit(&ctl->empty[slot]);
-                        if (h == L::kHalves - 1) tc::commit(&ctl->o_done[e & 1]);
+                        __syncwarp();
                     }
-                    __syncwarp();
                 }
                 return true;
             };
@@ -510,20 +515,18 @@ __global__ void __launch_bounds__(kThreadsPacked, 1) packed_attention_kernel(con
             const bool masked = (j + 1) * kTile > lowest;
             const int lim = limit - j * kTile;
             uint32_t s[kTile];
-            float top[2] = {-INFINITY, -INFINITY};
-            tc::tmem_ld_32x32b_x32(s_at, *reinterpret_cast<uint32_t(*)[32]>(s));
+            float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int c = 0; c < kTile; c += 32) {        // the next 32 columns on their way while the maximum of these is taken
-                tmem_ld_wait_for(s + c);
-                if (c + 32 < kTile) tc::tmem_ld_32x32b_x32(s_at + c + 32, *reinterpret_cast<uint32_t(*)[32]>(s + (c + 32) % kTile));
-                if (masked) {
+            for (int c = 0; c < kTile; c += 32) tc::tmem_ld_32x32b_x32(s_at + c, *reinterpret_cast<uint32_t(*)[32]>(s + c));
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) s[c + i] = c + i < lim ? s[c + i] : 0xff800000u;
-                }
+            for (int c = 0; c < kTile; c += 32) tmem_ld_wait_for(s + c);
+            if (masked) {
 #pragma unroll
-                for (int i = 0; i < 32; i += 2) top[(i >> 1) & 1] = max3(top[(i >> 1) & 1], __uint_as_float(s[c + i]), __uint_as_float(s[c + i + 1]));
+                for (int i = 0; i < kTile; ++i) s[i] = i < lim ? s[i] : 0xff800000u;
             }
-            const float high = fmaxf(top[0], top[1]) * P.scale2;
+#pragma unroll
+            for (int i = 0; i < kTile; i += 2) top[(i >> 1) & 3] = max3(top[(i >> 1) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+            const float high = max3(fmaxf(top[0], top[1]), top[2], top[3]) * P.scale2;
             if (!L::kTwo && e > 0) {     // the reference after the event before, from the other group
                 if (!wait_warp(&ctl->ref_ready[x ^ 1][quarter], ((e - 1) >> 1) & 1)) { ok = false; break; }
                 ref = ctl->ref[row];
@@ -561,10 +564,10 @@ __global__ void __launch_bounds__(kThreadsPacked, 1) packed_attention_kernel(con
             uint64_t sum[2] = {pair(0.0f, 0.0f), pair(0.0f, 0.0f)};
             auto weights = [&](auto poly) {
 #pragma unroll
-                for (int c = 0; c < kTile / 2; c += 16) {
-                    uint32_t p[16];
+                for (int c = 0; c < kTile / 2; c += 32) {
+                    uint32_t p[32];
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
+                    for (int i = 0; i < 32; ++i) {
                         uint64_t w = fma2(pair(__uint_as_float(s[2 * (c + i)]), __uint_as_float(s[2 * (c + i) + 1])), scale, minus);
                         float a, b;
                         if (decltype(poly)::value && i % 4 == 3) {
@@ -579,7 +582,11 @@ __global__ void __launch_bounds__(kThreadsPacked, 1) packed_attention_kernel(con
                         sum[i & 1] = add2(sum[i & 1], w);
                         p[i] = Half16<T>::pack(a, b);
                     }
-                    tmem_st_x16(s_at + c, p);
+                    tmem_st_x32(s_at + c, p);
+                    tmem_st_done();
+                    tc::fence_before_thread_sync();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&ctl->p_ready[x][c / 32]);
                 }
             };
             // masked scores are -inf and have to become zeros; with one row tile the products take twice the exponentials' time
@@ -588,10 +595,6 @@ __global__ void __launch_bounds__(kThreadsPacked, 1) packed_attention_kernel(con
             float a, b;
             unpair(add2(sum[0], sum[1]), a, b);
             l += a + b;
-            tmem_st_done();
-            tc::fence_before_thread_sync();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&ctl->p_ready[x]);
         }
         // ------------------------------------------------------------ O / l -> the rows
         if (!L::kTwo) {
