@@ -122,13 +122,6 @@ __device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t* r) {
         "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
 }
-__device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t* r) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};\n" ::"r"(taddr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-        : "memory");
-}
 // Waits for the loads into r, which nothing may read before: the operands keep the compiler from moving a use up
 __device__ __forceinline__ void tmem_ld_wait_for(uint32_t* r) {
     asm volatile("tcgen05.wait::ld.sync.aligned;"
@@ -325,7 +318,6 @@ __global__ void __launch_bounds__(kThreadsPacked, 1) packed_attention_kernel(con
     // the order of the line of events: which are computed, and where the tiles of K and V stand in the ring
     auto active = [&](int e) { return L::kTwo ? (e >> 1) < tiles[e & 1] : true; };
     auto key_tile = [&](int e) { return L::kTwo ? e >> 1 : e; };
-    auto last_use = [&](int e) { return !L::kTwo || (e & 1) == 1 || tiles[1] == 0; };
     auto k_unit = [&](int j) { return L::kHalves * (L::kTwo ? 2 * j : (j < 2 ? j : 2 * j - 1)); };
     auto v_unit = [&](int j) { return L::kHalves * (L::kTwo ? 2 * j + 1 : (j == n_tiles - 1 ? 2 * j + 1 : 2 * j + 2)); };
 
@@ -374,66 +366,127 @@ __global__ void __launch_bounds__(kThreadsPacked, 1) packed_attention_kernel(con
             // -------------------------------------------------------- products
             const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
             const uint32_t q16 = (smem_u32(sQ) & 0x3FFFFu) >> 4, r16 = (smem_u32(ring) & 0x3FFFFu) >> 4;
-            const int ksteps = (P.head_dim + 15) >> 4;
             constexpr uint32_t kDescHiMnSw128 = (1024u >> 4) | (1u << 14) | (static_cast<uint32_t>(tc::kSwizzle128B) << 29);
             constexpr uint32_t kLboField = (static_cast<uint32_t>(kBlockBytes) >> 4) << 16;
-            bool ok = wait_warp(&ctl->q_full, 0);
-            auto scores = [&](int e) {
-                const int u0 = k_unit(key_tile(e));
-                const uint32_t qa = q16 + (L::kTwo ? (e & 1) * (L::kBlocks * kBlockBytes >> 4) : 0);
-#pragma unroll
-                for (int h = 0; h < L::kHalves; ++h) {
-                    const int slot = (u0 + h) % L::kUnits;
-                    if (!wait_warp(&ctl->full[slot], ((u0 + h) / L::kUnits) & 1)) return false;
-                    tc::fence_after_thread_sync();
-                    if (tc::elect_one()) {
-                        const uint32_t ka = r16 + (slot * L::kUnitBytes >> 4);
-                        const int steps = min(ksteps - h * L::kUnitBlocks * 4, L::kUnitBlocks * 4);
-                        for (int kk = 0; kk < steps; ++kk) {
-                            const uint32_t off = static_cast<uint32_t>((kk >> 2) * kBlockBytes + (kk & 3) * 32) >> 4;
-                            mma_ss(tm + (e & 1) * kTile, tc::desc_from_words(qa + h * (L::kUnitBytes >> 4) + off, tc::kDescHiKmajorSw128),
-                                   tc::desc_from_words(ka + off, tc::kDescHiKmajorSw128), P.idesc_s, (h | kk) > 0 ? 1u : 0u);
-                        }
-                        if (last_use(e)) tc::commit(&ctl->empty[slot]);
-                        if (h == L::kHalves - 1) tc::commit(&ctl->s_ready[e & 1]);
-                    }
-                    __syncwarp();
-                }
-                return true;
+            // Issuing a product takes about as long as it runs (64 cycles for N = 128), so what the warp does between them is
+            // lost: barriers are tested before products are issued and the outcome looked at behind them, and the second product of head
+            // sizes above 128 has N = 256.
+            auto test = [&](uint64_t* bar, uint32_t parity) { return mbar_test_wait(bar, parity); };
+            auto seen = [&](bool early, uint64_t* bar, uint32_t parity) {
+                const bool ok = __all_sync(0xffffffffu, early) || wait_warp(bar, parity);
+                tc::fence_after_thread_sync();
+                return ok;
             };
-            // the first half of the keys' weights is multiplied while the second is computed
-            auto values = [&](int e) {
-                const int j = key_tile(e), u0 = v_unit(j);
+            auto unit_full = [&](int u) { return &ctl->full[u % L::kUnits]; };
+            auto unit_parity = [&](int u) -> uint32_t { return (u / L::kUnits) & 1; };
+            // scores of one unit of K (past head_dim both operands are zero), row tile x, into buffer x
+            auto scores = [&](int x, int u, int h) {
+                const uint32_t qa = q16 + ((L::kTwo ? x * L::kBlocks * kBlockBytes : h * L::kUnitBytes) >> 4), ka = r16 + (u % L::kUnits * L::kUnitBytes >> 4);
 #pragma unroll
-                for (int part = 0; part < 2; ++part) {
-                    if (!wait_warp(&ctl->p_ready[e & 1][part], (e >> 1) & 1)) return false;
+                for (int kk = 0; kk < L::kUnitBlocks * 4; ++kk) {
+                    const uint32_t off = static_cast<uint32_t>((kk >> 2) * kBlockBytes + (kk & 3) * 32) >> 4;
+                    mma_ss(tm + x * kTile, tc::desc_from_words(qa + off, tc::kDescHiKmajorSw128), tc::desc_from_words(ka + off, tc::kDescHiKmajorSw128),
+                           P.idesc_s, (h | kk) > 0 ? 1u : 0u);
+                }
+            };
+            // the product of half of a tile's keys, weights in buffer x; a tile's units lie one behind the other
+            auto values = [&](int x, int u, int part, uint32_t more) {
+                const uint32_t va = r16 + (u % L::kUnits * L::kUnitBytes >> 4), d = tm + kColO + (L::kTwo ? x * DP : 0);
 #pragma unroll
-                    for (int h = 0; h < L::kHalves; ++h) {
-                        const int slot = (u0 + h) % L::kUnits;
-                        if (part == 0 && !wait_warp(&ctl->full[slot], ((u0 + h) / L::kUnits) & 1)) return false;
-                        tc::fence_after_thread_sync();
-                        if (tc::elect_one()) {
-                            const uint32_t va = r16 + (slot * L::kUnitBytes >> 4);
-                            const uint32_t d = tm + kColO + (L::kTwo ? (e & 1) * DP : h * 128);
+                for (int kk = part * 4; kk < part * 4 + 4; ++kk) {
+                    mma_ts(d, tm + x * kTile + kk * 8, tc::desc_from_words((va + (kk * 2048 >> 4)) | kLboField, kDescHiMnSw128), P.idesc_o,
+                           kk > 0 ? 1u : more);
+                }
+            };
+            bool ok = wait_warp(&ctl->q_full, 0);
+            if constexpr (L::kTwo) {
+                const int t0 = __shfl_sync(0xffffffffu, tiles[0], 0), t1 = __shfl_sync(0xffffffffu, tiles[1], 0), n = max(t0, t1);
+                ok = ok && wait_warp(unit_full(0), 0);
+                tc::fence_after_thread_sync();
+                if (ok && tc::elect_one()) {
+                    if (t0 > 0) {
+                        scores(0, 0, 0);
+                        tc::commit(&ctl->s_ready[0]);
+                    }
+                    if (t1 > 0) {
+                        scores(1, 0, 0);
+                        tc::commit(&ctl->s_ready[1]);
+                    }
+                    tc::commit(&ctl->empty[0]);
+                }
+                __syncwarp();
+                bool p0 = false;
+                for (int j = 0; j < n && ok; ++j) {
+                    const int v = 2 * j + 1, k = 2 * j + 2;
 #pragma unroll
-                            for (int kk = part * 4; kk < part * 4 + 4; ++kk) {
-                                mma_ts(d, tm + (e & 1) * kTile + kk * 8, tc::desc_from_words((va + (kk * 2048 >> 4)) | kLboField, kDescHiMnSw128),
-                                       P.idesc_o, (j | kk) > 0 ? 1u : 0u);
-                            }
-                            if (part == 1 && last_use(e)) tc::commit(&ctl->empty[slot]);
-                            if (part == 1 && h == L::kHalves - 1) tc::commit(&ctl->o_done[e & 1]);
+                    for (int x = 0; x < 2; ++x) {
+                        const int t = x == 0 ? t0 : t1;
+                        const bool last_use = x == 1 || t1 == 0;
+                        if (j >= t || !ok) continue;
+                        ok = seen(p0, &ctl->p_ready[x][0], j & 1) && seen(test(unit_full(v), unit_parity(v)), unit_full(v), unit_parity(v));
+                        const bool p1 = test(&ctl->p_ready[x][1], j & 1);
+                        if (ok && tc::elect_one()) values(x, v, 0, j > 0 ? 1u : 0u);
+                        __syncwarp();
+                        ok = ok && seen(p1, &ctl->p_ready[x][1], j & 1);
+                        const bool next = j + 1 < t, kf = next && test(unit_full(k), unit_parity(k));
+                        if (ok && tc::elect_one()) {
+                            values(x, v, 1, 1);
+                            if (last_use) tc::commit(&ctl->empty[v % L::kUnits]);
+                            if (!next) tc::commit(&ctl->o_done[x]);
+                        }
+                        __syncwarp();
+                        // of the event that comes next: the other row tile's where it has one
+                        const bool other = x == 0 ? j < t1 : j + 1 < t0;
+                        p0 = test(&ctl->p_ready[other ? x ^ 1 : x][0], (x == 0 && other ? j : j + 1) & 1);
+                        if (!next) continue;
+                        ok = ok && seen(kf, unit_full(k), unit_parity(k));
+                        if (ok && tc::elect_one()) {
+                            scores(x, k, 0);
+                            tc::commit(&ctl->s_ready[x]);
+                            if (last_use) tc::commit(&ctl->empty[k % L::kUnits]);
                         }
                         __syncwarp();
                     }
                 }
-                return true;
-            };
-            if (ok && active(0)) ok = scores(0);
-            if (ok && events > 1 && active(1)) ok = scores(1);
-            for (int e = 0; e < events && ok; ++e) {
-                if (!active(e)) continue;
-                ok = values(e);
-                if (ok && e + 2 < events && active(e + 2)) ok = scores(e + 2);
+            } else {
+                const int n = __shfl_sync(0xffffffffu, n_tiles, 0);
+                auto issue_scores = [&](int e, bool early) {
+                    const int u = k_unit(e);
+#pragma unroll
+                    for (int h = 0; h < L::kHalves; ++h) {
+                        ok = ok && seen(early, unit_full(u + h), unit_parity(u + h));
+                        early = test(unit_full(u + 1), unit_parity(u + 1));
+                        if (ok && tc::elect_one()) {
+                            scores(e & 1, u + h, h);
+                            tc::commit(&ctl->empty[(u + h) % L::kUnits]);
+                            if (h == L::kHalves - 1) tc::commit(&ctl->s_ready[e & 1]);
+                        }
+                        __syncwarp();
+                    }
+                };
+                issue_scores(0, false);
+                if (n > 1) issue_scores(1, false);
+                bool p0 = false;
+                for (int e = 0; e < n && ok; ++e) {
+                    const int v = L::kHalves * (e == n - 1 ? 2 * e + 1 : 2 * e + 2), x = e & 1;
+                    const uint32_t phase = (e >> 1) & 1;
+                    const bool v0 = test(unit_full(v), unit_parity(v)), v1 = test(unit_full(v + 1), unit_parity(v + 1));
+                    ok = seen(p0, &ctl->p_ready[x][0], phase) && seen(v0, unit_full(v), unit_parity(v)) && seen(v1, unit_full(v + 1), unit_parity(v + 1));
+                    const bool p1 = test(&ctl->p_ready[x][1], phase);
+                    if (ok && tc::elect_one()) values(x, v, 0, e > 0 ? 1u : 0u);
+                    __syncwarp();
+                    ok = ok && seen(p1, &ctl->p_ready[x][1], phase);
+                    const bool next = e + 2 < n, kf = next && test(unit_full(k_unit(e + 2)), unit_parity(k_unit(e + 2)));
+                    if (ok && tc::elect_one()) {
+                        values(x, v, 1, 1);
+                        tc::commit(&ctl->empty[v % L::kUnits]);
+                        tc::commit(&ctl->empty[(v + 1) % L::kUnits]);
+                        tc::commit(&ctl->o_done[x]);
+                    }
+                    __syncwarp();
+                    p0 = test(&ctl->p_ready[x ^ 1][0], ((e + 1) >> 1) & 1);
+                    if (next) issue_scores(e + 2, kf);
+                }
             }
             if (!ok && lane == 0) {
                 record_error(kErrPackedBarrierTimeout);
@@ -538,9 +591,9 @@ __global__ void __launch_bounds__(kThreadsPacked, 1) packed_attention_kernel(con
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&ctl->ref_ready[x][quarter]);
             }
-            const int before = L::kTwo ? e - 2 : e - 1;                    // the last product into this O
-            if (__any_sync(0xffffffffu, raise) && before >= 0) {
-                if (!wait_warp(&ctl->o_done[before & 1], (before >> 1) & 1)) { ok = false; break; }
+            if (__any_sync(0xffffffffu, raise) && e >= L::kRowTiles) {
+                // the last product into this O: with two row tiles it was issued before these scores, and is complete
+                if (!L::kTwo && !wait_warp(&ctl->o_done[x ^ 1], ((e - 1) >> 1) & 1)) { ok = false; break; }
                 tc::fence_after_thread_sync();
                 const float f = raise ? ex2(ref - now) : 1.0f;
                 for (int c = 0; c < DP; c += 32) {
@@ -606,8 +659,7 @@ __global__ void __launch_bounds__(kThreadsPacked, 1) packed_attention_kernel(con
         }
         const int mine = L::kTwo ? tiles[x] : tiles[0];
         if (ok && mine > 0) {
-            const int last = L::kTwo ? 2 * (mine - 1) + x : mine - 1;
-            if (!wait_warp(&ctl->o_done[last & 1], (last >> 1) & 1)) ok = false;
+            if (!wait_warp(&ctl->o_done[L::kTwo ? x : (mine - 1) & 1], L::kTwo ? 0 : ((mine - 1) >> 1) & 1)) ok = false;
             tc::fence_after_thread_sync();
         }
         if (!ok && lane == 0) {
@@ -757,7 +809,7 @@ extern "C" int tpb200_packed_attention(const tpb200_packed_attention_args* a, tp
     // instruction descriptor: fp32 sums, A and B bf16 (1) or fp16 (0), [13] negate A, [16] B MN-major, N >> 3 at 17, M >> 4 at 24
     const uint32_t types = (1u << 4) | (bf ? (1u << 7) | (1u << 10) : 0u) | ((128u >> 4) << 24);
     P.idesc_s = types | (a->scale < 0.0f ? 1u << 13 : 0u) | ((128u >> 3) << 17);
-    P.idesc_o = types | (1u << 16) | (static_cast<uint32_t>(std::min(DP, 128) >> 3) << 17);
+    P.idesc_o = types | (1u << 16) | (static_cast<uint32_t>(DP >> 3) << 17);
     const int rows_tokens = kTile / pack;
     if (!rows_map(&P.q, a->q, a->head_dim, a->q_heads, a->q_stride[1], a->q_tokens, a->q_stride[0], pack, rows_tokens)) return TPB200_ERR_SHAPE;
     if (a->k_tokens > 0) {
