@@ -21,9 +21,6 @@
 //                         shared memory.
 // While one group works the other's products run.
 //
-// The exponentials are what is left to speed up once the products are fed: 16 a cycle on an SM, 1024 cycles for a tile of 128 x 128, as
-// many as its products take at head size 128.  A quarter of them is therefore computed on the FMA pipes (exp2_pair).
-//
 // What may stand in masked places does not matter: scores are selected, not biased.  Rows of V behind a sequence's end are zeroed in
 // shared memory, and in tiles that hold masked pairs V is searched for infinities and NaN (weight 0 times those would be NaN): they are
 // taken out and added to the rows that do see them at the end.
@@ -39,8 +36,6 @@ namespace {
 
 constexpr int kTile = 128;               // rows of a query tile, keys of a key tile
 constexpr int kBlockBytes = kTile * 128; // 128 rows x 64 columns of 16 bits
-constexpr int kThreadsPacked = 384;
-constexpr uint32_t kTmemCols = 512, kColO = 256;
 constexpr long long kWait = 200000000LL; // about 0.1 s: the bound of each wait
 constexpr float kRaise = 8.0f;
 constexpr int kBadTiles = 4;             // key tiles with masked pairs at most: 256 rows on the diagonal and the sequence's end
@@ -60,16 +55,23 @@ struct PackedParams {
     int causal;
 };
 
-template <int DP>
+// DP: head_dim rounded up to 64, 128 or 256; R: tiles of 128 rows per CTA, two only up to 128
+template <int DP, int R>
 struct Layout {
-    static constexpr bool kTwo = DP <= 128;
-    static constexpr int kRowTiles = kTwo ? 2 : 1;
+    static constexpr bool kOwn = DP <= 128;                        // every row tile has a group, a buffer of scores and an O of its own
+    static constexpr int kGroups = kOwn ? R : 2;
+    static constexpr int kThreads = 128 + 128 * kGroups;
+    static constexpr int kCtas = kOwn && R == 1 ? 2 : 1;           // on an SM
+    static constexpr uint32_t kTmemCols = kCtas == 2 ? 256 : 512, kColO = kGroups * kTile;
     static constexpr int kBlocks = DP / 64;                        // 64-column blocks of a row
     static constexpr int kUnitBlocks = DP < 128 ? 1 : 2;           // a unit: 128 keys x up to 128 columns
     static constexpr int kHalves = kBlocks / kUnitBlocks;          // units of a tile
     static constexpr int kUnitBytes = kUnitBlocks * kBlockBytes;
-    static constexpr int kUnits = DP < 128 ? 8 : 4;
-    static constexpr int kQBytes = kRowTiles * kBlocks * kBlockBytes;
+    static constexpr int kUnits = kCtas == 2 ? (DP < 128 ? 4 : 2) : (DP < 128 ? 8 : 4);
+    static constexpr int kQBytes = R * kBlocks * kBlockBytes;
+    // registers move over to the softmax: threads x registers at launch (168 or 128 each) on both sides
+    static constexpr int kFewRegs = kCtas == 2 ? 56 : 64, kManyRegs = kCtas == 2 ? 200 : 216;
+    static_assert(R == 1 || kOwn, "");
 };
 
 struct PackedControl {
@@ -87,9 +89,10 @@ struct PackedControl {
     float part_l[2][kTile], part_m[2][kTile];
 };
 
-template <int DP>
+template <int DP, int R>
 constexpr int packed_smem() {
-    return Layout<DP>::kQBytes + Layout<DP>::kUnits * Layout<DP>::kUnitBytes + static_cast<int>(sizeof(PackedControl)) + 1024;
+    using L = Layout<DP, R>;
+    return std::max(L::kQBytes + L::kUnits * L::kUnitBytes + static_cast<int>(sizeof(PackedControl)) + 1024, min_smem_of_columns(L::kTmemCols));
 }
 
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
@@ -157,50 +160,11 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     return r;
 }
 
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
-__device__ __forceinline__ float max_nan(float a, float b) {        // NaN stays NaN
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
-}
-
-// 2^x of a pair for x <= 8 without the special-function unit, after Cody and Waite: x = n + f with n the nearest integer (it falls out
-// of adding 1.5 * 2^23), |f| <= 1/2, 2^f by the polynomial of least relative error (Remez exchange), times 2^n assembled as a float.
-// Degree 3 is off by 7.5e-5 at most, a fiftieth of bf16's half step; degree 4, for fp16, by 2.7e-6.  x below -126 gives
-// 2^-126: such a weight is nothing beside the row's largest.
-template <typename T>
-__device__ __forceinline__ uint64_t exp2_pair(uint64_t x) {
-    float a, b;
-    unpair(x, a, b);
-    x = pair(max_nan(a, -126.0f), max_nan(b, -126.0f));
-    constexpr float kShift = 12582912.0f;
-    const uint64_t t = add2(x, pair(kShift, kShift)), n = add2(t, pair(-kShift, -kShift));
-    const uint64_t f = fma2(n, pair(-1.0f, -1.0f), x);
-    uint64_t p;
-    auto c = [](float v) { return pair(v, v); };
-    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-        p = fma2(c(0.0551716685f), f, c(0.242611125f));
-        p = fma2(p, f, c(0.693260968f));
-        p = fma2(p, f, c(0.999928057f));
-    } else {
-        p = fma2(c(0.00957010221f), f, c(0.0559178591f));
-        p = fma2(p, f, c(0.240247443f));
-        p = fma2(p, f, c(0.693121791f));
-        p = fma2(p, f, c(0.999999285f));
-    }
-    unpair(t, a, b);
-    return mul2(p, pair(__uint_as_float((__float_as_uint(a) << 23) + 0x3f800000u), __uint_as_float((__float_as_uint(b) << 23) + 0x3f800000u)));
-}
-
 __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity) {
     return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, kWait));
 }
@@ -211,9 +175,14 @@ __device__ __forceinline__ int row_limit(const PackedParams& P, int nq, int nk, 
     return P.causal ? max(0, min(nk, nk - nq + token + 1)) : nk;
 }
 
-template <typename T, int DP>
-__global__ void __launch_bounds__(kThreadsPacked, 1) packed_attention_kernel(const __grid_constant__ PackedParams P) {
-    using L = Layout<DP>;
+template <int kRegs>
+__device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs)); }
+template <int kRegs>
+__device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs)); }
+
+template <typename T, int DP, int R>
+__global__ void __launch_bounds__(Layout<DP, R>::kThreads, Layout<DP, R>::kCtas) packed_attention_kernel(const __grid_constant__ PackedParams P) {
+    using L = Layout<DP, R>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* sQ = smem;
@@ -221,7 +190,7 @@ __global__ void __launch_bounds__(kThreadsPacked, 1) packed_attention_kernel(con
     PackedControl* ctl = reinterpret_cast<PackedControl*>(ring + L::kUnits * L::kUnitBytes);
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int head_group = blockIdx.x % P.head_groups;
-    constexpr int kRowsCta = L::kRowTiles * kTile;
+    constexpr int kRowsCta = R * kTile;
     const int tokens_cta = kRowsCta >> P.pack_shift;
 
     pdl_wait_prior_grids();              // the offsets may come from the previous kernel too
@@ -293,7 +262,7 @@ __global__ void __launch_bounds__(kThreadsPacked, 1) packed_attention_kernel(con
         return;
     }
     if (warp == 2) {
-        tc::tmem_alloc(&ctl->tmem_base, kTmemCols);
+        tc::tmem_alloc(&ctl->tmem_base, L::kTmemCols);
         tc::tmem_relinquish();
     }
     tc::fence_before_thread_sync();
@@ -309,20 +278,20 @@ __global__ void __launch_bounds__(kThreadsPacked, 1) packed_attention_kernel(con
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
         const int first = token0 + x * tokens_tile, last = min(first + tokens_tile, nq) - 1;
-        tiles[x] = (x < L::kRowTiles && last >= first) ? (row_limit(P, nq, nk, last) + kTile - 1) / kTile : 0;
+        tiles[x] = (x < R && last >= first) ? (row_limit(P, nq, nk, last) + kTile - 1) / kTile : 0;
     }
-    if (!L::kTwo) tiles[1] = 0;
+    if (!L::kOwn) tiles[1] = 0;
     const int n_tiles = max(tiles[0], tiles[1]);
     const int first_masked = row_limit(P, nq, nk, token0) / kTile;       // key tiles from here on hold masked pairs: kBadTiles at most
-    const int events = L::kTwo ? 2 * n_tiles : n_tiles;
+    const int events = L::kOwn ? 2 * n_tiles : n_tiles;
     // the order of the line of events: which are computed, and where the tiles of K and V stand in the ring
-    auto active = [&](int e) { return L::kTwo ? (e >> 1) < tiles[e & 1] : true; };
-    auto key_tile = [&](int e) { return L::kTwo ? e >> 1 : e; };
-    auto k_unit = [&](int j) { return L::kHalves * (L::kTwo ? 2 * j : (j < 2 ? j : 2 * j - 1)); };
-    auto v_unit = [&](int j) { return L::kHalves * (L::kTwo ? 2 * j + 1 : (j == n_tiles - 1 ? 2 * j + 1 : 2 * j + 2)); };
+    auto active = [&](int e) { return L::kOwn ? (e >> 1) < tiles[e & 1] : true; };
+    auto key_tile = [&](int e) { return L::kOwn ? e >> 1 : e; };
+    auto k_unit = [&](int j) { return L::kHalves * (L::kOwn ? 2 * j : (j < 2 ? j : 2 * j - 1)); };
+    auto v_unit = [&](int j) { return L::kHalves * (L::kOwn ? 2 * j + 1 : (j == n_tiles - 1 ? 2 * j + 1 : 2 * j + 2)); };
 
     if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        fewer_registers<L::kFewRegs>();
         if (warp == 0 && n_tiles > 0) {
             // -------------------------------------------------------- producer
             const int kv_head = head_group / P.groups_per_kv;
@@ -349,7 +318,7 @@ __global__ void __launch_bounds__(kThreadsPacked, 1) packed_attention_kernel(con
                     }
                     return true;
                 };
-                if (L::kTwo) {
+                if (L::kOwn) {
                     for (int j = 0; j < n_tiles && ok; ++j) ok = request(&P.k, j) && request(&P.v, j, true);
                 } else {
                     ok = request(&P.k, 0);
@@ -381,7 +350,7 @@ __global__ void __launch_bounds__(kThreadsPacked, 1) packed_attention_kernel(con
             auto unit_parity = [&](int u) -> uint32_t { return (u / L::kUnits) & 1; };
             // scores of one unit of K (past head_dim both operands are zero), row tile x, into buffer x
             auto scores = [&](int x, int u, int h) {
-                const uint32_t qa = q16 + ((L::kTwo ? x * L::kBlocks * kBlockBytes : h * L::kUnitBytes) >> 4), ka = r16 + (u % L::kUnits * L::kUnitBytes >> 4);
+                const uint32_t qa = q16 + ((L::kOwn ? x * L::kBlocks * kBlockBytes : h * L::kUnitBytes) >> 4), ka = r16 + (u % L::kUnits * L::kUnitBytes >> 4);
 #pragma unroll
                 for (int kk = 0; kk < L::kUnitBlocks * 4; ++kk) {
                     const uint32_t off = static_cast<uint32_t>((kk >> 2) * kBlockBytes + (kk & 3) * 32) >> 4;
@@ -391,7 +360,7 @@ __global__ void __launch_bounds__(kThreadsPacked, 1) packed_attention_kernel(con
             };
             // the product of half of a tile's keys, weights in buffer x; a tile's units lie one behind the other
             auto values = [&](int x, int u, int part, uint32_t more) {
-                const uint32_t va = r16 + (u % L::kUnits * L::kUnitBytes >> 4), d = tm + kColO + (L::kTwo ? x * DP : 0);
+                const uint32_t va = r16 + (u % L::kUnits * L::kUnitBytes >> 4), d = tm + L::kColO + (L::kOwn ? x * DP : 0);
 #pragma unroll
                 for (int kk = part * 4; kk < part * 4 + 4; ++kk) {
                     mma_ts(d, tm + x * kTile + kk * 8, tc::desc_from_words((va + (kk * 2048 >> 4)) | kLboField, kDescHiMnSw128), P.idesc_o,
@@ -399,7 +368,7 @@ __global__ void __launch_bounds__(kThreadsPacked, 1) packed_attention_kernel(con
                 }
             };
             bool ok = wait_warp(&ctl->q_full, 0);
-            if constexpr (L::kTwo) {
+            if constexpr (L::kOwn) {
                 const int t0 = __shfl_sync(0xffffffffu, tiles[0], 0), t1 = __shfl_sync(0xffffffffu, tiles[1], 0), n = max(t0, t1);
                 ok = ok && wait_warp(unit_full(0), 0);
                 tc::fence_after_thread_sync();
@@ -548,12 +517,12 @@ __global__ void __launch_bounds__(kThreadsPacked, 1) packed_attention_kernel(con
         }
     } else {
         // ------------------------------------------------------------ softmax: group x, thread = row of a tile
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        more_registers<L::kManyRegs>();
         const int x = (warp >> 2) - 1;
         const int quarter = warp & 3, row = quarter * 32 + lane;
         const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
-        const uint32_t s_at = lanes + x * kTile, o_at = lanes + kColO + (L::kTwo ? x * DP : 0);
-        const int my_tile = L::kTwo ? x : 0;
+        const uint32_t s_at = lanes + x * kTile, o_at = lanes + L::kColO + (L::kOwn ? x * DP : 0);
+        const int my_tile = L::kOwn ? x : 0;
         const int token = token0 + my_tile * tokens_tile + (row >> P.pack_shift);
         const int limit = row_limit(P, nq, nk, token);
         const int lowest = row_limit(P, nq, nk, token0 + my_tile * tokens_tile);     // of the tile's rows that exist
@@ -580,20 +549,20 @@ __global__ void __launch_bounds__(kThreadsPacked, 1) packed_attention_kernel(con
 #pragma unroll
             for (int i = 0; i < kTile; i += 2) top[(i >> 1) & 3] = max3(top[(i >> 1) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
             const float high = max3(fmaxf(top[0], top[1]), top[2], top[3]) * P.scale2;
-            if (!L::kTwo && e > 0) {     // the reference after the event before, from the other group
+            if (!L::kOwn && e > 0) {     // the reference after the event before, from the other group
                 if (!wait_warp(&ctl->ref_ready[x ^ 1][quarter], ((e - 1) >> 1) & 1)) { ok = false; break; }
                 ref = ctl->ref[row];
             }
             const bool raise = high > ref + kRaise || (ref == -INFINITY && high > ref);
             const float now = raise ? high : ref;
-            if (!L::kTwo) {
+            if (!L::kOwn) {
                 ctl->ref[row] = now;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&ctl->ref_ready[x][quarter]);
             }
-            if (__any_sync(0xffffffffu, raise) && e >= L::kRowTiles) {
+            if (__any_sync(0xffffffffu, raise) && e >= R) {
                 // the last product into this O: with two row tiles it was issued before these scores, and is complete
-                if (!L::kTwo && !wait_warp(&ctl->o_done[x ^ 1], ((e - 1) >> 1) & 1)) { ok = false; break; }
+                if (!L::kOwn && !wait_warp(&ctl->o_done[x ^ 1], ((e - 1) >> 1) & 1)) { ok = false; break; }
                 tc::fence_after_thread_sync();
                 const float f = raise ? ex2(ref - now) : 1.0f;
                 for (int c = 0; c < DP; c += 32) {
@@ -615,64 +584,53 @@ __global__ void __launch_bounds__(kThreadsPacked, 1) packed_attention_kernel(con
             // P = 2^(scale2 S - m), its row sum, rounded pairs into the columns S was in
             const uint64_t scale = pair(P.scale2, P.scale2), minus = pair(-base, -base);
             uint64_t sum[2] = {pair(0.0f, 0.0f), pair(0.0f, 0.0f)};
-            auto weights = [&](auto poly) {
 #pragma unroll
-                for (int c = 0; c < kTile / 2; c += 32) {
-                    uint32_t p[32];
+            for (int c = 0; c < kTile / 2; c += 32) {
+                uint32_t p[32];
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        uint64_t w = fma2(pair(__uint_as_float(s[2 * (c + i)]), __uint_as_float(s[2 * (c + i) + 1])), scale, minus);
-                        float a, b;
-                        if (decltype(poly)::value && i % 4 == 3) {
-                            w = exp2_pair<T>(w);
-                            unpair(w, a, b);
-                        } else {
-                            unpair(w, a, b);
-                            a = ex2(a);
-                            b = ex2(b);
-                            w = pair(a, b);
-                        }
-                        sum[i & 1] = add2(sum[i & 1], w);
-                        p[i] = Half16<T>::pack(a, b);
-                    }
-                    tmem_st_x32(s_at + c, p);
-                    tmem_st_done();
-                    tc::fence_before_thread_sync();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&ctl->p_ready[x][c / 32]);
+                for (int i = 0; i < 32; ++i) {
+                    float a, b;
+                    unpair(fma2(pair(__uint_as_float(s[2 * (c + i)]), __uint_as_float(s[2 * (c + i) + 1])), scale, minus), a, b);
+                    a = ex2(a);
+                    b = ex2(b);
+                    sum[i & 1] = add2(sum[i & 1], pair(a, b));
+                    p[i] = Half16<T>::pack(a, b);
                 }
-            };
-            // masked scores are -inf and have to become zeros; with one row tile the products take twice the exponentials' time
-            if (masked || !L::kTwo) weights(std::false_type{});
-            else weights(std::true_type{});
+                tmem_st_x32(s_at + c, p);
+                tmem_st_done();
+                tc::fence_before_thread_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&ctl->p_ready[x][c / 32]);
+            }
             float a, b;
             unpair(add2(sum[0], sum[1]), a, b);
             l += a + b;
         }
         // ------------------------------------------------------------ O / l -> the rows
-        if (!L::kTwo) {
+        if (!L::kOwn) {
             ctl->part_l[x][row] = l;
             ctl->part_m[x][row] = l_ref;
             asm volatile("bar.sync 1, 256;" ::: "memory");
             const float m = fmaxf(ctl->part_m[0][row], ctl->part_m[1][row]), base = m == -INFINITY ? 0.0f : m;
             l = ctl->part_l[0][row] * ex2(ctl->part_m[0][row] - base) + ctl->part_l[1][row] * ex2(ctl->part_m[1][row] - base);
         }
-        const int mine = L::kTwo ? tiles[x] : tiles[0];
+        const int mine = L::kOwn ? tiles[x] : tiles[0];
         if (ok && mine > 0) {
-            if (!wait_warp(&ctl->o_done[L::kTwo ? x : (mine - 1) & 1], L::kTwo ? 0 : ((mine - 1) >> 1) & 1)) ok = false;
+            if (!wait_warp(&ctl->o_done[L::kOwn ? x : (mine - 1) & 1], L::kOwn ? 0 : ((mine - 1) >> 1) & 1)) ok = false;
             tc::fence_after_thread_sync();
         }
         if (!ok && lane == 0) {
             record_error(kErrPackedBarrierTimeout);
             ctl->failed = 1;
         }
-        if (ok && (L::kTwo || x == 0 || DP > 128)) {
+        if (ok) {
             const float inv = mine > 0 ? 1.0f / l : 0.0f;
             // through shared memory where Q was (its products are done), each warp its own rows, so that whole rows leave together
-            constexpr int kCols = L::kTwo ? DP : DP / 2, kChunks = kCols / 8, kRowsIter = 32 / kChunks;
-            const int c_lo = L::kTwo ? 0 : x * kCols;
+            constexpr int kCols = L::kOwn ? DP : DP / 2, kChunks = kCols / 8, kRowsIter = 32 / kChunks;
+            const int c_lo = L::kOwn ? 0 : x * kCols;
             uint8_t* stage = sQ + (x * 4 + quarter) * 32 * kCols * 2;
             const bool any_bad = mine > 0 && ctl->bad_any != 0;
+#pragma unroll 1
             for (int c = 0; c < kCols; c += 32) {
                 uint32_t o[32];
                 if (mine > 0) {
@@ -726,26 +684,26 @@ __global__ void __launch_bounds__(kThreadsPacked, 1) packed_attention_kernel(con
         __syncthreads();
     }
     tc::fence_after_thread_sync();
-    if (warp == 2) tc::tmem_dealloc(tmem, kTmemCols);
+    if (warp == 2) tc::tmem_dealloc(tmem, L::kTmemCols);
 }
 
-template <typename T, int DP>
+template <typename T, int DP, int R>
 int launch_packed(const PackedParams& P, unsigned blocks, int flags, cudaStream_t stream) {
-    constexpr int smem = packed_smem<DP>();
-    static_assert(smem <= 227 * 1024, "shared memory of a CTA");
+    constexpr int smem = packed_smem<DP, R>();
+    static_assert(Layout<DP, R>::kCtas * (smem + 1024) <= 228 * 1024, "shared memory of an SM");
     static std::atomic<uint64_t> configured{0};
     int dev = 0;
     cudaGetDevice(&dev);
     const uint64_t bit = 1ull << (dev & 63);
     if (!(configured.load(std::memory_order_relaxed) & bit)) {
-        if (cudaFuncSetAttribute(packed_attention_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
+        if (cudaFuncSetAttribute(packed_attention_kernel<T, DP, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
             return TPB200_ERR_CUDA;
         }
         configured.fetch_or(bit, std::memory_order_relaxed);
     }
     cudaLaunchAttribute attr;
-    const cudaLaunchConfig_t cfg = paged_config(blocks, kThreadsPacked, smem, flags, &attr, stream);
-    return cudaLaunchKernelEx(&cfg, packed_attention_kernel<T, DP>, P) == cudaSuccess ? TPB200_OK : TPB200_ERR_CUDA;
+    const cudaLaunchConfig_t cfg = paged_config(blocks, Layout<DP, R>::kThreads, smem, flags, &attr, stream);
+    return cudaLaunchKernelEx(&cfg, packed_attention_kernel<T, DP, R>, P) == cudaSuccess ? TPB200_OK : TPB200_ERR_CUDA;
 }
 
 // [tokens][heads][head_dim] with element strides, boxes of 64 columns x `heads` x `rows` tokens
@@ -818,14 +776,20 @@ extern "C" int tpb200_packed_attention(const tpb200_packed_attention_args* a, tp
             return TPB200_ERR_SHAPE;
         }
     }
+    // Up to head size 128, two row tiles per CTA where sequences are long (each unit of K and V serves both), else one, and two CTAs on an
+    // SM: half the rows to fill up, and one's loads and output beside the other's products.  KSHORT
+    const bool two = DP <= 128 && static_cast<long long>(a->k_tokens) > 1024ll * a->seqs;
     // no more tiles than whole ones and a ragged one per sequence
-    const int tokens_cta = rows_tokens * (DP <= 128 ? 2 : 1);
-    const long long tiles = static_cast<long long>(a->q_tokens) / tokens_cta + std::min(a->seqs, a->q_tokens);
+    const long long tiles = static_cast<long long>(a->q_tokens) / (rows_tokens * (two ? 2 : 1)) + std::min(a->seqs, a->q_tokens);
     const long long blocks = tiles * P.head_groups;
     TPB_REQUIRE(blocks <= 0x7fffffff, TPB200_ERR_SHAPE);
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     const unsigned n = static_cast<unsigned>(blocks);
-    if (DP == 64) return bf ? launch_packed<__nv_bfloat16, 64>(P, n, a->flags, s) : launch_packed<__half, 64>(P, n, a->flags, s);
-    if (DP == 128) return bf ? launch_packed<__nv_bfloat16, 128>(P, n, a->flags, s) : launch_packed<__half, 128>(P, n, a->flags, s);
-    return bf ? launch_packed<__nv_bfloat16, 256>(P, n, a->flags, s) : launch_packed<__half, 256>(P, n, a->flags, s);
+    auto launch = [&](auto type) {
+        using T = decltype(type);
+        if (DP == 64) return two ? launch_packed<T, 64, 2>(P, n, a->flags, s) : launch_packed<T, 64, 1>(P, n, a->flags, s);
+        if (DP == 128) return two ? launch_packed<T, 128, 2>(P, n, a->flags, s) : launch_packed<T, 128, 1>(P, n, a->flags, s);
+        return launch_packed<T, 256, 1>(P, n, a->flags, s);
+    };
+    return bf ? launch(__nv_bfloat16()) : launch(__half());
 }
