@@ -204,3 +204,32 @@ def test_offsets_outside_the_tensors_are_clamped(cuda_device):
     assert torch.equal(ops.packed_attention(q, k, v, cu, 0.125, out=out)[:150], want[:150])
     assert bool((out[150:] == 0).all())
     _no_error()
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("hq,hk,D", [(8, 2, 128), (16, 4, 64), (3, 1, 72), (4, 4, 64)])
+def test_two_row_tiles_per_cta(cuda_device, hq, hk, D, dtype, causal):
+    """Sequences long enough on average for the form with two row tiles: ragged ends, a tile of rows on its own, queries without keys,
+    short sequences between long ones."""
+    lens, klens = [129, 40, 300, 7, 128], [4500, 1300, 130, 3000, 128]
+    _run(cuda_device, lens, klens, hq, hk, D, dtype, causal, seed=D)
+
+
+def test_masked_places_with_two_row_tiles(cuda_device):
+    from turbopi_b200 import ops
+    lens, klens = [300, 200], [300, 3000]
+    cu, cuk = _offsets(lens, cuda_device), _offsets(klens, cuda_device)
+    q, k, v = _problem(lens, klens, 8, 2, 128, torch.bfloat16, cuda_device, seed=11)
+    clean = ops.packed_attention(q, k, v, cu, 0.09, cu_keys=cuk)
+    for value in (float("nan"), float("inf")):
+        for at in (2850, 2900, 2999, 10):                        # the first query sees 2801
+            v2 = v.clone()
+            v2[300 + at, 0, 64:] = value
+            out = ops.packed_attention(q, k, v2, cu, 0.09, cu_keys=cuk)
+            sees = torch.arange(200, device=cuda_device) + 2800 >= at
+            assert torch.equal(out[:300], clean[:300]) and torch.equal(out[300:][~sees], clean[300:][~sees])
+            bad = out[300:][sees][:, :4, 64:]
+            assert bool((bad.isnan() if value != value else (bad == value)).all())
+            assert torch.equal(out[300:, :, :64], clean[300:, :, :64]) and torch.equal(out[300:, 4:], clean[300:, 4:])
+    _no_error()
