@@ -257,10 +257,7 @@ __global__ void __launch_bounds__(Layout<DP, R>::kThreads, Layout<DP, R>::kCtas)
         }
     }
     __syncthreads();
-    if (ctl->seq < 0) {
-        pdl_launch_dependents();
-        return;
-    }
+    if (ctl->seq < 0) return;
     if (warp == 2) {
         tc::tmem_alloc(&ctl->tmem_base, L::kTmemCols);
         tc::tmem_relinquish();

@@ -14,7 +14,7 @@ namespace tpb {
 namespace {
 
 constexpr int kAppendThreads = 256;
-constexpr int kAppendUnits = 4;          // units a thread has in flight: 64 KB of loads per SM at full occupancy
+constexpr int kAppendLoads = 4;          // tokens whose unit a thread has in flight: 32 bytes each
 constexpr int kMaxTokensPerBlock = 16;
 
 struct AppendParams {
@@ -71,9 +71,10 @@ __device__ __forceinline__ void load_table(const void* p, int dtype, size_t at, 
 }
 
 // A unit is V values of a row and the V values half a row further on (rotated, or a plain copy of both), so that a rotation
-// needs one thread.  V = 8 where half a row is a multiple of 8, else 4.
+// needs one thread.  V = 8 where half a row is a multiple of 8, else 4.  A thread keeps its unit (which tensor, head and columns) for all
+// tokens of the block: one division per thread and not per token (77 -> 54 us for the prompts of six sequences, 10.5 k tokens, 4.9 TB/s).
 template <typename T, int V>
-__global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const __grid_constant__ AppendParams P) {
+__global__ void __launch_bounds__(kAppendThreads, 3) paged_append_kernel(const __grid_constant__ AppendParams P) {
     __shared__ int seq[kMaxTokensPerBlock];
     __shared__ int position[kMaxTokensPerBlock];
     __shared__ long long row_at[kMaxTokensPerBlock];     // element offset of the token's row in the pages, -1: not written
@@ -82,76 +83,74 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const __gr
     const int t0 = blockIdx.x * P.tokens_per_block;
     const int count = min(P.tokens_per_block, P.tokens - t0);
     const int per_token = P.units_q + P.units_k + P.units_v;
-    const int total = count * per_token;
     const int half = P.cache.head_dim / 2, per_row = half / V;
     bool placed = false;
-    for (int base = 0; base < total; base += kAppendThreads * kAppendUnits) {
-        Vec<V> a[kAppendUnits], b[kAppendUnits];
-        int token[kAppendUnits], kind[kAppendUnits], head[kAppendUnits], at[kAppendUnits];
+    for (int base = 0; base < per_token; base += kAppendThreads) {
+        const int u = base + threadIdx.x;
+        const bool mine = u < per_token;
+        const int kind = u < P.units_q ? 0 : (u < P.units_q + P.units_k ? 1 : 2);        // queries, keys, values
+        const int r = u - (kind == 0 ? 0 : (kind == 1 ? P.units_q : P.units_q + P.units_k)), head = r / per_row, at = (r - head * per_row) * V;
+        const long long* st = kind == 0 ? P.q_stride : (kind == 1 ? P.k_stride : P.v_stride);
+        const long long step = st[0];
+        const uint16_t* src = (kind == 0 ? P.q : (kind == 1 ? P.k : P.v)) + t0 * step + head * st[1] + at;
+        const bool turn = P.rope_positions > 0 && kind < 2;
+        uint16_t* dst = kind == 0 ? P.q_out + t0 * P.o_stride[0] + head * P.o_stride[1] + at
+                                  : static_cast<uint16_t*>(kind == 1 ? P.cache.k_pages : P.cache.v_pages) + head * P.cache.head_stride + at;
+        for (int first = 0; first < count; first += kAppendLoads) {
+            Vec<V> a[kAppendLoads], b[kAppendLoads];
 #pragma unroll
-        for (int i = 0; i < kAppendUnits; ++i) {
-            const int u = base + i * kAppendThreads + threadIdx.x;
-            kind[i] = -1;
-            if (u >= total) continue;
-            token[i] = u / per_token;
-            int r = u - token[i] * per_token;
-            kind[i] = r < P.units_q ? 0 : (r < P.units_q + P.units_k ? 1 : 2);
-            r -= kind[i] == 0 ? 0 : (kind[i] == 1 ? P.units_q : P.units_q + P.units_k);
-            head[i] = r / per_row;
-            at[i] = (r - head[i] * per_row) * V;
-            const uint16_t* src = kind[i] == 0 ? P.q : (kind[i] == 1 ? P.k : P.v);
-            const long long* st = kind[i] == 0 ? P.q_stride : (kind[i] == 1 ? P.k_stride : P.v_stride);
-            src += (t0 + token[i]) * st[0] + head[i] * st[1] + at[i];
-            a[i] = load_vec<V>(src);
-            b[i] = load_vec<V>(src + half);
-        }
-        if (!placed) {
-            // the tokens' rows, behind the first loads: which sequence, which position, which page
-            placed = true;
-            if (threadIdx.x < kMaxTokensPerBlock) seq[threadIdx.x] = 0x7fffffff;
-            __syncthreads();
-            for (int s = threadIdx.x; s < P.cache.seqs; s += kAppendThreads) {
-                const int lo = max(P.cu[s], t0), hi = min(P.cu[s + 1], t0 + count);
-                for (int t = lo; t < hi; ++t) atomicMin(&seq[t - t0], s);
-            }
-            __syncthreads();
-            if (threadIdx.x < count) {
-                const int s = seq[threadIdx.x];
-                long long row = -1;
-                int pos = -1;
-                if (s != 0x7fffffff) {                   // tokens behind the last sequence belong to nobody
-                    pos = P.cache.lengths[s] - (P.cu[s + 1] - (t0 + static_cast<int>(threadIdx.x)));
-                    row = P.cache.row_offset(s, pos);
-                    if (row >= 0 && P.rope_positions > 0 && pos >= P.rope_positions) row = -1;
-                    if (row < 0) record_error(kErrPagedIndex);
-                }
-                row_at[threadIdx.x] = row;
-                position[threadIdx.x] = pos;
-            }
-            __syncthreads();
-        }
-#pragma unroll
-        for (int i = 0; i < kAppendUnits; ++i) {
-            if (kind[i] < 0) continue;
-            const long long row = row_at[token[i]];
-            if (row < 0) continue;
-            if (P.rope_positions > 0 && kind[i] < 2) {
-                float c[V], s[V];
-                const size_t e = static_cast<size_t>(position[token[i]]) * half + at[i];
-                load_table<V>(P.cos, P.rope_dtype, e, c);
-                load_table<V>(P.sin, P.rope_dtype, e, s);
-#pragma unroll
-                for (int j = 0; j < V / 2; ++j) {        // in fp32, rounded once
-                    const float2 x = Half16<T>::unpack(a[i].w[j]), y = Half16<T>::unpack(b[i].w[j]);
-                    a[i].w[j] = Half16<T>::pack(x.x * c[2 * j] - y.x * s[2 * j], x.y * c[2 * j + 1] - y.y * s[2 * j + 1]);
-                    b[i].w[j] = Half16<T>::pack(y.x * c[2 * j] + x.x * s[2 * j], y.y * c[2 * j + 1] + x.y * s[2 * j + 1]);
+            for (int i = 0; i < kAppendLoads; ++i) {
+                if (mine && first + i < count) {
+                    a[i] = load_vec<V>(src + (first + i) * step);
+                    b[i] = load_vec<V>(src + (first + i) * step + half);
                 }
             }
-            uint16_t* dst;
-            if (kind[i] == 0) dst = P.q_out + (t0 + token[i]) * P.o_stride[0] + head[i] * P.o_stride[1] + at[i];
-            else dst = static_cast<uint16_t*>(kind[i] == 1 ? P.cache.k_pages : P.cache.v_pages) + row + head[i] * P.cache.head_stride + at[i];
-            store_vec<V>(dst, a[i]);
-            store_vec<V>(dst + half, b[i]);
+            if (!placed) {
+                // the tokens' rows, behind the first loads: which sequence, which position, which page
+                placed = true;
+                if (threadIdx.x < kMaxTokensPerBlock) seq[threadIdx.x] = 0x7fffffff;
+                __syncthreads();
+                for (int s = threadIdx.x; s < P.cache.seqs; s += kAppendThreads) {
+                    const int lo = max(P.cu[s], t0), hi = min(P.cu[s + 1], t0 + count);
+                    for (int t = lo; t < hi; ++t) atomicMin(&seq[t - t0], s);
+                }
+                __syncthreads();
+                if (threadIdx.x < count) {
+                    const int s = seq[threadIdx.x];
+                    long long row = -1;
+                    int pos = -1;
+                    if (s != 0x7fffffff) {               // tokens behind the last sequence belong to nobody
+                        pos = P.cache.lengths[s] - (P.cu[s + 1] - (t0 + static_cast<int>(threadIdx.x)));
+                        row = P.cache.row_offset(s, pos);
+                        if (row >= 0 && P.rope_positions > 0 && pos >= P.rope_positions) row = -1;
+                        if (row < 0) record_error(kErrPagedIndex);
+                    }
+                    row_at[threadIdx.x] = row;
+                    position[threadIdx.x] = pos;
+                }
+                __syncthreads();
+            }
+#pragma unroll
+            for (int i = 0; i < kAppendLoads; ++i) {
+                if (!mine || first + i >= count) continue;
+                const long long row = row_at[first + i];
+                if (row < 0) continue;
+                if (turn) {
+                    float c[V], s[V];
+                    const size_t e = static_cast<size_t>(position[first + i]) * half + at;
+                    load_table<V>(P.cos, P.rope_dtype, e, c);
+                    load_table<V>(P.sin, P.rope_dtype, e, s);
+#pragma unroll
+                    for (int j = 0; j < V / 2; ++j) {    // in fp32, rounded once
+                        const float2 x = Half16<T>::unpack(a[i].w[j]), y = Half16<T>::unpack(b[i].w[j]);
+                        a[i].w[j] = Half16<T>::pack(x.x * c[2 * j] - y.x * s[2 * j], x.y * c[2 * j + 1] - y.y * s[2 * j + 1]);
+                        b[i].w[j] = Half16<T>::pack(y.x * c[2 * j] + x.x * s[2 * j], y.y * c[2 * j + 1] + x.y * s[2 * j + 1]);
+                    }
+                }
+                uint16_t* to = dst + (kind == 0 ? (first + i) * P.o_stride[0] : row);
+                store_vec<V>(to, a[i]);
+                store_vec<V>(to + half, b[i]);
+            }
         }
     }
 }
@@ -248,9 +247,8 @@ extern "C" int tpb200_paged_append(const tpb200_paged_append_args* a, tpb200_str
     TPB_REQUIRE(units <= (1 << 24), TPB200_ERR_SHAPE);
     P.units_q = static_cast<int>(per_head * P.q_heads);
     P.units_k = P.units_v = static_cast<int>(per_head * P.cache.kv_heads);
-    // a block takes as many tokens as fill its threads' units, but leaves no SM without a block
-    const int fill = std::max<int>(1, static_cast<int>(kAppendThreads * kAppendUnits / units));
-    P.tokens_per_block = std::max(1, std::min({fill, kMaxTokensPerBlock, a->tokens / 296}));
+    // eight tokens share a block's look-up, fewer where that would leave SMs without a block
+    P.tokens_per_block = std::max(1, std::min(8, a->tokens / 444));
     const unsigned blocks = static_cast<unsigned>((a->tokens + P.tokens_per_block - 1) / P.tokens_per_block);
     const bool bf = a->cache.dtype == TPB200_BF16;
     auto kernel = bf ? (V == 8 ? paged_append_kernel<__nv_bfloat16, 8> : paged_append_kernel<__nv_bfloat16, 4>)
