@@ -233,3 +233,17 @@ def test_masked_places_with_two_row_tiles(cuda_device):
             assert bool((bad.isnan() if value != value else (bad == value)).all())
             assert torch.equal(out[300:, :, :64], clean[300:, :, :64]) and torch.equal(out[300:, 4:], clean[300:, 4:])
     _no_error()
+
+
+def test_rows_without_keys_beside_rows_with_keys(cuda_device):
+    """One row tile of a CTA is done before the CTA's queries have landed where outputs are staged; many launches."""
+    from turbopi_b200 import ops
+    n, m = 256, 100                                              # 128 rows without keys, then 28 more, then 100 with
+    lens, klens = [n] * 40 + [16], [m] * 40 + [90000]            # the long one: two row tiles per CTA
+    q, k, v = _problem(lens, klens, 1, 1, 64, torch.bfloat16, cuda_device, seed=12)
+    cu, cuk = _offsets(lens, cuda_device), _offsets(klens, cuda_device)
+    for _ in range(30):
+        out = ops.packed_attention(q, k, v, cu, 0.125, cu_keys=cuk)
+        assert bool((out[:n * 40].view(40, n, 64)[:, :n - m] == 0).all())
+    _check(out[:n], q, k, v, [n], [m], 0.125, True)
+    _no_error()

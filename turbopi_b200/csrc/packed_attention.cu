@@ -197,12 +197,17 @@ __global__ void __launch_bounds__(Layout<DP, R>::kThreads, Layout<DP, R>::kCtas)
     if (warp == 0) {
         // which tile of which sequence: tiles are dealt from the last one back, so that within a sequence the long rows come first
         const int want = static_cast<int>(gridDim.x / P.head_groups - 1 - blockIdx.x / P.head_groups);
-        int before = 0, found = -1, tile = 0;
+        int before = 0;
+        if (lane == 0) ctl->seq = -1;
+        __syncwarp();
         for (int s0 = 0; s0 < P.seqs; s0 += 32) {
             const int s = s0 + lane;
-            int n = 0;
+            int n = 0, a = 0, b = 0, ka = 0, kb = 0;
             if (s < P.seqs) {
-                const int a = min(max(P.cu[s], 0), P.q_tokens), b = min(max(P.cu[s + 1], a), P.q_tokens);
+                a = min(max(P.cu[s], 0), P.q_tokens);
+                b = min(max(P.cu[s + 1], a), P.q_tokens);
+                ka = min(max(P.cu_keys[s], 0), P.k_tokens);
+                kb = min(max(P.cu_keys[s + 1], ka), P.k_tokens);
                 n = (b - a + tokens_cta - 1) / tokens_cta;
             }
             int upto = n;
@@ -211,26 +216,17 @@ __global__ void __launch_bounds__(Layout<DP, R>::kThreads, Layout<DP, R>::kCtas)
                 const int y = __shfl_up_sync(0xffffffffu, upto, o);
                 if (lane >= o) upto += y;
             }
-            const uint32_t hit = __ballot_sync(0xffffffffu, want >= before + upto - n && want < before + upto);
-            if (hit != 0) {
-                const int at = __ffs(hit) - 1;
-                found = s0 + at;
-                tile = want - before - __shfl_sync(0xffffffffu, upto - n, at);
-                break;
-            }
-            before += __shfl_sync(0xffffffffu, upto, 31);
-        }
-        if (lane == 0) {
-            ctl->seq = found;
-            ctl->tile = tile;
-            if (found >= 0) {
-                const int a = min(max(P.cu[found], 0), P.q_tokens);
+            const bool mine = want >= before + upto - n && want < before + upto;
+            if (mine) {
+                ctl->seq = s;
+                ctl->tile = want - before - (upto - n);
                 ctl->q0 = a;
-                ctl->nq = min(max(P.cu[found + 1], a), P.q_tokens) - a;
-                const int ka = min(max(P.cu_keys[found], 0), P.k_tokens);
+                ctl->nq = b - a;
                 ctl->k0 = ka;
-                ctl->nk = min(max(P.cu_keys[found + 1], ka), P.k_tokens) - ka;
+                ctl->nk = kb - ka;
             }
+            if (__any_sync(0xffffffffu, mine)) break;
+            before += __shfl_sync(0xffffffffu, upto, 31);
         }
     }
     if (threadIdx.x == 32) {
@@ -256,8 +252,6 @@ __global__ void __launch_bounds__(Layout<DP, R>::kThreads, Layout<DP, R>::kCtas)
             tc::prefetch_tensormap(&P.v);
         }
     }
-    __syncthreads();
-    if (ctl->seq < 0) return;
     if (warp == 2) {
         tc::tmem_alloc(&ctl->tmem_base, L::kTmemCols);
         tc::tmem_relinquish();
@@ -267,6 +261,10 @@ __global__ void __launch_bounds__(Layout<DP, R>::kThreads, Layout<DP, R>::kCtas)
     tc::fence_after_thread_sync();
     pdl_launch_dependents();
     const uint32_t tmem = ctl->tmem_base;
+    if (ctl->seq < 0) {                  // more tiles were launched than there are
+        if (warp == 2) tc::tmem_dealloc(tmem, L::kTmemCols);
+        return;
+    }
     const int nq = ctl->nq, nk = ctl->nk, q0 = ctl->q0, k0 = ctl->k0;
     const int token0 = ctl->tile * tokens_cta;
     const int tokens_tile = kTile >> P.pack_shift;
@@ -541,7 +539,11 @@ __global__ void __launch_bounds__(Layout<DP, R>::kThreads, Layout<DP, R>::kCtas)
             for (int c = 0; c < kTile; c += 32) tmem_ld_wait_for(s + c);
             if (masked) {
 #pragma unroll
-                for (int i = 0; i < kTile; ++i) s[i] = i < lim ? s[i] : 0xff800000u;
+                for (int c = 0; c < kTile; c += 32) {    // a bit per column that is seen
+                    const uint32_t sees = lim >= c + 32 ? 0xffffffffu : (lim > c ? (1u << (lim - c)) - 1 : 0u);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) s[c + i] = (sees >> i) & 1 ? s[c + i] : 0xff800000u;
+                }
             }
 #pragma unroll
             for (int i = 0; i < kTile; i += 2) top[(i >> 1) & 3] = max3(top[(i >> 1) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
@@ -616,6 +618,8 @@ __global__ void __launch_bounds__(Layout<DP, R>::kThreads, Layout<DP, R>::kCtas)
             if (!wait_warp(&ctl->o_done[L::kOwn ? x : (mine - 1) & 1], L::kOwn ? 0 : ((mine - 1) >> 1) & 1)) ok = false;
             tc::fence_after_thread_sync();
         }
+        // rows that see no key while the CTA's other row tile does: their queries may still be on the way to where the output is staged
+        if (ok && mine == 0 && n_tiles > 0) ok = wait_warp(&ctl->q_full, 0);
         if (!ok && lane == 0) {
             record_error(kErrPackedBarrierTimeout);
             ctl->failed = 1;
@@ -663,7 +667,7 @@ __global__ void __launch_bounds__(Layout<DP, R>::kThreads, Layout<DP, R>::kCtas)
             }
             __syncwarp();
             const int chunk = lane % kChunks;
-#pragma unroll
+#pragma unroll 4
             for (int r0 = 0; r0 < 32; r0 += kRowsIter) {
                 const int r = r0 + lane / kChunks, t = token0 + my_tile * tokens_tile + ((quarter * 32 + r) >> P.pack_shift);
                 if (t >= nq || c_lo + chunk * 8 >= P.head_dim) continue;
@@ -685,7 +689,7 @@ __global__ void __launch_bounds__(Layout<DP, R>::kThreads, Layout<DP, R>::kCtas)
 }
 
 template <typename T, int DP, int R>
-int launch_packed(const PackedParams& P, unsigned blocks, int flags, cudaStream_t stream) {
+int launch_packed(const PackedParams& P, unsigned blocks, cudaStream_t stream) {
     constexpr int smem = packed_smem<DP, R>();
     static_assert(Layout<DP, R>::kCtas * (smem + 1024) <= 228 * 1024, "shared memory of an SM");
     static std::atomic<uint64_t> configured{0};
@@ -699,7 +703,7 @@ int launch_packed(const PackedParams& P, unsigned blocks, int flags, cudaStream_
         configured.fetch_or(bit, std::memory_order_relaxed);
     }
     cudaLaunchAttribute attr;
-    const cudaLaunchConfig_t cfg = paged_config(blocks, Layout<DP, R>::kThreads, smem, flags, &attr, stream);
+    const cudaLaunchConfig_t cfg = paged_config(blocks, Layout<DP, R>::kThreads, smem, &attr, stream);
     return cudaLaunchKernelEx(&cfg, packed_attention_kernel<T, DP, R>, P) == cudaSuccess ? TPB200_OK : TPB200_ERR_CUDA;
 }
 
@@ -784,9 +788,9 @@ extern "C" int tpb200_packed_attention(const tpb200_packed_attention_args* a, tp
     const unsigned n = static_cast<unsigned>(blocks);
     auto launch = [&](auto type) {
         using T = decltype(type);
-        if (DP == 64) return two ? launch_packed<T, 64, 2>(P, n, a->flags, s) : launch_packed<T, 64, 1>(P, n, a->flags, s);
-        if (DP == 128) return two ? launch_packed<T, 128, 2>(P, n, a->flags, s) : launch_packed<T, 128, 1>(P, n, a->flags, s);
-        return launch_packed<T, 256, 1>(P, n, a->flags, s);
+        if (DP == 64) return two ? launch_packed<T, 64, 2>(P, n, s) : launch_packed<T, 64, 1>(P, n, s);
+        if (DP == 128) return two ? launch_packed<T, 128, 2>(P, n, s) : launch_packed<T, 128, 1>(P, n, s);
+        return launch_packed<T, 256, 1>(P, n, s);
     };
     return bf ? launch(__nv_bfloat16()) : launch(__half());
 }

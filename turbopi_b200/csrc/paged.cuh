@@ -72,8 +72,9 @@ static inline int paged_view(const tpb200_paged_cache& c, PagedView* v) {
     return TPB200_OK;
 }
 
-static inline cudaLaunchConfig_t paged_config(unsigned blocks, int threads, size_t smem, int flags, cudaLaunchAttribute* attr,
-                                              cudaStream_t stream) {
+// These kernels wait for the launch before them ahead of everything they read or write, so they are always launched as dependents
+// (TPB200_FLAG_PDL or not): their CTAs start while it drains.
+static inline cudaLaunchConfig_t paged_config(unsigned blocks, int threads, size_t smem, cudaLaunchAttribute* attr, cudaStream_t stream) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(blocks, 1, 1);
     cfg.blockDim = dim3(threads, 1, 1);
@@ -82,7 +83,7 @@ static inline cudaLaunchConfig_t paged_config(unsigned blocks, int threads, size
     attr->id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr->val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = (flags & TPB200_FLAG_PDL) ? 1 : 0;
+    cfg.numAttrs = 1;
     return cfg;
 }
 

@@ -836,7 +836,7 @@ DecodeScratch decode_scratch(int ctas, int rows, int head_dim) {
 int decode_rows(int group) { return group <= 8 ? 8 : 16; }
 
 template <typename T, int DP, int NT, bool kAligned>
-int launch_decode(const DecodeParams& P, int ctas, int flags, cudaStream_t stream) {
+int launch_decode(const DecodeParams& P, int ctas, cudaStream_t stream) {
     constexpr int smem = smem_bytes<DP, NT>();
     static_assert(kCtasPerSm * (smem + 1024) <= 228 * 1024, "two CTAs of an SM");
     static std::atomic<uint64_t> configured{0};
@@ -850,15 +850,15 @@ int launch_decode(const DecodeParams& P, int ctas, int flags, cudaStream_t strea
         configured.fetch_or(bit, std::memory_order_relaxed);
     }
     cudaLaunchAttribute attr;
-    const cudaLaunchConfig_t cfg = paged_config(static_cast<unsigned>(ctas), kThreads, smem, flags, &attr, stream);
+    const cudaLaunchConfig_t cfg = paged_config(static_cast<unsigned>(ctas), kThreads, smem, &attr, stream);
     return cudaLaunchKernelEx(&cfg, paged_attention_kernel<T, DP, NT, kAligned>, P) == cudaSuccess ? TPB200_OK : TPB200_ERR_CUDA;
 }
 
 template <typename T, int DP>
-int launch_decode(const DecodeParams& P, int ctas, int flags, cudaStream_t stream) {
+int launch_decode(const DecodeParams& P, int ctas, cudaStream_t stream) {
     const bool aligned = P.cache.page_size % 16 == 0;
-    if (P.group <= 8) return aligned ? launch_decode<T, DP, 1, true>(P, ctas, flags, stream) : launch_decode<T, DP, 1, false>(P, ctas, flags, stream);
-    return aligned ? launch_decode<T, DP, 2, true>(P, ctas, flags, stream) : launch_decode<T, DP, 2, false>(P, ctas, flags, stream);
+    if (P.group <= 8) return aligned ? launch_decode<T, DP, 1, true>(P, ctas, stream) : launch_decode<T, DP, 1, false>(P, ctas, stream);
+    return aligned ? launch_decode<T, DP, 2, true>(P, ctas, stream) : launch_decode<T, DP, 2, false>(P, ctas, stream);
 }
 
 }  // namespace
@@ -914,16 +914,16 @@ extern "C" int tpb200_paged_attention(const tpb200_paged_attention_args* a, tpb2
     const bool bf = a->cache.dtype == TPB200_BF16;
     const int D = P.cache.head_dim;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    const int done = D <= 64 ? (bf ? launch_decode<__nv_bfloat16, 64>(P, ctas, a->flags, s) : launch_decode<__half, 64>(P, ctas, a->flags, s))
-                   : D <= 128 ? (bf ? launch_decode<__nv_bfloat16, 128>(P, ctas, a->flags, s) : launch_decode<__half, 128>(P, ctas, a->flags, s))
-                              : (bf ? launch_decode<__nv_bfloat16, 256>(P, ctas, a->flags, s) : launch_decode<__half, 256>(P, ctas, a->flags, s));
+    const int done = D <= 64 ? (bf ? launch_decode<__nv_bfloat16, 64>(P, ctas, s) : launch_decode<__half, 64>(P, ctas, s))
+                   : D <= 128 ? (bf ? launch_decode<__nv_bfloat16, 128>(P, ctas, s) : launch_decode<__half, 128>(P, ctas, s))
+                              : (bf ? launch_decode<__nv_bfloat16, 256>(P, ctas, s) : launch_decode<__half, 256>(P, ctas, s));
     if (done != TPB200_OK) return done;
-    // Always dependent: its launch hides behind the first kernel, which it waits for.  Where items are few they have many parts each
+    // Its launch hides behind the first kernel, which it waits for.  Where items are few they have many parts each
     // (eight lanes of eight loads), else few (two of four, so that the whole launch is resident at once).
     const bool few = items * 8 < static_cast<long long>(ctas) * kWarps;
     const int quads = kJoinThreads / (few ? 8 : 2);
     cudaLaunchAttribute attr;
-    cudaLaunchConfig_t cfg = paged_config(static_cast<unsigned>(P.join_by_item ? items : ctas * kWarps - 1), kJoinThreads, 0, TPB200_FLAG_PDL, &attr, s);
+    cudaLaunchConfig_t cfg = paged_config(static_cast<unsigned>(P.join_by_item ? items : ctas * kWarps - 1), kJoinThreads, 0, &attr, s);
     cfg.gridDim.y = static_cast<unsigned>((P.rows * D / 4 + quads - 1) / quads);
     const auto join = few ? (bf ? paged_attention_join_kernel<__nv_bfloat16, 8, 8> : paged_attention_join_kernel<__half, 8, 8>)
                           : (bf ? paged_attention_join_kernel<__nv_bfloat16, 2, 4> : paged_attention_join_kernel<__half, 2, 4>);

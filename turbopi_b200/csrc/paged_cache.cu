@@ -254,7 +254,7 @@ extern "C" int tpb200_paged_append(const tpb200_paged_append_args* a, tpb200_str
     auto kernel = bf ? (V == 8 ? paged_append_kernel<__nv_bfloat16, 8> : paged_append_kernel<__nv_bfloat16, 4>)
                      : (V == 8 ? paged_append_kernel<__half, 8> : paged_append_kernel<__half, 4>);
     cudaLaunchAttribute attr;
-    const cudaLaunchConfig_t cfg = paged_config(blocks, kAppendThreads, 0, a->flags, &attr, reinterpret_cast<cudaStream_t>(stream));
+    const cudaLaunchConfig_t cfg = paged_config(blocks, kAppendThreads, 0, &attr, reinterpret_cast<cudaStream_t>(stream));
     return cudaLaunchKernelEx(&cfg, kernel, P) == cudaSuccess ? TPB200_OK : TPB200_ERR_CUDA;
 }
 
@@ -295,7 +295,7 @@ extern "C" int tpb200_copy_pages(void* pages, long long slab_bytes, int slabs, l
         P.units = parts * slabs * n;
         cudaLaunchAttribute attr;
         const cudaLaunchConfig_t cfg = paged_config(static_cast<unsigned>((P.units + kCopyWarps - 1) / kCopyWarps), kCopyWarps * 32, 0,
-                                                    flags, &attr, reinterpret_cast<cudaStream_t>(stream));
+                                                    &attr, reinterpret_cast<cudaStream_t>(stream));
         if (cudaLaunchKernelEx(&cfg, copy_pages_kernel, P) != cudaSuccess) return TPB200_ERR_CUDA;
     }
     return TPB200_OK;
