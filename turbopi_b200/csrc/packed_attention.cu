@@ -627,7 +627,7 @@ __global__ void __launch_bounds__(Layout<DP, R>::kThreads, Layout<DP, R>::kCtas)
         if (ok) {
             const float inv = mine > 0 ? 1.0f / l : 0.0f;
             // through shared memory where Q was (its products are done), each warp its own rows, so that whole rows leave together
-            constexpr int kCols = L::kOwn ? DP : DP / 2, kChunks = kCols / 8, kRowsIter = 32 / kChunks;
+            constexpr int kCols = L::kOwn ? DP : DP / 2, kChunks = kCols / 8, kRowsIter = 32 / kChunks, kSwap = 7;
             const int c_lo = L::kOwn ? 0 : x * kCols;
             uint8_t* stage = sQ + (x * 4 + quarter) * 32 * kCols * 2;
             const bool any_bad = mine > 0 && ctl->bad_any != 0;
@@ -662,18 +662,25 @@ __global__ void __launch_bounds__(Layout<DP, R>::kThreads, Layout<DP, R>::kCtas)
                             w[i] = Half16<T>::pack(__uint_as_float(o[n + 2 * i]) * inv, __uint_as_float(o[n + 2 * i + 1]) * inv);
                         }
                     }
-                    *reinterpret_cast<uint4*>(stage + lane * (kCols * 2) + ((((c + n) >> 3) ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                    *reinterpret_cast<uint4*>(stage + lane * (kCols * 2) + ((((c + n) >> 3) ^ (lane & kSwap)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
                 }
             }
             __syncwarp();
-            const int chunk = lane % kChunks;
+            // kRowsIter rows at a time: they are heads of one token, or whole tokens, so a lane's offset stays and the step's is uniform
+            const int chunk = lane % kChunks, lane_row = lane / kChunks, first_row = quarter * 32, mask = P.pack - 1;
+            uint16_t* to = P.out + static_cast<long long>(q0 + token0 + my_tile * tokens_tile + ((first_row + lane_row) >> P.pack_shift)) * P.o_stride[0] +
+                           ((head_group << P.pack_shift) + ((first_row + lane_row) & mask)) * P.o_stride[1] + c_lo + chunk * 8;
+            const int rows_left = ((nq - token0 - my_tile * tokens_tile) << P.pack_shift) - first_row;       // of this warp that exist
+            const uint8_t* from = stage + lane_row * (kCols * 2);
+            const bool column = c_lo + chunk * 8 < P.head_dim;
 #pragma unroll 4
             for (int r0 = 0; r0 < 32; r0 += kRowsIter) {
-                const int r = r0 + lane / kChunks, t = token0 + my_tile * tokens_tile + ((quarter * 32 + r) >> P.pack_shift);
-                if (t >= nq || c_lo + chunk * 8 >= P.head_dim) continue;
-                const int head = (head_group << P.pack_shift) + ((quarter * 32 + r) & (P.pack - 1));
-                const uint4 v = *reinterpret_cast<const uint4*>(stage + r * (kCols * 2) + ((chunk ^ (r & 7)) << 4));
-                *reinterpret_cast<uint4*>(P.out + static_cast<long long>(q0 + t) * P.o_stride[0] + head * P.o_stride[1] + c_lo + chunk * 8) = v;
+                const int r = r0 + lane_row;
+                const uint4 v = *reinterpret_cast<const uint4*>(from + r0 * (kCols * 2) + ((chunk ^ (r & kSwap)) << 4));
+                if (r < rows_left && column) {
+                    const int row0 = first_row + r0, token_step = (row0 >> P.pack_shift) - (first_row >> P.pack_shift), head_step = (row0 & mask) - (first_row & mask);
+                    *reinterpret_cast<uint4*>(to + token_step * P.o_stride[0] + head_step * P.o_stride[1]) = v;
+                }
             }
         }
         tc::fence_before_thread_sync();
@@ -778,8 +785,9 @@ extern "C" int tpb200_packed_attention(const tpb200_packed_attention_args* a, tp
         }
     }
     // Up to head size 128, two row tiles per CTA where sequences are long (each unit of K and V serves both), else one, and two CTAs on an
-    // SM: half the rows to fill up, and one's loads and output beside the other's products.  KSHORT
-    const bool two = DP <= 128 && static_cast<long long>(a->k_tokens) > 1024ll * a->seqs;
+    // SM: half the rows to fill up, and one's loads and output beside the other's products.  The border is where the two meet on average:
+    // 24 sequences of 100 / 8 of 1536, 16 heads of 64: 13.5 us with one, 18.1 with two / 91.6, 92.6; 16 heads of 128: 21.0, 25.2 / 129, 118.
+    const bool two = DP <= 128 && static_cast<long long>(a->k_tokens) > (DP == 64 ? 1000ll : 200ll) * a->seqs;
     // no more tiles than whole ones and a ragged one per sequence
     const long long tiles = static_cast<long long>(a->q_tokens) / (rows_tokens * (two ? 2 : 1)) + std::min(a->seqs, a->q_tokens);
     const long long blocks = tiles * P.head_groups;
