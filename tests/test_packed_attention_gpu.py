@@ -247,3 +247,64 @@ def test_rows_without_keys_beside_rows_with_keys(cuda_device):
         assert bool((out[:n * 40].view(40, n, 64)[:, :n - m] == 0).all())
     _check(out[:n], q, k, v, [n], [m], 0.125, True)
     _no_error()
+
+
+@pytest.mark.parametrize("seed", range(8))
+def test_drawn_batches(cuda_device, seed):
+    import random
+    rng = random.Random(seed)
+    hq, hk, D = rng.choice([(8, 1, 256), (32, 8, 128), (16, 4, 64), (16, 16, 64), (12, 4, 128), (16, 16, 72), (16, 2, 96), (4, 4, 256)])
+    lens = [rng.choice([0, 1, rng.randint(1, 130), rng.randint(1, 700)]) for _ in range(rng.randint(1, 20))]
+    klens = lens if rng.random() < 0.4 else [max(0, n + rng.choice([0, 5, 300, 2000, -50])) for n in lens]
+    _run(cuda_device, lens, klens, hq, hk, D, rng.choice([torch.bfloat16, torch.float16]), rng.random() < 0.7, seed=seed)
+
+
+def test_output_in_place_of_the_queries(cuda_device):
+    from turbopi_b200 import ops
+    for D in (64, 256):
+        q, k, v = _problem([300, 40, 129], [300, 40, 129], 4, 2, D, torch.bfloat16, cuda_device)
+        cu = _offsets([300, 40, 129], cuda_device)
+        want = ops.packed_attention(q, k, v, cu, 0.1)
+        assert ops.packed_attention(q, k, v, cu, 0.1, out=q) is q and torch.equal(q, want)
+
+
+def test_tokens_in_front_of_the_first_sequence_are_left_alone(cuda_device):
+    from turbopi_b200 import ops
+    q, k, v = _problem([50, 200], [50, 200], 2, 1, 128, torch.float16, cuda_device)
+    out = torch.full_like(q, 6.0)
+    ops.packed_attention(q, k, v, torch.tensor([50, 250], dtype=torch.int32, device=cuda_device), 0.1, out=out)
+    assert bool((out[:50] == 6).all())
+    _check(out[50:], q[50:], k[50:], v[50:], [200], [200], 0.1, True)
+
+
+def test_launches_behind_copies_fills_and_another_stream(cuda_device):
+    """These launches start while what is before them drains: a host copy, a fill, a wait for another stream, captured too."""
+    from turbopi_b200 import ops
+    lens = [90, 33]
+    q, k, v = _problem(lens, lens, 4, 1, 64, torch.bfloat16, cuda_device)
+    want = ops.packed_attention(q, k, v, _offsets(lens, cuda_device), 0.125)
+    host = q.cpu().pin_memory()
+    side = torch.cuda.Stream()
+    q2, k2, cu = torch.zeros_like(q), torch.empty_like(k), _offsets(lens, cuda_device)
+    torch.cuda.synchronize()
+
+    def chain(out):
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            k2.copy_(k)
+        q2.copy_(host, non_blocking=True)
+        out.fill_(3)
+        torch.cuda.current_stream().wait_stream(side)
+        ops.packed_attention(q2, k2, v, cu, 0.125, out=out)
+        q2.zero_()
+        k2.zero_()
+    for _ in range(50):
+        out = torch.empty_like(q)
+        chain(out)
+        assert torch.equal(out, want)
+    graph, out = torch.cuda.CUDAGraph(), torch.empty_like(q)
+    with torch.cuda.graph(graph):
+        chain(out)
+    for _ in range(20):
+        graph.replay()
+        assert torch.equal(out, want)

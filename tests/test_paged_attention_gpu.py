@@ -207,3 +207,46 @@ def test_what_the_table_must_not_hold_is_reported(cuda_device):
     n[1] = -3                                                    # no keys
     assert bool((ops.paged_attention(q, k, v, table, n, 0.1)[1] == 0).all())
     assert lib.tpb200_device_error(1) == 0
+
+
+def test_more_sequences_than_lengths_are_staged(cuda_device):
+    """1500 sequences: their lengths are read where they lie."""
+    from turbopi_b200 import ops
+    lens = [(i * 7) % 40 for i in range(1500)]
+    q, k, v, table, lengths, rows = _problem(lens, 4, 2, 64, 16, torch.float16, cuda_device, seed=9, poison=False)
+    out = ops.paged_attention(q, k, v, table, lengths, 0.125)
+    for i in list(range(0, 1500, 37)) + [1499]:
+        want, allow = attend(q[i:i + 1], gather(k, rows[i], lens[i]), gather(v, rows[i], lens[i]), 0.125)
+        check(out[i:i + 1], want, allow)
+    _no_error()
+
+
+@pytest.mark.parametrize("hq", [1, 8, 9, 16])
+@pytest.mark.parametrize("n", [1, 15, 16, 31, 32, 33, 47, 48, 49, 63, 64, 65, 80, 129, 192, 193, 1000])
+def test_lines_of_few_slots(cuda_device, n, hq):
+    """Lines too short to give every warp a slot, CTAs inside one item, items that end where a CTA does."""
+    from turbopi_b200 import ops
+    for D in (64, 256):
+        q, k, v, table, lengths, rows = _problem([n], hq, 1, D, 16, torch.bfloat16, cuda_device, seed=n)
+        _check(ops.paged_attention(q, k, v, table, lengths, D ** -0.5), q, k, v, rows, [n], D ** -0.5)
+    _no_error()
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_drawn_lengths(cuda_device, seed):
+    import random
+
+    from turbopi_b200 import ops
+    rng = random.Random(seed)
+    hq, hk, D = rng.choice([(8, 1, 256), (8, 2, 128), (16, 16, 64), (12, 4, 128), (16, 2, 96)])
+    lens = [rng.choice([0, 1, rng.randint(1, 60), rng.randint(1, 700), rng.randint(1, 4000)]) for _ in range(rng.randint(1, 60))]
+    q, k, v, table, lengths, rows = _problem(lens, hq, hk, D, rng.choice([16, 24, 64]), torch.bfloat16, cuda_device, seed=seed, poison=False)
+    _check(ops.paged_attention(q, k, v, table, lengths, D ** -0.5), q, k, v, rows, lens, D ** -0.5)
+    _no_error()
+
+
+def test_output_in_place_of_the_queries(cuda_device):
+    from turbopi_b200 import ops
+    q, k, v, table, lengths, rows = _problem([3000, 5, 700, 64], 16, 1, 128, 16, torch.bfloat16, cuda_device)
+    want = ops.paged_attention(q, k, v, table, lengths, 0.1)
+    assert ops.paged_attention(q, k, v, table, lengths, 0.1, out=q) is q and torch.equal(q, want)

@@ -166,3 +166,29 @@ def test_copies_beyond_32_bits(cuda_device):
     pages[:, 19999].normal_()
     ops.copy_pages(pages, [5, 19999], [19998, 7])
     assert torch.equal(pages[:, 19998], pages[:, 5]) and torch.equal(pages[:, 7], pages[:, 19999])
+
+
+def test_captured_copies(cuda_device):
+    """The pairs are part of the launch: a graph moves the same pages whatever the lists hold later."""
+    from turbopi_b200 import ops
+    pages = torch.randn(2, 1200, 4, 1, 8, device=cuda_device).to(torch.float16)
+    src, dst = list(range(500)), list(range(600, 1100))          # more than one launch's worth
+    ops.copy_pages(pages, [0], [1199])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.copy_pages(pages, src, dst)
+    src[:], dst[:] = dst, src
+    pages[:, :600].normal_()
+    want = pages.clone()
+    want[:, 600:1100] = pages[:, :500]
+    graph.replay()
+    assert torch.equal(pages, want)
+
+
+def test_ids_that_would_wrap_are_refused(cuda_device):
+    from turbopi_b200 import ops
+    from turbopi_b200._lib import TurboPiError
+    pages = torch.zeros(4, 2, 1, 8, device=cuda_device)
+    for bad in ([2 ** 32], [2 ** 70], [1.0], [True], [None]):
+        with pytest.raises(TurboPiError):
+            ops.copy_pages(pages, bad, [2])

@@ -106,3 +106,42 @@ def test_packed_attention_refuses_cpu_tensors():
     q = torch.zeros(4, 2, 64, dtype=torch.bfloat16)
     with pytest.raises(TurboPiError, match="CUDA"):
         ops.packed_attention(q, q, q, torch.zeros(2, dtype=torch.int32), 1.0)
+
+
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), float("-inf")])
+def test_scales_that_are_no_numbers(scale):
+    lib = _lib.load()
+    packed = _lib.PackedAttentionArgs(q=64, k=64, v=64, out=64, q_stride=Two(1024, 256), k_stride=Two(512, 256), v_stride=Two(512, 256),
+                                      o_stride=Two(1024, 256), cu=64, seqs=1, q_tokens=9, k_tokens=9, q_heads=4, kv_heads=2, head_dim=256,
+                                      dtype=_lib.BF16, scale=scale, causal=1)
+    paged = _lib.PagedAttentionArgs(cache=_cache(), q=64, out=64, q_stride=Two(2048, 256), o_stride=Two(2048, 256), q_heads=8, scale=scale,
+                                    workspace=256, workspace_bytes=1 << 30)
+    assert lib.tpb200_packed_attention(packed, None) == SHAPE and lib.tpb200_paged_attention(paged, None) == SHAPE
+
+
+def test_outputs_whose_rows_overlap():
+    """An expanded output would be written by several heads or sequences at once."""
+    lib = _lib.load()
+    base = dict(cache=_cache(), q=64, out=64, q_stride=Two(2048, 256), o_stride=Two(2048, 256), q_heads=8, scale=1.0, workspace=256,
+                workspace_bytes=1 << 30)
+    for o_stride in (Two(0, 256), Two(2048, 0), Two(2048, 128)):
+        assert lib.tpb200_paged_attention(_lib.PagedAttentionArgs(**{**base, "o_stride": o_stride}), None) == SHAPE
+
+
+def test_capacities_whose_plan_would_not_fit():
+    """The plan counts in 32 bits, for sequences as long as the table; with larger slots (smaller heads) more of them fit."""
+    lib = _lib.load()
+    wide = dict(page_size=1024, table_width=1024, table_stride=1024, seqs=40000)
+    args = dict(q=64, out=64, q_stride=Two(2048, 256), o_stride=Two(2048, 256), q_heads=8, scale=1.0, workspace=256, workspace_bytes=1 << 30)
+    assert lib.tpb200_paged_attention(_lib.PagedAttentionArgs(cache=_cache(page_stride=1024 * 256, **wide), **args), None) == SHAPE
+
+
+def test_structures_follow_the_header_field_by_field():
+    import re
+    from pathlib import Path
+    header = (Path(__file__).resolve().parent.parent / "include" / "turbopi_b200.h").read_text()
+    for name, mirror in {"tpb200_paged_cache": _lib.PagedCacheView, "tpb200_paged_attention_args": _lib.PagedAttentionArgs,
+                         "tpb200_paged_append_args": _lib.PagedAppendArgs, "tpb200_packed_attention_args": _lib.PackedAttentionArgs}.items():
+        body = re.sub(r"/\*.*?\*/", "", re.search(r"typedef struct\s*\{([^}]*)\}\s*" + name + r"\s*;", header, re.S).group(1), flags=re.S)
+        fields = [part.strip().split()[-1].split("[")[0].lstrip("*") for d in body.split(";") if d.strip() for part in d.split(",")]
+        assert fields == [f[0] for f in mirror._fields_], name

@@ -26,6 +26,7 @@
 // taken out and added to the rows that do see them at the end.
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <type_traits>
 
 #include "paged.cuh"
@@ -167,6 +168,17 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity) {
     return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, kWait));
+}
+
+// Warps 2 and 3 meet, and learn whether both are fine
+__device__ __forceinline__ bool meet_and(bool ok) {
+    uint32_t all;
+    asm volatile(
+        "{\n .reg .pred p, q;\n setp.ne.u32 q, %1, 0;\n barrier.cta.red.and.pred p, 2, 64, q;\n selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(all)
+        : "r"(static_cast<uint32_t>(ok))
+        : "memory");
+    return all != 0;
 }
 
 // The keys a query row sees: [0, limit)
@@ -469,20 +481,20 @@ __global__ void __launch_bounds__(Layout<DP, R>::kThreads, Layout<DP, R>::kCtas)
                         for (int b = 0; b < L::kUnitBlocks; ++b) {
                             uint4* at = reinterpret_cast<uint4*>(ring + (u0 + h) % L::kUnits * L::kUnitBytes + b * kBlockBytes + r * 128);
                             uint4 v[8];
-                            uint32_t sum = 0;
+                            uint32_t sum[4] = {0, 0, 0, 0};          // four chains: the check is in the way of short sequences
 #pragma unroll
                             for (int c = 0; c < 8; ++c) v[c] = at[c ^ (r & 7)];
 #pragma unroll
                             for (int c = 0; c < 8; ++c) {
-                                sum = Half16<T>::add_zeros(v[c].x, sum);
-                                sum = Half16<T>::add_zeros(v[c].y, sum);
-                                sum = Half16<T>::add_zeros(v[c].z, sum);
-                                sum = Half16<T>::add_zeros(v[c].w, sum);
+                                sum[0] = Half16<T>::add_zeros(v[c].x, sum[0]);
+                                sum[1] = Half16<T>::add_zeros(v[c].y, sum[1]);
+                                sum[2] = Half16<T>::add_zeros(v[c].z, sum[2]);
+                                sum[3] = Half16<T>::add_zeros(v[c].w, sum[3]);
                             }
                             if (!there) {
 #pragma unroll
                                 for (int c = 0; c < 8; ++c) at[c] = make_uint4(0, 0, 0, 0);
-                            } else if ((sum & 0x7fff7fffu) != 0) {
+                            } else if (((sum[0] | sum[1] | sum[2] | sum[3]) & 0x7fff7fffu) != 0) {
                                 bad = true;
                                 uint16_t* x = reinterpret_cast<uint16_t*>(at);
                                 constexpr uint16_t kExp = std::is_same<T, __nv_bfloat16>::value ? 0x7f80 : 0x7c00;
@@ -499,8 +511,7 @@ __global__ void __launch_bounds__(Layout<DP, R>::kThreads, Layout<DP, R>::kCtas)
                     }
                 }
                 fence_proxy_async_smem();
-                asm volatile("bar.sync 2, 64;" ::: "memory");
-                if (!ok) {               // the units stay empty: the products' wait runs out too
+                if (!meet_and(ok)) {     // both warps leave; the units stay empty, and the products' wait runs out too
                     if (lane == 0) {
                         record_error(kErrPackedBarrierTimeout);
                         ctl->failed = 1;
@@ -742,15 +753,13 @@ extern "C" int tpb200_packed_attention(const tpb200_packed_attention_args* a, tp
     TPB_REQUIRE(a->q && a->out && a->cu && (a->k_tokens == 0 || (a->k && a->v)), TPB200_ERR_NULL);
     TPB_REQUIRE(tpb_aligned16(a->q) && tpb_aligned16(a->k) && tpb_aligned16(a->v) && tpb_aligned16(a->out), TPB200_ERR_ALIGN);
     PackedParams P = {};
+    TPB_REQUIRE(std::isfinite(a->scale), TPB200_ERR_SHAPE);
     for (int i = 0; i < 2; ++i) {
-        TPB_REQUIRE(a->q_stride[i] % 8 == 0 && a->k_stride[i] % 8 == 0 && a->v_stride[i] % 8 == 0 && a->o_stride[i] % 8 == 0,
-                    TPB200_ERR_ALIGN);
         const int qn = i == 0 ? a->q_tokens : a->q_heads, kn = i == 0 ? a->k_tokens : a->kv_heads;
-        TPB_REQUIRE((qn <= 1 || (a->q_stride[i] >= a->head_dim && a->o_stride[i] >= a->head_dim)) &&
-                        (kn <= 1 || (a->k_stride[i] >= a->head_dim && a->v_stride[i] >= a->head_dim)),
-                    TPB200_ERR_SHAPE);
-        P.o_stride[i] = a->o_stride[i];
-        P.v_stride[i] = a->v_stride[i];
+        for (const long long st : {a->q_stride[i], a->o_stride[i]}) TPB_REQUIRE(paged_stride(st, qn, a->head_dim) == TPB200_OK, paged_stride(st, qn, a->head_dim));
+        for (const long long st : {a->k_stride[i], a->v_stride[i]}) TPB_REQUIRE(paged_stride(st, kn, a->head_dim) == TPB200_OK, paged_stride(st, kn, a->head_dim));
+        P.o_stride[i] = qn > 1 ? a->o_stride[i] : 0;
+        P.v_stride[i] = kn > 1 ? a->v_stride[i] : 0;
     }
     const int group = a->q_heads / a->kv_heads;
     int pack = 1;

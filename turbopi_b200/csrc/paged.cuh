@@ -57,6 +57,13 @@ struct PagedView {
     }
 };
 
+// A stride between `n` rows of head_dim values: of one row it does not matter, else the rows lie apart, whole 16-byte groups
+static inline int paged_stride(long long stride, int n, int head_dim) {
+    TPB_REQUIRE(n <= 1 || stride % 8 == 0, TPB200_ERR_ALIGN);
+    TPB_REQUIRE(stride >= 0 && (n <= 1 || stride >= head_dim), TPB200_ERR_SHAPE);
+    return TPB200_OK;
+}
+
 static inline int paged_view(const tpb200_paged_cache& c, PagedView* v) {
     TPB_REQUIRE(c.seqs >= 0 && c.num_pages >= 1 && c.page_size >= 1 && c.kv_heads >= 1 && c.table_width >= 1, TPB200_ERR_SHAPE);
     TPB_REQUIRE(c.head_dim >= 8 && c.head_dim <= 256 && c.head_dim % 8 == 0, TPB200_ERR_SHAPE);
@@ -65,15 +72,22 @@ static inline int paged_view(const tpb200_paged_cache& c, PagedView* v) {
     TPB_REQUIRE(c.k_pages && c.v_pages, TPB200_ERR_NULL);
     TPB_REQUIRE(c.seqs == 0 || (c.table && c.lengths), TPB200_ERR_NULL);
     TPB_REQUIRE(tpb_aligned16(c.k_pages) && tpb_aligned16(c.v_pages), TPB200_ERR_ALIGN);
-    TPB_REQUIRE(c.page_stride % 8 == 0 && c.row_stride % 8 == 0 && c.head_stride % 8 == 0, TPB200_ERR_ALIGN);
-    TPB_REQUIRE(c.page_stride >= 0 && c.row_stride >= 0 && c.head_stride >= 0 && c.table_stride >= 0, TPB200_ERR_SHAPE);
-    *v = {c.k_pages, c.v_pages, c.page_stride, c.row_stride, c.head_stride, c.table, c.lengths, c.table_stride,
-          c.num_pages, c.page_size, c.kv_heads, c.head_dim, c.table_width, c.seqs};
+    TPB_REQUIRE(c.seqs <= 1 || c.table_stride >= 0, TPB200_ERR_SHAPE);
+    const long long strides[3] = {c.page_stride, c.row_stride, c.head_stride};
+    const int sizes[3] = {c.num_pages, c.page_size, c.kv_heads};
+    for (int i = 0; i < 3; ++i) {
+        const int st = paged_stride(strides[i], sizes[i], c.head_dim);
+        if (st != TPB200_OK) return st;
+    }
+    auto used = [](long long stride, int n) { return n > 1 ? stride : 0; };
+    *v = {c.k_pages, c.v_pages, used(c.page_stride, c.num_pages), used(c.row_stride, c.page_size), used(c.head_stride, c.kv_heads), c.table,
+          c.lengths, used(c.table_stride, c.seqs), c.num_pages, c.page_size, c.kv_heads, c.head_dim, c.table_width, c.seqs};
     return TPB200_OK;
 }
 
 // These kernels wait for the launch before them ahead of everything they read or write, so they are always launched as dependents
-// (TPB200_FLAG_PDL or not): their CTAs start while it drains.
+// (TPB200_FLAG_PDL or not): their CTAs start while it drains.  They let the next launch in behind that wait, not before it: what was
+// enqueued ahead of one of them is complete when a launch behind it starts, as behind any launch without the flag.
 static inline cudaLaunchConfig_t paged_config(unsigned blocks, int threads, size_t smem, cudaLaunchAttribute* attr, cudaStream_t stream) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(blocks, 1, 1);

@@ -19,6 +19,7 @@
 //     rows or columns of queries; this needs a seventh of the instruction slots that an SM's share of the stream leaves (16 KB per 700 cycles).
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <type_traits>
 
 #include "paged.cuh"
@@ -188,8 +189,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attention_kernel(c
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int heads = P.cache.kv_heads * P.tiles;
     const int D = P.cache.head_dim;
-    pdl_launch_dependents();
     pdl_wait_prior_grids();
+    pdl_launch_dependents();
 
     // ------------------------------------------------ this warp's piece of the line
     // Every warp for itself, without a barrier: slots and units before each lane's run of sequences, then the places where its piece
@@ -740,8 +741,8 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attention_join_kernel(cons
     constexpr int kQuads = kJoinThreads / kLanes;
     __shared__ float4 sums[kLanes][kQuads];
     __shared__ float2 mls[kLanes][kQuads];
-    pdl_launch_dependents();
     pdl_wait_prior_grids();
+    pdl_launch_dependents();
     const int4 join = P.joins[blockIdx.x];
     if (join.x < 0) return;
     const int heads = P.cache.kv_heads * P.tiles, D = P.cache.head_dim;
@@ -885,17 +886,23 @@ extern "C" int tpb200_paged_attention(const tpb200_paged_attention_args* a, tpb2
     TPB_REQUIRE((a->flags & ~TPB200_FLAG_PDL) == 0, TPB200_ERR_ENUM);
     TPB_REQUIRE(a->q_heads >= 1 && a->q_heads % P.cache.kv_heads == 0, TPB200_ERR_SHAPE);
     TPB_REQUIRE(tpb_aligned16(a->q) && tpb_aligned16(a->out), TPB200_ERR_ALIGN);
+    TPB_REQUIRE(std::isfinite(a->scale), TPB200_ERR_SHAPE);
     for (int i = 0; i < 2; ++i) {
-        TPB_REQUIRE(a->q_stride[i] % 8 == 0 && a->o_stride[i] % 8 == 0, TPB200_ERR_ALIGN);
-        P.q_stride[i] = a->q_stride[i];
-        P.o_stride[i] = a->o_stride[i];
+        const int n = i == 0 ? P.cache.seqs : a->q_heads;
+        for (const long long stride : {a->q_stride[i], a->o_stride[i]}) {
+            const int fine = paged_stride(stride, n, P.cache.head_dim);
+            if (fine != TPB200_OK) return fine;
+        }
+        P.q_stride[i] = n > 1 ? a->q_stride[i] : 0;
+        P.o_stride[i] = n > 1 ? a->o_stride[i] : 0;
     }
     if (P.cache.seqs == 0) return TPB200_OK;
     P.group = a->q_heads / P.cache.kv_heads;
     P.tiles = (P.group + decode_rows(P.group) - 1) / decode_rows(P.group);
     P.rows = std::min(P.group, decode_rows(P.group));
-    // the line's length must fit an int, with 16 keys to a slot at the least
-    const long long most = (static_cast<long long>(P.cache.page_size) * P.cache.table_width + 15) / 16;
+    // the line's length must fit an int, were every sequence as long as the table
+    const int slot_keys = P.cache.head_dim <= 64 ? 64 : (P.cache.head_dim <= 128 ? 32 : 16);
+    const long long most = (static_cast<long long>(P.cache.page_size) * P.cache.table_width + slot_keys - 1) / slot_keys;
     const long long items = static_cast<long long>(P.cache.kv_heads) * P.tiles * P.cache.seqs;
     TPB_REQUIRE(items <= 0x7fffffff && (most * kSlotUnits + kItemUnits) * items <= 0x7fffffff, TPB200_ERR_SHAPE);
     const int ctas = decode_ctas();

@@ -78,8 +78,8 @@ __global__ void __launch_bounds__(kAppendThreads, 3) paged_append_kernel(const _
     __shared__ int seq[kMaxTokensPerBlock];
     __shared__ int position[kMaxTokensPerBlock];
     __shared__ long long row_at[kMaxTokensPerBlock];     // element offset of the token's row in the pages, -1: not written
-    pdl_launch_dependents();
     pdl_wait_prior_grids();
+    pdl_launch_dependents();
     const int t0 = blockIdx.x * P.tokens_per_block;
     const int count = min(P.tokens_per_block, P.tokens - t0);
     const int per_token = P.units_q + P.units_k + P.units_v;
@@ -172,8 +172,8 @@ struct CopyParams {
 };
 
 __global__ void __launch_bounds__(kCopyWarps * 32) copy_pages_kernel(const __grid_constant__ CopyParams P) {
-    pdl_launch_dependents();
     pdl_wait_prior_grids();
+    pdl_launch_dependents();
     const long long unit = static_cast<long long>(blockIdx.x) * kCopyWarps + (threadIdx.x >> 5);
     if (unit >= P.units) return;
     const int per_pair = P.slabs * P.parts;
@@ -223,8 +223,11 @@ extern "C" int tpb200_paged_append(const tpb200_paged_append_args* a, tpb200_str
     }
     TPB_REQUIRE(tpb_aligned16(a->k) && tpb_aligned16(a->v) && tpb_aligned16(a->q) && tpb_aligned16(a->q_out), TPB200_ERR_ALIGN);
     for (int i = 0; i < 2; ++i) {
-        TPB_REQUIRE(a->k_stride[i] % 8 == 0 && a->v_stride[i] % 8 == 0 && a->q_stride[i] % 8 == 0 && a->o_stride[i] % 8 == 0,
-                    TPB200_ERR_ALIGN);
+        const int n = i == 0 ? a->tokens : P.cache.kv_heads, qn = a->q == nullptr ? 0 : (i == 0 ? a->tokens : a->q_heads);
+        for (const int st : {paged_stride(a->k_stride[i], n, P.cache.head_dim), paged_stride(a->v_stride[i], n, P.cache.head_dim),
+                             paged_stride(a->q_stride[i], qn, P.cache.head_dim), paged_stride(a->o_stride[i], qn, P.cache.head_dim)}) {
+            if (st != TPB200_OK) return st;
+        }
         P.k_stride[i] = a->k_stride[i];
         P.v_stride[i] = a->v_stride[i];
         P.q_stride[i] = a->q_stride[i];

@@ -872,11 +872,14 @@ def copy_pages(pages, src, dst):
             if x.is_cuda or x.is_floating_point() or x.dim() != 1:
                 raise TurboPiError("copy_pages: src and dst are sequences of ints or 1-D integer tensors on the CPU")
             x = x.tolist()
-        lists.append(x)
+        lists.append(list(x))
     n = len(lists[0])
     if len(lists[1]) != n:
         raise TurboPiError("copy_pages: src and dst differ in length")
     P = pages.shape[-4]
+    for x in lists:
+        if any(type(i) is bool or not isinstance(i, int) or not 0 <= i < P for i in x):
+            raise TurboPiError(f"copy_pages: a page id outside the supported range [0, {P}), or no int")
     slab = pages.stride(-4) * P * pages.element_size()
     if n == 0 or pages.numel() == 0:
         if n:
