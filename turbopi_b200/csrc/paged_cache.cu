@@ -3,7 +3,8 @@
 //   append   the new tokens' keys and values go to the rows the page table names, keys (and the queries beside them) rotated to
 //            their positions on the way: one launch where the parts would be two rotations, a gather of row addresses and two
 //            scattered writes.  Bound by HBM for prompts; for a decode step by the chain offsets -> length -> page id -> store.
-//   copy     pages of every layer, keys and values, moved for a fork or a compaction.  Bound by HBM.
+//   copy     pages of every layer, keys and values, moved for a fork or a compaction.  Bound by HBM: 900 pages of 16 x 256 in 18 layers
+//            (531 MB read and written) take 87 us = 6.1 TB/s = 0.93 of the measured copy rate.
 #include <stdlib.h>
 
 #include <algorithm>
@@ -14,8 +15,8 @@ namespace tpb {
 namespace {
 
 constexpr int kAppendThreads = 256;
-constexpr int kAppendLoads = 4;          // tokens whose unit a thread has in flight: 32 bytes each
-constexpr int kMaxTokensPerBlock = 16;
+constexpr int kAppendLoads = 2;          // tokens whose unit a thread has in flight: 32 bytes each, 80 KB on an SM with five blocks
+constexpr int kMaxTokensPerBlock = 4;
 
 struct AppendParams {
     PagedView cache;
@@ -72,9 +73,11 @@ __device__ __forceinline__ void load_table(const void* p, int dtype, size_t at, 
 
 // A unit is V values of a row and the V values half a row further on (rotated, or a plain copy of both), so that a rotation
 // needs one thread.  V = 8 where half a row is a multiple of 8, else 4.  A thread keeps its unit (which tensor, head and columns) for all
-// tokens of the block: one division per thread and not per token (77 -> 54 us for the prompts of six sequences, 10.5 k tokens, 4.9 TB/s).
+// tokens of the block: one division per thread and not per token: 77 -> 54 us for the prompts of six sequences (10.5 k tokens, 32 on 8 heads of 128,
+// 265 MB), and 48 us = 5.5 TB/s = 0.85 of the measured copy rate with five blocks on an SM that take four tokens each (three blocks of
+// eight: 53; sixteen tokens: 60; six blocks, which spill: 61).
 template <typename T, int V>
-__global__ void __launch_bounds__(kAppendThreads, 3) paged_append_kernel(const __grid_constant__ AppendParams P) {
+__global__ void __launch_bounds__(kAppendThreads, 5) paged_append_kernel(const __grid_constant__ AppendParams P) {
     __shared__ int seq[kMaxTokensPerBlock];
     __shared__ int position[kMaxTokensPerBlock];
     __shared__ long long row_at[kMaxTokensPerBlock];     // element offset of the token's row in the pages, -1: not written
@@ -250,8 +253,8 @@ extern "C" int tpb200_paged_append(const tpb200_paged_append_args* a, tpb200_str
     TPB_REQUIRE(units <= (1 << 24), TPB200_ERR_SHAPE);
     P.units_q = static_cast<int>(per_head * P.q_heads);
     P.units_k = P.units_v = static_cast<int>(per_head * P.cache.kv_heads);
-    // eight tokens share a block's look-up, fewer where that would leave SMs without a block
-    P.tokens_per_block = std::max(1, std::min(8, a->tokens / 444));
+    // four tokens share a block's look-up, fewer where that would leave SMs without a block
+    P.tokens_per_block = std::max(1, std::min(kMaxTokensPerBlock, a->tokens / 444));
     const unsigned blocks = static_cast<unsigned>((a->tokens + P.tokens_per_block - 1) / P.tokens_per_block);
     const bool bf = a->cache.dtype == TPB200_BF16;
     auto kernel = bf ? (V == 8 ? paged_append_kernel<__nv_bfloat16, 8> : paged_append_kernel<__nv_bfloat16, 4>)
