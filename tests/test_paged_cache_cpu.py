@@ -146,3 +146,45 @@ def test_batches_are_refused_after_pages_have_moved(cpu_copies):
     again = cache.extend([b], [0], out=batch)
     assert again is batch and batch.table[0, 0] == 0
     cache._current(batch)
+
+
+@pytest.mark.parametrize("what", ["freed", "truncated", "copied"])
+def test_a_batch_whose_pages_may_be_others_is_refused(cpu_copies, monkeypatch, what):
+    monkeypatch.setattr(ops, "paged_append", lambda *a, **k: "appended")
+    monkeypatch.setattr(ops, "paged_attention", lambda *a, **k: "attended")
+    cache = _cache()
+    a, other = cache.add(), cache.add()
+    batch, kv = cache.extend([a, other], [5, 2]), torch.zeros(7, 1, 8)
+    alone = cache.extend([other], [1])
+    # what leaves the pages of the batch with their sequences leaves the batch as it is
+    cache.extend([a], [1])
+    fork = cache.fork(a)
+    assert cache.append(0, batch, kv, kv) == "appended" and cache.attention(0, batch, kv, 1.0) == "attended"
+    if what == "freed":
+        cache.free(a)
+    elif what == "truncated":
+        cache.truncate(a, 3)
+    else:
+        cache.extend([a], [1])
+    for call in (lambda: cache.append(0, batch, kv, kv), lambda: cache.attention(0, batch, kv, 1.0)):
+        with pytest.raises(TurboPiError, match=what):
+            call()
+    assert cache.attention(0, alone, kv, 1.0) == "attended"
+    cache.extend([fork, other], [1, 1], out=batch)           # written anew, it holds again, and for these sequences
+    assert cache.append(0, batch, kv[:2], kv[:2]) == "appended"
+    if what != "freed":
+        cache.free(a)
+        assert cache.attention(0, batch, kv, 1.0) == "attended"
+    cache.free(fork)
+    with pytest.raises(TurboPiError, match="freed"):
+        cache.attention(0, batch, kv, 1.0)
+
+
+def test_a_batch_of_another_cache_is_refused(cpu_copies):
+    one, two = _cache(), _cache()
+    batch, seq = one.extend([one.add()], [1]), two.add()
+    kv = torch.zeros(1, 1, 8)
+    for call in (lambda: two.append(0, batch, kv, kv), lambda: two.attention(0, batch, kv, 1.0), lambda: two.extend([seq], [1], out=batch)):
+        with pytest.raises(TurboPiError, match="another cache"):
+            call()
+    assert two.length(seq) == 0 and two.free_pages == two.num_pages

@@ -13,13 +13,29 @@
 // 2 and 3 look tiles with masked pairs over, two groups of four warps do the softmax, a thread per row, with registers moved over to
 // them from the others (setmaxnreg).
 // The products are a line of events e; event e computes S into tensor-memory buffer e & 1, group e & 1 turns it into P in the same
-// columns, the product with V reads P from there:
+// columns, the product with V reads P from there, the first half of the keys while the weights of the second are computed:
 //   head sizes up to 128  two tiles of 128 rows per CTA, one per group: event e is key tile e / 2 of row tile e & 1; each unit of K
-//                         and V is read by both, which halves what comes through L2 (a row tile of its own would need 64 KB per
-//                         1024 cycles of products, twice what an SM gets);
+//                         and V is read by both, which halves what comes through L2 (a row tile of its own needs 64 KB per
+//                         1024 cycles of products, more than an SM gets);
+//                         short sequences: one row tile and one group (256 threads), two CTAs on an SM;
 //   above                 one row tile (its O alone is 256 columns), the groups take alternate key tiles and hand m on through
 //                         shared memory.
 // While one group works the other's products run.
+//
+// What bounds it, measured on one B200 (calls in a CUDA graph):
+//   one sequence of 8191 tokens, causal, 8 on 1 heads of 256: 203 us = 1.35 PFLOP/s, 0.82 of the measured bf16 rate; the tensor pipe works in
+//   68 % of the cycles.  When all of it took 209 us, the line of products without loads and without the arithmetic of the softmax took
+//   203: what is missing goes into the hand-overs from product to softmax and back.
+//   4 sequences, 24.6 k tokens, causal, 32 on 8 heads of 128: 1.6 ms = 1.07 PFLOP/s, 0.65.  The exponentials of a 128 x 128 tile take the
+//   special-function unit 1024 cycles (16 each), and its products the tensor pipe as long; both groups at once finish a tile
+//   every 1000-1150.  About 6 us of each CTA's 70 pass in its first loads and its output.
+//   One sequence of 200 tokens, 8 on 1 heads of 256: 10.9 us: look-up 0.6, tensor memory and barriers 0.3, loads 1-2, 1.1 of softmax per tile,
+//   1.4 for the output, one after the other.
+// Issuing a 128 x 128 x 16 product takes the issuing warp about the 64 cycles it runs, so none queue up and a wait between two of them is
+// lost time: barriers are tested while products ahead of them run (209 -> 201 us, 1.72 -> 1.71 ms).  Tried without gain: a quarter of the
+// exponentials as polynomials on the FMA pipes (1.61 ms without, 1.71 with); four groups, two threads per row (1.75 -> 1.94 ms;
+// sequences of 100 tokens gain 7 %, those of 1 to 1200 lose 6 %); pairs of CTAs on one product (cta_group::2, M = 256: 2.47 ms, the single
+// sequence 250 us, each hand-over crosses the cluster).
 //
 // What may stand in masked places does not matter: scores are selected, not biased.  Rows of V behind a sequence's end are zeroed in
 // shared memory, and in tiles that hold masked pairs V is searched for infinities and NaN (weight 0 times those would be NaN): they are

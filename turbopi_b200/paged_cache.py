@@ -16,9 +16,12 @@ same pages); the bytes are moved by `ops.copy_pages`, written by `ops.paged_appe
         q = cache.append(l, batch, k, v, q=q, cos=cos, sin=sin)
         out = cache.attention(l, batch, q, scale)
 
-Calls that move or write pages enqueue on the current stream; use one stream per cache, or order them yourself.
+A batch holds for its cache until one of its sequences is freed, truncated or had a shared page copied, or pages have moved (compact);
+then `append` and `attention` refuse it, since its table may name pages of others.  Calls that move or write pages enqueue on the
+current stream; use one stream per cache, or order them yourself.
 """
 import heapq
+import weakref
 
 import torch
 
@@ -30,9 +33,9 @@ class PagedBatch:
     """What the kernels read of some sequences: table int32 [S, max_pages], lengths int32 [S] (the new tokens among them) and cu int32
     [S + 1], the offsets of the new tokens; `tokens` is their number."""
 
-    def __init__(self, table, lengths, cu, tokens, moves):
+    def __init__(self, table, lengths, cu, tokens, cache):
         self.table, self.lengths, self.cu, self.tokens = table, lengths, cu, tokens
-        self._moves = moves                # page moves the cache had seen when the table was made
+        self._cache, self._seqs, self._stale = weakref.ref(cache), [], None       # _stale: why it no longer holds
 
 
 class PagedCache:
@@ -49,9 +52,8 @@ class PagedCache:
         self.pages = torch.zeros((layers, 2, num_pages, page_size, kv_heads, head_dim), dtype=dtype, device=self.device)
         self._free = list(range(num_pages))           # a heap
         self._refs = [0] * num_pages
-        self._seqs = {}                               # id -> [page ids, length]
+        self._seqs = {}                               # id -> [page ids, length, batches that name its pages]
         self._next = 0
-        self._moves = 0
 
     # ------------------------------------------------------------------ sequences
     def _get(self, seq):
@@ -63,7 +65,7 @@ class PagedCache:
     def add(self):
         """A new sequence without tokens; returns its id."""
         self._next += 1
-        self._seqs[self._next] = [[], 0]
+        self._seqs[self._next] = [[], 0, weakref.WeakSet()]
         return self._next
 
     def length(self, seq):
@@ -83,18 +85,20 @@ class PagedCache:
 
     def free(self, seq):
         """Gives the sequence up; pages that no other one shares are free again."""
-        for page in self._get(seq)[0]:
+        entry = self._get(seq)
+        for page in entry[0]:
             self._release(page)
+        self._outdate(entry, f"sequence {seq} was freed")
         del self._seqs[seq]
 
     def fork(self, seq):
         """A second sequence with the same tokens, on the same pages; returns its id.  Nothing is copied until one of them is extended
         within the page they share last."""
-        pages, length = self._get(seq)
+        pages, length, _ = self._get(seq)
         for page in pages:
             self._refs[page] += 1
         self._next += 1
-        self._seqs[self._next] = [list(pages), length]
+        self._seqs[self._next] = [list(pages), length, weakref.WeakSet()]
         return self._next
 
     def truncate(self, seq, length):
@@ -105,7 +109,15 @@ class PagedCache:
         keep = -(-length // self.page_size)
         for page in entry[0][keep:]:
             self._release(page)
+        if length < entry[1]:
+            self._outdate(entry, f"sequence {seq} was truncated")
         entry[0], entry[1] = entry[0][:keep], length
+
+    @staticmethod
+    def _outdate(entry, why):
+        for batch in entry[2]:
+            batch._stale = why
+        entry[2].clear()
 
     # ------------------------------------------------------------------ room for tokens
     def extend(self, seqs, new, out=None):
@@ -116,12 +128,12 @@ class PagedCache:
         seqs, new = list(seqs), [int(n) for n in new]
         if len(seqs) != len(new) or len(set(seqs)) != len(seqs) or any(n < 0 for n in new):
             raise TurboPiError("PagedCache: extend takes different sequences and a number of new tokens >= 0 for each")
-        if out is not None and out.lengths.shape[0] != len(seqs):
-            raise TurboPiError("PagedCache: `out` is a batch of another number of sequences")
+        if out is not None and (out._cache() is not self or out.lengths.shape[0] != len(seqs)):
+            raise TurboPiError("PagedCache: `out` is a batch of another cache or number of sequences")
         page, plan, taken = self.page_size, [], 0
         refs = {}                                     # of shared last pages, as the plan leaves them
         for seq, n in zip(seqs, new):
-            pages, length = self._get(seq)
+            pages, length, _ = self._get(seq)
             total = -(-(length + n) // page)
             if total > self.max_pages:
                 raise TurboPiError(f"PagedCache: {length + n} tokens need more than {self.max_pages} pages")
@@ -144,6 +156,7 @@ class PagedCache:
                 dst.append(fresh)
                 self._release(entry[0][-1])
                 entry[0][-1] = fresh
+                self._outdate(entry, f"a shared page of sequence {seq} was copied")
             entry[0].extend(self._take() for _ in range(more))
             entry[1] += n
         if src:
@@ -175,11 +188,18 @@ class PagedCache:
         flat = self._upload(rows + [self._seqs[s][1] for s in seqs] + cu, (-1,))
         table, lengths, offsets = flat[:S * W].view(S, W), flat[S * W:S * W + S], flat[S * W + S:]
         if out is None:
-            return PagedBatch(table, lengths, offsets, cu[-1], self._moves)
-        out.table.copy_(table)
-        out.lengths.copy_(lengths)
-        out.cu.copy_(offsets)
-        out.tokens, out._moves = cu[-1], self._moves
+            out = PagedBatch(table, lengths, offsets, cu[-1], self)
+        else:
+            for seq in out._seqs:
+                if seq in self._seqs:
+                    self._seqs[seq][2].discard(out)
+            out.table.copy_(table)
+            out.lengths.copy_(lengths)
+            out.cu.copy_(offsets)
+            out.tokens, out._stale = cu[-1], None
+        out._seqs = seqs
+        for seq in seqs:
+            self._seqs[seq][2].add(out)
         return out
 
     # ------------------------------------------------------------------ the device side
@@ -188,8 +208,10 @@ class PagedCache:
         return self.pages[layer, 0], self.pages[layer, 1]
 
     def _current(self, batch):
-        if batch._moves != self._moves:
-            raise TurboPiError("PagedCache: pages have moved since this batch was made (compact); make it again")
+        if batch._cache() is not self:
+            raise TurboPiError("PagedCache: a batch of another cache")
+        if batch._stale:
+            raise TurboPiError(f"PagedCache: {batch._stale} since this batch was made; make it again")
 
     def append(self, layer, batch, k, v, q=None, cos=None, sin=None, q_out=None):
         """ops.paged_append of the batch's new tokens: k, v (and q) [batch.tokens, heads, head_dim], sequence by sequence."""
@@ -215,8 +237,8 @@ class PagedCache:
         to = dict(zip(high, low))
         for entry in self._seqs.values():
             entry[0] = [to.get(p, p) for p in entry[0]]
+            self._outdate(entry, "pages have moved (compact)")
         for a, b in to.items():
             self._refs[b], self._refs[a] = self._refs[a], 0
         self._free = list(range(used, self.num_pages))          # sorted, which is a heap
-        self._moves += 1
         return used
