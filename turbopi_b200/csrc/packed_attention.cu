@@ -186,6 +186,9 @@ __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity) {
     return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, kWait));
 }
 
+// The value all lanes hold, where the compiler knows that they do: operands of products live in uniform registers
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __reduce_or_sync(0xffffffffu, x); }
+
 // Warps 2 and 3 meet, and learn whether both are fine
 __device__ __forceinline__ bool meet_and(bool ok) {
     uint32_t all;
@@ -356,7 +359,7 @@ __global__ void __launch_bounds__(Layout<DP, R>::kThreads, Layout<DP, R>::kCtas)
             __syncwarp();
         } else if (warp == 1 && n_tiles > 0) {
             // -------------------------------------------------------- products
-            const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+            const uint32_t tm = uniform(tmem);
             const uint32_t q16 = (smem_u32(sQ) & 0x3FFFFu) >> 4, r16 = (smem_u32(ring) & 0x3FFFFu) >> 4;
             constexpr uint32_t kDescHiMnSw128 = (1024u >> 4) | (1u << 14) | (static_cast<uint32_t>(tc::kSwizzle128B) << 29);
             constexpr uint32_t kLboField = (static_cast<uint32_t>(kBlockBytes) >> 4) << 16;
@@ -364,11 +367,6 @@ __global__ void __launch_bounds__(Layout<DP, R>::kThreads, Layout<DP, R>::kCtas)
             // lost: barriers are tested before products are issued and the outcome looked at behind them, and the second product of head
             // sizes above 128 has N = 256.
             auto test = [&](uint64_t* bar, uint32_t parity) { return mbar_test_wait(bar, parity); };
-            auto seen = [&](bool early, uint64_t* bar, uint32_t parity) {
-                const bool ok = __all_sync(0xffffffffu, early) || wait_warp(bar, parity);
-                tc::fence_after_thread_sync();
-                return ok;
-            };
             auto unit_full = [&](int u) { return &ctl->full[u % L::kUnits]; };
             auto unit_parity = [&](int u) -> uint32_t { return (u / L::kUnits) & 1; };
             // scores of one unit of K (past head_dim both operands are zero), row tile x, into buffer x
@@ -392,97 +390,102 @@ __global__ void __launch_bounds__(Layout<DP, R>::kThreads, Layout<DP, R>::kCtas)
             };
             bool ok = wait_warp(&ctl->q_full, 0);
             if constexpr (L::kOwn) {
-                const int t0 = __shfl_sync(0xffffffffu, tiles[0], 0), t1 = __shfl_sync(0xffffffffu, tiles[1], 0), n = max(t0, t1);
+                const int t0 = uniform(tiles[0]), t1 = uniform(tiles[1]), n = max(t0, t1);
                 ok = ok && wait_warp(unit_full(0), 0);
-                tc::fence_after_thread_sync();
-                if (ok && tc::elect_one()) {
-                    if (t0 > 0) {
+                if (tc::elect_one()) {
+                    if (ok && t0 > 0) {
                         scores(0, 0, 0);
                         tc::commit(&ctl->s_ready[0]);
                     }
-                    if (t1 > 0) {
-                        scores(1, 0, 0);
-                        tc::commit(&ctl->s_ready[1]);
+                    if (R == 2 && ok && t1 > 0) {
+                        scores(R - 1, 0, 0);
+                        tc::commit(&ctl->s_ready[R - 1]);
                     }
-                    tc::commit(&ctl->empty[0]);
-                }
-                __syncwarp();
-                bool p0 = false;
-                for (int j = 0; j < n && ok; ++j) {
-                    const int v = 2 * j + 1, k = 2 * j + 2;
+                    if (ok) tc::commit(&ctl->empty[0]);
+                    bool p0 = false, vf = false;
+                    for (int j = 0; j < n && ok; ++j) {
+                        const int v = 2 * j + 1, k = 2 * j + 2;
 #pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        const int t = x == 0 ? t0 : t1;
-                        const bool last_use = x == 1 || t1 == 0;
-                        if (j >= t || !ok) continue;
-                        ok = seen(p0, &ctl->p_ready[x][0], j & 1) && seen(test(unit_full(v), unit_parity(v)), unit_full(v), unit_parity(v));
-                        const bool p1 = test(&ctl->p_ready[x][1], j & 1);
-                        if (ok && tc::elect_one()) values(x, v, 0, j > 0 ? 1u : 0u);
-                        __syncwarp();
-                        ok = ok && seen(p1, &ctl->p_ready[x][1], j & 1);
-                        const bool next = j + 1 < t, kf = next && test(unit_full(k), unit_parity(k));
-                        if (ok && tc::elect_one()) {
+                        for (int x = 0; x < R; ++x) {
+                            const int t = x == 0 ? t0 : t1;
+                            const bool last_use = x == R - 1 || t1 == 0;
+                            if (j >= t || !ok) continue;
+                            ok = (p0 || mbar_wait_bounded(&ctl->p_ready[x][0], j & 1, kWait)) &&
+                                 (vf || mbar_wait_bounded(unit_full(v), unit_parity(v), kWait));
+                            if (!ok) continue;
+                            tc::fence_after_thread_sync();
+                            const bool p1 = test(&ctl->p_ready[x][1], j & 1);
+                            values(x, v, 0, j > 0 ? 1u : 0u);
+                            ok = p1 || mbar_wait_bounded(&ctl->p_ready[x][1], j & 1, kWait);
+                            if (!ok) continue;
+                            tc::fence_after_thread_sync();
+                            const bool next = j + 1 < t, kf = next && test(unit_full(k), unit_parity(k));
+                            // of the event that comes next: the other row tile's where it has one
+                            const bool other = R == 2 && (x == 0 ? j < t1 : j + 1 < t0);
                             values(x, v, 1, 1);
                             if (last_use) tc::commit(&ctl->empty[v % L::kUnits]);
                             if (!next) tc::commit(&ctl->o_done[x]);
-                        }
-                        __syncwarp();
-                        // of the event that comes next: the other row tile's where it has one
-                        const bool other = x == 0 ? j < t1 : j + 1 < t0;
-                        p0 = test(&ctl->p_ready[other ? x ^ 1 : x][0], (x == 0 && other ? j : j + 1) & 1);
-                        if (!next) continue;
-                        ok = ok && seen(kf, unit_full(k), unit_parity(k));
-                        if (ok && tc::elect_one()) {
+                            p0 = test(&ctl->p_ready[other ? x ^ 1 : x][0], (x == 0 && other ? j : j + 1) & 1);
+                            vf = x == 0 && other ? true : test(unit_full(v + 2), unit_parity(v + 2));
+                            if (!next) continue;
+                            ok = kf || mbar_wait_bounded(unit_full(k), unit_parity(k), kWait);
+                            if (!ok) continue;
                             scores(x, k, 0);
                             tc::commit(&ctl->s_ready[x]);
                             if (last_use) tc::commit(&ctl->empty[k % L::kUnits]);
                         }
-                        __syncwarp();
+                    }
+                    if (!ok) {
+                        record_error(kErrPackedBarrierTimeout);
+                        ctl->failed = 1;
                     }
                 }
+                __syncwarp();
             } else {
-                const int n = __shfl_sync(0xffffffffu, n_tiles, 0);
-                auto issue_scores = [&](int e, bool early) {
-                    const int u = k_unit(e);
+                const int n = uniform(n_tiles);
+                if (tc::elect_one()) {
+                    auto issue_scores = [&](int e, bool early) {
+                        const int u = k_unit(e);
 #pragma unroll
-                    for (int h = 0; h < L::kHalves; ++h) {
-                        ok = ok && seen(early, unit_full(u + h), unit_parity(u + h));
-                        early = test(unit_full(u + 1), unit_parity(u + 1));
-                        if (ok && tc::elect_one()) {
+                        for (int h = 0; h < L::kHalves; ++h) {
+                            ok = ok && (early || mbar_wait_bounded(unit_full(u + h), unit_parity(u + h), kWait));
+                            if (!ok) return;
+                            early = test(unit_full(u + 1), unit_parity(u + 1));
                             scores(e & 1, u + h, h);
                             tc::commit(&ctl->empty[(u + h) % L::kUnits]);
-                            if (h == L::kHalves - 1) tc::commit(&ctl->s_ready[e & 1]);
                         }
-                        __syncwarp();
-                    }
-                };
-                issue_scores(0, false);
-                if (n > 1) issue_scores(1, false);
-                bool p0 = false;
-                for (int e = 0; e < n && ok; ++e) {
-                    const int v = L::kHalves * (e == n - 1 ? 2 * e + 1 : 2 * e + 2), x = e & 1;
-                    const uint32_t phase = (e >> 1) & 1;
-                    const bool v0 = test(unit_full(v), unit_parity(v)), v1 = test(unit_full(v + 1), unit_parity(v + 1));
-                    ok = seen(p0, &ctl->p_ready[x][0], phase) && seen(v0, unit_full(v), unit_parity(v)) && seen(v1, unit_full(v + 1), unit_parity(v + 1));
-                    const bool p1 = test(&ctl->p_ready[x][1], phase);
-                    if (ok && tc::elect_one()) values(x, v, 0, e > 0 ? 1u : 0u);
-                    __syncwarp();
-                    ok = ok && seen(p1, &ctl->p_ready[x][1], phase);
-                    const bool next = e + 2 < n, kf = next && test(unit_full(k_unit(e + 2)), unit_parity(k_unit(e + 2)));
-                    if (ok && tc::elect_one()) {
+                        tc::commit(&ctl->s_ready[e & 1]);
+                    };
+                    issue_scores(0, false);
+                    if (n > 1) issue_scores(1, false);
+                    bool p0 = false;
+                    for (int e = 0; e < n && ok; ++e) {
+                        const int v = L::kHalves * (e == n - 1 ? 2 * e + 1 : 2 * e + 2), x = e & 1;
+                        const uint32_t phase = (e >> 1) & 1;
+                        const bool v0 = test(unit_full(v), unit_parity(v)), v1 = test(unit_full(v + 1), unit_parity(v + 1));
+                        ok = (p0 || mbar_wait_bounded(&ctl->p_ready[x][0], phase, kWait)) && (v0 || mbar_wait_bounded(unit_full(v), unit_parity(v), kWait)) &&
+                             (v1 || mbar_wait_bounded(unit_full(v + 1), unit_parity(v + 1), kWait));
+                        if (!ok) break;
+                        tc::fence_after_thread_sync();
+                        const bool p1 = test(&ctl->p_ready[x][1], phase);
+                        values(x, v, 0, e > 0 ? 1u : 0u);
+                        ok = p1 || mbar_wait_bounded(&ctl->p_ready[x][1], phase, kWait);
+                        if (!ok) break;
+                        tc::fence_after_thread_sync();
+                        const bool next = e + 2 < n, kf = next && test(unit_full(k_unit(e + 2)), unit_parity(k_unit(e + 2)));
                         values(x, v, 1, 1);
                         tc::commit(&ctl->empty[v % L::kUnits]);
                         tc::commit(&ctl->empty[(v + 1) % L::kUnits]);
                         tc::commit(&ctl->o_done[x]);
+                        p0 = test(&ctl->p_ready[x ^ 1][0], ((e + 1) >> 1) & 1);
+                        if (next) issue_scores(e + 2, kf);
                     }
-                    __syncwarp();
-                    p0 = test(&ctl->p_ready[x ^ 1][0], ((e + 1) >> 1) & 1);
-                    if (next) issue_scores(e + 2, kf);
+                    if (!ok) {
+                        record_error(kErrPackedBarrierTimeout);
+                        ctl->failed = 1;
+                    }
                 }
-            }
-            if (!ok && lane == 0) {
-                record_error(kErrPackedBarrierTimeout);
-                ctl->failed = 1;
+                __syncwarp();
             }
         } else if (warp >= 2) {
             // -------------------------------------------------------- V of tiles with masked pairs
