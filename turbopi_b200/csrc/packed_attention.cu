@@ -23,17 +23,19 @@
 // While one group works the other's products run.
 //
 // What bounds it, measured on one B200 (calls in a CUDA graph):
-//   one sequence of 8191 tokens, causal, 8 on 1 heads of 256: 203 us = 1.35 PFLOP/s, 0.82 of the measured bf16 rate; the tensor pipe works in
-//   68 % of the cycles.  When all of it took 209 us, the line of products without loads and without the arithmetic of the softmax took
-//   203: what is missing goes into the hand-overs from product to softmax and back.
-//   4 sequences, 24.6 k tokens, causal, 32 on 8 heads of 128: 1.6 ms = 1.07 PFLOP/s, 0.65.  The exponentials of a 128 x 128 tile take the
-//   special-function unit 1024 cycles (16 each), and its products the tensor pipe as long; both groups at once finish a tile
-//   every 1000-1150.  About 6 us of each CTA's 70 pass in its first loads and its output.
-//   One sequence of 200 tokens, 8 on 1 heads of 256: 10.9 us: look-up 0.6, tensor memory and barriers 0.3, loads 1-2, 1.1 of softmax per tile,
+//   one sequence of 8191 tokens, causal, 8 on 1 heads of 256: 195 us = 1.41 PFLOP/s, 0.86 of the measured bf16 rate: hand-overs from product to
+//   softmax and back.
+//   4 sequences, 24.6 k tokens, causal, 32 on 8 heads of 128: 1.38 ms = 1.23 PFLOP/s, 0.75, at 1965 MHz; after some 10 ms of it the board
+//   is at its 1000 W, the clock goes to 1.6 GHz and the call to 1.56-1.62 ms.  At full clock two tiles take 3350 cycles, of which their products
+//   need 2048 and so do their exponentials (16 a cycle and SM): a group's softmax takes 2000 (1300 to the first half of P) while the
+//   other's runs too, then 1130 pass until its next scores are there.  About 6 us of each CTA's 60 pass in its first loads and its output.
+//   One sequence of 200 tokens, 8 on 1 heads of 256: 10.7 us: look-up 0.6, tensor memory and barriers 0.3, loads 1-2, 1.1 of softmax per tile,
 //   1.4 for the output, one after the other.
-// Issuing a 128 x 128 x 16 product takes the issuing warp about the 64 cycles it runs, so none queue up and a wait between two of them is
-// lost time: barriers are tested while products ahead of them run (209 -> 201 us, 1.72 -> 1.71 ms).  Tried without gain: a quarter of the
-// exponentials as polynomials on the FMA pipes (1.61 ms without, 1.71 with); four groups, two threads per row (1.75 -> 1.94 ms;
+// One thread issues the products, from operands that the compiler knows to be the same in all lanes (uniform()), and tests barriers while
+// products ahead of them run.  With operands it had to move over for every product, issuing took as long as running, and of an event's 1760
+// cycles 690 went between products (one sequence 201 -> 195 us, four 1414 -> 1381 unthrottled, 1645 -> 1605 throttled).
+// Tried without gain: an eighth to a half of the exponentials as polynomials on the FMA pipes (four sequences 1555 us without, 1585-1620 with:
+// their energy); two threads issuing, one per row tile (1725 us: the two no longer alternate); four groups, two threads per row (1.75 -> 1.94 ms;
 // sequences of 100 tokens gain 7 %, those of 1 to 1200 lose 6 %); pairs of CTAs on one product (cta_group::2, M = 256: 2.47 ms, the single
 // sequence 250 us, each hand-over crosses the cluster).
 //
@@ -80,6 +82,10 @@ struct Layout {
     static constexpr int kThreads = 128 + 128 * kGroups;
     static constexpr int kCtas = kOwn && R == 1 ? 2 : 1;           // on an SM
     static constexpr uint32_t kTmemCols = kCtas == 2 ? 256 : 512, kColO = kGroups * kTile;
+    // Where tensor memory has room for P beside S, the next scores are computed while the exponentials of these are: 8192 tokens, 16 heads
+    // of 64, 203 -> 194 us.  With one row tile the other CTA fills the gaps: 16 sequences of 512 36.0 us, ahead 36.4.
+    static constexpr bool kAhead = DP == 64 && R == 2;
+    static constexpr uint32_t kColP = kAhead ? kColO + kGroups * DP : 0, kStepP = kAhead ? kTile / 2 : kTile;
     static constexpr int kBlocks = DP / 64;                        // 64-column blocks of a row
     static constexpr int kUnitBlocks = DP < 128 ? 1 : 2;           // a unit: 128 keys x up to 128 columns
     static constexpr int kHalves = kBlocks / kUnitBlocks;          // units of a tile
@@ -95,6 +101,7 @@ struct PackedControl {
     uint64_t q_full;
     uint64_t full[8], empty[8];
     uint64_t s_ready[2], p_ready[2][2], o_done[2];       // p_ready: by half of the tile's keys
+    uint64_t s_read[2];                  // scores are in registers, the next ones may take their place (kAhead)
     uint64_t ref_ready[2][4];            // one row tile: the reference of event e, by quarter of the rows
     uint64_t v_landed[kBadTiles];        // V of a tile with masked pairs, which is looked over before its units count as full
     uint32_t tmem_base;
@@ -270,6 +277,7 @@ __global__ void __launch_bounds__(Layout<DP, R>::kThreads, Layout<DP, R>::kCtas)
             mbar_init(&ctl->s_ready[i], 1);
             for (int h = 0; h < 2; ++h) mbar_init(&ctl->p_ready[i][h], 4);
             mbar_init(&ctl->o_done[i], 1);
+            mbar_init(&ctl->s_read[i], 4);
             for (int w = 0; w < 4; ++w) mbar_init(&ctl->ref_ready[i][w], 1);
         }
         for (int i = 0; i < kBadTiles; ++i) mbar_init(&ctl->v_landed[i], L::kHalves);
@@ -363,9 +371,8 @@ __global__ void __launch_bounds__(Layout<DP, R>::kThreads, Layout<DP, R>::kCtas)
             const uint32_t q16 = (smem_u32(sQ) & 0x3FFFFu) >> 4, r16 = (smem_u32(ring) & 0x3FFFFu) >> 4;
             constexpr uint32_t kDescHiMnSw128 = (1024u >> 4) | (1u << 14) | (static_cast<uint32_t>(tc::kSwizzle128B) << 29);
             constexpr uint32_t kLboField = (static_cast<uint32_t>(kBlockBytes) >> 4) << 16;
-            // Issuing a product takes about as long as it runs (64 cycles for N = 128), so what the warp does between them is
-            // lost: barriers are tested before products are issued and the outcome looked at behind them, and the second product of head
-            // sizes above 128 has N = 256.
+            // Barriers are tested before products are issued and the outcome is looked at behind them; the second product of head sizes
+            // above 128 has N = 256.
             auto test = [&](uint64_t* bar, uint32_t parity) { return mbar_test_wait(bar, parity); };
             auto unit_full = [&](int u) { return &ctl->full[u % L::kUnits]; };
             auto unit_parity = [&](int u) -> uint32_t { return (u / L::kUnits) & 1; };
@@ -384,7 +391,7 @@ __global__ void __launch_bounds__(Layout<DP, R>::kThreads, Layout<DP, R>::kCtas)
                 const uint32_t va = r16 + (u % L::kUnits * L::kUnitBytes >> 4), d = tm + L::kColO + (L::kOwn ? x * DP : 0);
 #pragma unroll
                 for (int kk = part * 4; kk < part * 4 + 4; ++kk) {
-                    mma_ts(d, tm + x * kTile + kk * 8, tc::desc_from_words((va + (kk * 2048 >> 4)) | kLboField, kDescHiMnSw128), P.idesc_o,
+                    mma_ts(d, tm + L::kColP + x * L::kStepP + kk * 8, tc::desc_from_words((va + (kk * 2048 >> 4)) | kLboField, kDescHiMnSw128), P.idesc_o,
                            kk > 0 ? 1u : more);
                 }
             };
@@ -410,6 +417,20 @@ __global__ void __launch_bounds__(Layout<DP, R>::kThreads, Layout<DP, R>::kCtas)
                             const int t = x == 0 ? t0 : t1;
                             const bool last_use = x == R - 1 || t1 == 0;
                             if (j >= t || !ok) continue;
+                            const bool next = j + 1 < t;
+                            auto next_scores = [&](bool early) {
+                                ok = early || mbar_wait_bounded(unit_full(k), unit_parity(k), kWait);
+                                if (!ok) return;
+                                scores(x, k, 0);
+                                tc::commit(&ctl->s_ready[x]);
+                                if (last_use) tc::commit(&ctl->empty[k % L::kUnits]);
+                            };
+                            if (L::kAhead && next) {
+                                ok = mbar_wait_bounded(&ctl->s_read[x], j & 1, kWait);
+                                tc::fence_after_thread_sync();
+                                if (ok) next_scores(false);
+                                if (!ok) continue;
+                            }
                             ok = (p0 || mbar_wait_bounded(&ctl->p_ready[x][0], j & 1, kWait)) &&
                                  (vf || mbar_wait_bounded(unit_full(v), unit_parity(v), kWait));
                             if (!ok) continue;
@@ -419,20 +440,15 @@ __global__ void __launch_bounds__(Layout<DP, R>::kThreads, Layout<DP, R>::kCtas)
                             ok = p1 || mbar_wait_bounded(&ctl->p_ready[x][1], j & 1, kWait);
                             if (!ok) continue;
                             tc::fence_after_thread_sync();
-                            const bool next = j + 1 < t, kf = next && test(unit_full(k), unit_parity(k));
+                            const bool kf = !L::kAhead && next && test(unit_full(k), unit_parity(k));
                             // of the event that comes next: the other row tile's where it has one
                             const bool other = R == 2 && (x == 0 ? j < t1 : j + 1 < t0);
                             values(x, v, 1, 1);
                             if (last_use) tc::commit(&ctl->empty[v % L::kUnits]);
-                            if (!next) tc::commit(&ctl->o_done[x]);
+                            if (L::kAhead || !next) tc::commit(&ctl->o_done[x]);
                             p0 = test(&ctl->p_ready[other ? x ^ 1 : x][0], (x == 0 && other ? j : j + 1) & 1);
                             vf = x == 0 && other ? true : test(unit_full(v + 2), unit_parity(v + 2));
-                            if (!next) continue;
-                            ok = kf || mbar_wait_bounded(unit_full(k), unit_parity(k), kWait);
-                            if (!ok) continue;
-                            scores(x, k, 0);
-                            tc::commit(&ctl->s_ready[x]);
-                            if (last_use) tc::commit(&ctl->empty[k % L::kUnits]);
+                            if (!L::kAhead && next) next_scores(kf);
                         }
                     }
                     if (!ok) {
@@ -546,7 +562,7 @@ __global__ void __launch_bounds__(Layout<DP, R>::kThreads, Layout<DP, R>::kCtas)
         const int x = (warp >> 2) - 1;
         const int quarter = warp & 3, row = quarter * 32 + lane;
         const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
-        const uint32_t s_at = lanes + x * kTile, o_at = lanes + L::kColO + (L::kOwn ? x * DP : 0);
+        const uint32_t s_at = lanes + x * kTile, p_at = lanes + L::kColP + x * L::kStepP, o_at = lanes + L::kColO + (L::kOwn ? x * DP : 0);
         const int my_tile = L::kOwn ? x : 0;
         const int token = token0 + my_tile * tokens_tile + (row >> P.pack_shift);
         const int limit = row_limit(P, nq, nk, token);
@@ -567,6 +583,11 @@ __global__ void __launch_bounds__(Layout<DP, R>::kThreads, Layout<DP, R>::kCtas)
             for (int c = 0; c < kTile; c += 32) tc::tmem_ld_32x32b_x32(s_at + c, *reinterpret_cast<uint32_t(*)[32]>(s + c));
 #pragma unroll
             for (int c = 0; c < kTile; c += 32) tmem_ld_wait_for(s + c);
+            if (L::kAhead) {
+                tc::fence_before_thread_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&ctl->s_read[x]);
+            }
             if (masked) {
 #pragma unroll
                 for (int c = 0; c < kTile; c += 32) {    // a bit per column that is seen
@@ -589,8 +610,12 @@ __global__ void __launch_bounds__(Layout<DP, R>::kThreads, Layout<DP, R>::kCtas)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&ctl->ref_ready[x][quarter]);
             }
-            if (__any_sync(0xffffffffu, raise) && e >= R) {
-                // the last product into this O: with two row tiles it was issued before these scores, and is complete
+            if (L::kAhead && e >= 2) {       // the last product into this O, which reads what P is written over
+                if (!wait_warp(&ctl->o_done[x], ((e >> 1) - 1) & 1)) { ok = false; break; }
+                tc::fence_after_thread_sync();
+            }
+            if (__any_sync(0xffffffffu, raise) && e >= (L::kOwn ? 2 : 1)) {
+                // the last product into this O: where P lies in S's columns it was issued before these scores, and is complete
                 if (!L::kOwn && !wait_warp(&ctl->o_done[x ^ 1], ((e - 1) >> 1) & 1)) { ok = false; break; }
                 tc::fence_after_thread_sync();
                 const float f = raise ? ex2(ref - now) : 1.0f;
@@ -625,7 +650,7 @@ __global__ void __launch_bounds__(Layout<DP, R>::kThreads, Layout<DP, R>::kCtas)
                     sum[i & 1] = add2(sum[i & 1], pair(a, b));
                     p[i] = Half16<T>::pack(a, b);
                 }
-                tmem_st_x32(s_at + c, p);
+                tmem_st_x32(p_at + c, p);
                 tmem_st_done();
                 tc::fence_before_thread_sync();
                 __syncwarp();
@@ -645,7 +670,7 @@ __global__ void __launch_bounds__(Layout<DP, R>::kThreads, Layout<DP, R>::kCtas)
         }
         const int mine = L::kOwn ? tiles[x] : tiles[0];
         if (ok && mine > 0) {
-            if (!wait_warp(&ctl->o_done[L::kOwn ? x : (mine - 1) & 1], L::kOwn ? 0 : ((mine - 1) >> 1) & 1)) ok = false;
+            if (!wait_warp(&ctl->o_done[L::kOwn ? x : (mine - 1) & 1], L::kAhead ? (mine - 1) & 1 : (L::kOwn ? 0 : ((mine - 1) >> 1) & 1))) ok = false;
             tc::fence_after_thread_sync();
         }
         // rows that see no key while the CTA's other row tile does: their queries may still be on the way to where the output is staged
