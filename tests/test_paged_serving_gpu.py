@@ -128,3 +128,32 @@ def test_a_decode_step_as_a_graph(cuda_device):
             assert torch.equal(keys, m.seen[s][0][0]) and torch.equal(values, m.seen[s][0][1])
             want, allow = attend(q[j:j + 1], keys, values, m.scale)
             check(out[j:j + 1], want, allow)
+
+
+@pytest.mark.parametrize("hq,hk,D,dtype", [(8, 1, 256, torch.bfloat16), (6, 2, 64, torch.float16)])
+def test_prompts_from_a_fused_projection(cuda_device, hq, hk, D, dtype):
+    """Queries and keys are neighbouring columns of a projection: rotated together, the keys come back packed, as they lie in the pages."""
+    from turbopi_b200 import ops
+    from turbopi_b200.paged_cache import PagedCache
+    cache = PagedCache(1, 40, 16, hk, D, 12, dtype=dtype, device=cuda_device)
+    g = torch.Generator(device=cuda_device).manual_seed(5)
+    lens = [37, 1, 150]
+    seqs = [cache.add() for _ in lens]
+    qkv = torch.randn((sum(lens), hq + 2 * hk, D), generator=g, device=cuda_device, dtype=dtype)
+    cos, sin = ops.rope_tables(160, D, device=cuda_device)
+    batch, v = cache.extend(seqs, lens), qkv[:, hq + hk:]
+    turned = cache.append(0, batch, qkv[:, hq:hq + hk], v, q=qkv[:, :hq + hk], cos=cos, sin=sin)
+    out = ops.packed_attention(turned[:, :hq], turned[:, hq:], v, batch.cu, D ** -0.5)
+    at = 0
+    for s, n in zip(seqs, lens):
+        ids = torch.tensor(cache.page_ids(s), device=cuda_device)
+        keys, values = (p[ids].flatten(0, 1)[:n] for p in cache.layer(0))
+        assert torch.equal(keys, turned[at:at + n, hq:]) and torch.equal(values, v[at:at + n])
+        pos = torch.arange(n, device=cuda_device)
+        wanted = rotate(qkv[at:at + n, :hq].double(), cos[pos], sin[pos])
+        # rounded once, the rotation itself in fp32: half a step, and three roundings of 2^-24 of the pair's largest product
+        half, size = torch.finfo(dtype).eps / 2, qkv[at:at + n, :hq].double().abs().amax(-1, keepdim=True)
+        assert bool(((turned[at:at + n, :hq].double() - wanted).abs() <= half * wanted.abs() + 8 * 2.0 ** -24 * size + torch.finfo(dtype).tiny).all())
+        want, allow = attend(turned[at:at + n, :hq], keys, values, D ** -0.5, 0)
+        check(out[at:at + n], want, allow)
+        at += n
