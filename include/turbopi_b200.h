@@ -423,7 +423,8 @@ int tpb200_attention_describe(int n_rows, int n_keys, int head_dim, int groups, 
  * keys gives zeros.  Query heads [h * g, (h + 1) * g) read key head h.  q / out [q_tokens, q_heads, head_dim], k / v
  * [k_tokens, kv_heads, head_dim] with element strides of a token and a head, multiples of 8 that do not overlap; bf16 or fp16;
  * head_dim a multiple of 8, <= 256.  Tokens before cu[0] and behind cu[seqs] are left alone; out may be q.  The offsets are read on the
- * device (a captured call follows them); ones outside the tensors are clamped to them.  What stands in masked places (keys and
+ * device (a captured call follows them); ones outside the tensors are clamped to them.  An output that shares
+ * elements with k or v, or with q other than row on row, is refused.  What stands in masked places (keys and
  * values of later tokens, of other sequences, of nobody) does not matter, infinities and NaN included.
  * ------------------------------------------------------------------------------------------- */
 typedef struct {
@@ -457,7 +458,7 @@ typedef struct {
  * (the new token's own key among them); query heads [h * g, (h + 1) * g) read key head h, g = q_heads / kv_heads; fp32 sums,
  * outputs rounded once.  A sequence of length 0 gives zeros.  q / out: element strides of a sequence and of a head, multiples of 8.
  * The lengths' sum is cut into equal pieces over the GPU whatever the single lengths; items that cross a cut are joined by a second
- * small kernel through `workspace` (no initialisation needed; its size depends on the heads only).  out may be q.  All lengths decide
+ * small kernel through `workspace` (no initialisation needed; its size depends on the heads only).  out may be q (row on row, not in part).  All lengths decide
  * where the cuts fall, and so the order of a sequence's sums; the same call gives the same bits. */
 typedef struct {
     tpb200_paged_cache cache;
@@ -475,7 +476,8 @@ int tpb200_paged_attention(const tpb200_paged_attention_args* args, tpb200_strea
  * lengths are those after the call.  Tokens behind cu[seqs] are left alone.  With cos / sin ([rope_positions, head_dim / 2], rows
  * contiguous, fp32, fp16 or bf16) the keys, and the queries where given, are rotated at their positions in rotate-half form:
  *   y[d] = x[d] cos[d] - x[d + D/2] sin[d],  y[d + D/2] = x[d + D/2] cos[d] + x[d] sin[d]
- * in fp32, rounded once (modeling_gemma.py:132-197); q_out may be q.  A token without a place (501) writes nothing; no two tokens
+ * in fp32, rounded once (modeling_gemma.py:132-197); q_out may be q, and shares no other elements with q, k or v.  Key and value pages
+ * are different memory, and what is written there is not read as a token of the same call.  A token without a place (501) writes nothing; no two tokens
  * of a call may have the same place. */
 typedef struct {
     tpb200_paged_cache cache;

@@ -145,3 +145,57 @@ def test_structures_follow_the_header_field_by_field():
         body = re.sub(r"/\*.*?\*/", "", re.search(r"typedef struct\s*\{([^}]*)\}\s*" + name + r"\s*;", header, re.S).group(1), flags=re.S)
         fields = [part.strip().split()[-1].split("[")[0].lstrip("*") for d in body.split(";") if d.strip() for part in d.split(",")]
         assert fields == [f[0] for f in mirror._fields_], name
+
+
+def _elements(at, stride, tokens, heads, D):
+    return [{at // 2 + t * stride[0] + h * stride[1] + d for d in range(D)} for t in range(tokens) for h in range(heads)]
+
+
+def test_outputs_in_part_where_inputs_lie():
+    """Random views around one place, against sets of their elements: an output on its input row on row is fine, one that shares only some of
+    its elements, or its own rows, is refused; views with different token strides are refused where their ranges meet."""
+    import random
+    rng, lib, seen = random.Random(3), _lib.load(), {True: 0, False: 0}
+    for _ in range(1500):
+        D, tokens, heads = rng.choice([8, 16, 24]), rng.randint(1, 4), rng.randint(1, 4)
+
+        def view():
+            return rng.choice([1024, 1024 + 16 * rng.randint(-12, 12)]), (rng.choice([D * heads, D * heads * 2, D + 8 * rng.randint(0, 12)]),
+                                                                         rng.choice([D, D, D + 8, 2 * D, D + 8 * rng.randint(0, 12)]))
+        q, q_stride = view()
+        out, o_stride = (q, q_stride) if rng.random() < 0.2 else view()
+        if rng.random() < 0.6:
+            o_stride = (q_stride[0], o_stride[1])
+        rows, written = _elements(q, q_stride, tokens, heads, D), _elements(out, o_stride, tokens, heads, D)
+        a, b = set().union(*rows), set().union(*written)
+        ranges = min(a) <= max(b) and min(b) <= max(a)
+        crossed = len(b) < len(written) * D
+        bad = crossed or (rows != written and (bool(a & b) or (tokens > 1 and q_stride[0] != o_stride[0] and ranges)))
+        args = _lib.PagedAttentionArgs(cache=_cache(head_dim=D, seqs=tokens, page_stride=16 * 256), q=q, out=out, q_stride=Two(*q_stride),
+                                       o_stride=Two(*o_stride), q_heads=heads, scale=1.0)
+        assert (lib.tpb200_paged_attention(args, None) == SHAPE) == bad, (D, tokens, heads, q, q_stride, out, o_stride)
+        seen[bad] += 1
+    assert min(seen.values()) > 300
+
+
+@pytest.mark.parametrize("change", [dict(out=64 + 512), dict(k=1 << 20), dict(v=1 << 20), dict(v=(1 << 20) + 1024 * 2 * 9 - 16)])
+def test_packed_outputs_where_others_read(change):
+    base = dict(q=64, k=1 << 21, v=1 << 22, out=1 << 20, q_stride=Two(1024, 256), k_stride=Two(512, 256), v_stride=Two(512, 256),
+                o_stride=Two(1024, 256), cu=64, seqs=1, q_tokens=9, k_tokens=9, q_heads=4, kv_heads=2, head_dim=256, dtype=_lib.BF16, scale=1.0)
+    assert _lib.load().tpb200_packed_attention(_lib.PackedAttentionArgs(**{**base, **change}), None) == SHAPE
+
+
+@pytest.mark.parametrize("change", [dict(q_out=64 + 512), dict(q_out=(1 << 20) - 512), dict(q_out=1 << 21), dict(o_stride=Two(512, 256)),
+                                    dict(cache=_cache(v_pages=1024)),
+                                    dict(q=64, q_out=64, q_heads=9, k=64 + 8 * 512, q_stride=Two(2560, 256), o_stride=Two(2560, 256),
+                                         k_stride=Two(2560, 256), v=64 + 9 * 512, v_stride=Two(2560, 256))])
+def test_appends_that_write_where_others_read(change):
+    """The last one: queries and keys of a fused projection turned in place together, while the keys are read for their pages."""
+    base = dict(cache=_cache(), k=1 << 20, v=1 << 21, k_stride=Two(256, 256), v_stride=Two(256, 256), cu=64, tokens=3, q=64, q_out=1 << 22, q_heads=8,
+                q_stride=Two(2048, 256), o_stride=Two(2048, 256), cos=64, sin=64, rope_positions=4, rope_dtype=_lib.F32)
+    assert _lib.load().tpb200_paged_append(_lib.PagedAppendArgs(**{**base, **change}), None) == SHAPE
+
+
+def test_scales_too_large_for_the_exponent():
+    base = dict(cache=_cache(), q=64, out=64, q_stride=Two(2048, 256), o_stride=Two(2048, 256), q_heads=8, scale=3e38, workspace=256, workspace_bytes=1 << 30)
+    assert _lib.load().tpb200_paged_attention(_lib.PagedAttentionArgs(**base), None) == SHAPE

@@ -823,6 +823,12 @@ extern "C" int tpb200_packed_attention(const tpb200_packed_attention_args* a, tp
     P.causal = a->causal != 0;
     // the sign of the scale goes into the product (operand A negated), its size into the exponent; none at all would lose the mask
     P.scale2 = fmaxf(fabsf(a->scale) * 1.4426950408889634f, 1.1754944e-38f);
+    TPB_REQUIRE(std::isfinite(P.scale2), TPB200_ERR_SHAPE);
+    // CTAs read keys and values while others write rows of the output
+    const RowSet q_rows(a->q, a->q_stride, a->q_tokens, a->q_heads, a->head_dim), o_rows(a->out, a->o_stride, a->q_tokens, a->q_heads, a->head_dim);
+    TPB_REQUIRE(output_fits(o_rows, q_rows), TPB200_ERR_SHAPE);
+    TPB_REQUIRE(!rows_meet(o_rows, RowSet(a->k, a->k_stride, a->k_tokens, a->kv_heads, a->head_dim)) &&
+                !rows_meet(o_rows, RowSet(a->v, a->v_stride, a->k_tokens, a->kv_heads, a->head_dim)), TPB200_ERR_SHAPE);
     const int DP = a->head_dim <= 64 ? 64 : (a->head_dim <= 128 ? 128 : 256);
     const bool bf = a->dtype == TPB200_BF16;
     // instruction descriptor: fp32 sums, A and B bf16 (1) or fp16 (0), [13] negate A, [16] B MN-major, N >> 3 at 17, M >> 4 at 24

@@ -1,6 +1,8 @@
 // What the kernels on a cache of pages share: the view of the cache, its checks, 16-bit pairs.
 #pragma once
 
+#include <algorithm>
+
 #include "common.cuh"
 
 namespace tpb {
@@ -63,6 +65,55 @@ static inline int paged_stride(long long stride, int n, int head_dim) {
     TPB_REQUIRE(stride >= 0 && (n <= 1 || stride >= head_dim), TPB200_ERR_SHAPE);
     return TPB200_OK;
 }
+
+// Rows of head_dim 16-bit values, [n0][n1] with element strides; where heads lie side by side a token is one run
+struct RowSet {
+    long long at, s0, s1;
+    int n0, n1, width;
+    RowSet(const void* p, const long long (&stride)[2], int tokens, int heads, int head_dim)
+        : at(static_cast<long long>(reinterpret_cast<uintptr_t>(p) / 2)), s0(stride[0]), s1(stride[1]), n0(tokens), n1(heads), width(head_dim) {
+        if (n1 > 1 && s1 == width) {
+            width *= n1;
+            n1 = 1;
+        }
+    }
+    long long token() const { return (n1 - 1) * s1 + width; }
+    long long end() const { return at + (n0 - 1) * s0 + token(); }
+};
+
+// Whether runs of `a` and `b` values, the second `d` behind the first, meet when the second moves on by t * s0 for a t in [first, last]
+static inline bool runs_meet(long long d, int a, int b, long long s0, long long first, long long last) {
+    const long long lo = 1 - b - d, hi = a - 1 - d;              // what t * s0 has to lie between
+    const long long t_lo = lo > 0 ? (lo + s0 - 1) / s0 : -(-lo / s0), t_hi = hi >= 0 ? hi / s0 : -((-hi + s0 - 1) / s0);
+    return std::max(t_lo, first) <= std::min(t_hi, last);
+}
+// Whether two sets share an element.  Views of one tensor (equal token strides) are compared row by row; sets of different
+// strides whose ranges meet count as meeting.
+static inline bool rows_meet(const RowSet& a, const RowSet& b) {
+    if (a.n0 < 1 || b.n0 < 1 || a.at >= b.end() || b.at >= a.end()) return false;
+    if (a.n0 > 1 && b.n0 > 1 && a.s0 != b.s0) return true;
+    const long long s0 = a.n0 > 1 ? a.s0 : (b.n0 > 1 ? b.s0 : 1);
+    for (int i = 0; i < a.n1; ++i) {
+        for (int j = 0; j < b.n1; ++j) {
+            if (runs_meet(b.at + j * b.s1 - a.at - i * a.s1, a.width, b.width, s0, 1ll - a.n0, b.n0 - 1ll)) return true;
+        }
+    }
+    return false;
+}
+// Whether two rows of an output share an element
+static inline bool rows_cross(const RowSet& a) {
+    if (a.n0 < 2) return false;          // heads do not: their stride is at least a row
+    if (a.s0 < a.width) return true;
+    for (int i = 1; i < a.n1; ++i) {
+        if (runs_meet(i * a.s1, a.width, a.width, a.s0, 1ll - a.n0, a.n0 - 1ll)) return true;
+    }
+    return false;
+}
+static inline bool rows_same(const RowSet& a, const RowSet& b) {
+    return a.at == b.at && a.width == b.width && a.n1 == b.n1 && (a.n1 < 2 || a.s1 == b.s1) && (a.n0 < 2 || a.s0 == b.s0);
+}
+// An output may lie where its input lies, row on row, and else shares nothing with it or with itself
+static inline bool output_fits(const RowSet& out, const RowSet& in) { return !rows_cross(out) && (rows_same(in, out) || !rows_meet(in, out)); }
 
 static inline int paged_view(const tpb200_paged_cache& c, PagedView* v) {
     TPB_REQUIRE(c.seqs >= 0 && c.num_pages >= 1 && c.page_size >= 1 && c.kv_heads >= 1 && c.table_width >= 1, TPB200_ERR_SHAPE);

@@ -893,7 +893,8 @@ extern "C" int tpb200_paged_attention(const tpb200_paged_attention_args* a, tpb2
     TPB_REQUIRE((a->flags & ~TPB200_FLAG_PDL) == 0, TPB200_ERR_ENUM);
     TPB_REQUIRE(a->q_heads >= 1 && a->q_heads % P.cache.kv_heads == 0, TPB200_ERR_SHAPE);
     TPB_REQUIRE(tpb_aligned16(a->q) && tpb_aligned16(a->out), TPB200_ERR_ALIGN);
-    TPB_REQUIRE(std::isfinite(a->scale), TPB200_ERR_SHAPE);
+    P.scale2 = a->scale * 1.4426950408889634f;
+    TPB_REQUIRE(std::isfinite(P.scale2), TPB200_ERR_SHAPE);
     for (int i = 0; i < 2; ++i) {
         const int n = i == 0 ? P.cache.seqs : a->q_heads;
         for (const long long stride : {a->q_stride[i], a->o_stride[i]}) {
@@ -904,6 +905,8 @@ extern "C" int tpb200_paged_attention(const tpb200_paged_attention_args* a, tpb2
         P.o_stride[i] = n > 1 ? a->o_stride[i] : 0;
     }
     if (P.cache.seqs == 0) return TPB200_OK;
+    TPB_REQUIRE(output_fits(RowSet(a->out, a->o_stride, P.cache.seqs, a->q_heads, P.cache.head_dim),
+                            RowSet(a->q, a->q_stride, P.cache.seqs, a->q_heads, P.cache.head_dim)), TPB200_ERR_SHAPE);
     P.group = a->q_heads / P.cache.kv_heads;
     P.tiles = (P.group + decode_rows(P.group) - 1) / decode_rows(P.group);
     P.rows = std::min(P.group, decode_rows(P.group));
@@ -924,7 +927,6 @@ extern "C" int tpb200_paged_attention(const tpb200_paged_attention_args* a, tpb2
     P.join_by_item = items < static_cast<long long>(ctas) * kWarps;
     P.q = static_cast<const uint16_t*>(a->q);
     P.out = static_cast<uint16_t*>(a->out);
-    P.scale2 = a->scale * 1.4426950408889634f;
     const bool bf = a->cache.dtype == TPB200_BF16;
     const int D = P.cache.head_dim;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);

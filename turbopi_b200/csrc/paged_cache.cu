@@ -237,6 +237,14 @@ extern "C" int tpb200_paged_append(const tpb200_paged_append_args* a, tpb200_str
         P.o_stride[i] = a->o_stride[i];
     }
     if (a->tokens == 0 || P.cache.seqs == 0) return TPB200_OK;
+    TPB_REQUIRE(a->cache.k_pages != a->cache.v_pages, TPB200_ERR_SHAPE);
+    if (a->q != nullptr) {               // other threads read what lies there
+        const int D = P.cache.head_dim, H = P.cache.kv_heads;
+        const RowSet out(a->q_out, a->o_stride, a->tokens, a->q_heads, D);
+        TPB_REQUIRE(output_fits(out, RowSet(a->q, a->q_stride, a->tokens, a->q_heads, D)), TPB200_ERR_SHAPE);
+        TPB_REQUIRE(!rows_meet(out, RowSet(a->k, a->k_stride, a->tokens, H, D)) && !rows_meet(out, RowSet(a->v, a->v_stride, a->tokens, H, D)),
+                    TPB200_ERR_SHAPE);
+    }
     P.k = static_cast<const uint16_t*>(a->k);
     P.v = static_cast<const uint16_t*>(a->v);
     P.q = static_cast<const uint16_t*>(a->q);

@@ -815,7 +815,8 @@ def paged_append(k, v, k_pages, v_pages, table, cu, lengths, q=None, cos=None, s
     k / v [T, Hk, D], q [T, Hq, D]: the sequences' tokens one behind the other, sequence s at [cu[s], cu[s + 1]) (cu int32 [S + 1]);
     its last token goes to position lengths[s] - 1.  Tokens behind cu[S] are left alone, in q_out too.
     cos / sin [positions, D / 2] (fp32, fp16 or bf16): keys and queries are rotated (rotate-half, in fp32, rounded once); q_out
-    may be q."""
+    may be q and shares no other elements with q, k or v.  Keys for packed_attention come back rotated when they are passed with the
+    queries: q = qkv[:, :Hq + Hk], k = qkv[:, Hq:Hq + Hk]."""
     done = (_lib._native or _lib.native()).paged_append(k, v, k_pages, v_pages, table, cu, lengths, q, cos, sin, q_out, _flags.value)
     if done is not None:
         done = _result(done, "tpb200_paged_append")
