@@ -704,8 +704,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attention_kernel(c
     const bool whole = whole_item;
     const int kvh = work.h / P.tiles, row0 = (work.h - kvh * P.tiles) * S::kRows;
     const long long part = 2ll * kWarps * cta;
-    for (int u = threadIdx.x; u < min(P.group - row0, S::kRows) * (D / 4); u += kThreads) {
-        const int row = u / (D / 4), col = (u - row * (D / 4)) * 4;
+    const int rows = min(P.group - row0, S::kRows);
+#pragma unroll 4
+    for (int u = threadIdx.x; u < S::kRows * (DP / 4); u += kThreads) {
+        const int row = u / (DP / 4), col = u % (DP / 4) * 4;
+        if (row >= rows || col >= D) continue;
         float M = -INFINITY, L = 0.0f;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) M = fmaxf(M, ctl->ml[w][row][0]);
