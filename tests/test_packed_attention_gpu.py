@@ -308,3 +308,20 @@ def test_launches_behind_copies_fills_and_another_stream(cuda_device):
     for _ in range(20):
         graph.replay()
         assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("hq,hk,D", [(4, 2, 64), (3, 1, 40), (4, 2, 128)])
+def test_growing_maxima_with_two_row_tiles(cuda_device, hq, hk, D, dtype):
+    """Long sequences, the reference raised in every tile: small heads have the next scores, and the last product, under way meanwhile."""
+    from turbopi_b200 import ops
+    lens, klens = [1300, 1150], [1300, 1400]
+    q, k, v = _problem(lens, klens, hq, hk, D, dtype, cuda_device, seed=9)
+    k *= torch.linspace(0.05, 8, sum(klens), device=cuda_device).to(k.dtype)[:, None, None]
+    cu, cuk = _offsets(lens, cuda_device), _offsets(klens, cuda_device)
+    for causal in (True, False):
+        first = ops.packed_attention(q, k, v, cu, 0.3, causal=causal, cu_keys=cuk)
+        _check(first, q, k, v, lens, klens, 0.3, causal)
+        for _ in range(5):
+            assert torch.equal(ops.packed_attention(q, k, v, cu, 0.3, causal=causal, cu_keys=cuk), first)
+    _no_error()

@@ -20,7 +20,7 @@
 //     side, eight of its rows zeros, 16 KB of cache took 1043 warp instructions and 48 ragged sequences 55 us instead of 45.)
 //
 // What bounds it: inside a piece the stream runs at 6.2-6.6 TB/s, the measured copy rate; around it lie 2 us until a warp knows its piece,
-// a spread of 12 % between SMs, and 3-5 us for the second kernel.  Calls in a CUDA graph: 3 sequences, 260 k keys, fp16, 8 on 1 heads
+// SMs that get 5-10 % less of the bandwidth (the same ones in every run), and 3-5 us for the second kernel.  Calls in a CUDA graph: 3 sequences, 260 k keys, fp16, 8 on 1 heads
 // of 256 (267 MB) 54 us = 4.9 TB/s; 48 sequences of 1 to 4096, 32 on 8 of 128 (160 MB) 38 us = 4.2; 128 of 16 to 2000, 16 on 16 of
 // 64 (215 MB) 49 us = 4.4; one sequence of 762 keys 9.6 us, all latency.  Equal pieces per CTA, items not weighed, took 45 and 69 us for
 // the two batches: CTAs with many short items were done last.
