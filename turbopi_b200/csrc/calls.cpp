@@ -3,7 +3,8 @@
 // reference for what is accepted: whatever a function here does not recognise as its plain case (a CPU tensor, another
 // device, a dtype or a stride that needs a conversion) returns None and takes the Python form, which converts or refuses.
 // A non-zero status of the C ABI comes back as an int.  Time to issue a call (us, Python form -> here): one-token INT4 linear
-// 13.1 -> 7.1, 50-token MLP 31.2 -> 17.4, attention 18.2 -> 8.2, W4A4 linear 21.7 -> 12.4, FP8 quantiser + W4A8 launcher 24.4 -> 18.1.
+// 13.1 -> 7.1, 50-token MLP 31.2 -> 17.4, attention 18.2 -> 8.2, W4A4 linear 21.7 -> 12.4, FP8 quantiser + W4A8 launcher 24.4 -> 18.1,
+// attention on packed prompts or a paged cache, appends, page copies 20-50 -> 4-8.
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
