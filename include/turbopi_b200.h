@@ -441,8 +441,9 @@ int tpb200_packed_attention(const tpb200_packed_attention_args* args, tpb200_str
  * elements, multiples of 8): row r of head h of page p starts at p * page_stride + r * row_stride + h * head_stride.  Position j of
  * sequence s is row j % page_size of page table[s * table_stride + j / page_size].  bf16 or fp16; head_dim a multiple of 8, <= 256.
  * table and lengths are read on the device, so a captured call follows them.  What they must not hold is checked
- * there: a page id outside the pool, a position outside the table or a length beyond table_width * page_size is skipped, and
- * tpb200_device_error() reports 501.  table_width * page_size < 2^31.
+ * there and skipped, and tpb200_device_error() reports 501: positions whose page id lies outside the pool (the -1 behind a sequence's
+ * pages) and positions beyond table_width * page_size are no keys of their sequence, and nothing is written there.
+ * table_width * page_size < 2^31.
  * The launches of this section and of packed attention wait for what is before them ahead of everything they touch, so they start as
  * dependents with or without TPB200_FLAG_PDL, and let the next launch in behind that wait.
  * ------------------------------------------------------------------------------------------- */
@@ -456,7 +457,7 @@ typedef struct {
 
 /* Attention of one new token per sequence on the cache: out[s] = softmax(scale * q[s] K^T) V over the first lengths[s] positions
  * (the new token's own key among them); query heads [h * g, (h + 1) * g) read key head h, g = q_heads / kv_heads; fp32 sums,
- * outputs rounded once.  A sequence of length 0 gives zeros.  q / out: element strides of a sequence and of a head, multiples of 8.
+ * outputs rounded once.  A sequence without keys (length 0, or none of its pages in the pool) gives zeros.  q / out: element strides of a sequence and of a head, multiples of 8.
  * The lengths' sum is cut into equal pieces over the GPU whatever the single lengths; items that cross a cut are joined by a second
  * small kernel through `workspace` (no initialisation needed; its size depends on the heads only).  out may be q (row on row, not in part).  All lengths decide
  * where the cuts fall, and so the order of a sequence's sums; the same call gives the same bits. */

@@ -26,6 +26,7 @@
 // the two batches: CTAs with many short items were done last.
 #include <algorithm>
 #include <atomic>
+#include <cfloat>
 #include <cmath>
 #include <type_traits>
 
@@ -40,6 +41,7 @@ constexpr int kSlotBytes = 8192;
 constexpr int kSlots = 3;
 constexpr int kCtasPerSm = 2;
 constexpr int kSlotUnits = 2, kItemUnits = 1;      // what a slot costs, and an item besides: queries, sums, the output
+constexpr float kLowest = -FLT_MAX;      // the least reference of a row with a key
 constexpr int kLengths = 1024;           // lengths kept in shared memory; with more sequences they are read where they lie
 
 struct DecodeParams {
@@ -122,6 +124,9 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+
+// 1 over the sum of the weights; a row without any key (its reference never left -infinity) gives zeros
+__device__ __forceinline__ float inverse(float reference, float sum) { return reference == -INFINITY ? 0.0f : 1.0f / sum; }
 
 // keys of a sequence that the cache can hold: a length beyond the table's pages is an error, not an address
 __device__ __forceinline__ int keys_of(const PagedView& c, int s) {
@@ -317,6 +322,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attention_kernel(c
     int page_id[kPlaces];                // of this lane's rows of the next slot to load
     long long row_at[kPlaces];           // of the slot whose keys were asked for last: element offsets, -1: no such row
     int there = 0;                       // its keys
+    // Keys whose page is not in the pool, a bit per group of 16 (aligned) or per key: of the slot whose keys were asked for last, and of the
+    // one before it, which is the one that is worked on.
+    constexpr int kKeysPerBit = kAligned ? 16 : 1;
+    using Absent = std::conditional_t<(S::kKeys / kKeysPerBit > 32), uint64_t, uint32_t>;
+    Absent absent_next = 0, absent = 0;
 
     // the key whose place lane `lane` looks up: aligned, the first of a group of 16; else its own
     auto own_key = [&](int o) { return load.ci * S::kKeys + (kAligned ? (lane * 16) % S::kKeys : o * 32 + lane); };
@@ -336,13 +346,16 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attention_kernel(c
         for (int o = 0; o < kPlaces; ++o) {
             const int key = own_key(o);
             row_at[o] = -1;
-            if (key < load.len && (kAligned || o * 32 + lane < S::kKeys)) {
-                if (static_cast<unsigned>(page_id[o]) < static_cast<unsigned>(P.cache.num_pages)) {
-                    row_at[o] = page_id[o] * P.cache.page_stride + (key % P.cache.page_size) * P.cache.row_stride +
-                                load.h / P.tiles * P.cache.head_stride;
-                } else {
-                    record_error(kErrPagedIndex);
-                }
+            const bool in = key < load.len && (kAligned || o * 32 + lane < S::kKeys);
+            const bool known = static_cast<unsigned>(page_id[o]) < static_cast<unsigned>(P.cache.num_pages);
+            if (in && known) {
+                row_at[o] = page_id[o] * P.cache.page_stride + (key % P.cache.page_size) * P.cache.row_stride +
+                            load.h / P.tiles * P.cache.head_stride;
+            }
+            const uint32_t gone = __ballot_sync(0xffffffffu, in && !known);
+            if (gone != 0) {
+                record_error(kErrPagedIndex);
+                absent_next |= kAligned ? gone & ((1u << (S::kKeys / 16)) - 1) : static_cast<Absent>(gone) << (o * 32);
             }
         }
         --left;
@@ -516,18 +529,21 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attention_kernel(c
                         for (int j = 0; j < 4; ++j) sc[b][n][j] += odd[b][n][j];
                 // ---- a query head's scores lie in the lanes of equal lane % 4.  The reference is raised only when a score passes
                 // it by 8 (weights stay below 2^8), so the maximum crosses the lanes hardly ever.
+                // A slot with a key has a finite reference, whatever the score: one of -infinity at the end means that there was no key.
+                const bool some = absent == 0 || __popcll(absent) < (min(valid, S::kKeys) + kKeysPerBit - 1) / kKeysPerBit;
                 float top[NT][2];
 #pragma unroll
-                for (int n = 0; n < NT; ++n) top[n][0] = top[n][1] = -INFINITY;
-                if (valid < S::kKeys) {
+                for (int n = 0; n < NT; ++n) top[n][0] = top[n][1] = some ? kLowest : -INFINITY;
+                if (valid < S::kKeys || absent != 0) {
 #pragma unroll
                     for (int b = 0; b < S::kKeys / 16; ++b)
 #pragma unroll
-                        for (int n = 0; n < NT; ++n)
+                        for (int j = 0; j < 4; ++j) {
+                            const int key = b * 16 + (lane >> 2) + (j >> 1) * 8;
+                            const bool seen = key < valid && ((absent >> (kAligned ? b : key)) & 1) == 0;
 #pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                sc[b][n][j] = b * 16 + (lane >> 2) + (j >> 1) * 8 < valid ? sc[b][n][j] * P.scale2 : -INFINITY;
-                            }
+                            for (int n = 0; n < NT; ++n) sc[b][n][j] = seen ? sc[b][n][j] * P.scale2 : -INFINITY;
+                        }
                 } else {
 #pragma unroll
                     for (int b = 0; b < S::kKeys / 16; ++b)
@@ -595,6 +611,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attention_kernel(c
             }
             __syncwarp();
         }
+        if ((t & 1) == 0) {
+            absent = absent_next;
+            absent_next = 0;
+        }
         if (t < uses) {
             if ((t & 1) == 0) enter_slot();
             copy_rows(static_cast<const uint16_t*>((t & 1) == 0 ? P.cache.k_pages : P.cache.v_pages), at);
@@ -625,7 +645,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attention_kernel(c
             for (int j = 0; j < 2; ++j) {
 #pragma unroll
                 for (int x = 4; x < 32; x <<= 1) l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], x);
-                f[n][j] = whole ? 1.0f / l[n][j] : 1.0f;
+                f[n][j] = whole ? inverse(m[n][j], l[n][j]) : 1.0f;
                 const int row = n * 8 + (lane & 3) * 2 + j;
                 if (!whole && lane < 4 && row < P.rows) {
                     *reinterpret_cast<float2*>(P.part_ml + (part * P.rows + row) * 2) = make_float2(m[n][j], l[n][j]);
@@ -721,7 +741,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attention_kernel(c
             sum.x += y.x * f; sum.y += y.y * f; sum.z += y.z * f; sum.w += y.w * f;
         }
         if (whole) {
-            const float inv = 1.0f / L;
+            const float inv = inverse(M, L);
             uint16_t* to = P.out + work.s * P.o_stride[0] + (kvh * P.group + row0 + row) * P.o_stride[1] + col;
             *reinterpret_cast<uint2*>(to) = make_uint2(Half16<T>::pack(sum.x * inv, sum.y * inv), Half16<T>::pack(sum.z * inv, sum.w * inv));
         } else {
@@ -817,7 +837,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attention_join_kernel(cons
             l += ml.y * w;
             sum.x += x.x * w; sum.y += x.y * w; sum.z += x.z * w; sum.w += x.w * w;
         }
-        const float inv = 1.0f / l;
+        const float inv = inverse(m, l);
         uint16_t* to = P.out + s * P.o_stride[0] + (kvh * P.group + head) * P.o_stride[1] + col;
         *reinterpret_cast<uint2*>(to) = make_uint2(Half16<T>::pack(sum.x * inv, sum.y * inv), Half16<T>::pack(sum.z * inv, sum.w * inv));
     }

@@ -782,7 +782,7 @@ def paged_attention(q, k_pages, v_pages, table, lengths, scale, out=None, worksp
     q / out [S, Hq, D]; pages [P, page, Hk, D] (one layer; Hq a multiple of Hk, consecutive query heads share a key head); table
     int32 [S, W]: position j of sequence s is row j % page of page table[s, j // page]; lengths int32 [S], the new token among them.
     bf16 or fp16.  A sequence of length 0 gives zeros.  table and lengths are read on the device: a captured call follows
-    them, and what they must not hold is reported by tpb200_device_error()."""
+    them.  Positions without a page in the pool, or beyond the table, are left out and reported by tpb200_device_error()."""
     done = (_lib._native or _lib.native()).paged_attention(q, k_pages, v_pages, table, lengths, scale, out, workspace, _flags.value)
     if done is not None:
         return _result(done, "tpb200_paged_attention")
