@@ -419,7 +419,8 @@ int tpb200_attention_describe(int n_rows, int n_keys, int head_dim, int groups, 
 /* ---------------------------------------------------------------------------------------------
  * Attention over prompts packed one behind the other.  Sequence s has the queries [cu[s], cu[s + 1]) and the keys
  * [cu_keys[s], cu_keys[s + 1]) (cu_keys NULL: the same offsets); out = softmax(scale * Q K^T) V per sequence and head.  causal != 0: query i of
- * n sees the keys up to i + (m - n) of m, so queries may stand behind keys that were there before them.  A query without
+ * n sees the keys up to i + (m - n) of m, so queries may stand behind keys that were there before them.  Weights are rounded to the tensors'
+ * type for their product with the values, sums are fp32, outputs rounded once.  A query without
  * keys gives zeros.  Query heads [h * g, (h + 1) * g) read key head h.  q / out [q_tokens, q_heads, head_dim], k / v
  * [k_tokens, kv_heads, head_dim] with element strides of a token and a head, multiples of 8 that do not overlap; bf16 or fp16;
  * head_dim a multiple of 8, <= 256.  Tokens before cu[0] and behind cu[seqs] are left alone; out may be q.  The offsets are read on the
@@ -456,8 +457,8 @@ typedef struct {
 } tpb200_paged_cache;
 
 /* Attention of one new token per sequence on the cache: out[s] = softmax(scale * q[s] K^T) V over the first lengths[s] positions
- * (the new token's own key among them); query heads [h * g, (h + 1) * g) read key head h, g = q_heads / kv_heads; fp32 sums,
- * outputs rounded once.  A sequence without keys (length 0, or none of its pages in the pool) gives zeros.  q / out: element strides of a sequence and of a head, multiples of 8.
+ * (the new token's own key among them); query heads [h * g, (h + 1) * g) read key head h, g = q_heads / kv_heads; weights
+ * rounded to the cache's type for their product with the values, fp32 sums, outputs rounded once.  A sequence without keys (length 0, or none of its pages in the pool) gives zeros.  q / out: element strides of a sequence and of a head, multiples of 8.
  * The lengths' sum is cut into equal pieces over the GPU whatever the single lengths; items that cross a cut are joined by a second
  * small kernel through `workspace` (no initialisation needed; its size depends on the heads only).  out may be q (row on row, not in part).  All lengths decide
  * where the cuts fall, and so the order of a sequence's sums; the same call gives the same bits. */

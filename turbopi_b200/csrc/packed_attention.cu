@@ -3,8 +3,9 @@
 //
 // One pass over the keys per tile of 128 query rows, with the running reference m of a softmax:
 //     S = Q K_j^T,  P = 2^(scale2 S - m),  O += P V_j,  l += rowsum P,      out = O / l
-// m is raised (and O, l scaled by 2^(m_old - m_new)) only when a row's maximum passes m by 8: P stays below 2^8, which costs no
-// relative precision in either type, and after the first tiles O is hardly ever touched between its products.
+// m is raised (and O, l scaled by 2^(m_old - m_new)) only when a row's maximum passes m by 8, a published way to run a softmax: P stays below
+// 2^8 and after the first tiles O is hardly ever touched between its products.  P is rounded to the tensors' type; fp16 holds it 2^7 times
+// larger (Half16::kLift), so that small weights keep their bits.
 //
 // A row of a tile is a (token, head) pair: `pack` query heads of one key head, the largest power of two in the group, side by side,
 // so that short prompts fill tiles and the heads of a group read their keys once.
@@ -635,8 +636,8 @@ __global__ void __launch_bounds__(Layout<DP, R>::kThreads, Layout<DP, R>::kCtas)
                 l *= ex2(l_ref - base);
                 l_ref = ref;
             }
-            // P = 2^(scale2 S - m), its row sum, rounded pairs into the columns S was in
-            const uint64_t scale = pair(P.scale2, P.scale2), minus = pair(-base, -base);
+            // P = 2^(scale2 S - m), its row sum (before rounding), rounded pairs into the columns S was in
+            const uint64_t scale = pair(P.scale2, P.scale2), minus = pair(Half16<T>::kLift - base, Half16<T>::kLift - base);
             uint64_t sum[2] = {pair(0.0f, 0.0f), pair(0.0f, 0.0f)};
 #pragma unroll
             for (int c = 0; c < kTile / 2; c += 32) {

@@ -7,11 +7,15 @@
 
 namespace tpb {
 
-// Pairs of a 16-bit type in a 32-bit word
+// Pairs of a 16-bit type in a 32-bit word.  kLift: softmax weights, which are rounded to the type for their product with the values, are held
+// 2^kLift times larger than against their reference, which the sum's division takes out again.  fp16 has no exponents below -14 and steps of
+// 2^-24 there; a weight is at most 2^8 of its reference, so seven bits are free at the other end (2^15 < 65504), and weights keep their eleven bits
+// down to 2^-21 and vanish below 2^-32.  bf16 has fp32's exponents.
 template <typename T>
 struct Half16;
 template <>
 struct Half16<__nv_bfloat16> {
+    static constexpr float kLift = 0.0f;
     static __device__ __forceinline__ float2 unpack(uint32_t w) {
         return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
     }
@@ -28,6 +32,7 @@ struct Half16<__nv_bfloat16> {
 };
 template <>
 struct Half16<__half> {
+    static constexpr float kLift = 7.0f;
     static __device__ __forceinline__ float2 unpack(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
     static __device__ __forceinline__ uint32_t pack(float a, float b) {
         const __half2 h = __floats2half2_rn(a, b);

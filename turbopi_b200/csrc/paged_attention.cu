@@ -581,10 +581,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attention_kernel(c
                         }
                     }
                 }
-                // ---- weights, rounded to the values' type for the second product, transposed into its B operand
+                // ---- weights, rounded to the values' type for the second product (their sum is that of the unrounded ones), transposed into
+                // its B operand
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    const float b0 = m[n][0] == -INFINITY ? 0.0f : m[n][0], b1 = m[n][1] == -INFINITY ? 0.0f : m[n][1];
+                    const float b0 = (m[n][0] == -INFINITY ? 0.0f : m[n][0]) - Half16<T>::kLift, b1 = (m[n][1] == -INFINITY ? 0.0f : m[n][1]) - Half16<T>::kLift;
 #pragma unroll
                     for (int b = 0; b < S::kKeys / 16; ++b) {
                         float w[4];
