@@ -135,6 +135,10 @@ __device__ __forceinline__ int keys_of(const PagedView& c, int s) {
     return max(0, min(n, most));
 }
 
+// Lengths go up to 2^31 - 1: a length rounded up to whole slots, and the place of a key behind the last one in its slot, are unsigned
+template <int kKeys>
+__device__ __forceinline__ int slots_of(int len) { return static_cast<int>((static_cast<unsigned>(len) + kKeys - 1) / kKeys); }
+
 // A place in the line of slots: slot `ci` of item (sequence, tile of query heads)
 template <int kKeys>
 struct Place {
@@ -146,7 +150,7 @@ struct Place {
             len = P.cache.seqs <= kLengths ? lengths[s] : keys_of(P.cache, s);
             if (len > 0) break;
         }
-        n = (len + kKeys - 1) / kKeys;
+        n = slots_of<kKeys>(len);
         h = ci = 0;
     }
     __device__ __forceinline__ void next(const DecodeParams& P, const int* lengths) {
@@ -212,7 +216,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attention_kernel(c
     int slots_here = 0, units_here = 0;
     bool empty = false;
     for (int s = s0; s < s1; ++s) {
-        const int len = keys_of(P.cache, s), n = (len + S::kKeys - 1) / S::kKeys;
+        const int len = keys_of(P.cache, s), n = slots_of<S::kKeys>(len);
         if (staged) ctl->lengths[s] = len;
         slots_here += n * heads;
         units_here += n > 0 ? (n * kSlotUnits + kItemUnits) * heads : 0;
@@ -258,7 +262,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attention_kernel(c
         int s = s0, slots = slots_to - slots_here, units = units_to - units_here;
         if (here) {
             for (;; ++s) {
-                const int n = (length(s) + S::kKeys - 1) / S::kKeys, more = n > 0 ? (n * kSlotUnits + kItemUnits) * heads : 0;
+                const int n = slots_of<S::kKeys>(length(s)), more = n > 0 ? (n * kSlotUnits + kItemUnits) * heads : 0;
                 if (unit < units + more) break;
                 slots += n * heads;
                 units += more;
@@ -270,7 +274,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attention_kernel(c
         units = __shfl_sync(0xffffffffu, units, from);
         work.s = s;
         work.len = length(s);
-        work.n = (work.len + S::kKeys - 1) / S::kKeys;
+        work.n = slots_of<S::kKeys>(work.len);
         const int item = work.n * kSlotUnits + kItemUnits;
         work.h = (unit - units) / item;
         work.units = item_first = units + work.h * item;
@@ -329,13 +333,13 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attention_kernel(c
     Absent absent_next = 0, absent = 0;
 
     // the key whose place lane `lane` looks up: aligned, the first of a group of 16; else its own
-    auto own_key = [&](int o) { return load.ci * S::kKeys + (kAligned ? (lane * 16) % S::kKeys : o * 32 + lane); };
+    auto own_key = [&](int o) { return static_cast<unsigned>(load.ci * S::kKeys) + (kAligned ? (lane * 16) % S::kKeys : o * 32 + lane); };
     auto fetch_ids = [&]() {             // page ids of the slot at `load`, asked for one slot ahead of their use
 #pragma unroll
         for (int o = 0; o < kPlaces; ++o) {
-            const int key = own_key(o);
+            const unsigned key = own_key(o);
             page_id[o] = -1;
-            if (left > 0 && key < load.len && (kAligned || o * 32 + lane < S::kKeys)) {
+            if (left > 0 && key < static_cast<unsigned>(load.len) && (kAligned || o * 32 + lane < S::kKeys)) {
                 page_id[o] = P.cache.table[load.s * P.cache.table_stride + key / P.cache.page_size];
             }
         }
@@ -344,9 +348,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attention_kernel(c
         there = min(load.len - load.ci * S::kKeys, S::kKeys);
 #pragma unroll
         for (int o = 0; o < kPlaces; ++o) {
-            const int key = own_key(o);
+            const unsigned key = own_key(o);
             row_at[o] = -1;
-            const bool in = key < load.len && (kAligned || o * 32 + lane < S::kKeys);
+            const bool in = key < static_cast<unsigned>(load.len) && (kAligned || o * 32 + lane < S::kKeys);
             const bool known = static_cast<unsigned>(page_id[o]) < static_cast<unsigned>(P.cache.num_pages);
             if (in && known) {
                 row_at[o] = page_id[o] * P.cache.page_stride + (key % P.cache.page_size) * P.cache.row_stride +
