@@ -423,7 +423,7 @@ int tpb200_attention_describe(int n_rows, int n_keys, int head_dim, int groups, 
  * type for their product with the values, sums are fp32, outputs rounded once.  A query without
  * keys gives zeros.  Query heads [h * g, (h + 1) * g) read key head h.  q / out [q_tokens, q_heads, head_dim], k / v
  * [k_tokens, kv_heads, head_dim] with element strides of a token and a head, multiples of 8 that do not overlap; bf16 or fp16;
- * head_dim a multiple of 8, <= 256.  Tokens before cu[0] and behind cu[seqs] are left alone; out may be q.  The offsets are read on the
+ * head_dim a multiple of 8, <= 256; up to 2^31 - 1024 queries and keys.  Tokens before cu[0] and behind cu[seqs] are left alone; out may be q.  The offsets are read on the
  * device (a captured call follows them); ones outside the tensors are clamped to them.  An output that shares
  * elements with k or v, or with q other than row on row, is refused.  What stands in masked places (keys and
  * values of later tokens, of other sequences, of nobody) does not matter, infinities and NaN included.

@@ -58,6 +58,7 @@ constexpr int kTile = 128;               // rows of a query tile, keys of a key 
 constexpr int kBlockBytes = kTile * 128; // 128 rows x 64 columns of 16 bits
 constexpr long long kWait = 200000000LL; // about 0.1 s: the bound of each wait
 constexpr float kRaise = 8.0f;
+constexpr int kMaxTokens = 0x7fffffff - 1023;        // positions are 32 bits, and up to four tiles' rows behind the last one are counted
 constexpr int kBadTiles = 4;             // key tiles with masked pairs at most: 256 rows on the diagonal and the sequence's end
 
 struct PackedParams {
@@ -792,6 +793,7 @@ extern "C" int tpb200_packed_attention(const tpb200_packed_attention_args* a, tp
     TPB_REQUIRE((a->flags & ~TPB200_FLAG_PDL) == 0, TPB200_ERR_ENUM);
     TPB_REQUIRE(a->dtype == TPB200_BF16 || a->dtype == TPB200_F16, TPB200_ERR_ENUM);
     TPB_REQUIRE(a->seqs >= 0 && a->q_tokens >= 0 && a->k_tokens >= 0, TPB200_ERR_SHAPE);
+    TPB_REQUIRE(a->q_tokens <= kMaxTokens && a->k_tokens <= kMaxTokens, TPB200_ERR_SHAPE);
     TPB_REQUIRE(a->q_heads >= 1 && a->kv_heads >= 1 && a->q_heads % a->kv_heads == 0, TPB200_ERR_SHAPE);
     TPB_REQUIRE(a->head_dim >= 8 && a->head_dim <= 256 && a->head_dim % 8 == 0, TPB200_ERR_SHAPE);
     if (a->seqs == 0 || a->q_tokens == 0) return TPB200_OK;
