@@ -210,7 +210,7 @@ extern "C" int tpb200_paged_append(const tpb200_paged_append_args* a, tpb200_str
     AppendParams P = {};
     const int st = paged_view(a->cache, &P.cache);
     if (st != TPB200_OK) return st;
-    TPB_REQUIRE(a->k && a->v && a->cu, TPB200_ERR_NULL);
+    TPB_REQUIRE(a->tokens == 0 || (a->k && a->v && a->cu), TPB200_ERR_NULL);      // tensors of no tokens have no memory
     TPB_REQUIRE((a->flags & ~TPB200_FLAG_PDL) == 0, TPB200_ERR_ENUM);
     TPB_REQUIRE(a->tokens >= 0, TPB200_ERR_SHAPE);
     const bool rope = a->cos != nullptr || a->sin != nullptr;
