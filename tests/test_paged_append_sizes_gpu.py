@@ -1,4 +1,4 @@
-"""ops.paged_append of no tokens at all."""
+"""ops.paged_append of no tokens at all, and of as many as 32 bits count."""
 import pytest
 import torch
 
@@ -27,3 +27,17 @@ def test_no_tokens(cuda_device, monkeypatch, native):
     empty = cache.extend([], [])
     assert cache.append(0, empty, k, k) is None
     assert torch.equal(cache.pages, before) and _lib.load().tpb200_device_error(0) == 0
+
+
+def test_as_many_tokens_as_32_bits_count(cuda_device):
+    """2^31 - 1 tokens (34 GB, keys and values the same ones), of which the last three have a place."""
+    from turbopi_b200 import _lib, ops
+    n = 2 ** 31 - 1
+    kv = torch.empty((n, 1, 8), dtype=torch.bfloat16, device=cuda_device)
+    kv[-4:] = torch.arange(32, device=cuda_device, dtype=torch.bfloat16).view(4, 1, 8)
+    pages = torch.zeros((2, 2, 16, 1, 8), dtype=torch.bfloat16, device=cuda_device)
+    want = pages.clone()
+    want[:, 1, 14:, 0], want[:, 0, 0, 0] = kv[-3:-1, 0], kv[-1, 0]
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda_device)      # noqa: E731
+    ops.paged_append(kv, kv, pages[0], pages[1], ints([[1, 0]]), ints([n - 3, n]), ints([17]))
+    assert torch.equal(pages, want) and _lib.load().tpb200_device_error(0) == 0

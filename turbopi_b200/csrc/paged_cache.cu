@@ -263,7 +263,7 @@ extern "C" int tpb200_paged_append(const tpb200_paged_append_args* a, tpb200_str
     P.units_k = P.units_v = static_cast<int>(per_head * P.cache.kv_heads);
     // four tokens share a block's look-up, fewer where that would leave SMs without a block
     P.tokens_per_block = std::max(1, std::min(kMaxTokensPerBlock, a->tokens / 444));
-    const unsigned blocks = static_cast<unsigned>((a->tokens + P.tokens_per_block - 1) / P.tokens_per_block);
+    const unsigned blocks = static_cast<unsigned>((a->tokens - 1) / P.tokens_per_block + 1);
     const bool bf = a->cache.dtype == TPB200_BF16;
     auto kernel = bf ? (V == 8 ? paged_append_kernel<__nv_bfloat16, 8> : paged_append_kernel<__nv_bfloat16, 4>)
                      : (V == 8 ? paged_append_kernel<__half, 8> : paged_append_kernel<__half, 4>);
