@@ -258,11 +258,19 @@ py::object nvfp4_linear(const at::Tensor& x, const at::Tensor& w, int64_t N, dou
 }
 
 // ------------------------------------------------------------------------------------------------ a cache of pages
+// sizes that the 32 bits of the C structures hold; others are refused by the Python forms
+bool fits(at::IntArrayRef sizes) {
+    for (const int64_t n : sizes) {
+        if (n > 0x7fffffff) return false;
+    }
+    return true;
+}
+
 bool half(const at::Tensor& t) { return t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf; }
 
 // [tokens, heads, D] of one type and device with a contiguous last dimension
 bool rows(const at::Tensor& t, int dev, int64_t tokens, int64_t heads, int64_t D, at::ScalarType type) {
-    return on(t, dev) && t.dim() == 3 && t.size(0) == tokens && t.size(1) == heads && t.size(2) == D && t.scalar_type() == type && t.stride(2) == 1;
+    return on(t, dev) && t.dim() == 3 && t.size(0) == tokens && t.size(1) == heads && t.size(2) == D && fits(t.sizes()) && t.scalar_type() == type && t.stride(2) == 1;
 }
 bool offsets(const at::Tensor& t, int dev, int64_t n) {
     return on(t, dev) && t.dim() == 1 && t.numel() == n && t.scalar_type() == at::kInt && t.is_contiguous();
@@ -276,7 +284,7 @@ bool paged(const at::Tensor& k, const at::Tensor& v, const at::Tensor& table, co
     if (!on(k, dev) || !on(v, dev) || !on(table, dev) || !on(lengths, dev) || k.dim() != 4 || !half(k) || v.scalar_type() != k.scalar_type() ||
         v.sizes() != k.sizes() || v.strides() != k.strides() || k.stride(3) != 1 || table.dim() != 2 || table.scalar_type() != at::kInt ||
         lengths.dim() != 1 || lengths.scalar_type() != at::kInt || lengths.numel() != table.size(0) || !lengths.is_contiguous() ||
-        (table.size(1) > 1 && table.stride(1) != 1)) {
+        (table.size(1) > 1 && table.stride(1) != 1) || !fits(k.sizes()) || !fits(table.sizes())) {
         return false;
     }
     c.k_pages = k.data_ptr();
@@ -344,7 +352,7 @@ py::object paged_append(const at::Tensor& k, const at::Tensor& v, const at::Tens
     }
     if (cos.has_value()) {
         if (!on(*cos, dev) || !on(*sin, dev) || cos->dim() != 2 || cos->sizes() != sin->sizes() || cos->size(1) != D / 2 ||
-            cos->scalar_type() != sin->scalar_type() || code_of(cos->scalar_type()) < 0 || !cos->is_contiguous() || !sin->is_contiguous()) {
+            cos->scalar_type() != sin->scalar_type() || code_of(cos->scalar_type()) < 0 || !cos->is_contiguous() || !sin->is_contiguous() || !fits(cos->sizes())) {
             return py::none();
         }
         a.cos = cos->data_ptr();
@@ -385,7 +393,7 @@ py::object packed_attention(const at::Tensor& q, const at::Tensor& k, const at::
     const int64_t T = q.size(0), H = q.size(1), D = q.size(2), Tk = k.size(0), Hk = k.size(1);
     const auto type = q.scalar_type();
     if (!rows(q, dev, T, H, D, type) || !rows(k, dev, Tk, Hk, D, type) || !rows(v, dev, Tk, Hk, D, type) || cu.numel() < 1 ||
-        !offsets(cu, dev, cu.numel()) || (cu_keys.has_value() ? !offsets(*cu_keys, dev, cu.numel()) : Tk != T) ||
+        !offsets(cu, dev, cu.numel()) || !fits(cu.sizes()) || (cu_keys.has_value() ? !offsets(*cu_keys, dev, cu.numel()) : Tk != T) ||
         (out.has_value() && !rows(*out, dev, T, H, D, type))) {
         return py::none();
     }
@@ -435,10 +443,12 @@ py::object copy_pages(const at::Tensor& pages, const py::object& src, const py::
         }
     }
     const int64_t P = pages.size(-4), page_bytes = pages.stride(-4) * pages.element_size(), slab = page_bytes * P;
+    const int64_t slabs = static_cast<int64_t>(pages.nbytes()) / slab;
+    if (!fits({P, slabs})) return py::none();
     void* base = pages.data_ptr();
     const tpb200_stream_t s = stream_of(dev);
     const int st = launch([&] {
-        return g.copy_pages(base, slab, static_cast<int>(pages.nbytes() / slab), page_bytes, static_cast<int>(P), ids.data(), ids.data() + n,
+        return g.copy_pages(base, slab, static_cast<int>(slabs), page_bytes, static_cast<int>(P), ids.data(), ids.data() + n,
                             static_cast<int>(n), flags, s);
     });
     return st == 0 ? py::object(py::bool_(true)) : py::int_(st);

@@ -712,8 +712,14 @@ def _paged_view(what, k_pages, v_pages, table, lengths):
         raise TurboPiError(f"{what}: one contiguous length per row of the table, rows contiguous")
     _one_device(what, k_pages, v_pages, table, lengths)
     P, page, H, D = k_pages.shape
+    _counts(what, P, page, H, W, S)
     return _lib.PagedCacheView(_ptr(k_pages), _ptr(v_pages), k_pages.stride(0), k_pages.stride(1), k_pages.stride(2), P, page, H, D,
                                _HALF[k_pages.dtype], _ptr(table), table.stride(0), W, _ptr(lengths), S)
+
+
+def _counts(what, *sizes):
+    if any(n >= 2 ** 31 for n in sizes):
+        raise TurboPiError(f"{what}: sizes are 32 bits wide, {max(sizes)} is not")
 
 
 def _one_device(what, first, *others):
@@ -759,6 +765,7 @@ def packed_attention(q, k, v, cu, scale, out=None, causal=True, cu_keys=None):
     if cu.numel() < 1 or (cu_keys is None and Tk != T):
         raise TurboPiError("packed_attention: keys of another number than the queries need cu_keys, cu an entry more than sequences")
     _one_device("packed_attention", q, k, v, cu, out, cu_keys)
+    _counts("packed_attention", T, Hq, Tk, Hk, cu.numel() - 1)
     args = _lib.PackedAttentionArgs(q=_ptr(q), k=_ptr(k), v=_ptr(v), out=_ptr(out), q_stride=_strides(q), k_stride=_strides(k),
                                     v_stride=_strides(v), o_stride=_strides(out), cu=_ptr(cu), cu_keys=_ptr(cu_keys),
                                     seqs=cu.numel() - 1, q_tokens=T, k_tokens=Tk, q_heads=Hq, kv_heads=Hk, head_dim=D,
@@ -803,6 +810,7 @@ def paged_attention(q, k_pages, v_pages, table, lengths, scale, out=None, worksp
     if workspace is None:
         workspace = paged_attention_workspace(Hq, view.kv_heads, view.head_dim, q.device)
     _one_device("paged_attention", k_pages, q, out, workspace)
+    _counts("paged_attention", Hq)
     args = _lib.PagedAttentionArgs(cache=view, q=_ptr(q), out=_ptr(out), q_stride=_strides(q), o_stride=_strides(out), q_heads=Hq,
                                    scale=float(scale), workspace=_ptr(workspace),
                                    workspace_bytes=workspace.numel() * workspace.element_size(), flags=_flags.value)
@@ -845,6 +853,7 @@ def paged_append(k, v, k_pages, v_pages, table, cu, lengths, q=None, cos=None, s
         else:
             _rows_of_heads("paged_append", "q_out", q_out, T, q.shape[1], D, dtype)
     _one_device("paged_append", k_pages, k, v, cu, q, cos, sin, q_out)
+    _counts("paged_append", T, 0 if q is None else q.shape[1], 0 if cos is None else cos.shape[0])
     args = _lib.PagedAppendArgs(cache=view, k=_ptr(k), v=_ptr(v), q=_ptr(q), q_out=_ptr(q_out), k_stride=_strides(k),
                                 v_stride=_strides(v), q_stride=_strides(q) if q is not None else _Two(0, 0),
                                 o_stride=_strides(q_out) if q is not None else _Two(0, 0), cu=_ptr(cu), tokens=T,
@@ -886,9 +895,10 @@ def copy_pages(pages, src, dst):
         if n:
             raise TurboPiError("copy_pages: the pool is empty")
         return
+    slabs = pages.numel() * pages.element_size() // slab
+    _counts("copy_pages", n, P, slabs)
     arrays = [(ctypes.c_int * n)(*x) for x in lists]
-    st = _run(pages, _lib.load().tpb200_copy_pages, _ptr(pages), slab, pages.numel() * pages.element_size() // slab,
-              slab // P, P, arrays[0], arrays[1], n, _flags.value)
+    st = _run(pages, _lib.load().tpb200_copy_pages, _ptr(pages), slab, slabs, slab // P, P, arrays[0], arrays[1], n, _flags.value)
     _lib.check(st, "tpb200_copy_pages")
 
 
