@@ -442,7 +442,9 @@ py::object copy_pages(const at::Tensor& pages, const py::object& src, const py::
             ids[side * n + i] = static_cast<int>(id);
         }
     }
-    const int64_t P = pages.size(-4), page_bytes = pages.stride(-4) * pages.element_size(), slab = page_bytes * P;
+    if (n == 0) return py::bool_(true);
+    // not by strides: those of one page may be anything
+    const int64_t P = pages.size(-4), page_bytes = pages.size(-3) * pages.size(-2) * pages.size(-1) * pages.element_size(), slab = page_bytes * P;
     const int64_t slabs = static_cast<int64_t>(pages.nbytes()) / slab;
     if (!fits({P, slabs})) return py::none();
     void* base = pages.data_ptr();

@@ -890,11 +890,11 @@ def copy_pages(pages, src, dst):
     for x in lists:
         if any(type(i) is bool or not isinstance(i, int) or not 0 <= i < P for i in x):
             raise TurboPiError(f"copy_pages: a page id outside the supported range [0, {P}), or no int")
-    slab = pages.stride(-4) * P * pages.element_size()
     if n == 0 or pages.numel() == 0:
         if n:
             raise TurboPiError("copy_pages: the pool is empty")
         return
+    slab = P * pages.shape[-3:].numel() * pages.element_size()           # not by strides: those of one page may be anything
     slabs = pages.numel() * pages.element_size() // slab
     _counts("copy_pages", n, P, slabs)
     arrays = [(ctypes.c_int * n)(*x) for x in lists]
