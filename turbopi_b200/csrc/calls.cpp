@@ -313,6 +313,7 @@ py::object paged_attention(const at::Tensor& q, const at::Tensor& k, const at::T
     if (dev < 0 || !paged(k, v, table, lengths, dev, a.cache) || q.dim() != 3 || a.cache.seqs < 1 || a.cache.kv_heads < 1) return py::none();
     const int64_t H = q.size(1);
     if (!rows(q, dev, a.cache.seqs, H, a.cache.head_dim, k.scalar_type()) || !on(workspace, dev) || H < 1 || H % a.cache.kv_heads != 0 ||
+        (workspace.has_value() && !workspace->is_contiguous()) ||
         (out.has_value() && !rows(*out, dev, a.cache.seqs, H, a.cache.head_dim, k.scalar_type()))) {
         return py::none();
     }

@@ -809,6 +809,8 @@ def paged_attention(q, k_pages, v_pages, table, lengths, scale, out=None, worksp
         return out
     if workspace is None:
         workspace = paged_attention_workspace(Hq, view.kv_heads, view.head_dim, q.device)
+    if not workspace.is_contiguous():
+        raise TurboPiError("paged_attention: the workspace must be contiguous")
     _one_device("paged_attention", k_pages, q, out, workspace)
     _counts("paged_attention", Hq)
     args = _lib.PagedAttentionArgs(cache=view, q=_ptr(q), out=_ptr(out), q_stride=_strides(q), o_stride=_strides(out), q_heads=Hq,
