@@ -38,6 +38,13 @@ class PagedBatch:
         self._cache, self._seqs, self._stale = weakref.ref(cache), [], None       # _stale: why it no longer holds
 
 
+def _whole(x):
+    n = int(x)
+    if n != x:
+        raise ValueError(f"{x} is no whole number")
+    return n
+
+
 class PagedCache:
     def __init__(self, layers, num_pages, page_size, kv_heads, head_dim, max_pages, dtype=torch.bfloat16, device="cuda"):
         if min(layers, num_pages, page_size, kv_heads, max_pages) < 1 or not 8 <= head_dim <= 256 or head_dim % 8:
@@ -104,6 +111,10 @@ class PagedCache:
     def truncate(self, seq, length):
         """Forgets the tokens from position `length` on."""
         entry = self._get(seq)
+        try:
+            length = _whole(length)
+        except (TypeError, ValueError, OverflowError):
+            raise TurboPiError(f"PagedCache: cannot truncate to {length!r} tokens") from None
         if not 0 <= length <= entry[1]:
             raise TurboPiError(f"PagedCache: cannot truncate {entry[1]} tokens to {length}")
         keep = -(-length // self.page_size)
@@ -125,8 +136,12 @@ class PagedCache:
         allocated, and a half-filled last page that another sequence shares is copied first (every layer).  All or nothing: where pages
         run out, nothing has changed.  `out`: a PagedBatch of as many sequences whose tensors are written (a captured graph
         reads them)."""
-        seqs, new = list(seqs), [int(n) for n in new]
-        if len(seqs) != len(new) or len(set(seqs)) != len(seqs) or any(n < 0 for n in new):
+        try:
+            seqs, new = list(seqs), [_whole(n) for n in new]
+            fine = len(seqs) == len(new) and len(set(seqs)) == len(seqs) and all(n >= 0 for n in new)
+        except (TypeError, ValueError, OverflowError):
+            fine = False
+        if not fine:
             raise TurboPiError("PagedCache: extend takes different sequences and a number of new tokens >= 0 for each")
         if out is not None and (out._cache() is not self or out.lengths.shape[0] != len(seqs)):
             raise TurboPiError("PagedCache: `out` is a batch of another cache or number of sequences")
@@ -165,7 +180,10 @@ class PagedCache:
 
     def batch(self, seqs):
         """The PagedBatch of sequences as they are, without new tokens."""
-        seqs = list(seqs)
+        try:
+            seqs = list(seqs)
+        except TypeError:
+            raise TurboPiError("PagedCache: batch takes sequences") from None
         return self.extend(seqs, [0] * len(seqs))
 
     def _take(self):
