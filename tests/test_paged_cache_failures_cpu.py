@@ -45,3 +45,65 @@ def test_arguments_of_other_kinds_that_are_fine():
     a, b = cache.add(), cache.add()
     assert cache.extend((a, b), torch.tensor([2, 0])).lengths.tolist() == [2, 0]
     assert cache.extend(iter([b]), (3.0,)).lengths.tolist() == [3]
+
+
+def _pages(cache):
+    return {s: (cache.page_ids(s), cache.length(s)) for s in cache._seqs}, list(cache._refs), sorted(cache._free)
+
+
+def _shared(cache):
+    """Two sequences on one half-filled page, a third beside them, and a batch of each."""
+    a, c = cache.add(), cache.add()
+    cache.extend([a, c], [6, 5])
+    b = cache.fork(a)
+    return a, b, c, [cache.batch([s]) for s in (a, b, c)]
+
+
+@pytest.mark.parametrize("out", [False, True])
+@pytest.mark.parametrize("what", ["copy", "upload"])
+def test_extend_changes_nothing_when_a_step_of_it_fails(monkeypatch, what, out):
+    """The copy of a shared page, or the upload of the tables: pages, lengths and batches are as they were, and the next call works."""
+    cache = _cache()
+    a, b, c, batches = _shared(cache)
+    before, tables = _pages(cache), [x.table.clone() for x in batches]
+
+    def fail(*args):
+        raise TurboPiError("this step fails")
+    with monkeypatch.context() as m:
+        m.setattr(*((ops, "copy_pages", fail) if what == "copy" else (cache, "_upload", fail)))
+        if what == "upload":
+            m.setattr(ops, "copy_pages", lambda *args: None)
+        with pytest.raises(TurboPiError, match="this step fails"):
+            cache.extend([a, c, b], [7, 4, 1], out=cache.batch([a, c, b]) if out and what == "copy" else None)
+    assert _pages(cache) == before
+    for batch, table in zip(batches, tables):
+        cache._current(batch)
+        assert torch.equal(batch.table, table)
+    copied = []
+    monkeypatch.setattr(ops, "copy_pages", lambda pages, src, dst: copied.append((src, dst)))
+    last = cache.page_ids(a)[1]
+    batch = cache.extend([a, c, b], [7, 4, 1])
+    assert batch.lengths.tolist() == [13, 9, 7]
+    assert copied == [([last], [cache.page_ids(a)[1]])] and cache.page_ids(b)[1] == last
+    # the copied page's sequence has to have its batches made again, the others hold
+    with pytest.raises(TurboPiError, match="copied"):
+        cache._current(batches[0])
+    cache._current(batches[1])
+    cache._current(batches[2])
+
+
+def test_compaction_changes_nothing_when_its_copy_fails(monkeypatch):
+    cache = _cache()
+    a, b, c, batches = _shared(cache)
+    cache.free(a)
+    cache.free(b)
+    before = _state(cache)
+
+    def fail(*args):
+        raise TurboPiError("this step fails")
+    with monkeypatch.context() as m:
+        m.setattr(ops, "copy_pages", fail)
+        with pytest.raises(TurboPiError, match="this step fails"):
+            cache.compact()
+    assert _state(cache) == before
+    cache._current(batches[2])

@@ -134,7 +134,7 @@ class PagedCache:
     def extend(self, seqs, new, out=None):
         """Room for new[i] >= 0 more tokens of sequence seqs[i]; returns the PagedBatch for `append` and `attention`.  Pages are
         allocated, and a half-filled last page that another sequence shares is copied first (every layer).  All or nothing: where pages
-        run out, nothing has changed.  `out`: a PagedBatch of as many sequences whose tensors are written (a captured graph
+        run out, or a step fails, nothing has changed.  `out`: a PagedBatch of as many sequences whose tensors are written (a captured graph
         reads them)."""
         try:
             seqs, new = list(seqs), [_whole(n) for n in new]
@@ -162,21 +162,34 @@ class PagedCache:
             taken += copied + total - len(pages)
         if taken > len(self._free):
             raise TurboPiError(f"PagedCache: {taken} pages needed, {len(self._free)} free")
-        src, dst = [], []
-        for seq, n, (copied, more) in zip(seqs, new, plan):
+        fresh = [heapq.heappop(self._free) for _ in range(taken)]
+        try:                                          # what may fail comes before anything is changed
+            take, held, src, dst = iter(fresh), [], [], []
+            for seq, (copied, more) in zip(seqs, plan):
+                pages = list(self._seqs[seq][0])
+                if copied:
+                    src.append(pages[-1])
+                    pages[-1] = next(take)
+                    dst.append(pages[-1])
+                pages.extend(next(take) for _ in range(more))
+                held.append(pages)
+            if src:
+                ops.copy_pages(self.pages, src, dst)
+            tensors = self._tensors(held, [self._seqs[seq][1] + n for seq, n in zip(seqs, new)], new)
+        except BaseException:
+            for p in fresh:
+                heapq.heappush(self._free, p)
+            raise
+        for p in fresh:
+            self._refs[p] = 1
+        for seq, n, pages, (copied, _) in zip(seqs, new, held, plan):
             entry = self._seqs[seq]
             if copied:
-                fresh = self._take()
-                src.append(entry[0][-1])
-                dst.append(fresh)
                 self._release(entry[0][-1])
-                entry[0][-1] = fresh
                 self._outdate(entry, f"a shared page of sequence {seq} was copied")
-            entry[0].extend(self._take() for _ in range(more))
+            entry[0] = pages
             entry[1] += n
-        if src:
-            ops.copy_pages(self.pages, src, dst)
-        return self._batch(seqs, new, out)
+        return self._batch(seqs, sum(new), tensors, out)
 
     def batch(self, seqs):
         """The PagedBatch of sequences as they are, without new tokens."""
@@ -186,27 +199,24 @@ class PagedCache:
             raise TurboPiError("PagedCache: batch takes sequences") from None
         return self.extend(seqs, [0] * len(seqs))
 
-    def _take(self):
-        page = heapq.heappop(self._free)
-        self._refs[page] = 1
-        return page
-
     def _upload(self, values, shape):
         t = torch.tensor(values, dtype=torch.int32).reshape(shape)
         return t.pin_memory().to(self.device, non_blocking=True) if self.device.type == "cuda" else t
 
-    def _batch(self, seqs, new, out):
-        S, W = len(seqs), self.max_pages
+    def _tensors(self, held, lengths, new):
+        """Tables, lengths and offsets in one copy to the device."""
+        S, W = len(held), self.max_pages
         rows, cu = [], [0]
-        for seq, n in zip(seqs, new):
-            pages = self._seqs[seq][0]
+        for pages, n in zip(held, new):
             rows += pages + [-1] * (W - len(pages))
             cu.append(cu[-1] + n)
-        # one copy to the device: tables, lengths, offsets
-        flat = self._upload(rows + [self._seqs[s][1] for s in seqs] + cu, (-1,))
-        table, lengths, offsets = flat[:S * W].view(S, W), flat[S * W:S * W + S], flat[S * W + S:]
+        flat = self._upload(rows + lengths + cu, (-1,))
+        return flat[:S * W].view(S, W), flat[S * W:S * W + S], flat[S * W + S:]
+
+    def _batch(self, seqs, tokens, tensors, out):
+        table, lengths, offsets = tensors
         if out is None:
-            out = PagedBatch(table, lengths, offsets, cu[-1], self)
+            out = PagedBatch(table, lengths, offsets, tokens, self)
         else:
             for seq in out._seqs:
                 if seq in self._seqs:
@@ -214,7 +224,7 @@ class PagedCache:
             out.table.copy_(table)
             out.lengths.copy_(lengths)
             out.cu.copy_(offsets)
-            out.tokens, out._stale = cu[-1], None
+            out.tokens, out._stale = tokens, None
         out._seqs = seqs
         for seq in seqs:
             self._seqs[seq][2].add(out)
