@@ -17,7 +17,8 @@ same pages); the bytes are moved by `ops.copy_pages`, written by `ops.paged_appe
         out = cache.attention(l, batch, q, scale)
 
 A batch holds for its cache until one of its sequences is freed, truncated or had a shared page copied, or pages have moved (compact);
-then `append` and `attention` refuse it, since its table may name pages of others.  Calls that move or write pages enqueue on the
+then `append` and `attention` refuse it, since its table may name pages of others.  `append` also refuses tokens whose page has been copied
+to a fork, which would lack them: write a batch's tokens before extending a fork of its sequences.  Calls that move or write pages enqueue on the
 current stream; use one stream per cache, or order them yourself.
 """
 import heapq
@@ -35,7 +36,9 @@ class PagedBatch:
 
     def __init__(self, table, lengths, cu, tokens, cache):
         self.table, self.lengths, self.cu, self.tokens = table, lengths, cu, tokens
-        self._cache, self._seqs, self._stale = weakref.ref(cache), [], None       # _stale: why it no longer holds
+        # _new: sequence -> [first, last + 1) of its new tokens' positions; _stale: why it no longer holds, _late: why its tokens can
+        # no longer be written in a layer that is not among _layers, the ones where `append` wrote them
+        self._cache, self._new, self._stale, self._late, self._layers = weakref.ref(cache), {}, None, None, set()
 
 
 def _whole(x):
@@ -100,7 +103,8 @@ class PagedCache:
 
     def fork(self, seq):
         """A second sequence with the same tokens, on the same pages; returns its id.  Nothing is copied until one of them is extended
-        within the page they share last."""
+        within the page they share last.  By then tokens that a batch has made room for there must be written, in every layer: the copy
+        lacks later ones, and `append` refuses to write them.  (A captured graph that writes them is not seen here.)"""
         pages, length, _ = self._get(seq)
         for page in pages:
             self._refs[page] += 1
@@ -185,11 +189,24 @@ class PagedCache:
         for seq, n, pages, (copied, _) in zip(seqs, new, held, plan):
             entry = self._seqs[seq]
             if copied:
+                self._copied(seq, entry[0], entry[1])
                 self._release(entry[0][-1])
                 self._outdate(entry, f"a shared page of sequence {seq} was copied")
             entry[0] = pages
             entry[1] += n
-        return self._batch(seqs, sum(new), tensors, out)
+        return self._batch(seqs, new, tensors, out)
+
+    def _copied(self, seq, pages, length):
+        """The last page of a sequence was copied for it: tokens that others were still to write there, below its length, are not in
+        the copy."""
+        i, page = len(pages) - 1, pages[-1]
+        for other, (held, _, batches) in self._seqs.items():
+            if other == seq or len(held) <= i or held[i] != page:            # a page has the same place in all that share it
+                continue
+            for batch in batches:
+                first, last = batch._new.get(other, (0, 0))
+                if max(first, i * self.page_size) < min(last, length):
+                    batch._late = f"a page with new tokens of sequence {other} was copied to sequence {seq}"
 
     def batch(self, seqs):
         """The PagedBatch of sequences as they are, without new tokens."""
@@ -213,19 +230,19 @@ class PagedCache:
         flat = self._upload(rows + lengths + cu, (-1,))
         return flat[:S * W].view(S, W), flat[S * W:S * W + S], flat[S * W + S:]
 
-    def _batch(self, seqs, tokens, tensors, out):
+    def _batch(self, seqs, new, tensors, out):
         table, lengths, offsets = tensors
         if out is None:
-            out = PagedBatch(table, lengths, offsets, tokens, self)
+            out = PagedBatch(table, lengths, offsets, sum(new), self)
         else:
-            for seq in out._seqs:
+            for seq in out._new:
                 if seq in self._seqs:
                     self._seqs[seq][2].discard(out)
             out.table.copy_(table)
             out.lengths.copy_(lengths)
             out.cu.copy_(offsets)
-            out.tokens, out._stale = tokens, None
-        out._seqs = seqs
+            out.tokens, out._stale, out._late, out._layers = sum(new), None, None, set()
+        out._new = {seq: (self._seqs[seq][1] - n, self._seqs[seq][1]) for seq, n in zip(seqs, new)}
         for seq in seqs:
             self._seqs[seq][2].add(out)
         return out
@@ -244,9 +261,14 @@ class PagedCache:
     def append(self, layer, batch, k, v, q=None, cos=None, sin=None, q_out=None):
         """ops.paged_append of the batch's new tokens: k, v (and q) [batch.tokens, heads, head_dim], sequence by sequence."""
         self._current(batch)
+        layer = range(self.pages.shape[0])[layer]
+        if batch._late and layer not in batch._layers:
+            raise TurboPiError(f"PagedCache: {batch._late} before this append; append in every layer before a fork is extended")
         if k.shape[0] != batch.tokens:
             raise TurboPiError(f"PagedCache: {k.shape[0]} rows for {batch.tokens} new tokens")
-        return ops.paged_append(k, v, *self.layer(layer), batch.table, batch.cu, batch.lengths, q=q, cos=cos, sin=sin, q_out=q_out)
+        out = ops.paged_append(k, v, *self.layer(layer), batch.table, batch.cu, batch.lengths, q=q, cos=cos, sin=sin, q_out=q_out)
+        batch._layers.add(layer)
+        return out
 
     def attention(self, layer, batch, q, scale, out=None, workspace=None):
         """ops.paged_attention of one query row per sequence of the batch, over all its tokens."""
