@@ -86,3 +86,70 @@ def test_truncated_below_the_reserved_tokens(cache):
     cache.truncate(b, 2)
     cache.extend([b], [1])                                       # its copy needs positions 0 and 1, not 2
     assert _append(cache, late) == "appended"
+
+
+@pytest.mark.parametrize("seed", range(20))
+def test_random_histories(monkeypatch, seed):
+    """Appends that come late, or never: what was appended without a refusal is what every sequence with those tokens reads."""
+    import random
+    rng, layers = random.Random(seed), 2
+    cache = PagedCache(layers, 14, 4, 1, 8, 5, dtype=torch.float16, device="cpu")
+    monkeypatch.setattr(ops, "copy_pages", lambda pages, src, dst: pages.index_copy_(2, torch.tensor(dst), pages[:, :, src].clone()))
+
+    def write(k, v, k_pages, v_pages, table, cu, lengths, **kw):
+        cu, lengths = cu.tolist(), lengths.tolist()
+        for s, row in enumerate(table.tolist()):
+            for t in range(cu[s], cu[s + 1]):
+                pos = lengths[s] - cu[s + 1] + t
+                k_pages[row[pos // 4], pos % 4] = k[t]
+    monkeypatch.setattr(ops, "paged_append", write)
+    want, open_batches, written, stamp, refused = {}, [], [set() for _ in range(layers)], 0, 0
+    for _ in range(400):
+        what = rng.choice(["add", "extend", "extend", "extend", "append", "append", "append", "fork", "fork", "free", "truncate", "compact"])
+        if what == "add" and len(want) < 5:
+            want[cache.add()] = []
+        elif what == "extend" and want:
+            seqs = rng.sample(sorted(want), rng.randint(1, len(want)))
+            new = [rng.choice([0, 1, 1, 2, 5]) for _ in seqs]
+            try:
+                batch = cache.extend(seqs, new)
+            except TurboPiError:
+                continue
+            tokens = [float(stamp + i) for i in range(sum(new))]
+            stamp += len(tokens)
+            open_batches.append((batch, tokens))
+            for s, n in zip(seqs, new):
+                want[s] = want[s] + tokens[:n]
+                tokens = tokens[n:]
+        elif what == "append" and open_batches:
+            batch, tokens = rng.choice(open_batches[-4:])
+            layer = rng.randrange(layers)
+            kv = torch.tensor(tokens).view(-1, 1, 1).expand(-1, 1, 8)
+            if layer in batch._layers:
+                continue
+            try:
+                cache.append(layer, batch, kv, kv)
+                written[layer].update(tokens)
+            except TurboPiError:
+                refused += 1
+        elif what == "fork" and want and len(want) < 5:
+            s = rng.choice(sorted(want))
+            want[cache.fork(s)] = list(want[s])
+        elif what == "free" and len(want) > 2:
+            s = rng.choice(sorted(want))
+            cache.free(s)
+            del want[s]
+        elif what == "truncate" and want:
+            s = rng.choice(sorted(want))
+            n = rng.randint(len(want[s]) // 2, len(want[s]))
+            cache.truncate(s, n)
+            want[s] = want[s][:n]
+        elif what == "compact":
+            cache.compact()
+        for s, tokens in want.items():
+            pages = cache.page_ids(s)
+            for layer in range(layers):
+                for pos, token in enumerate(tokens):
+                    if token in written[layer]:
+                        assert float(cache.pages[layer, 0, pages[pos // 4], pos % 4, 0, 0]) == token
+    assert refused and sum(map(len, written)) > 20

@@ -184,29 +184,33 @@ class PagedCache:
             for p in fresh:
                 heapq.heappush(self._free, p)
             raise
+        if src:
+            self._copied([(seq, *self._seqs[seq][:2]) for seq, (copied, _) in zip(seqs, plan) if copied])
         for p in fresh:
             self._refs[p] = 1
         for seq, n, pages, (copied, _) in zip(seqs, new, held, plan):
             entry = self._seqs[seq]
             if copied:
-                self._copied(seq, entry[0], entry[1])
                 self._release(entry[0][-1])
                 self._outdate(entry, f"a shared page of sequence {seq} was copied")
             entry[0] = pages
             entry[1] += n
         return self._batch(seqs, new, tensors, out)
 
-    def _copied(self, seq, pages, length):
-        """The last page of a sequence was copied for it: tokens that others were still to write there, below its length, are not in
-        the copy."""
-        i, page = len(pages) - 1, pages[-1]
+    def _copied(self, copies):
+        """The last pages of some sequences, (sequence, page ids, length) each, were copied for them: tokens that others were still to
+        write there, below that length, are not in the copy."""
+        page, where = self.page_size, {}
+        for seq, pages, length in copies:                        # a page has the same place in all that share it
+            where.setdefault((len(pages) - 1, pages[-1]), []).append((seq, length))
+        low, high = min(i for i, _ in where), max(i for i, _ in where)
         for other, (held, _, batches) in self._seqs.items():
-            if other == seq or len(held) <= i or held[i] != page:            # a page has the same place in all that share it
-                continue
             for batch in batches:
                 first, last = batch._new.get(other, (0, 0))
-                if max(first, i * self.page_size) < min(last, length):
-                    batch._late = f"a page with new tokens of sequence {other} was copied to sequence {seq}"
+                for i in range(max(low, first // page), min(high + 1, len(held), -(-last // page))):
+                    for seq, length in where.get((i, held[i]), ()):
+                        if other != seq and max(first, i * page) < min(last, length):
+                            batch._late = f"a page with new tokens of sequence {other} was copied to sequence {seq}"
 
     def batch(self, seqs):
         """The PagedBatch of sequences as they are, without new tokens."""
