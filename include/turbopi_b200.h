@@ -457,7 +457,7 @@ typedef struct {
 } tpb200_paged_cache;
 
 /* Attention of one new token per sequence on the cache: out[s] = softmax(scale * q[s] K^T) V over the first lengths[s] positions
- * (the new token's own key among them); query heads [h * g, (h + 1) * g) read key head h, g = q_heads / kv_heads; weights
+ * (the new token's own key among them); query heads [h * g, (h + 1) * g) read key head h, g = q_heads / kv_heads (a g above 16 reads the cache once per sixteen); weights
  * rounded to the cache's type for their product with the values, fp32 sums, outputs rounded once.  A sequence without keys (length 0, or none of its pages in the pool) gives zeros.  q / out: element strides of a sequence and of a head, multiples of 8.
  * The lengths' sum is cut into equal pieces over the GPU whatever the single lengths; items that cross a cut are joined by a second
  * small kernel through `workspace` (no initialisation needed; its size depends on the heads only).  out may be q (row on row, not in part).  All lengths decide

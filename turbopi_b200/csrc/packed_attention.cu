@@ -23,9 +23,9 @@
 //                         shared memory.
 // While one group works the other's products run.
 //
-// What bounds it, measured on one B200 (calls in a CUDA graph):
-//   one sequence of 8191 tokens, causal, 8 on 1 heads of 256: 195 us = 1.41 PFLOP/s, 0.86 of the measured bf16 rate: hand-overs from product to
-//   softmax and back.
+// What bounds it, measured on one B200 (ten calls in a CUDA graph, before the board's power limit; calls one after the other reach it):
+//   one sequence of 8191 tokens, causal, 8 on 1 heads of 256: 197 us = 1.40 PFLOP/s, 0.85 of the measured bf16 burst rate: hand-overs from product to
+//   softmax and back.  Call after call 237 us = 1.16, 0.83 of the rate that lasts for seconds.
 //   4 sequences, 24.6 k tokens, causal, 32 on 8 heads of 128: 1.38 ms = 1.23 PFLOP/s, 0.75, at 1965 MHz; after some 10 ms of it the board
 //   is at its 1000 W, the clock goes to 1.6 GHz and the call to 1.56-1.62 ms.  At full clock two tiles take 3350 cycles, of which their products
 //   need 2048 and so do their exponentials (16 a cycle and SM): a group's softmax takes 2000 (1300 to the first half of P) while the
@@ -849,6 +849,7 @@ extern "C" int tpb200_packed_attention(const tpb200_packed_attention_args* a, tp
     // Up to head size 128, two row tiles per CTA where sequences are long (each unit of K and V serves both), else one, and two CTAs on an
     // SM: half the rows to fill up, and one's loads and output beside the other's products.  The border is where the two meet on average:
     // 24 sequences of 100 / 8 of 1536, 16 heads of 64: 13.5 us with one, 18.1 with two / 91.6, 92.6; 16 heads of 128: 21.0, 25.2 / 129, 118.
+    // Batches of sequences alike; not measured where lengths differ much or queries are few beside the keys.
     const bool two = DP <= 128 && static_cast<long long>(a->k_tokens) > (DP == 64 ? 1000ll : 200ll) * a->seqs;
     // no more tiles than whole ones and a ragged one per sequence
     const long long tiles = static_cast<long long>(a->q_tokens) / (rows_tokens * (two ? 2 : 1)) + std::min(a->seqs, a->q_tokens);

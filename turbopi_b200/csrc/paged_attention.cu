@@ -21,8 +21,8 @@
 //
 // What bounds it: inside a piece the stream runs at 6.2-6.6 TB/s, the measured copy rate; around it lie 2 us until a warp knows its piece,
 // SMs that get 5-10 % less of the bandwidth (the same ones in every run), and 3-5 us for the second kernel.  Calls in a CUDA graph: 3 sequences, 260 k keys, fp16, 8 on 1 heads
-// of 256 (267 MB) 54 us = 4.9 TB/s; 48 sequences of 1 to 4096, 32 on 8 of 128 (160 MB) 38 us = 4.2; 128 of 16 to 2000, 16 on 16 of
-// 64 (215 MB) 49 us = 4.4; one sequence of 762 keys 9.6 us, all latency.  Equal pieces per CTA, items not weighed, took 45 and 69 us for
+// of 256 (267 MB) 54 us = 4.9 TB/s; 48 sequences of 1 to 4096, 32 on 8 of 128 (160 MB) 38 us = 4.2, with pages of 24 39; 128 of 16 to 2000, 16 on 16 of
+// 64 (215 MB) 50 us = 4.3; one sequence of 762 keys 9.6 us, all latency.  Equal pieces per CTA, items not weighed, took 45 and 69 us for
 // the two batches: CTAs with many short items were done last.
 #include <algorithm>
 #include <atomic>
@@ -868,7 +868,8 @@ DecodeScratch decode_scratch(int ctas, int rows, int head_dim) {
     return d;
 }
 
-// query heads that go through together: eight, or sixteen where a group has more
+// query heads that go through together: eight, or sixteen where a group has more; larger groups read the cache once per sixteen (48 sequences of 1 to
+// 4096, 4 key heads of 128, 80 MB: groups of 8 21 us, of 16 28, of 32 47)
 int decode_rows(int group) { return group <= 8 ? 8 : 16; }
 
 template <typename T, int DP, int NT, bool kAligned>
