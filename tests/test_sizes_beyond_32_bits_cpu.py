@@ -39,9 +39,9 @@ def test_what_fits_is_launched(launched):
 def test_packed_attention(launched):
     for q, k in ((LARGE, 4), (4, LARGE)):
         with pytest.raises(TurboPiError, match="32 bits"):
-            ops.packed_attention(_rows(q), _rows(k), _rows(k), _ints(2), 1.0, out=_rows(q), cu_keys=_ints(2))
+            ops.packed_attention(_rows(q), _rows(k), _rows(k), _ints(2), 1.0, cu_keys=_ints(2))
     with pytest.raises(TurboPiError, match="32 bits"):
-        ops.packed_attention(_rows(4, LARGE), _rows(4), _rows(4), _ints(2), 1.0, out=_rows(4, LARGE))
+        ops.packed_attention(_rows(4, LARGE), _rows(4), _rows(4), _ints(2), 1.0)
     assert not launched
 
 

@@ -755,6 +755,7 @@ def packed_attention(q, k, v, cu, scale, out=None, causal=True, cu_keys=None):
     _rows_of_heads("packed_attention", "q", q, T, Hq, D, q.dtype)
     _rows_of_heads("packed_attention", "k", k, Tk, Hk, D, q.dtype)
     _rows_of_heads("packed_attention", "v", v, Tk, Hk, D, q.dtype)
+    _counts("packed_attention", T, Hq, Tk, Hk, cu.numel() - 1)
     if out is None:
         out = torch.empty((T, Hq, D), dtype=q.dtype, device=q.device)
     else:
@@ -765,7 +766,6 @@ def packed_attention(q, k, v, cu, scale, out=None, causal=True, cu_keys=None):
     if cu.numel() < 1 or (cu_keys is None and Tk != T):
         raise TurboPiError("packed_attention: keys of another number than the queries need cu_keys, cu an entry more than sequences")
     _one_device("packed_attention", q, k, v, cu, out, cu_keys)
-    _counts("packed_attention", T, Hq, Tk, Hk, cu.numel() - 1)
     args = _lib.PackedAttentionArgs(q=_ptr(q), k=_ptr(k), v=_ptr(v), out=_ptr(out), q_stride=_strides(q), k_stride=_strides(k),
                                     v_stride=_strides(v), o_stride=_strides(out), cu=_ptr(cu), cu_keys=_ptr(cu_keys),
                                     seqs=cu.numel() - 1, q_tokens=T, k_tokens=Tk, q_heads=Hq, kv_heads=Hk, head_dim=D,
@@ -798,6 +798,7 @@ def paged_attention(q, k_pages, v_pages, table, lengths, scale, out=None, worksp
     if q.dim() != 3:
         raise TurboPiError("paged_attention: q must be [sequences, heads, D]")
     Hq = q.shape[1]
+    _counts("paged_attention", Hq)
     _rows_of_heads("paged_attention", "q", q, view.seqs, Hq, view.head_dim, k_pages.dtype)
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
@@ -812,7 +813,6 @@ def paged_attention(q, k_pages, v_pages, table, lengths, scale, out=None, worksp
     if not workspace.is_contiguous():
         raise TurboPiError("paged_attention: the workspace must be contiguous")
     _one_device("paged_attention", k_pages, q, out, workspace)
-    _counts("paged_attention", Hq)
     args = _lib.PagedAttentionArgs(cache=view, q=_ptr(q), out=_ptr(out), q_stride=_strides(q), o_stride=_strides(out), q_heads=Hq,
                                    scale=float(scale), workspace=_ptr(workspace),
                                    workspace_bytes=workspace.numel() * workspace.element_size(), flags=_flags.value)
@@ -846,16 +846,17 @@ def paged_append(k, v, k_pages, v_pages, table, cu, lengths, q=None, cos=None, s
     if cos is not None and (cos.dim() != 2 or cos.shape != sin.shape or cos.shape[1] != D // 2 or cos.dtype != sin.dtype
                             or cos.dtype not in _DTYPES or not cos.is_contiguous() or not sin.is_contiguous()):
         raise TurboPiError(f"paged_append: cos and sin must be contiguous [positions, {D // 2}] of one floating type")
+    _counts("paged_append", T, 0 if cos is None else cos.shape[0])
     if q is not None:
         if q.dim() != 3:
             raise TurboPiError("paged_append: q must be [tokens, heads, D]")
+        _counts("paged_append", q.shape[1])
         _rows_of_heads("paged_append", "q", q, T, q.shape[1], D, dtype)
         if q_out is None:
             q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         else:
             _rows_of_heads("paged_append", "q_out", q_out, T, q.shape[1], D, dtype)
     _one_device("paged_append", k_pages, k, v, cu, q, cos, sin, q_out)
-    _counts("paged_append", T, 0 if q is None else q.shape[1], 0 if cos is None else cos.shape[0])
     args = _lib.PagedAppendArgs(cache=view, k=_ptr(k), v=_ptr(v), q=_ptr(q), q_out=_ptr(q_out), k_stride=_strides(k),
                                 v_stride=_strides(v), q_stride=_strides(q) if q is not None else _Two(0, 0),
                                 o_stride=_strides(q_out) if q is not None else _Two(0, 0), cu=_ptr(cu), tokens=T,
