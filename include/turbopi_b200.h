@@ -436,6 +436,8 @@ typedef struct {
     float scale; int causal; int flags;
 } tpb200_packed_attention_args;
 int tpb200_packed_attention(const tpb200_packed_attention_args* args, tpb200_stream_t stream);
+/* The same (causal) over a sliding window: a query sees the last `window` >= 1 keys up to its own limit and its sequence's first `sinks` >= 0. */
+int tpb200_packed_attention_window(const tpb200_packed_attention_args* args, int window, int sinks, tpb200_stream_t stream);
 
 /* ---------------------------------------------------------------------------------------------
  * A cache of pages that many sequences share (one layer of it).  Key and value pages lie apart, with the same strides (in
@@ -474,6 +476,10 @@ typedef struct {
 size_t tpb200_paged_attention_workspace_size(int q_heads, int kv_heads, int head_dim);
 int tpb200_paged_attention(const tpb200_paged_attention_args* args, tpb200_stream_t stream);
 
+/* The same over a sliding window: the token sees the last `window` >= 1 keys (its own among them) and the first `sinks` >= 0.  Pages that hold
+ * none of them are not read and need not be in the table. */
+int tpb200_paged_attention_window(const tpb200_paged_attention_args* args, int window, int sinks, tpb200_stream_t stream);
+
 /* New tokens into the cache.  Sequence s brings the tokens [cu[s], cu[s + 1]); its last one goes to position lengths[s] - 1, so
  * lengths are those after the call.  Tokens behind cu[seqs] are left alone.  With cos / sin ([rope_positions, head_dim / 2], rows
  * contiguous, fp32, fp16 or bf16) the keys, and the queries where given, are rotated at their positions in rotate-half form:
@@ -490,6 +496,62 @@ typedef struct {
     int flags;
 } tpb200_paged_append_args;
 int tpb200_paged_append(const tpb200_paged_append_args* args, tpb200_stream_t stream);
+
+/* One layer of a paged cache held in 4 bits (NVFP4).  With G = ceil(head_dim / 32), a page has page_size / 16 tiles for each key head, a tile of 16
+ * tokens is 288 G bytes: 16 rows of 16 G bytes of E2M1 codes (value 2 i in the low half of byte i, 2 i + 1 in the high half, zeros behind
+ * head_dim), then 16 rows of 2 G E4M3 scales, one for every 16 values.  A key is k_scale * scale * code, a value v_scale * scale * code; k_scale and
+ * v_scale are powers of two from 2^-63 to 2^64.  scale * code is exact in fp16 and bf16.  page_size is a multiple of 16; the strides are in bytes,
+ * multiples of 16: from page to page, from head to head, from tile to tile.  Table and lengths as in tpb200_paged_cache. */
+typedef struct {
+    void* k_pages; void* v_pages;
+    long long page_stride, head_stride, tile_stride;
+    int num_pages, page_size, kv_heads, head_dim;
+    float k_scale, v_scale;
+    const int* table; long long table_stride; int table_width;
+    const int* lengths; int seqs;
+} tpb200_paged_nvfp4_cache;
+
+/* tpb200_paged_attention on such a cache.  window 0 (and sinks 0): all keys, else as in tpb200_paged_attention_window.  q / out: bf16 or fp16
+ * (`dtype`).  Values are multiplied as fp16, bf16 queries after division by a power of two per head; weights are rounded to fp16, sums are fp32, the
+ * outputs are rounded once.  A group of query heads above 16 (head_dim above 128: 8) reads the cache more than once. */
+typedef struct {
+    tpb200_paged_nvfp4_cache cache;
+    const void* q; void* out; int dtype;
+    long long q_stride[2]; long long o_stride[2];
+    int q_heads;
+    float scale;
+    int window, sinks;
+    void* workspace; size_t workspace_bytes;
+    int flags;
+} tpb200_paged_attention_nvfp4_args;
+size_t tpb200_paged_attention_nvfp4_workspace_size(int q_heads, int kv_heads, int head_dim);
+int tpb200_paged_attention_nvfp4(const tpb200_paged_attention_nvfp4_args* args, tpb200_stream_t stream);
+
+/* tpb200_paged_append into such a cache: k, v, q and q_out are bf16 or fp16 (`dtype`).  Keys are rotated where tables are given and rounded to
+ * `dtype`; then 16 values at a time, divided by k_scale or v_scale, get the scale s = max |x| / 6, rounded to the nearest E4M3 (at most 448), and
+ * the codes x / s, rounded to the nearest E2M1 (ties to the even code, at most 6); s = 0 gives zeros.  16 values with an infinity or a NaN among them
+ * get a scale that is NaN. */
+typedef struct {
+    tpb200_paged_nvfp4_cache cache;
+    const void* k; const void* v; const void* q; void* q_out; int dtype;
+    long long k_stride[2]; long long v_stride[2]; long long q_stride[2]; long long o_stride[2];
+    const int* cu; int tokens; int q_heads;
+    const void* cos; const void* sin; int rope_dtype; int rope_positions;
+    int flags;
+} tpb200_paged_append_nvfp4_args;
+int tpb200_paged_append_nvfp4(const tpb200_paged_append_nvfp4_args* args, tpb200_stream_t stream);
+
+/* Tokens out of a cache, one sequence behind the other, as packed attention takes them: rows [cu[s], cu[s + 1]) of k and v get sequence s's last
+ * cu[s + 1] - cu[s] positions, the last one lengths[s] - 1.  Rows behind cu[seqs] are left alone; a row without a place (501) gets zeros.  The 16-bit form
+ * copies, the 4-bit one gives the values that are held, in `dtype`, exactly where k_scale or v_scale does not take them out of its range. */
+typedef struct {
+    void* k; void* v; int dtype;
+    long long k_stride[2]; long long v_stride[2];
+    const int* cu; int tokens;
+    int flags;
+} tpb200_paged_rows;
+int tpb200_paged_read(const tpb200_paged_cache* cache, const tpb200_paged_rows* rows, tpb200_stream_t stream);
+int tpb200_paged_read_nvfp4(const tpb200_paged_nvfp4_cache* cache, const tpb200_paged_rows* rows, tpb200_stream_t stream);
 
 /* Pages copied within their pool, in each of `slabs` slabs (a layer's keys or values: num_pages pages of page_bytes bytes, slab_bytes
  * apart): page dst[i] <- page src[i].  src / dst are HOST arrays, read before the call returns.  TPB200_ERR_SHAPE for an index

@@ -129,6 +129,32 @@ class PackedAttentionArgs(ctypes.Structure):
                 ("kv_heads", c_int), ("head_dim", c_int), ("dtype", c_int), ("scale", c_float), ("causal", c_int), ("flags", c_int)]
 
 
+class PagedNvfp4CacheView(ctypes.Structure):
+    _fields_ = [("k_pages", c_void_p), ("v_pages", c_void_p),
+                ("page_stride", c_longlong), ("head_stride", c_longlong), ("tile_stride", c_longlong),
+                ("num_pages", c_int), ("page_size", c_int), ("kv_heads", c_int), ("head_dim", c_int),
+                ("k_scale", c_float), ("v_scale", c_float),
+                ("table", c_void_p), ("table_stride", c_longlong), ("table_width", c_int), ("lengths", c_void_p), ("seqs", c_int)]
+
+
+class PagedAttentionNvfp4Args(ctypes.Structure):
+    _fields_ = [("cache", PagedNvfp4CacheView), ("q", c_void_p), ("out", c_void_p), ("dtype", c_int), ("q_stride", c_longlong * 2),
+                ("o_stride", c_longlong * 2), ("q_heads", c_int), ("scale", c_float), ("window", c_int), ("sinks", c_int),
+                ("workspace", c_void_p), ("workspace_bytes", c_size_t), ("flags", c_int)]
+
+
+class PagedAppendNvfp4Args(ctypes.Structure):
+    _fields_ = [("cache", PagedNvfp4CacheView), ("k", c_void_p), ("v", c_void_p), ("q", c_void_p), ("q_out", c_void_p), ("dtype", c_int),
+                ("k_stride", c_longlong * 2), ("v_stride", c_longlong * 2), ("q_stride", c_longlong * 2),
+                ("o_stride", c_longlong * 2), ("cu", c_void_p), ("tokens", c_int), ("q_heads", c_int), ("cos", c_void_p),
+                ("sin", c_void_p), ("rope_dtype", c_int), ("rope_positions", c_int), ("flags", c_int)]
+
+
+class PagedRows(ctypes.Structure):
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("dtype", c_int), ("k_stride", c_longlong * 2), ("v_stride", c_longlong * 2),
+                ("cu", c_void_p), ("tokens", c_int), ("flags", c_int)]
+
+
 class ActTc(ctypes.Structure):
     _fields_ = [("x", c_void_p), ("ldx", c_int), ("K", c_int), ("x_image", c_void_p), ("x_row_scale", c_void_p)]
 
@@ -193,6 +219,13 @@ SIGNATURES = {
     "tpb200_paged_attention_workspace_size": (c_size_t, [c_int, c_int, c_int]),
     "tpb200_paged_attention": (c_int, [ctypes.POINTER(PagedAttentionArgs), c_void_p]),
     "tpb200_paged_append": (c_int, [ctypes.POINTER(PagedAppendArgs), c_void_p]),
+    "tpb200_packed_attention_window": (c_int, [ctypes.POINTER(PackedAttentionArgs), c_int, c_int, c_void_p]),
+    "tpb200_paged_attention_window": (c_int, [ctypes.POINTER(PagedAttentionArgs), c_int, c_int, c_void_p]),
+    "tpb200_paged_attention_nvfp4_workspace_size": (c_size_t, [c_int, c_int, c_int]),
+    "tpb200_paged_attention_nvfp4": (c_int, [ctypes.POINTER(PagedAttentionNvfp4Args), c_void_p]),
+    "tpb200_paged_append_nvfp4": (c_int, [ctypes.POINTER(PagedAppendNvfp4Args), c_void_p]),
+    "tpb200_paged_read": (c_int, [ctypes.POINTER(PagedCacheView), ctypes.POINTER(PagedRows), c_void_p]),
+    "tpb200_paged_read_nvfp4": (c_int, [ctypes.POINTER(PagedNvfp4CacheView), ctypes.POINTER(PagedRows), c_void_p]),
     "tpb200_copy_pages": (c_int, [c_void_p, c_longlong, c_int, c_longlong, c_int, ctypes.POINTER(c_int), ctypes.POINTER(c_int),
                                   c_int, c_int, c_void_p]),
     "tpb200_w4a16_gemm": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_int,
@@ -223,7 +256,9 @@ _native = None
 _NATIVE_ENTRIES = ("tpb200_w4_gemm", "tpb200_w4a16_gemv", "tpb200_w4a16_gemm", "tpb200_attention", "quantizeActivationToFP8",
                    "tpb200_last_error", "tpb200_nvfp4_tiled_a_bytes", "tpb200_nvfp4_quantize_act_tiled", "tpb200_nvfp4_gemm_ex",
                    "tpb200_packed_attention", "tpb200_paged_attention_workspace_size", "tpb200_paged_attention", "tpb200_paged_append",
-                   "tpb200_copy_pages")
+                   "tpb200_copy_pages", "tpb200_packed_attention_window", "tpb200_paged_attention_window",
+                   "tpb200_paged_attention_nvfp4_workspace_size", "tpb200_paged_attention_nvfp4", "tpb200_paged_append_nvfp4",
+                   "tpb200_paged_read", "tpb200_paged_read_nvfp4")
 
 
 def calls_path():

@@ -7,6 +7,7 @@
 // attention on packed prompts or a paged cache, appends, page copies 20-50 -> 4-8.
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/extension.h>
 
 #include <optional>
@@ -30,6 +31,13 @@ struct Entries {
     decltype(&tpb200_paged_attention) paged_attention;
     decltype(&tpb200_paged_append) paged_append;
     decltype(&tpb200_copy_pages) copy_pages;
+    decltype(&tpb200_packed_attention_window) packed_attention_window;
+    decltype(&tpb200_paged_attention_window) paged_attention_window;
+    decltype(&tpb200_paged_attention_nvfp4_workspace_size) paged_nvfp4_workspace;
+    decltype(&tpb200_paged_attention_nvfp4) paged_attention_nvfp4;
+    decltype(&tpb200_paged_append_nvfp4) paged_append_nvfp4;
+    decltype(&tpb200_paged_read) paged_read;
+    decltype(&tpb200_paged_read_nvfp4) paged_read_nvfp4;
 } g;
 
 using OptTensor = std::optional<at::Tensor>;
@@ -305,9 +313,9 @@ bool paged(const at::Tensor& k, const at::Tensor& v, const at::Tensor& table, co
     return true;
 }
 
-// ops.paged_attention
-py::object paged_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& table, const at::Tensor& lengths,
-                           double scale, const OptTensor& out, const OptTensor& workspace, int flags) {
+// ops.paged_attention; window 0: all keys
+py::object paged_attention_window(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& table, const at::Tensor& lengths,
+                                  double scale, const OptTensor& out, const OptTensor& workspace, int window, int sinks, int flags) {
     const int dev = here(q);
     tpb200_paged_attention_args a = {};
     if (dev < 0 || !paged(k, v, table, lengths, dev, a.cache) || q.dim() != 3 || a.cache.seqs < 1 || a.cache.kv_heads < 1) return py::none();
@@ -335,36 +343,162 @@ py::object paged_attention(const at::Tensor& q, const at::Tensor& k, const at::T
     a.workspace_bytes = ws.nbytes();
     a.flags = flags;
     const tpb200_stream_t s = stream_of(dev);
-    return done(launch([&] { return g.paged_attention(&a, s); }), y);
+    return done(launch([&] { return window > 0 ? g.paged_attention_window(&a, window, sinks, s) : g.paged_attention(&a, s); }), y);
+}
+py::object paged_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& table, const at::Tensor& lengths,
+                           double scale, const OptTensor& out, const OptTensor& workspace, int flags) {
+    return paged_attention_window(q, k, v, table, lengths, scale, out, workspace, 0, 0, flags);
 }
 
-// ops.paged_append; True where there are no queries to give back
-py::object paged_append(const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_pages, const at::Tensor& v_pages, const at::Tensor& table,
-                        const at::Tensor& cu, const at::Tensor& lengths, const OptTensor& q, const OptTensor& cos, const OptTensor& sin,
-                        const OptTensor& q_out, int flags) {
-    const int dev = here(k);
-    tpb200_paged_append_args a = {};
-    if (dev < 0 || !paged(k_pages, v_pages, table, lengths, dev, a.cache) || k.dim() != 3) return py::none();
-    const int64_t T = k.size(0), D = a.cache.head_dim;
-    const auto type = k_pages.scalar_type();
-    if (!rows(k, dev, T, a.cache.kv_heads, D, type) || !rows(v, dev, T, a.cache.kv_heads, D, type) || !offsets(cu, dev, a.cache.seqs + 1) ||
-        cos.has_value() != sin.has_value() || (q.has_value() && !cos.has_value()) || (!q.has_value() && q_out.has_value())) {
+// one layer of a cache of 4-bit pages
+bool paged_nvfp4(const at::Tensor& k, const at::Tensor& v, const at::Tensor& table, const at::Tensor& lengths, int64_t head_dim, double k_scale,
+                 double v_scale, int dev, tpb200_paged_nvfp4_cache& c) {
+    if (!on(k, dev) || !on(v, dev) || !on(table, dev) || !on(lengths, dev) || k.dim() != 4 || k.scalar_type() != at::kByte ||
+        v.scalar_type() != at::kByte || v.sizes() != k.sizes() || v.strides() != k.strides() || k.stride(3) != 1 || head_dim < 8 || head_dim > 256 ||
+        k.size(3) != 288 * ((head_dim + 31) / 32) || table.dim() != 2 || table.scalar_type() != at::kInt || lengths.dim() != 1 ||
+        lengths.scalar_type() != at::kInt || lengths.numel() != table.size(0) || !lengths.is_contiguous() ||
+        (table.size(1) > 1 && table.stride(1) != 1) || !fits({k.size(0), k.size(1), 16 * k.size(2)}) || !fits(table.sizes())) {
+        return false;
+    }
+    c.k_pages = k.data_ptr();
+    c.v_pages = v.data_ptr();
+    c.page_stride = k.stride(0);
+    c.head_stride = k.stride(1);
+    c.tile_stride = k.stride(2);
+    c.num_pages = static_cast<int>(k.size(0));
+    c.page_size = static_cast<int>(16 * k.size(2));
+    c.kv_heads = static_cast<int>(k.size(1));
+    c.head_dim = static_cast<int>(head_dim);
+    c.k_scale = static_cast<float>(k_scale);
+    c.v_scale = static_cast<float>(v_scale);
+    c.table = static_cast<const int*>(table.data_ptr());
+    c.table_stride = table.stride(0);
+    c.table_width = static_cast<int>(table.size(1));
+    c.lengths = static_cast<const int*>(lengths.data_ptr());
+    c.seqs = static_cast<int>(table.size(0));
+    return true;
+}
+
+// ops.paged_attention_nvfp4
+py::object paged_attention_nvfp4(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& table, const at::Tensor& lengths,
+                                 double scale, const OptTensor& out, const OptTensor& workspace, int window, int sinks, double k_scale,
+                                 double v_scale, int flags) {
+    const int dev = here(q);
+    tpb200_paged_attention_nvfp4_args a = {};
+    if (dev < 0 || q.dim() != 3 || !half(q) || !paged_nvfp4(k, v, table, lengths, q.size(2), k_scale, v_scale, dev, a.cache) || a.cache.seqs < 1 ||
+        a.cache.kv_heads < 1) {
         return py::none();
+    }
+    const int64_t H = q.size(1), D = q.size(2);
+    if (!rows(q, dev, a.cache.seqs, H, D, q.scalar_type()) || !on(workspace, dev) || H < 1 || H % a.cache.kv_heads != 0 ||
+        (workspace.has_value() && !workspace->is_contiguous()) || (out.has_value() && !rows(*out, dev, a.cache.seqs, H, D, q.scalar_type()))) {
+        return py::none();
+    }
+    at::Tensor ws;
+    if (workspace.has_value()) ws = *workspace;
+    else {
+        const size_t n = g.paged_nvfp4_workspace(static_cast<int>(H), a.cache.kv_heads, a.cache.head_dim);
+        if (n == 0) return py::none();
+        ws = at::empty({static_cast<int64_t>(n)}, q.options().dtype(at::kByte));
+    }
+    const at::Tensor y = out.has_value() ? *out : at::empty(q.sizes(), q.options());
+    a.q = q.data_ptr();
+    a.out = y.data_ptr();
+    a.dtype = code_of(q.scalar_type());
+    strides(q, a.q_stride);
+    strides(y, a.o_stride);
+    a.q_heads = static_cast<int>(H);
+    a.scale = static_cast<float>(scale);
+    a.window = window;
+    a.sinks = sinks;
+    a.workspace = ws.data_ptr();
+    a.workspace_bytes = ws.nbytes();
+    a.flags = flags;
+    const tpb200_stream_t s = stream_of(dev);
+    return done(launch([&] { return g.paged_attention_nvfp4(&a, s); }), y);
+}
+
+// (k, v) as the rows that a read gives; false where they are not the plain case
+bool read_rows(const at::Tensor& pages, int64_t heads, int64_t D, at::ScalarType type, const at::Tensor& cu, int64_t seqs, int64_t tokens,
+               const OptTensor& k, const OptTensor& v, int dev, at::Tensor (&y)[2], tpb200_paged_rows& a) {
+    if (!offsets(cu, dev, seqs + 1) || tokens < 0 || !fits({tokens}) || k.has_value() != v.has_value() ||
+        (k.has_value() && (!rows(*k, dev, tokens, heads, D, type) || !rows(*v, dev, tokens, heads, D, type)))) {
+        return false;
+    }
+    for (int i = 0; i < 2; ++i) {
+        y[i] = k.has_value() ? *(i == 0 ? k : v) : at::empty({tokens, heads, D}, pages.options().dtype(type));
+    }
+    a.k = y[0].data_ptr();
+    a.v = y[1].data_ptr();
+    a.dtype = code_of(type);
+    strides(y[0], a.k_stride);
+    strides(y[1], a.v_stride);
+    a.cu = static_cast<const int*>(cu.data_ptr());
+    a.tokens = static_cast<int>(tokens);
+    return true;
+}
+py::object pair_of(int status, const at::Tensor (&y)[2]) { return status == 0 ? py::object(py::make_tuple(y[0], y[1])) : py::int_(status); }
+
+// ops.paged_read
+py::object paged_read(const at::Tensor& k_pages, const at::Tensor& v_pages, const at::Tensor& table, const at::Tensor& cu, const at::Tensor& lengths,
+                      const py::object& tokens, const OptTensor& k, const OptTensor& v, int flags) {
+    const int dev = here(k_pages);
+    tpb200_paged_cache c = {};
+    tpb200_paged_rows a = {};
+    at::Tensor y[2];
+    if (dev < 0 || !PyLong_CheckExact(tokens.ptr()) || !paged(k_pages, v_pages, table, lengths, dev, c)) return py::none();
+    int overflow = 0;
+    const int64_t n = PyLong_AsLongAndOverflow(tokens.ptr(), &overflow);
+    if (overflow != 0 || !read_rows(k_pages, c.kv_heads, c.head_dim, k_pages.scalar_type(), cu, c.seqs, n, k, v, dev, y, a)) return py::none();
+    a.flags = flags;
+    const tpb200_stream_t s = stream_of(dev);
+    return pair_of(launch([&] { return g.paged_read(&c, &a, s); }), y);
+}
+
+// ops.paged_read_nvfp4
+py::object paged_read_nvfp4(const at::Tensor& k_pages, const at::Tensor& v_pages, const at::Tensor& table, const at::Tensor& cu, const at::Tensor& lengths,
+                            const py::object& head_dim, const py::object& tokens, const py::object& dtype, const OptTensor& k, const OptTensor& v,
+                            double k_scale, double v_scale, int flags) {
+    const int dev = here(k_pages);
+    tpb200_paged_nvfp4_cache c = {};
+    tpb200_paged_rows a = {};
+    at::Tensor y[2];
+    if (dev < 0 || !PyLong_CheckExact(tokens.ptr()) || !PyLong_CheckExact(head_dim.ptr()) || !THPDtype_Check(dtype.ptr())) return py::none();
+    const auto type = reinterpret_cast<THPDtype*>(dtype.ptr())->scalar_type;
+    int overflow = 0, too_wide = 0;
+    const int64_t n = PyLong_AsLongAndOverflow(tokens.ptr(), &overflow), D = PyLong_AsLongAndOverflow(head_dim.ptr(), &too_wide);
+    if (overflow != 0 || too_wide != 0 || (type != at::kBFloat16 && type != at::kHalf) ||
+        !paged_nvfp4(k_pages, v_pages, table, lengths, D, k_scale, v_scale, dev, c) ||
+        !read_rows(k_pages, c.kv_heads, D, type, cu, c.seqs, n, k, v, dev, y, a)) {
+        return py::none();
+    }
+    a.flags = flags;
+    const tpb200_stream_t s = stream_of(dev);
+    return pair_of(launch([&] { return g.paged_read_nvfp4(&c, &a, s); }), y);
+}
+
+// the rows, offsets and tables of an append; false where they are not the plain case
+template <class Args>
+bool append_rows(const at::Tensor& k, const at::Tensor& v, const at::Tensor& cu, const OptTensor& q, const OptTensor& cos, const OptTensor& sin,
+                 const OptTensor& q_out, at::ScalarType type, int heads, int64_t D, int seqs, int dev, at::Tensor& y, Args& a) {
+    const int64_t T = k.size(0);
+    if (!rows(k, dev, T, heads, D, type) || !rows(v, dev, T, heads, D, type) || !offsets(cu, dev, seqs + 1ll) ||
+        cos.has_value() != sin.has_value() || (q.has_value() && !cos.has_value()) || (!q.has_value() && q_out.has_value())) {
+        return false;
     }
     if (cos.has_value()) {
         if (!on(*cos, dev) || !on(*sin, dev) || cos->dim() != 2 || cos->sizes() != sin->sizes() || cos->size(1) != D / 2 ||
             cos->scalar_type() != sin->scalar_type() || code_of(cos->scalar_type()) < 0 || !cos->is_contiguous() || !sin->is_contiguous() || !fits(cos->sizes())) {
-            return py::none();
+            return false;
         }
         a.cos = cos->data_ptr();
         a.sin = sin->data_ptr();
         a.rope_dtype = code_of(cos->scalar_type());
         a.rope_positions = static_cast<int>(cos->size(0));
     }
-    at::Tensor y;
     if (q.has_value()) {
         if (q->dim() != 3 || !rows(*q, dev, T, q->size(1), D, type) || (q_out.has_value() && !rows(*q_out, dev, T, q->size(1), D, type))) {
-            return py::none();
+            return false;
         }
         y = q_out.has_value() ? *q_out : at::empty(q->sizes(), q->options());
         a.q = q->data_ptr();
@@ -379,6 +513,18 @@ py::object paged_append(const at::Tensor& k, const at::Tensor& v, const at::Tens
     strides(v, a.v_stride);
     a.cu = static_cast<const int*>(cu.data_ptr());
     a.tokens = static_cast<int>(T);
+    return true;
+}
+
+// ops.paged_append; True where there are no queries to give back
+py::object paged_append(const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_pages, const at::Tensor& v_pages, const at::Tensor& table,
+                        const at::Tensor& cu, const at::Tensor& lengths, const OptTensor& q, const OptTensor& cos, const OptTensor& sin,
+                        const OptTensor& q_out, int flags) {
+    const int dev = here(k);
+    tpb200_paged_append_args a = {};
+    if (dev < 0 || !paged(k_pages, v_pages, table, lengths, dev, a.cache) || k.dim() != 3) return py::none();
+    at::Tensor y;
+    if (!append_rows(k, v, cu, q, cos, sin, q_out, k_pages.scalar_type(), a.cache.kv_heads, a.cache.head_dim, a.cache.seqs, dev, y, a)) return py::none();
     a.flags = flags;
     const tpb200_stream_t s = stream_of(dev);
     const int st = launch([&] { return g.paged_append(&a, s); });
@@ -386,9 +532,28 @@ py::object paged_append(const at::Tensor& k, const at::Tensor& v, const at::Tens
     return q.has_value() ? py::cast(y) : py::object(py::bool_(true));
 }
 
-// ops.packed_attention
-py::object packed_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& cu, double scale,
-                            const OptTensor& out, bool causal, const OptTensor& cu_keys, int flags) {
+// ops.paged_append_nvfp4; True where there are no queries to give back
+py::object paged_append_nvfp4(const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_pages, const at::Tensor& v_pages, const at::Tensor& table,
+                              const at::Tensor& cu, const at::Tensor& lengths, const OptTensor& q, const OptTensor& cos, const OptTensor& sin,
+                              const OptTensor& q_out, double k_scale, double v_scale, int flags) {
+    const int dev = here(k);
+    tpb200_paged_append_nvfp4_args a = {};
+    if (dev < 0 || k.dim() != 3 || !half(k) || !paged_nvfp4(k_pages, v_pages, table, lengths, k.size(2), k_scale, v_scale, dev, a.cache)) {
+        return py::none();
+    }
+    at::Tensor y;
+    if (!append_rows(k, v, cu, q, cos, sin, q_out, k.scalar_type(), a.cache.kv_heads, a.cache.head_dim, a.cache.seqs, dev, y, a)) return py::none();
+    a.dtype = code_of(k.scalar_type());
+    a.flags = flags;
+    const tpb200_stream_t s = stream_of(dev);
+    const int st = launch([&] { return g.paged_append_nvfp4(&a, s); });
+    if (st != 0) return py::int_(st);
+    return q.has_value() ? py::cast(y) : py::object(py::bool_(true));
+}
+
+// ops.packed_attention; window 0: all keys
+py::object packed(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& cu, double scale,
+                  const OptTensor& out, bool causal, const OptTensor& cu_keys, int window, int sinks, int flags) {
     const int dev = here(q);
     if (dev < 0 || q.dim() != 3 || k.dim() != 3 || !half(q)) return py::none();
     const int64_t T = q.size(0), H = q.size(1), D = q.size(2), Tk = k.size(0), Hk = k.size(1);
@@ -421,7 +586,15 @@ py::object packed_attention(const at::Tensor& q, const at::Tensor& k, const at::
     a.causal = causal;
     a.flags = flags;
     const tpb200_stream_t s = stream_of(dev);
-    return done(launch([&] { return g.packed_attention(&a, s); }), y);
+    return done(launch([&] { return window > 0 ? g.packed_attention_window(&a, window, sinks, s) : g.packed_attention(&a, s); }), y);
+}
+py::object packed_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& cu, double scale,
+                            const OptTensor& out, bool causal, const OptTensor& cu_keys, int flags) {
+    return packed(q, k, v, cu, scale, out, causal, cu_keys, 0, 0, flags);
+}
+py::object packed_attention_window(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& cu, double scale,
+                                   const OptTensor& out, const OptTensor& cu_keys, int window, int sinks, int flags) {
+    return packed(q, k, v, cu, scale, out, true, cu_keys, window, sinks, flags);
 }
 
 // ops.copy_pages on lists of ints; True when done
@@ -471,4 +644,10 @@ PYBIND11_MODULE(_calls, m) {
     m.def("paged_attention", &paged_attention);
     m.def("paged_append", &paged_append);
     m.def("copy_pages", &copy_pages);
+    m.def("packed_attention_window", &packed_attention_window);
+    m.def("paged_attention_window", &paged_attention_window);
+    m.def("paged_attention_nvfp4", &paged_attention_nvfp4);
+    m.def("paged_append_nvfp4", &paged_append_nvfp4);
+    m.def("paged_read", &paged_read);
+    m.def("paged_read_nvfp4", &paged_read_nvfp4);
 }

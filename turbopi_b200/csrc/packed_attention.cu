@@ -74,6 +74,7 @@ struct PackedParams {
     float scale2;                        // |scale| log2 e
     uint32_t idesc_s, idesc_o;
     int causal;
+    int window, sinks;                   // a query sees the last `window` keys up to its own and the first `sinks` (kWindow)
 };
 
 // DP: head_dim rounded up to 64, 128 or 256; R: tiles of 128 rows per CTA, two only up to 128
@@ -105,12 +106,12 @@ struct PackedControl {
     uint64_t s_ready[2], p_ready[2][2], o_done[2];       // p_ready: by half of the tile's keys
     uint64_t s_read[2];                  // scores are in registers, the next ones may take their place (kAhead)
     uint64_t ref_ready[2][4];            // one row tile: the reference of event e, by quarter of the rows
-    uint64_t v_landed[kBadTiles];        // V of a tile with masked pairs, which is looked over before its units count as full
+    uint64_t v_landed[2 * kBadTiles];    // V of a tile with masked pairs, which is looked over before its units count as full
     uint32_t tmem_base;
     int failed;
     int seq, tile, q0, nq, k0, nk;       // the CTA's work
     int bad_any;
-    uint32_t bad[kBadTiles][4];          // keys of masked tiles with infinities or NaN in V, from the first masked tile on
+    uint32_t bad[2 * kBadTiles][4];      // keys of masked tiles with infinities or NaN in V
     float ref[kTile];
     float part_l[2][kTile], part_m[2][kTile];
 };
@@ -220,7 +221,7 @@ __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec
 template <int kRegs>
 __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs)); }
 
-template <typename T, int DP, int R>
+template <typename T, int DP, int R, bool kWindow>
 __global__ void __launch_bounds__(Layout<DP, R>::kThreads, Layout<DP, R>::kCtas) packed_attention_kernel(const __grid_constant__ PackedParams P) {
     using L = Layout<DP, R>;
     extern __shared__ uint8_t smem_raw[];
@@ -282,11 +283,11 @@ __global__ void __launch_bounds__(Layout<DP, R>::kThreads, Layout<DP, R>::kCtas)
             mbar_init(&ctl->s_read[i], 4);
             for (int w = 0; w < 4; ++w) mbar_init(&ctl->ref_ready[i][w], 1);
         }
-        for (int i = 0; i < kBadTiles; ++i) mbar_init(&ctl->v_landed[i], L::kHalves);
+        for (int i = 0; i < (kWindow ? 2 : 1) * kBadTiles; ++i) mbar_init(&ctl->v_landed[i], L::kHalves);
         fence_mbar_init();
         ctl->failed = 0;
         ctl->bad_any = 0;
-        for (int i = 0; i < kBadTiles * 4; ++i) ctl->bad[i >> 2][i & 3] = 0;
+        for (int i = 0; i < (kWindow ? 2 : 1) * kBadTiles * 4; ++i) ctl->bad[i >> 2][i & 3] = 0;
         tc::prefetch_tensormap(&P.q);
         if (P.k_tokens > 0) {
             tc::prefetch_tensormap(&P.k);
@@ -317,8 +318,30 @@ __global__ void __launch_bounds__(Layout<DP, R>::kThreads, Layout<DP, R>::kCtas)
         tiles[x] = (x < R && last >= first) ? (row_limit(P, nq, nk, last) + kTile - 1) / kTile : 0;
     }
     if (!L::kOwn) tiles[1] = 0;
+    // With a window, the key tiles between those of the sinks and the first one that the first row's window reaches are left out: tile j of the
+    // CTA is key tile real(j).  Those from left_begin to left_end hold pairs hidden by the window, kBadTiles at most: the last one of the sinks, and
+    // where the windows of 256 rows begin.
+    int skip = 0, sink_tiles = 0, left_begin = 0, left_end = 0;
+    if (kWindow) {
+        const int first = row_limit(P, nq, nk, token0), last = row_limit(P, nq, nk, min(token0 + tokens_cta, nq) - 1);
+        sink_tiles = static_cast<int>((static_cast<unsigned>(P.sinks) + kTile - 1) / kTile);
+        skip = max(0, max(0, first - P.window) / kTile - sink_tiles);
+        const int behind = last - P.window;              // of the keys that some row does not see, but for the sinks
+        if (behind > P.sinks) {
+            left_begin = min(P.sinks / kTile, first / kTile - skip);
+            left_end = max(sink_tiles, (behind + kTile - 1) / kTile - skip);
+        }
+#pragma unroll
+        for (int x = 0; x < 2; ++x) tiles[x] = max(0, tiles[x] - skip);
+    }
+    auto real = [&](int j) { return kWindow && j >= sink_tiles ? j + skip : j; };
     const int n_tiles = max(tiles[0], tiles[1]);
-    const int first_masked = row_limit(P, nq, nk, token0) / kTile;       // key tiles from here on hold masked pairs: kBadTiles at most
+    const int first_masked = row_limit(P, nq, nk, token0) / kTile - skip;      // tiles from here on hold masked pairs: kBadTiles at most
+    const int right_begin = kWindow ? max(first_masked, left_end) : first_masked;
+    // the places of tiles with masked pairs in v_landed and bad
+    auto looked_over = [&](int j) { return j >= first_masked || (kWindow && j >= left_begin && j < left_end); };
+    auto place = [&](int j) { return kWindow ? (j < left_end ? j - left_begin : kBadTiles + j - right_begin) : j - first_masked; };
+    auto tile_at = [&](int place) { return kWindow ? (place < kBadTiles ? left_begin + place : right_begin + place - kBadTiles) : first_masked + place; };
     const int events = L::kOwn ? 2 * n_tiles : n_tiles;
     // the order of the line of events: which are computed, and where the tiles of K and V stand in the ring
     auto active = [&](int e) { return L::kOwn ? (e >> 1) < tiles[e & 1] : true; };
@@ -345,11 +368,11 @@ __global__ void __launch_bounds__(Layout<DP, R>::kThreads, Layout<DP, R>::kCtas)
                     for (int h = 0; h < L::kHalves; ++h, ++u) {
                         const int slot = u % L::kUnits;
                         if (!mbar_wait_bounded(&ctl->empty[slot], ((u / L::kUnits) & 1) ^ 1, kWait)) return false;
-                        uint64_t* bar = values && j >= first_masked ? &ctl->v_landed[j - first_masked] : &ctl->full[slot];
+                        uint64_t* bar = values && looked_over(j) ? &ctl->v_landed[place(j)] : &ctl->full[slot];
                         mbar_expect_tx(bar, L::kUnitBytes);
                         for (int b = 0; b < L::kUnitBlocks; ++b) {
                             tma_load_3d(ring + slot * L::kUnitBytes + b * kBlockBytes, map, (h * L::kUnitBlocks + b) * 64, kv_head,
-                                        k0 + j * kTile, bar);
+                                        k0 + real(j) * kTile, bar);
                         }
                     }
                     return true;
@@ -508,11 +531,12 @@ __global__ void __launch_bounds__(Layout<DP, R>::kThreads, Layout<DP, R>::kCtas)
         } else if (warp >= 2) {
             // -------------------------------------------------------- V of tiles with masked pairs
             // Rows behind the sequence's end to zero, infinities and NaN out of the product.  x * 0 summed up is NaN if there is one.
-            for (int j = first_masked; j < n_tiles; ++j) {
+            for (int j = kWindow && left_begin < left_end ? left_begin : first_masked; j < n_tiles; ++j) {
+                if (kWindow && !looked_over(j)) continue;
                 const int u0 = v_unit(j);
-                bool ok = wait_warp(&ctl->v_landed[j - first_masked], 0);
+                bool ok = wait_warp(&ctl->v_landed[place(j)], 0);
                 for (int r = (warp - 2) * 32 + lane; r < kTile && ok; r += 64) {
-                    const bool there = j * kTile + r < nk;
+                    const bool there = real(j) * kTile + r < nk;
                     bool bad = false;
                     for (int h = 0; h < L::kHalves; ++h) {
                         for (int b = 0; b < L::kUnitBlocks; ++b) {
@@ -543,7 +567,7 @@ __global__ void __launch_bounds__(Layout<DP, R>::kThreads, Layout<DP, R>::kCtas)
                     }
                     const uint32_t word = __ballot_sync(0xffffffffu, bad);
                     if (lane == 0 && word != 0) {
-                        ctl->bad[j - first_masked][r >> 5] = word;
+                        ctl->bad[place(j)][r >> 5] = word;
                         ctl->bad_any = 1;
                     }
                 }
@@ -569,6 +593,8 @@ __global__ void __launch_bounds__(Layout<DP, R>::kThreads, Layout<DP, R>::kCtas)
         const int token = token0 + my_tile * tokens_tile + (row >> P.pack_shift);
         const int limit = row_limit(P, nq, nk, token);
         const int lowest = row_limit(P, nq, nk, token0 + my_tile * tokens_tile);     // of the tile's rows that exist
+        // of the tile's rows that exist: behind the last key that the window hides from one
+        const int behind = kWindow ? row_limit(P, nq, nk, min(token0 + (my_tile + 1) * tokens_tile, nq) - 1) - P.window : 0;
         float ref = -INFINITY, l = 0.0f;
         float l_ref = -INFINITY;         // the reference that l is relative to (one row tile: the groups share ref)
         bool ok = true;
@@ -577,8 +603,9 @@ __global__ void __launch_bounds__(Layout<DP, R>::kThreads, Layout<DP, R>::kCtas)
             const int j = key_tile(e);
             if (!wait_warp(&ctl->s_ready[x], (e >> 1) & 1)) { ok = false; break; }
             tc::fence_after_thread_sync();
-            const bool masked = (j + 1) * kTile > lowest;
-            const int lim = limit - j * kTile;
+            const int key0 = real(j) * kTile;
+            const bool masked = key0 + kTile > lowest || (kWindow && key0 < behind && key0 + kTile > P.sinks);
+            const int lim = limit - key0;
             uint32_t s[kTile];
             float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -593,7 +620,12 @@ __global__ void __launch_bounds__(Layout<DP, R>::kThreads, Layout<DP, R>::kCtas)
             if (masked) {
 #pragma unroll
                 for (int c = 0; c < kTile; c += 32) {    // a bit per column that is seen
-                    const uint32_t sees = lim >= c + 32 ? 0xffffffffu : (lim > c ? (1u << (lim - c)) - 1 : 0u);
+                    uint32_t sees = lim >= c + 32 ? 0xffffffffu : (lim > c ? (1u << (lim - c)) - 1 : 0u);
+                    if (kWindow) {                       // but not [sinks, limit - window)
+                        const int from = min(max(P.sinks - key0 - c, 0), 32), to = min(max(lim - P.window - c, 0), 32);
+                        const uint32_t below_to = to == 32 ? 0xffffffffu : (1u << to) - 1, below_from = from == 32 ? 0xffffffffu : (1u << from) - 1;
+                        sees &= ~(below_to & ~below_from);
+                    }
 #pragma unroll
                     for (int i = 0; i < 32; ++i) s[c + i] = (sees >> i) & 1 ? s[c + i] : 0xff800000u;
                 }
@@ -696,9 +728,10 @@ __global__ void __launch_bounds__(Layout<DP, R>::kThreads, Layout<DP, R>::kCtas)
                     tc::tmem_ld_wait();
                 }
                 if (any_bad && token < nq) {             // what was taken out of V, for the rows that see it
-                    for (int i = 0; i < kBadTiles * kTile; ++i) {
-                        const int key = (first_masked + i / kTile) * kTile + i % kTile;
+                    for (int i = 0; i < (kWindow ? 2 : 1) * kBadTiles * kTile; ++i) {
+                        const int key = real(tile_at(i / kTile)) * kTile + i % kTile;
                         if (!((ctl->bad[i >> 7][(i >> 5) & 3] >> (i & 31)) & 1) || key >= limit) continue;
+                        if (kWindow && key >= P.sinks && key < limit - P.window) continue;
                         const uint16_t* from = P.v_rows + static_cast<long long>(k0 + key) * P.v_stride[0] +
                                                head_group / P.groups_per_kv * P.v_stride[1];
 #pragma unroll
@@ -752,7 +785,7 @@ __global__ void __launch_bounds__(Layout<DP, R>::kThreads, Layout<DP, R>::kCtas)
     if (warp == 2) tc::tmem_dealloc(tmem, L::kTmemCols);
 }
 
-template <typename T, int DP, int R>
+template <typename T, int DP, int R, bool kWindow>
 int launch_packed(const PackedParams& P, unsigned blocks, cudaStream_t stream) {
     constexpr int smem = packed_smem<DP, R>();
     static_assert(Layout<DP, R>::kCtas * (smem + 1024) <= 228 * 1024, "shared memory of an SM");
@@ -761,14 +794,14 @@ int launch_packed(const PackedParams& P, unsigned blocks, cudaStream_t stream) {
     cudaGetDevice(&dev);
     const uint64_t bit = 1ull << (dev & 63);
     if (!(configured.load(std::memory_order_relaxed) & bit)) {
-        if (cudaFuncSetAttribute(packed_attention_kernel<T, DP, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
+        if (cudaFuncSetAttribute(packed_attention_kernel<T, DP, R, kWindow>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
             return TPB200_ERR_CUDA;
         }
         configured.fetch_or(bit, std::memory_order_relaxed);
     }
     cudaLaunchAttribute attr;
     const cudaLaunchConfig_t cfg = paged_config(blocks, Layout<DP, R>::kThreads, smem, &attr, stream);
-    return cudaLaunchKernelEx(&cfg, packed_attention_kernel<T, DP, R>, P) == cudaSuccess ? TPB200_OK : TPB200_ERR_CUDA;
+    return cudaLaunchKernelEx(&cfg, packed_attention_kernel<T, DP, R, kWindow>, P) == cudaSuccess ? TPB200_OK : TPB200_ERR_CUDA;
 }
 
 // [tokens][heads][head_dim] with element strides, boxes of 64 columns x `heads` x `rows` tokens
@@ -787,8 +820,11 @@ int device_error_packed_attention(int clear) { return read_device_error(clear); 
 
 }  // namespace tpb
 
-extern "C" int tpb200_packed_attention(const tpb200_packed_attention_args* a, tpb200_stream_t stream) {
-    using namespace tpb;
+namespace tpb {
+namespace {
+
+// window 0: all keys up to a query's own
+int attend(const tpb200_packed_attention_args* a, int window, int sinks, tpb200_stream_t stream) {
     TPB_REQUIRE(a != nullptr, TPB200_ERR_NULL);
     TPB_REQUIRE((a->flags & ~TPB200_FLAG_PDL) == 0, TPB200_ERR_ENUM);
     TPB_REQUIRE(a->dtype == TPB200_BF16 || a->dtype == TPB200_F16, TPB200_ERR_ENUM);
@@ -824,6 +860,9 @@ extern "C" int tpb200_packed_attention(const tpb200_packed_attention_args* a, tp
     P.out = static_cast<uint16_t*>(a->out);
     P.v_rows = static_cast<const uint16_t*>(a->v);
     P.causal = a->causal != 0;
+    const bool hides = window > 0 && window < a->k_tokens;       // else no query has a key that it does not see
+    P.window = window;
+    P.sinks = std::min(sinks, a->k_tokens);
     // the sign of the scale goes into the product (operand A negated), its size into the exponent; none at all would lose the mask
     P.scale2 = fmaxf(fabsf(a->scale) * 1.4426950408889634f, 1.1754944e-38f);
     TPB_REQUIRE(std::isfinite(P.scale2), TPB200_ERR_SHAPE);
@@ -850,18 +889,32 @@ extern "C" int tpb200_packed_attention(const tpb200_packed_attention_args* a, tp
     // SM: half the rows to fill up, and one's loads and output beside the other's products.  The border is where the two meet on average:
     // 24 sequences of 100 / 8 of 1536, 16 heads of 64: 13.5 us with one, 18.1 with two / 91.6, 92.6; 16 heads of 128: 21.0, 25.2 / 129, 118.
     // Batches of sequences alike; not measured where lengths differ much or queries are few beside the keys.
-    const bool two = DP <= 128 && static_cast<long long>(a->k_tokens) > (DP == 64 ? 1000ll : 200ll) * a->seqs;
+    const long long keys = hides ? std::min<long long>(a->k_tokens, (static_cast<long long>(window) + P.sinks) * a->seqs) : a->k_tokens;
+    const bool two = DP <= 128 && keys > (DP == 64 ? 1000ll : 200ll) * a->seqs;
     // no more tiles than whole ones and a ragged one per sequence
     const long long tiles = static_cast<long long>(a->q_tokens) / (rows_tokens * (two ? 2 : 1)) + std::min(a->seqs, a->q_tokens);
     const long long blocks = tiles * P.head_groups;
     TPB_REQUIRE(blocks <= 0x7fffffff, TPB200_ERR_SHAPE);
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     const unsigned n = static_cast<unsigned>(blocks);
-    auto launch = [&](auto type) {
+    auto launch = [&](auto type, auto windowed) {
         using T = decltype(type);
-        if (DP == 64) return two ? launch_packed<T, 64, 2>(P, n, s) : launch_packed<T, 64, 1>(P, n, s);
-        if (DP == 128) return two ? launch_packed<T, 128, 2>(P, n, s) : launch_packed<T, 128, 1>(P, n, s);
-        return launch_packed<T, 256, 1>(P, n, s);
+        constexpr bool W = decltype(windowed)::value;
+        if (DP == 64) return two ? launch_packed<T, 64, 2, W>(P, n, s) : launch_packed<T, 64, 1, W>(P, n, s);
+        if (DP == 128) return two ? launch_packed<T, 128, 2, W>(P, n, s) : launch_packed<T, 128, 1, W>(P, n, s);
+        return launch_packed<T, 256, 1, W>(P, n, s);
     };
-    return bf ? launch(__nv_bfloat16()) : launch(__half());
+    if (hides) return bf ? launch(__nv_bfloat16(), std::true_type()) : launch(__half(), std::true_type());
+    return bf ? launch(__nv_bfloat16(), std::false_type()) : launch(__half(), std::false_type());
+}
+
+}  // namespace
+}  // namespace tpb
+
+extern "C" int tpb200_packed_attention(const tpb200_packed_attention_args* a, tpb200_stream_t stream) { return tpb::attend(a, 0, 0, stream); }
+
+extern "C" int tpb200_packed_attention_window(const tpb200_packed_attention_args* a, int window, int sinks, tpb200_stream_t stream) {
+    TPB_REQUIRE(a != nullptr, TPB200_ERR_NULL);
+    TPB_REQUIRE(window >= 1 && sinks >= 0 && a->causal, TPB200_ERR_SHAPE);
+    return tpb::attend(a, window, sinks, stream);
 }

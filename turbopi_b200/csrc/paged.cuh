@@ -2,6 +2,7 @@
 #pragma once
 
 #include <algorithm>
+#include <cmath>
 
 #include "common.cuh"
 
@@ -44,6 +45,48 @@ struct Half16<__half> {
         return *reinterpret_cast<const uint32_t*>(&h);
     }
 };
+
+// V values of a 16-bit type
+template <int V>
+struct Vec { uint32_t w[V / 2]; };
+
+template <int V>
+__device__ __forceinline__ Vec<V> load_vec(const uint16_t* p) {
+    Vec<V> r;
+    if constexpr (V == 8) {
+        const uint4 u = *reinterpret_cast<const uint4*>(p);
+        r.w[0] = u.x; r.w[1] = u.y; r.w[2] = u.z; r.w[3] = u.w;
+    } else {
+        const uint2 u = *reinterpret_cast<const uint2*>(p);
+        r.w[0] = u.x; r.w[1] = u.y;
+    }
+    return r;
+}
+template <int V>
+__device__ __forceinline__ void store_vec(uint16_t* p, const Vec<V>& r) {
+    if constexpr (V == 8) *reinterpret_cast<uint4*>(p) = make_uint4(r.w[0], r.w[1], r.w[2], r.w[3]);
+    else *reinterpret_cast<uint2*>(p) = make_uint2(r.w[0], r.w[1]);
+}
+
+// V consecutive table entries as floats
+template <int V>
+__device__ __forceinline__ void load_table(const void* p, int dtype, size_t at, float (&f)[V]) {
+    if (dtype == TPB200_F32) {
+#pragma unroll
+        for (int i = 0; i < V; i += 4) {
+            const float4 t = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p) + at + i));
+            f[i] = t.x; f[i + 1] = t.y; f[i + 2] = t.z; f[i + 3] = t.w;
+        }
+    } else {
+        const Vec<V> t = load_vec<V>(static_cast<const uint16_t*>(p) + at);
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) {
+            const float2 x = dtype == TPB200_F16 ? Half16<__half>::unpack(t.w[i]) : Half16<__nv_bfloat16>::unpack(t.w[i]);
+            f[2 * i] = x.x;
+            f[2 * i + 1] = x.y;
+        }
+    }
+}
 
 // The cache as a kernel sees it.  Offsets are in elements and 64 bits wide: a pool of pages passes 2^31 elements at 4 GB.
 struct PagedView {
@@ -137,6 +180,32 @@ static inline int paged_view(const tpb200_paged_cache& c, PagedView* v) {
     }
     auto used = [](long long stride, int n) { return n > 1 ? stride : 0; };
     *v = {c.k_pages, c.v_pages, used(c.page_stride, c.num_pages), used(c.row_stride, c.page_size), used(c.head_stride, c.kv_heads), c.table,
+          c.lengths, used(c.table_stride, c.seqs), c.num_pages, c.page_size, c.kv_heads, c.head_dim, c.table_width, c.seqs};
+    return TPB200_OK;
+}
+
+// A cache of 4-bit values as a PagedView: strides in bytes, row_stride from one tile of 16 tokens to the next
+static inline int paged_view_nvfp4(const tpb200_paged_nvfp4_cache& c, PagedView* v) {
+    TPB_REQUIRE(c.seqs >= 0 && c.num_pages >= 1 && c.kv_heads >= 1 && c.table_width >= 1, TPB200_ERR_SHAPE);
+    TPB_REQUIRE(c.page_size >= 16 && c.page_size % 16 == 0, TPB200_ERR_SHAPE);
+    TPB_REQUIRE(c.head_dim >= 8 && c.head_dim <= 256 && c.head_dim % 8 == 0, TPB200_ERR_SHAPE);
+    TPB_REQUIRE(static_cast<long long>(c.page_size) * c.table_width <= 0x7fffffff, TPB200_ERR_SHAPE);   // positions are 32 bits
+    TPB_REQUIRE(c.k_pages && c.v_pages, TPB200_ERR_NULL);
+    TPB_REQUIRE(c.seqs == 0 || (c.table && c.lengths), TPB200_ERR_NULL);
+    TPB_REQUIRE(tpb_aligned16(c.k_pages) && tpb_aligned16(c.v_pages), TPB200_ERR_ALIGN);
+    TPB_REQUIRE(c.seqs <= 1 || c.table_stride >= 0, TPB200_ERR_SHAPE);
+    for (const float f : {c.k_scale, c.v_scale}) {           // powers of two: what is held stays exact in 16 bits
+        int e = 0;
+        TPB_REQUIRE(std::isfinite(f) && std::frexp(f, &e) == 0.5f && e >= -62 && e <= 65, TPB200_ERR_SHAPE);
+    }
+    const long long tile = 288ll * ((c.head_dim + 31) / 32), strides[3] = {c.page_stride, c.head_stride, c.tile_stride};
+    const int sizes[3] = {c.num_pages, c.kv_heads, c.page_size / 16};
+    for (int i = 0; i < 3; ++i) {
+        TPB_REQUIRE(sizes[i] <= 1 || strides[i] % 16 == 0, TPB200_ERR_ALIGN);
+        TPB_REQUIRE(strides[i] >= 0 && (sizes[i] <= 1 || strides[i] >= tile), TPB200_ERR_SHAPE);
+    }
+    auto used = [](long long stride, int n) { return n > 1 ? stride : 0; };
+    *v = {c.k_pages, c.v_pages, used(c.page_stride, c.num_pages), used(c.tile_stride, c.page_size / 16), used(c.head_stride, c.kv_heads), c.table,
           c.lengths, used(c.table_stride, c.seqs), c.num_pages, c.page_size, c.kv_heads, c.head_dim, c.table_width, c.seqs};
     return TPB200_OK;
 }

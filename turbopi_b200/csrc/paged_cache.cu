@@ -30,47 +30,6 @@ struct AppendParams {
     int units_q, units_k, units_v;       // units per token of the queries, the keys, the values
 };
 
-template <int V>
-struct Vec { uint32_t w[V / 2]; };
-
-template <int V>
-__device__ __forceinline__ Vec<V> load_vec(const uint16_t* p) {
-    Vec<V> r;
-    if constexpr (V == 8) {
-        const uint4 u = *reinterpret_cast<const uint4*>(p);
-        r.w[0] = u.x; r.w[1] = u.y; r.w[2] = u.z; r.w[3] = u.w;
-    } else {
-        const uint2 u = *reinterpret_cast<const uint2*>(p);
-        r.w[0] = u.x; r.w[1] = u.y;
-    }
-    return r;
-}
-template <int V>
-__device__ __forceinline__ void store_vec(uint16_t* p, const Vec<V>& r) {
-    if constexpr (V == 8) *reinterpret_cast<uint4*>(p) = make_uint4(r.w[0], r.w[1], r.w[2], r.w[3]);
-    else *reinterpret_cast<uint2*>(p) = make_uint2(r.w[0], r.w[1]);
-}
-
-// V consecutive table entries as floats
-template <int V>
-__device__ __forceinline__ void load_table(const void* p, int dtype, size_t at, float (&f)[V]) {
-    if (dtype == TPB200_F32) {
-#pragma unroll
-        for (int i = 0; i < V; i += 4) {
-            const float4 t = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p) + at + i));
-            f[i] = t.x; f[i + 1] = t.y; f[i + 2] = t.z; f[i + 3] = t.w;
-        }
-    } else {
-        const Vec<V> t = load_vec<V>(static_cast<const uint16_t*>(p) + at);
-#pragma unroll
-        for (int i = 0; i < V / 2; ++i) {
-            const float2 x = dtype == TPB200_F16 ? Half16<__half>::unpack(t.w[i]) : Half16<__nv_bfloat16>::unpack(t.w[i]);
-            f[2 * i] = x.x;
-            f[2 * i + 1] = x.y;
-        }
-    }
-}
-
 // A unit is V values of a row and the V values half a row further on (rotated, or a plain copy of both), so that a rotation
 // needs one thread.  V = 8 where half a row is a multiple of 8, else 4.  A thread keeps its unit (which tensor, head and columns) for all
 // tokens of the block: one division per thread and not per token: 77 -> 54 us for the prompts of six sequences (10.5 k tokens, 32 on 8 heads of 128,

@@ -172,6 +172,8 @@ int device_error_pi05_inputs(int clear);
 int device_error_paged_cache(int clear);
 int device_error_paged_attention(int clear);
 int device_error_packed_attention(int clear);
+int device_error_paged_attention_nvfp4(int clear);
+int device_error_paged_nvfp4(int clear);
 
 }  // namespace tpb
 
@@ -205,7 +207,8 @@ int tpb200_device_error(int clear) {
                                      tpb::device_error_nvfp4_gemm, tpb::device_error_gemv_tc,
                                      tpb::device_error_attention, tpb::device_error_w4_gemm,
                                      tpb::device_error_pi05_inputs, tpb::device_error_paged_cache,
-                                     tpb::device_error_paged_attention, tpb::device_error_packed_attention};
+                                     tpb::device_error_paged_attention, tpb::device_error_packed_attention,
+                                     tpb::device_error_paged_attention_nvfp4, tpb::device_error_paged_nvfp4};
     int first = 0;
     for (auto r : readers) {
         const int v = r(clear);

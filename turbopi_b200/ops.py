@@ -11,6 +11,7 @@ and add the B200-native forms (bf16 in/out, E4M3 block-16 scales, grouped launch
 Every tensor must live on a CUDA device; nothing here computes on the CPU.
 """
 import ctypes
+import operator
 import threading
 
 import torch
@@ -737,14 +738,33 @@ def _strides(t):
     return _Two(t.stride(0), t.stride(1))
 
 
-def packed_attention(q, k, v, cu, scale, out=None, causal=True, cu_keys=None):
+def _window(what, window, sinks):
+    """The keys a query sees, as the C ABI takes them: (0, 0) for all, else the last `window` and the first `sinks`."""
+    try:
+        w, s = 0 if window is None else operator.index(window), operator.index(sinks)
+    except TypeError:
+        raise TurboPiError(f"{what}: window and sinks are whole numbers") from None
+    if s < 0 or (window is None and s > 0) or (window is not None and w < 1):
+        raise TurboPiError(f"{what}: a window of at least one key, and no sinks without a window")
+    return min(w, 2 ** 31 - 1), min(s, 2 ** 31 - 1)
+
+
+def packed_attention(q, k, v, cu, scale, out=None, causal=True, cu_keys=None, window=None, sinks=0):
     """out = softmax(scale * q k^T) v for prompts packed one behind the other; returns out.
     q / out [T, Hq, D], k / v [Tk, Hk, D] (views such as columns of a fused projection are fine; Hq a multiple of Hk, consecutive
     query heads share a key head), bf16 or fp16.  cu int32 [S + 1]: sequence s has the tokens [cu[s], cu[s + 1]).  cu_keys: the
     same for the keys where a sequence has more (or fewer) of them; causal then means that the last query sees every key:
     query i of n sees the keys up to i + (m - n) of m.  A query without keys gives zeros; tokens behind cu[S] are left alone.  The
-    offsets are read on the device: a captured call follows them; ones outside the tensors are clamped."""
-    done = (_lib._native or _lib.native()).packed_attention(q, k, v, cu, scale, out, bool(causal), cu_keys, _flags.value)
+    offsets are read on the device: a captured call follows them; ones outside the tensors are clamped.
+    window (causal only): of these keys a query sees the last `window`, its own among them, and its sequence's first `sinks`; the tiles in
+    between are not read."""
+    w, s = _window("packed_attention", window, sinks)
+    if w == 0:
+        done = (_lib._native or _lib.native()).packed_attention(q, k, v, cu, scale, out, bool(causal), cu_keys, _flags.value)
+    elif not causal:
+        raise TurboPiError("packed_attention: a window goes with causal attention")
+    else:
+        done = (_lib._native or _lib.native()).packed_attention_window(q, k, v, cu, scale, out, cu_keys, w, s, _flags.value)
     if done is not None:
         return _result(done, "tpb200_packed_attention")
     _cuda(q, k, v, cu, out, cu_keys)
@@ -770,7 +790,10 @@ def packed_attention(q, k, v, cu, scale, out=None, causal=True, cu_keys=None):
                                     v_stride=_strides(v), o_stride=_strides(out), cu=_ptr(cu), cu_keys=_ptr(cu_keys),
                                     seqs=cu.numel() - 1, q_tokens=T, k_tokens=Tk, q_heads=Hq, kv_heads=Hk, head_dim=D,
                                     dtype=_HALF[q.dtype], scale=float(scale), causal=int(bool(causal)), flags=_flags.value)
-    _lib.check(_run(q, _lib.load().tpb200_packed_attention, args), "tpb200_packed_attention")
+    if w == 0:
+        _lib.check(_run(q, _lib.load().tpb200_packed_attention, args), "tpb200_packed_attention")
+    else:
+        _lib.check(_run(q, _lib.load().tpb200_packed_attention_window, args, w, s), "tpb200_packed_attention_window")
     return out
 
 
@@ -784,13 +807,20 @@ def paged_attention_workspace(q_heads, kv_heads, head_dim, device):
     return torch.empty(n, dtype=torch.uint8, device=device)
 
 
-def paged_attention(q, k_pages, v_pages, table, lengths, scale, out=None, workspace=None):
+def paged_attention(q, k_pages, v_pages, table, lengths, scale, out=None, workspace=None, window=None, sinks=0):
     """out[s] = softmax(scale * q[s] K^T) V for one new token of each sequence on a cache of pages; returns out.
     q / out [S, Hq, D]; pages [P, page, Hk, D] (one layer; Hq a multiple of Hk, consecutive query heads share a key head); table
     int32 [S, W]: position j of sequence s is row j % page of page table[s, j // page]; lengths int32 [S], the new token among them.
     bf16 or fp16.  A sequence of length 0 gives zeros.  table and lengths are read on the device: a captured call follows
-    them.  Positions without a page in the pool, or beyond the table, are left out and reported by tpb200_device_error()."""
-    done = (_lib._native or _lib.native()).paged_attention(q, k_pages, v_pages, table, lengths, scale, out, workspace, _flags.value)
+    them.  Positions without a page in the pool, or beyond the table, are left out and reported by tpb200_device_error().
+    window: the token sees the last `window` keys, its own among them, and the first `sinks`; pages that hold none of these are not read
+    and need not be in the table."""
+    w, s = _window("paged_attention", window, sinks)
+    if w == 0:
+        done = (_lib._native or _lib.native()).paged_attention(q, k_pages, v_pages, table, lengths, scale, out, workspace, _flags.value)
+    else:
+        done = (_lib._native or _lib.native()).paged_attention_window(q, k_pages, v_pages, table, lengths, scale, out, workspace, w, s,
+                                                                      _flags.value)
     if done is not None:
         return _result(done, "tpb200_paged_attention")
     view = _paged_view("paged_attention", k_pages, v_pages, table, lengths)
@@ -816,7 +846,10 @@ def paged_attention(q, k_pages, v_pages, table, lengths, scale, out=None, worksp
     args = _lib.PagedAttentionArgs(cache=view, q=_ptr(q), out=_ptr(out), q_stride=_strides(q), o_stride=_strides(out), q_heads=Hq,
                                    scale=float(scale), workspace=_ptr(workspace),
                                    workspace_bytes=workspace.numel() * workspace.element_size(), flags=_flags.value)
-    _lib.check(_run(q, _lib.load().tpb200_paged_attention, args), "tpb200_paged_attention")
+    if w == 0:
+        _lib.check(_run(q, _lib.load().tpb200_paged_attention, args), "tpb200_paged_attention")
+    else:
+        _lib.check(_run(q, _lib.load().tpb200_paged_attention_window, args, w, s), "tpb200_paged_attention_window")
     return out
 
 
@@ -867,9 +900,191 @@ def paged_append(k, v, k_pages, v_pages, table, cu, lengths, q=None, cos=None, s
     return q_out
 
 
+# ------------------------------------------------------------------------------------- a cache of pages in 4 bits
+def nvfp4_page_shape(kv_heads, page_size, head_dim):
+    """The last three sizes of a pool of 4-bit pages, uint8 [..., pages, kv_heads, page_size / 16, bytes of a tile]: per key head, tiles of 16
+    tokens.  With G = ceil(head_dim / 32) a tile is 16 rows of 16 G bytes of E2M1 codes (the even value in the low half of a byte), then 16
+    rows of 2 G E4M3 scales, one for every 16 values."""
+    if kv_heads < 1 or page_size < 16 or page_size % 16 or not 8 <= head_dim <= 256 or head_dim % 8:
+        raise TurboPiError("nvfp4 pages: page_size a multiple of 16, head_dim a multiple of 8 up to 256")
+    return kv_heads, page_size // 16, 288 * ((head_dim + 31) // 32)
+
+
+def _nvfp4_view(what, k_pages, v_pages, table, lengths, head_dim, k_scale, v_scale):
+    """The checks and the C view of one layer of a 4-bit paged cache."""
+    _cuda(k_pages, v_pages, table, lengths)
+    if not 8 <= head_dim <= 256 or head_dim % 8:
+        raise TurboPiError(f"{what}: head_dim must be a multiple of 8 up to 256")
+    if (k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != torch.uint8 or v_pages.dtype != torch.uint8
+            or k_pages.shape[3] != 288 * ((head_dim + 31) // 32)):
+        raise TurboPiError(f"{what}: key and value pages must be uint8 [pages, heads, page / 16, {288 * ((head_dim + 31) // 32)}] of one shape")
+    if k_pages.stride() != v_pages.stride() or k_pages.stride(3) != 1:
+        raise TurboPiError(f"{what}: key and value pages must have the same strides and a contiguous last dimension")
+    if table.dim() != 2 or lengths.dim() != 1 or table.dtype != torch.int32 or lengths.dtype != torch.int32:
+        raise TurboPiError(f"{what}: table must be int32 [sequences, pages], lengths int32 [sequences]")
+    S, W = table.shape
+    if lengths.numel() != S or (S > 1 and lengths.stride(0) != 1) or (W > 1 and table.stride(1) != 1):
+        raise TurboPiError(f"{what}: one contiguous length per row of the table, rows contiguous")
+    _one_device(what, k_pages, v_pages, table, lengths)
+    P, H, tiles, _ = k_pages.shape
+    _counts(what, P, H, 16 * tiles, W, S)
+    return _lib.PagedNvfp4CacheView(_ptr(k_pages), _ptr(v_pages), k_pages.stride(0), k_pages.stride(1), k_pages.stride(2), P, 16 * tiles, H,
+                                    head_dim, float(k_scale), float(v_scale), _ptr(table), table.stride(0), W, _ptr(lengths), S)
+
+
+def _new_rows(what, name, t, tokens, heads, D, dtype, device):
+    """`t` checked, or new rows [tokens, heads, D]."""
+    if t is None:
+        return torch.empty((tokens, heads, D), dtype=dtype, device=device)
+    _rows_of_heads(what, name, t, tokens, heads, D, dtype)
+    return t
+
+
+def paged_attention_nvfp4_workspace(q_heads, kv_heads, head_dim, device):
+    """Scratch for `paged_attention_nvfp4`, as `paged_attention_workspace`."""
+    with torch.cuda.device(device):
+        n = int(_lib.load().tpb200_paged_attention_nvfp4_workspace_size(int(q_heads), int(kv_heads), int(head_dim)))
+    if n == 0:
+        raise TurboPiError("paged_attention_nvfp4: unsupported heads")
+    return torch.empty(n, dtype=torch.uint8, device=device)
+
+
+def paged_attention_nvfp4(q, k_pages, v_pages, table, lengths, scale, out=None, workspace=None, window=None, sinks=0, k_scale=1.0,
+                          v_scale=1.0):
+    """`paged_attention` on a cache of 4-bit pages (`nvfp4_page_shape`): q / out [S, Hq, D] bf16 or fp16.  Keys are k_scale times what their codes and
+    scales stand for, values v_scale times that (powers of two).  The cached values enter the products as they are held, in fp16, which holds
+    them exactly; weights are rounded to fp16, sums are fp32, outputs are rounded once."""
+    w, s = _window("paged_attention_nvfp4", window, sinks)
+    done = (_lib._native or _lib.native()).paged_attention_nvfp4(q, k_pages, v_pages, table, lengths, scale, out, workspace, w, s, k_scale,
+                                                                 v_scale, _flags.value)
+    if done is not None:
+        return _result(done, "tpb200_paged_attention_nvfp4")
+    _cuda(q, out, workspace)
+    if q.dim() != 3 or q.dtype not in _HALF:
+        raise TurboPiError("paged_attention_nvfp4: q must be bf16 or fp16 [sequences, heads, D]")
+    _, Hq, D = q.shape
+    view = _nvfp4_view("paged_attention_nvfp4", k_pages, v_pages, table, lengths, D, k_scale, v_scale)
+    _counts("paged_attention_nvfp4", Hq)
+    _rows_of_heads("paged_attention_nvfp4", "q", q, view.seqs, Hq, D, q.dtype)
+    if Hq < 1 or view.kv_heads < 1 or Hq % view.kv_heads:
+        raise TurboPiError(f"paged_attention_nvfp4: {Hq} query heads on {view.kv_heads} key heads")
+    out = _new_rows("paged_attention_nvfp4", "out", out, view.seqs, Hq, D, q.dtype, q.device)
+    _one_device("paged_attention_nvfp4", k_pages, q, out, workspace)
+    if view.seqs == 0:
+        return out
+    if workspace is None:
+        workspace = paged_attention_nvfp4_workspace(Hq, view.kv_heads, D, q.device)
+    if not workspace.is_contiguous():
+        raise TurboPiError("paged_attention_nvfp4: the workspace must be contiguous")
+    args = _lib.PagedAttentionNvfp4Args(cache=view, q=_ptr(q), out=_ptr(out), dtype=_HALF[q.dtype], q_stride=_strides(q),
+                                        o_stride=_strides(out), q_heads=Hq, scale=float(scale), window=w, sinks=s,
+                                        workspace=_ptr(workspace), workspace_bytes=workspace.numel() * workspace.element_size(),
+                                        flags=_flags.value)
+    _lib.check(_run(q, _lib.load().tpb200_paged_attention_nvfp4, args), "tpb200_paged_attention_nvfp4")
+    return out
+
+
+def paged_append_nvfp4(k, v, k_pages, v_pages, table, cu, lengths, q=None, cos=None, sin=None, q_out=None, k_scale=1.0, v_scale=1.0):
+    """`paged_append` into 4-bit pages (`nvfp4_page_shape`): k, v [T, Hk, D] and q [T, Hq, D] in bf16 or fp16.  Keys are rotated and rounded
+    to their type, then 16 values at a time, over k_scale or v_scale (powers of two), get the scale max / 6, rounded to E4M3, and the codes
+    nearest to them (ties to the even code; past 448 * 6 they saturate; below 2^-10 * 6 the 16 become zeros).  An infinity or a NaN makes
+    its 16 values NaN."""
+    done = (_lib._native or _lib.native()).paged_append_nvfp4(k, v, k_pages, v_pages, table, cu, lengths, q, cos, sin, q_out, k_scale,
+                                                              v_scale, _flags.value)
+    if done is not None:
+        done = _result(done, "tpb200_paged_append_nvfp4")
+        return None if q is None else done
+    _cuda(k, v, cu, q, cos, sin, q_out)
+    if k.dim() != 3 or k.dtype not in _HALF:
+        raise TurboPiError("paged_append_nvfp4: k must be bf16 or fp16 [tokens, heads, D]")
+    T, _, D = k.shape
+    dtype = k.dtype
+    view = _nvfp4_view("paged_append_nvfp4", k_pages, v_pages, table, lengths, D, k_scale, v_scale)
+    H = view.kv_heads
+    _rows_of_heads("paged_append_nvfp4", "k", k, T, H, D, dtype)
+    _rows_of_heads("paged_append_nvfp4", "v", v, T, H, D, dtype)
+    if cu.dtype != torch.int32 or cu.dim() != 1 or cu.numel() != view.seqs + 1 or not cu.is_contiguous():
+        raise TurboPiError("paged_append_nvfp4: cu must be contiguous int32 [sequences + 1]")
+    if (cos is None) != (sin is None) or (q is not None and cos is None) or (q is None and q_out is not None):
+        raise TurboPiError("paged_append_nvfp4: cos and sin go together, q with them, q_out with q")
+    if cos is not None and (cos.dim() != 2 or cos.shape != sin.shape or cos.shape[1] != D // 2 or cos.dtype != sin.dtype
+                            or cos.dtype not in _DTYPES or not cos.is_contiguous() or not sin.is_contiguous()):
+        raise TurboPiError(f"paged_append_nvfp4: cos and sin must be contiguous [positions, {D // 2}] of one floating type")
+    _counts("paged_append_nvfp4", T, 0 if cos is None else cos.shape[0])
+    if q is not None:
+        if q.dim() != 3:
+            raise TurboPiError("paged_append_nvfp4: q must be [tokens, heads, D]")
+        _counts("paged_append_nvfp4", q.shape[1])
+        _rows_of_heads("paged_append_nvfp4", "q", q, T, q.shape[1], D, dtype)
+        q_out = _new_rows("paged_append_nvfp4", "q_out", q_out, T, q.shape[1], D, dtype, q.device)
+    _one_device("paged_append_nvfp4", k_pages, k, v, cu, q, cos, sin, q_out)
+    args = _lib.PagedAppendNvfp4Args(cache=view, k=_ptr(k), v=_ptr(v), q=_ptr(q), q_out=_ptr(q_out), dtype=_HALF[dtype], k_stride=_strides(k),
+                                     v_stride=_strides(v), q_stride=_strides(q) if q is not None else _Two(0, 0),
+                                     o_stride=_strides(q_out) if q is not None else _Two(0, 0), cu=_ptr(cu), tokens=T,
+                                     q_heads=q.shape[1] if q is not None else 0, cos=_ptr(cos), sin=_ptr(sin),
+                                     rope_dtype=_dt(cos) if cos is not None else F32,
+                                     rope_positions=cos.shape[0] if cos is not None else 0, flags=_flags.value)
+    _lib.check(_run(k, _lib.load().tpb200_paged_append_nvfp4, args), "tpb200_paged_append_nvfp4")
+    return q_out
+
+
+def _read_rows(what, view, heads, D, dtype, cu, tokens, out, device):
+    """The rest of paged_read and paged_read_nvfp4."""
+    if cu.dtype != torch.int32 or cu.dim() != 1 or cu.numel() != view.seqs + 1 or not cu.is_contiguous():
+        raise TurboPiError(f"{what}: cu must be contiguous int32 [sequences + 1]")
+    try:
+        tokens = operator.index(tokens)
+        k, v = (None, None) if out is None else out
+    except (TypeError, ValueError):
+        raise TurboPiError(f"{what}: tokens is the number of rows, out a pair of tensors") from None
+    if tokens < 0:
+        raise TurboPiError(f"{what}: tokens is the number of rows, out a pair of tensors")
+    _counts(what, tokens)
+    if out is not None and not (torch.is_tensor(k) and torch.is_tensor(v)):
+        raise TurboPiError(f"{what}: tokens is the number of rows, out a pair of tensors")
+    _cuda(cu, k, v)
+    k, v = _new_rows(what, "k", k, tokens, heads, D, dtype, device), _new_rows(what, "v", v, tokens, heads, D, dtype, device)
+    return k, v, _lib.PagedRows(k=_ptr(k), v=_ptr(v), dtype=_HALF[dtype], k_stride=_strides(k), v_stride=_strides(v), cu=_ptr(cu),
+                                tokens=tokens, flags=_flags.value)
+
+
+def paged_read(k_pages, v_pages, table, cu, lengths, tokens, out=None):
+    """(k, v) [tokens, Hk, D] of the pages' type: tokens of a cache one sequence behind the other, as `packed_attention` takes them (cu is
+    then its cu_keys).  Sequence s gives rows [cu[s], cu[s + 1]) its last cu[s + 1] - cu[s] positions, up to lengths[s] - 1.  Rows behind
+    cu[S] are left as they are; a row without a page gets zeros and is reported by tpb200_device_error().  out: (k, v) to write."""
+    k, v = (None, None) if out is None or len(out) != 2 else out
+    done = (_lib._native or _lib.native()).paged_read(k_pages, v_pages, table, cu, lengths, tokens, k, v, _flags.value) \
+        if out is None or len(out) == 2 else None
+    if done is not None:
+        return _result(done, "tpb200_paged_read")
+    view = _paged_view("paged_read", k_pages, v_pages, table, lengths)
+    k, v, rows = _read_rows("paged_read", view, view.kv_heads, view.head_dim, k_pages.dtype, cu, tokens, out, k_pages.device)
+    _one_device("paged_read", k_pages, cu, k, v)
+    _lib.check(_run(k_pages, _lib.load().tpb200_paged_read, view, rows), "tpb200_paged_read")
+    return k, v
+
+
+def paged_read_nvfp4(k_pages, v_pages, table, cu, lengths, head_dim, tokens, dtype=torch.bfloat16, out=None, k_scale=1.0, v_scale=1.0):
+    """`paged_read` out of 4-bit pages: the values that are held, in bf16 or fp16, which hold them exactly unless k_scale or v_scale
+    takes them out of the type's range."""
+    k, v = (None, None) if out is None or len(out) != 2 else out
+    done = (_lib._native or _lib.native()).paged_read_nvfp4(k_pages, v_pages, table, cu, lengths, head_dim, tokens, dtype, k, v, k_scale,
+                                                            v_scale, _flags.value) if out is None or len(out) == 2 else None
+    if done is not None:
+        return _result(done, "tpb200_paged_read_nvfp4")
+    if dtype not in _HALF:
+        raise TurboPiError("paged_read_nvfp4: bf16 or fp16")
+    view = _nvfp4_view("paged_read_nvfp4", k_pages, v_pages, table, lengths, head_dim, k_scale, v_scale)
+    k, v, rows = _read_rows("paged_read_nvfp4", view, view.kv_heads, head_dim, dtype, cu, tokens, out, k_pages.device)
+    _one_device("paged_read_nvfp4", k_pages, cu, k, v)
+    _lib.check(_run(k_pages, _lib.load().tpb200_paged_read_nvfp4, view, rows), "tpb200_paged_read_nvfp4")
+    return k, v
+
+
 def copy_pages(pages, src, dst):
     """pages[..., dst[i], :, :, :] = pages[..., src[i], :, :, :] for every i, in one pass over the moved bytes.
-    pages: contiguous [..., P, page, heads, D] of any type (PagedCache holds [layers, 2, P, page, heads, D]).  src / dst: sequences of
+    pages: contiguous [..., P, page, heads, D] of any type (PagedCache holds [layers, 2, P, page, heads, D], 4-bit pages [layers, 2, P, heads,
+    page / 16, tile]).  src / dst: sequences of
     ints or integer tensors on the CPU; an index outside the pool, a page written twice or a page both read and written is
     refused.  The lists are read before the call returns."""
     done = (_lib._native or _lib.native()).copy_pages(pages, src, dst, _flags.value)

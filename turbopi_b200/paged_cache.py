@@ -16,12 +16,17 @@ same pages); the bytes are moved by `ops.copy_pages`, written by `ops.paged_appe
         q = cache.append(l, batch, k, v, q=q, cos=cos, sin=sin)
         out = cache.attention(l, batch, q, scale)
 
+dtype="nvfp4" holds keys and values in 4 bits (`ops.nvfp4_page_shape`): 18 bytes for 32 values instead of 64, the same calls.  A prompt behind tokens
+that are cached attends through `cache.prompt_attention`, which reads them back (`cache.read`) for `ops.packed_attention`; window= and sinks=
+restrict either attention to a sliding window and the first tokens.
+
 A batch holds for its cache until one of its sequences is freed, truncated or had a shared page copied, or pages have moved (compact);
 then `append` and `attention` refuse it, since its table may name pages of others.  `append` also refuses tokens whose page has been copied
 to a fork, which would lack them: write a batch's tokens before extending a fork of its sequences.  Calls that move or write pages enqueue on the
 current stream; use one stream per cache, or order them yourself.
 """
 import heapq
+import math
 import weakref
 
 import torch
@@ -32,10 +37,11 @@ from ._lib import TurboPiError
 
 class PagedBatch:
     """What the kernels read of some sequences: table int32 [S, max_pages], lengths int32 [S] (the new tokens among them) and cu int32
-    [S + 1], the offsets of the new tokens; `tokens` is their number."""
+    [S + 1], the offsets of the new tokens; `tokens` is their number.  cu_keys int32 [S + 1] and `keys` are the same for all tokens of the
+    sequences."""
 
-    def __init__(self, table, lengths, cu, tokens, cache):
-        self.table, self.lengths, self.cu, self.tokens = table, lengths, cu, tokens
+    def __init__(self, table, lengths, cu, tokens, cache, cu_keys=None, keys=0):
+        self.table, self.lengths, self.cu, self.tokens, self.cu_keys, self.keys = table, lengths, cu, tokens, cu_keys, keys
         # _new: sequence -> [first, last + 1) of its new tokens' positions; _stale: why it no longer holds, _late: why its tokens can
         # no longer be written in a layer that is not among _layers, the ones where `append` wrote them
         self._cache, self._new, self._stale, self._late, self._layers = weakref.ref(cache), {}, None, None, set()
@@ -48,18 +54,37 @@ def _whole(x):
     return n
 
 
+def _power_of_two(x):
+    try:
+        x = float(x)
+    except (TypeError, ValueError, OverflowError):
+        return False
+    return 2.0 ** -63 <= x <= 2.0 ** 64 and math.frexp(x)[0] == 0.5
+
+
 class PagedCache:
-    def __init__(self, layers, num_pages, page_size, kv_heads, head_dim, max_pages, dtype=torch.bfloat16, device="cuda"):
+    """dtype: torch.bfloat16, torch.float16 or "nvfp4" (page_size a multiple of 16); k_scale and v_scale, powers of two, are what 4-bit keys and
+    values are multiplied with, for ones that 448 * 6 does not hold or that 2^-10 * 6 is too large for."""
+
+    def __init__(self, layers, num_pages, page_size, kv_heads, head_dim, max_pages, dtype=torch.bfloat16, device="cuda", k_scale=1.0,
+                 v_scale=1.0):
         if min(layers, num_pages, page_size, kv_heads, max_pages) < 1 or not 8 <= head_dim <= 256 or head_dim % 8:
             raise TurboPiError("PagedCache: sizes must be positive, head_dim a multiple of 8 up to 256")
         if page_size * max_pages >= 2 ** 31:
             raise TurboPiError("PagedCache: positions are 32 bits wide")
-        if dtype not in (torch.bfloat16, torch.float16):
-            raise TurboPiError("PagedCache: bf16 or fp16")
-        self.page_size, self.max_pages, self.num_pages = page_size, max_pages, num_pages
+        if dtype not in (torch.bfloat16, torch.float16, "nvfp4"):
+            raise TurboPiError('PagedCache: bf16, fp16 or "nvfp4"')
+        self.nvfp4 = dtype == "nvfp4"
+        if self.nvfp4 and page_size % 16:
+            raise TurboPiError("PagedCache: page_size of 4-bit pages must be a multiple of 16")
+        if not all(_power_of_two(x) for x in (k_scale, v_scale)) or (not self.nvfp4 and (k_scale != 1 or v_scale != 1)):
+            raise TurboPiError("PagedCache: k_scale and v_scale are powers of two, for 4-bit pages")
+        self.page_size, self.max_pages, self.num_pages, self.head_dim = page_size, max_pages, num_pages, head_dim
         self.device = torch.device(device)
+        self._scales = dict(k_scale=float(k_scale), v_scale=float(v_scale)) if self.nvfp4 else {}
         # zeroed once: rows of a page that no token has reached are masked, not left out of the copies
-        self.pages = torch.zeros((layers, 2, num_pages, page_size, kv_heads, head_dim), dtype=dtype, device=self.device)
+        shape, dtype = (ops.nvfp4_page_shape(kv_heads, page_size, head_dim), torch.uint8) if self.nvfp4 else ((page_size, kv_heads, head_dim), dtype)
+        self.pages = torch.zeros((layers, 2, num_pages, *shape), dtype=dtype, device=self.device)
         self._free = list(range(num_pages))           # a heap
         self._refs = [0] * num_pages
         self._seqs = {}                               # id -> [page ids, length, batches that name its pages]
@@ -227,17 +252,18 @@ class PagedCache:
     def _tensors(self, held, lengths, new):
         """Tables, lengths and offsets in one copy to the device."""
         S, W = len(held), self.max_pages
-        rows, cu = [], [0]
-        for pages, n in zip(held, new):
+        rows, cu, cu_keys = [], [0], [0]
+        for pages, length, n in zip(held, lengths, new):
             rows += pages + [-1] * (W - len(pages))
             cu.append(cu[-1] + n)
-        flat = self._upload(rows + lengths + cu, (-1,))
-        return flat[:S * W].view(S, W), flat[S * W:S * W + S], flat[S * W + S:]
+            cu_keys.append(min(cu_keys[-1] + length, 2 ** 31 - 1))       # `read` refuses more
+        flat = self._upload(rows + lengths + cu + cu_keys, (-1,))
+        return flat[:S * W].view(S, W), flat[S * W:S * W + S], flat[S * W + S:S * W + 2 * S + 1], flat[S * W + 2 * S + 1:]
 
     def _batch(self, seqs, new, tensors, out):
-        table, lengths, offsets = tensors
+        table, lengths, offsets, key_offsets = tensors
         if out is None:
-            out = PagedBatch(table, lengths, offsets, sum(new), self)
+            out = PagedBatch(table, lengths, offsets, sum(new), self, key_offsets)
         else:
             for seq in out._new:
                 if seq in self._seqs:
@@ -245,7 +271,9 @@ class PagedCache:
             out.table.copy_(table)
             out.lengths.copy_(lengths)
             out.cu.copy_(offsets)
+            out.cu_keys.copy_(key_offsets)
             out.tokens, out._stale, out._late, out._layers = sum(new), None, None, set()
+        out.keys = sum(self._seqs[seq][1] for seq in seqs)
         out._new = {seq: (self._seqs[seq][1] - n, self._seqs[seq][1]) for seq, n in zip(seqs, new)}
         for seq in seqs:
             self._seqs[seq][2].add(out)
@@ -253,7 +281,7 @@ class PagedCache:
 
     # ------------------------------------------------------------------ the device side
     def layer(self, layer):
-        """(key pages, value pages) of a layer, views [pages, page_size, kv_heads, head_dim]."""
+        """(key pages, value pages) of a layer, views [pages, page_size, kv_heads, head_dim]; of 4 bits [pages, kv_heads, page_size / 16, bytes]."""
         return self.pages[layer, 0], self.pages[layer, 1]
 
     def _current(self, batch):
@@ -263,21 +291,46 @@ class PagedCache:
             raise TurboPiError(f"PagedCache: {batch._stale} since this batch was made; make it again")
 
     def append(self, layer, batch, k, v, q=None, cos=None, sin=None, q_out=None):
-        """ops.paged_append of the batch's new tokens: k, v (and q) [batch.tokens, heads, head_dim], sequence by sequence."""
+        """ops.paged_append (paged_append_nvfp4) of the batch's new tokens: k, v (and q) [batch.tokens, heads, head_dim], sequence by sequence."""
         self._current(batch)
         layer = range(self.pages.shape[0])[layer]
         if batch._late and layer not in batch._layers:
             raise TurboPiError(f"PagedCache: {batch._late} before this append; append in every layer before a fork is extended")
         if k.shape[0] != batch.tokens:
             raise TurboPiError(f"PagedCache: {k.shape[0]} rows for {batch.tokens} new tokens")
-        out = ops.paged_append(k, v, *self.layer(layer), batch.table, batch.cu, batch.lengths, q=q, cos=cos, sin=sin, q_out=q_out)
+        if self.nvfp4 and k.shape[-1] != self.head_dim:
+            raise TurboPiError(f"PagedCache: rows of {k.shape[-1]} values for heads of {self.head_dim}")
+        call = ops.paged_append_nvfp4 if self.nvfp4 else ops.paged_append
+        out = call(k, v, *self.layer(layer), batch.table, batch.cu, batch.lengths, q=q, cos=cos, sin=sin, q_out=q_out, **self._scales)
         batch._layers.add(layer)
         return out
 
-    def attention(self, layer, batch, q, scale, out=None, workspace=None):
-        """ops.paged_attention of one query row per sequence of the batch, over all its tokens."""
+    def attention(self, layer, batch, q, scale, out=None, workspace=None, window=None, sinks=0):
+        """ops.paged_attention (paged_attention_nvfp4, whose workspace is another) of one query row per sequence of the batch, over all its
+        tokens or the last `window` and the first `sinks`."""
         self._current(batch)
-        return ops.paged_attention(q, *self.layer(layer), batch.table, batch.lengths, scale, out=out, workspace=workspace)
+        if self.nvfp4 and q.shape[-1] != self.head_dim:
+            raise TurboPiError(f"PagedCache: rows of {q.shape[-1]} values for heads of {self.head_dim}")
+        call = ops.paged_attention_nvfp4 if self.nvfp4 else ops.paged_attention
+        return call(q, *self.layer(layer), batch.table, batch.lengths, scale, out=out, workspace=workspace, window=window, sinks=sinks,
+                    **self._scales)
+
+    def read(self, layer, batch, dtype=torch.bfloat16, out=None):
+        """(k, v) [batch.keys, kv_heads, head_dim]: all tokens of the batch's sequences, one sequence behind the other (offsets: batch.cu_keys),
+        by ops.paged_read or paged_read_nvfp4.  dtype: of rows read out of 4 bits, else the pages' own.  out: (k, v) to write."""
+        self._current(batch)
+        if self.nvfp4:
+            return ops.paged_read_nvfp4(*self.layer(layer), batch.table, batch.cu_keys, batch.lengths, self.head_dim, batch.keys, dtype=dtype,
+                                        out=out, **self._scales)
+        return ops.paged_read(*self.layer(layer), batch.table, batch.cu_keys, batch.lengths, batch.keys, out=out)
+
+    def prompt_attention(self, layer, batch, q, scale, out=None, window=None, sinks=0):
+        """Causal attention of the batch's new tokens, q [batch.tokens, heads, head_dim], over all tokens of their sequences (or a window), new
+        and cached, as the cache holds them: `read`, then ops.packed_attention.  Append the new tokens first."""
+        if q.shape[0] != batch.tokens:
+            raise TurboPiError(f"PagedCache: {q.shape[0]} rows for {batch.tokens} new tokens")
+        k, v = self.read(layer, batch, dtype=q.dtype)
+        return ops.packed_attention(q, k, v, batch.cu, scale, out=out, cu_keys=batch.cu_keys, window=window, sinks=sinks)
 
     def compact(self):
         """Moves pages so that those in use are the lowest ids, each at most once; returns how many are in use.  Batches made before
