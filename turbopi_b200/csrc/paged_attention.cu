@@ -33,7 +33,7 @@ template <typename T, int DP, int NT, bool kAligned, bool kWindow>
 __global__ void __launch_bounds__(kThreads, Shape<Rows16, DP, NT>::kCtas) paged_attention_kernel(const __grid_constant__ DecodeParams P) {
     pdl_wait_prior_grids();
     pdl_launch_dependents();
-    attend_pages<Rows16, T, DP, NT, kAligned, kWindow>(P);
+    attend_rows<T, DP, NT, kAligned, kWindow>(P);
 }
 template <typename T, int kLanes, int kLoads>
 __global__ void __launch_bounds__(kJoinThreads) paged_attention_join_kernel(const __grid_constant__ DecodeParams P) {
@@ -75,7 +75,7 @@ int attend(const tpb200_paged_attention_args* a, int window, int sinks, cudaStre
     const DecodeCall call = {a->q, a->out, a->q_stride, a->o_stride, a->q_heads, a->scale, a->workspace, a->workspace_bytes, a->flags, window, sinks};
     const int group = a->q_heads / P.cache.kv_heads, slot_keys = P.cache.head_dim <= 64 ? 64 : (P.cache.head_dim <= 128 ? 32 : 16);
     const int ctas = decode_ctas(kCtasPerSm);
-    const int ready = prepare_decode(call, decode_rows(group), slot_keys, ctas, &P);
+    const int ready = prepare_decode(call, decode_rows(group), slot_keys, Rows16::kItemUnits, ctas, &P);
     if (ready != TPB200_OK || P.cache.seqs == 0) return ready;
     const bool bf = a->cache.dtype == TPB200_BF16;
     // a window that no sequence of the table passes hides nothing
@@ -83,8 +83,8 @@ int attend(const tpb200_paged_attention_args* a, int window, int sinks, cudaStre
     const int done = hides ? (bf ? launch_rows<__nv_bfloat16, true>(P, ctas, stream) : launch_rows<__half, true>(P, ctas, stream))
                            : (bf ? launch_rows<__nv_bfloat16, false>(P, ctas, stream) : launch_rows<__half, false>(P, ctas, stream));
     if (done != TPB200_OK) return done;
-    return bf ? launch_join(P, paged_attention_join_kernel<__nv_bfloat16, 8, 8>, paged_attention_join_kernel<__nv_bfloat16, 2, 4>, ctas, stream)
-              : launch_join(P, paged_attention_join_kernel<__half, 8, 8>, paged_attention_join_kernel<__half, 2, 4>, ctas, stream);
+    return bf ? launch_join(P, nullptr, paged_attention_join_kernel<__nv_bfloat16, 8, 8>, paged_attention_join_kernel<__nv_bfloat16, 2, 4>, ctas, stream)
+              : launch_join(P, nullptr, paged_attention_join_kernel<__half, 8, 8>, paged_attention_join_kernel<__half, 2, 4>, ctas, stream);
 }
 
 }  // namespace

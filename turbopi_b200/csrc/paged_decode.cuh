@@ -16,10 +16,8 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kSlots = 3;
-constexpr int kSlotUnits = 2, kItemUnits = 1;      // what a slot costs, and an item besides: queries, sums, the output
+constexpr int kSlotUnits = 2;            // what a slot costs; an item besides, for queries, sums and the output: Src::kItemUnits
 constexpr float kLowest = -FLT_MAX;      // the least reference of a row with a key
-constexpr int kLengths = 1024;           // lengths kept in shared memory; with more sequences they are read where they lie
 
 struct DecodeParams {
     PagedView cache;
@@ -44,19 +42,21 @@ struct DecodeParams {
 // the low half, then 16 rows of 2 G E4M3 scales, one for 16 values.
 struct Rows16 {
     static constexpr bool kQuant = false;
-    static constexpr int kSlotBytes = 8192;
+    static constexpr int kItemUnits = 1;
 };
 struct Nvfp4 {
     static constexpr bool kQuant = true;
-    static constexpr int kSlotBytes = 4608;
+    static constexpr int kItemUnits = 6;
 };
 
 // DP: head_dim rounded up to 64, 128 or 256.  NT: tiles of eight query heads that go through together.
 template <typename Src, int DP, int NT>
 struct Shape {
-    static constexpr int kSlotBytes = Src::kSlotBytes;
-    static constexpr int kKeys = Src::kQuant ? kSlotBytes / (DP / 2 + DP / 16) : kSlotBytes / (DP * 2);     // of a slot: 16, 32, 64 or 32, 64, 128
-    static constexpr int kCtas = Src::kQuant && DP <= 128 && NT == 1 ? 3 : 2;     // on an SM
+    static constexpr int kKeys = !Src::kQuant || DP < 256 ? 4096 / DP : 32;                     // of a slot: 16 or 32, 32, 64
+    static constexpr int kSlotBytes = Src::kQuant ? 2 * kKeys * (DP / 2 + DP / 16) : kKeys * DP * 2;     // tiles of keys and of values; rows of keys, or of values
+    static constexpr int kSlots = 3;                        // of a warp's ring
+    static constexpr int kCtas = Src::kQuant && DP < 256 ? 3 : 2;       // on an SM
+    static constexpr int kLengths = 1024;                   // lengths kept in shared memory; with more sequences they are read where they lie
     static constexpr int kLanesRow = Src::kQuant ? DP / 32 : DP / 8;        // lanes that copy a row
     static constexpr int kRowsIter = 32 / kLanesRow;        // rows a warp copies at a time
     static constexpr int kCopies = kKeys / kRowsIter;
@@ -83,16 +83,18 @@ struct Shape {
     }
 };
 
-template <int NT>
+template <typename S>
 struct Control {
-    int lengths[kLengths];
-    float ml[kWarps][8 * NT][2];
+    int lengths[S::kLengths];
+    float ml[kWarps][S::kRows][2];
 };
 
+// 4-bit tiles: sums pass through the slot whose tiles were used last
 template <typename Src, int DP, int NT>
 constexpr int smem_bytes() {
     using S = Shape<Src, DP, NT>;
-    return kWarps * kSlots * S::kSlotBytes + kWarps * S::kRows * S::kSlabPitch * 4 + static_cast<int>(sizeof(Control<NT>));
+    static_assert(!Src::kQuant || S::kRows * S::kSlabPitch * 4 <= S::kSlotBytes, "");
+    return kWarps * S::kSlots * S::kSlotBytes + (Src::kQuant ? 0 : kWarps * S::kRows * S::kSlabPitch * 4) + static_cast<int>(sizeof(Control<S>));
 }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
@@ -157,7 +159,7 @@ __device__ __forceinline__ Extent extent_of(const DecodeParams& P, int len) {
 }
 
 // A place in the line of slots: slot `ci` of item (sequence, tile of query heads)
-template <int kKeys, bool kWindow>
+template <typename Src, int kKeys, int kLengths, bool kWindow>
 struct Place {
     int s, h, ci, n, len;                // n: slots of the sequence's items
     int skip;                            // slots of the sequence that are left out behind those of the sinks
@@ -182,7 +184,7 @@ struct Place {
     __device__ __forceinline__ void next(const DecodeParams& P, const int* lengths) {
         ci += step;
         if (ci < n) return;
-        units += n * kSlotUnits + kItemUnits;
+        units += n * kSlotUnits + Src::kItemUnits;
         ci = 0;
         if (++h < P.cache.kv_heads * P.tiles) return;
         enter(P, lengths, s + 1);
@@ -192,9 +194,12 @@ struct Place {
 // The line cut into pieces of equal cost, over the CTAs and a CTA's over its warps, the first ones of each getting a unit more.  A
 // slot belongs to the piece in which its first unit lies, behind the item's own; pieces are two units at least, so a warp between the
 // first and the last of an item always has a slot of it.  A line shorter than that for four warps is one warp's.
+template <int kItemUnits>
 struct Share {
     int total, ctas, each, more;         // `more` CTAs of each + 1 units, the others of each
-    __device__ __forceinline__ Share(int units, int grid) : total(units), ctas(min(grid, max(1, units / (kWarps * kSlotUnits)))) {
+    __device__ __forceinline__ void cut(int units, int grid) {
+        total = units;
+        ctas = min(grid, max(1, units / (kWarps * kSlotUnits)));
         each = total / ctas;
         more = total - each * ctas;
     }
@@ -221,267 +226,278 @@ struct Share {
     }
 };
 
-// ------------------------------------------------------------------------------------------------ 4-bit values (Nvfp4)
-// A slot in shared memory: rows of DP / 2 bytes of codes, in 128-byte lines whose 16-byte chunks are exchanged so that the eight lanes of a phase
-// meet all banks, whether they read two rows (keys) or a column of chunks (values); then the tiles' scales, DP bytes each, rows of 2 groups.
-template <int DP>
-__device__ __forceinline__ uint32_t code_at(int row, int chunk) {
-    constexpr int kPerLine = 256 / DP;                   // rows of a line: 1, 2, 4
-    const int line = row / kPerLine, c = row % kPerLine * (DP / 32) + chunk;
-    const int turn = DP == 256 ? ((row >> 1) & 3) * 2 ^ (row & 1) * 4 : (DP == 128 ? (line & 3) * 2 : (line & 1) * 2);
-    return line * 128 + ((c ^ turn) << 4);
-}
-// The order of a row's values in the products with the queries is free.  A lane (of four) takes whole groups of 32 values, for DP = 64 a block of 16;
-// step kk of 16 takes four of each lane's.
-template <int DP>
-__device__ __forceinline__ int query_column(int kk, int t) {
-    return DP == 64 ? t * 16 + kk * 4 : (t + (kk >> 3) * 4) * 32 + (kk & 7) * 4;
-}
-__device__ __forceinline__ __half2 e4m3_pair(uint32_t two) {
-    __half2_raw r;
-    asm("{\n .reg .b32 t;\n cvt.rn.f16x2.e4m3x2 t, %2;\n mov.b32 {%0, %1}, t;\n}\n" : "=h"(r.x), "=h"(r.y) : "h"(static_cast<uint16_t>(two)));
-    return r;
-}
-__device__ __forceinline__ uint32_t bits_of(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
+// A warp's piece of the line: where it begins, and its slots
+template <typename Src, typename S, bool kWindow>
+struct Piece {
+    Place<Src, S::kKeys, S::kLengths, kWindow> work;
+    Share<Src::kItemUnits> line;
+    int slots;
+    bool merged, whole_item;             // the CTA lies inside one item; it is the whole of it
 
-// S^T = K Q^T of a slot: sc[16-key block][tile of heads].  Per 32 values of a row: 16 conversions and 16 products with the scale, exact in fp16.
-template <int DP, int NT, int kBlocks>
-__device__ __forceinline__ void scores4(float (&sc)[kBlocks][NT][4], const uint8_t* slot, int keys, int groups, int lane, const uint32_t (&qf)[DP / 16][NT][2]) {
-    constexpr int kRuns = DP == 256 ? 2 : 1;             // of 32 values, or of 16 (DP = 64), that a lane has of a row
-    constexpr int kWords = DP == 64 ? 2 : 4;
-    const int g = lane >> 2, t = lane & 3;
+    // false: the CTA has none.  Sequences without keys get their zeros here.
+    __device__ __forceinline__ bool find(const DecodeParams& P, int* lengths, int warp, int lane) {
+        const int heads = P.cache.kv_heads * P.tiles, D = P.cache.head_dim;
+        // Every warp for itself, without a barrier: slots and units before each lane's run of sequences, then the places where its piece
+        // begins and ends.
+        const bool staged = P.cache.seqs <= S::kLengths;     // all warps write the same lengths there, each reads its own
+        const int run = (P.cache.seqs + 31) / 32, s0 = min(P.cache.seqs, lane * run), s1 = min(P.cache.seqs, s0 + run);
+        int slots_here = 0, units_here = 0;
+        bool empty = false;
+        for (int s = s0; s < s1; ++s) {
+            const int len = keys_of(P.cache, s), n = extent_of<S::kKeys, kWindow>(P, len).n;
+            if (staged) lengths[s] = len;
+            slots_here += n * heads;
+            units_here += n > 0 ? (n * kSlotUnits + Src::kItemUnits) * heads : 0;
+            empty = empty || n == 0;
+        }
+        __syncwarp();
+        auto length = [&](int s) { return staged ? lengths[s] : keys_of(P.cache, s); };
+        int slots_to = slots_here, units_to = units_here;
 #pragma unroll
-    for (int b = 0; b < kBlocks; ++b) {
-#pragma unroll
-        for (int run = 0; run < kRuns; ++run) {
-            const int group = DP == 64 ? t >> 1 : t + run * 4;
-            uint32_t w[2][kWords];
-            __half2 scale[2][2];                         // [row][block of 16]: the scale twice
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const uint8_t* codes = slot + b * 8 * DP + r * 4 * DP + code_at<DP>(g, group);
-                const uint8_t* scales = slot + keys * (DP / 2) + b * DP + (g + r * 8) * 2 * groups;
-                if constexpr (DP == 64) {
-                    const uint2 x = *reinterpret_cast<const uint2*>(codes + (t & 1) * 8);
-                    w[r][0] = x.x; w[r][1] = x.y;
-                    scale[r][0] = __low2half2(e4m3_pair(group < groups ? scales[t] : 0));
-                    scale[r][1] = scale[r][0];
-                } else {
-                    const uint4 x = *reinterpret_cast<const uint4*>(codes);
-                    w[r][0] = x.x; w[r][1] = x.y; w[r][kWords - 2] = x.z; w[r][kWords - 1] = x.w;
-                    const __half2 two = e4m3_pair(group < groups ? *reinterpret_cast<const uint16_t*>(scales + 2 * group) : 0);
-                    scale[r][0] = __low2half2(two);
-                    scale[r][1] = __high2half2(two);
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, slots_to, o), y = __shfl_up_sync(0xffffffffu, units_to, o);
+            if (lane >= o) {
+                slots_to += x;
+                units_to += y;
+            }
+        }
+        line.cut(__shfl_sync(0xffffffffu, units_to, 31), static_cast<int>(gridDim.x));
+        const int cta = blockIdx.x, worker = cta * kWarps + warp;
+        // sequences without keys: zeros
+        if (__any_sync(0xffffffffu, empty)) {
+            for (int s = worker; s < P.cache.seqs; s += gridDim.x * kWarps) {
+                if (length(s) > 0) continue;
+                const int per_head = D / 8;
+                for (int i = lane; i < P.cache.kv_heads * P.group * per_head; i += 32) {
+                    const int hq = i / per_head, c = i - hq * per_head;
+                    *reinterpret_cast<uint4*>(P.out + s * P.o_stride[0] + hq * P.o_stride[1] + c * 8) = make_uint4(0, 0, 0, 0);
+                }
+                if (P.join_by_item) {
+                    for (int h = lane; h < heads; h += 32) P.joins[s * heads + h] = make_int4(-1, 0, 0, 0);
                 }
             }
-#pragma unroll
-            for (int i = 0; i < kWords; ++i) {
-                __half2 x[2][4];
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    decode_e2m1x8(w[r][i], x[r]);
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) x[r][c] = __hmul2(x[r][c], scale[r][i / 2]);
+        }
+        if (!P.join_by_item && lane == 0) P.joins[worker] = make_int4(-1, 0, 0, 0);
+        if (line.total == 0 || cta >= line.ctas) return false;
+
+        // The place of the first slot that begins at `unit` or behind it, and the slots of the line before it.  A lane whose run holds the unit
+        // finds the sequence, all lanes the rest.
+        int item_first = 0;                  // units of the line before the item that holds the unit, and behind it
+        int item_behind = 0;
+        auto find = [&](int unit) {
+            const bool here = unit >= units_to - units_here && unit < units_to;
+            int s = s0, slots = slots_to - slots_here, units = units_to - units_here;
+            if (here) {
+                for (;; ++s) {
+                    const int n = extent_of<S::kKeys, kWindow>(P, length(s)).n, more = n > 0 ? (n * kSlotUnits + Src::kItemUnits) * heads : 0;
+                    if (unit < units + more) break;
+                    slots += n * heads;
+                    units += more;
                 }
+            }
+            const int from = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
+            s = __shfl_sync(0xffffffffu, s, from);
+            slots = __shfl_sync(0xffffffffu, slots, from);
+            units = __shfl_sync(0xffffffffu, units, from);
+            work.s = s;
+            work.len = length(s);
+            work.set_extent(P);
+            const int item = work.n * kSlotUnits + Src::kItemUnits;
+            work.h = (unit - units) / item;
+            work.units = item_first = units + work.h * item;
+            item_behind = item_first + item;
+            const int in = unit - item_first;
+            work.ci = in <= Src::kItemUnits ? 0 : (in - Src::kItemUnits + kSlotUnits - 1) / kSlotUnits;
+            const int before = slots + work.h * work.n + work.ci;
+            if (work.ci == work.n) {         // behind the item's last slot
+                work.ci = work.n - 1;
+                work.step = 1;
+                work.next(P, lengths);
+            }
+            return before;
+        };
+        const int cta_first = line.cta_begin(cta), cta_behind = line.cta_begin(cta + 1);
+        const int unit_first = line.begin(cta, warp), unit_behind = line.begin(cta, warp + 1);
+        slots = 0;
+        merged = whole_item = false;
+        if (unit_first < unit_behind) {
+            if (unit_behind < line.total) slots = find(unit_behind);
+            else slots = __shfl_sync(0xffffffffu, slots_to, 31);
+            slots -= find(unit_first);
+            work.step = 1;
+            // A CTA inside one item adds its warps' sums up itself, and deals its slots to them in turn: neighbours are read together.
+            merged = cta_first >= item_first && cta_behind <= item_behind;
+        } else {                             // one warp's line
+            find(cta_first);
+            merged = cta_behind <= item_behind;
+        }
+        if (merged) {
+            auto slot_of = [&](int unit) {
+                const int in = unit - item_first;
+                return in <= Src::kItemUnits ? 0 : min(work.n, (in - Src::kItemUnits + kSlotUnits - 1) / kSlotUnits);
+            };
+            const int first = slot_of(cta_first), behind = slot_of(cta_behind);
+            whole_item = first == 0 && behind == work.n;
+            slots = max(0, (behind - first - warp + kWarps - 1) / kWarps);
+            work.ci = first + warp;
+            work.step = kWarps;
+        }
+        return true;
+    }
+};
+
+// A warp's sums of an item, or of its piece of one, to the output or to a part; through shared memory (`own`), so that rows leave in runs.
+// Returns whether they were the whole item's.
+template <typename Src, typename T, typename S, int DP, int NT, typename Work, typename Line>
+__device__ __forceinline__ bool store_item(const DecodeParams& P, const Work& work, const Line& line, float* own, int cta, int worker, int lane, int parts,
+                                           bool from_start, bool item_done, const float (&o)[DP / 16][NT][4], const float (&m)[NT][2], float (&l)[NT][2]) {
+    const int heads = P.cache.kv_heads * P.tiles, D = P.cache.head_dim;
+    const bool whole = from_start && item_done;
+    const int kvh = work.h / P.tiles, row0 = (work.h - kvh * P.tiles) * S::kRows;
+    const long long part = 2ll * worker + parts;
+    float f[NT][2];
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const uint32_t a[4] = {bits_of(x[0][2 * j]), bits_of(x[1][2 * j]), bits_of(x[0][2 * j + 1]), bits_of(x[1][2 * j + 1])};
-                    const int kk = run * 8 + i * 2 + j;
+    for (int n = 0; n < NT; ++n) {
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) mma16816<__half>(sc[b][n], a, qf[kk][n][0], qf[kk][n][1]);
-                }
+        for (int j = 0; j < 2; ++j) {
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], x);
+            f[n][j] = whole ? inverse(m[n][j], l[n][j]) : 1.0f;
+            if (Src::kQuant && whole) f[n][j] *= P.out_scale;
+            const int row = n * 8 + (lane & 3) * 2 + j;
+            if (!whole && lane < 4 && row < P.rows) {
+                *reinterpret_cast<float2*>(P.part_ml + (part * P.rows + row) * 2) = make_float2(m[n][j], l[n][j]);
             }
         }
     }
+    constexpr int kQuads = S::kSlab / 4;
+#pragma unroll
+    for (int x = 0; x < DP / S::kSlab; ++x) {
+#pragma unroll
+        for (int i = 0; i < S::kSlab / 16; ++i) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    own[(n * 8 + (lane & 3) * 2 + (j & 1)) * S::kSlabPitch + S::slab_column(i, lane, j)] =
+                        o[x * (S::kSlab / 16) + i][n][j] * f[n][j & 1];
+                }
+            }
+        }
+        __syncwarp();
+        for (int u = lane; u < min(P.group - row0, S::kRows) * kQuads; u += 32) {
+            const int row = u / kQuads, col = S::column_of_slab(x, u % kQuads * 4);
+            if (col >= D) continue;
+            const float4 y = *reinterpret_cast<const float4*>(own + row * S::kSlabPitch + u % kQuads * 4);
+            if (whole) {
+                uint16_t* to = P.out + work.s * P.o_stride[0] + (kvh * P.group + row0 + row) * P.o_stride[1] + col;
+                *reinterpret_cast<uint2*>(to) = make_uint2(Half16<T>::pack(y.x, y.y), Half16<T>::pack(y.z, y.w));
+            } else {
+                *reinterpret_cast<float4*>(P.part_o + (part * P.rows + row) * D + col) = y;
+            }
+        }
+        __syncwarp();
+    }
+    if (lane == 0 && from_start) {
+        const int item = work.s * heads + work.h;
+        if (whole) {
+            if (P.join_by_item) P.joins[item] = make_int4(-1, 0, 0, 0);
+        } else {                     // it begins here and ends with a later warp
+            const int by = line.last_worker(work.units, work.n);
+            P.joins[P.join_by_item ? item : worker] =
+                make_int4(item, static_cast<int>(part), by, by / kWarps != cta && line.ends_merged(work.units, work.n, by) ? 2 : 0);
+        }
+    }
+    return whole;
 }
 
-// O^T += V^T P^T of a slot.  The product wants neighbouring keys in a register: the halves of two keys' bytes are exchanged before they are
-// converted, four instructions for 16 values, so that a conversion gives the same column of both, and a product applies both scales.  A lane has
-// DP / 8 neighbouring columns of four keys out of 16.
-template <int DP, int NT, int kBlocks>
-__device__ __forceinline__ void values4(float (&o)[DP / 16][NT][4], const uint8_t* slot, int keys, int groups, int lane, const uint32_t (&p)[kBlocks][NT][2]) {
-    constexpr int kWords = DP / 64;                      // of 8 columns
-    const int g = lane >> 2, t = lane & 3;
-    const int chunk = DP == 256 ? g : (DP == 128 ? g >> 1 : g >> 2), in_chunk = DP == 256 ? 0 : (DP == 128 ? (g & 1) * 8 : (g & 3) * 4);
-    const int block = DP == 256 ? 2 * g : (DP == 128 ? g : g >> 1);
-    const bool there = block < 2 * groups;
+// The sums of a CTA inside one item, each warp's where its ring was
+template <typename Src, typename T, typename S, int DP, int NT, typename Work, typename Line>
+__device__ __forceinline__ void merge_cta(const DecodeParams& P, const Work& work, const Line& line, uint8_t* smem, float (&ml)[kWarps][S::kRows][2], int cta,
+                                          int warp, int lane, bool from_start, bool whole, const float (&o)[DP / 16][NT][4], const float (&m)[NT][2], float (&l)[NT][2]) {
+    constexpr int kSlotBytes = S::kSlotBytes, kSlots = S::kSlots;
+    const int heads = P.cache.kv_heads * P.tiles, D = P.cache.head_dim, worker = cta * kWarps;
+    float* sums = reinterpret_cast<float*>(smem + warp * kSlots * kSlotBytes);
+    __syncwarp();
 #pragma unroll
-    for (int b = 0; b < kBlocks; ++b) {
-        uint32_t w[4][kWords], s[4];                     // keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
+    for (int n = 0; n < NT; ++n) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int row = 2 * t + (k & 1);
-            const uint8_t* codes = slot + b * 8 * DP + (k >> 1) * 4 * DP + code_at<DP>(row, chunk) + in_chunk;
-            const uint8_t* scales = slot + keys * (DP / 2) + b * DP + (row + (k >> 1) * 8) * 2 * groups + block;
-            if constexpr (DP == 256) {
-                const uint4 x = *reinterpret_cast<const uint4*>(codes);
-                w[k][0] = x.x; w[k][1] = x.y; w[k][kWords - 2] = x.z; w[k][kWords - 1] = x.w;
-                s[k] = there ? *reinterpret_cast<const uint16_t*>(scales) : 0;
-            } else if constexpr (DP == 128) {
-                const uint2 x = *reinterpret_cast<const uint2*>(codes);
-                w[k][0] = x.x; w[k][kWords - 1] = x.y;
-                s[k] = there ? *scales : 0;
-            } else {
-                w[k][0] = *reinterpret_cast<const uint32_t*>(codes);
-                s[k] = there ? *scales : 0;
-            }
-        }
-        __half2 scale[2][DP == 256 ? 2 : 1];             // of a pair of keys, per block of 16 columns
+        for (int j = 0; j < 2; ++j) {
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            scale[k][0] = e4m3_pair(__byte_perm(s[2 * k], s[2 * k + 1], 0x0040));
-            if constexpr (DP == 256) scale[k][1] = e4m3_pair(__byte_perm(s[2 * k], s[2 * k + 1], 0x0051));
+            for (int x = 4; x < 32; x <<= 1) l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], x);
+            if (lane < 4) *reinterpret_cast<float2*>(ml[warp][n * 8 + lane * 2 + j]) = make_float2(m[n][j], l[n][j]);
         }
 #pragma unroll
-        for (int i = 0; i < kWords; ++i) {
-            __half2 x[2][2][4];                          // [pair of keys][even, odd columns]
+        for (int i = 0; i < DP / 16; ++i) {
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const uint32_t a = w[2 * k][i], c = w[2 * k + 1][i];
-                decode_e2m1x8((a & 0x0f0f0f0fu) | ((c << 4) & 0xf0f0f0f0u), x[k][0]);
-                decode_e2m1x8(((a >> 4) & 0x0f0f0f0fu) | (c & 0xf0f0f0f0u), x[k][1]);
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-#pragma unroll
-                    for (int n = 0; n < 4; ++n) x[k][j][n] = __hmul2(x[k][j][n], scale[k][DP == 256 ? i / 2 : 0]);
+            for (int j = 0; j < 4; ++j) {
+                sums[(n * 8 + (lane & 3) * 2 + (j & 1)) * S::kSumPitch + S::column(i, lane, j)] = o[i][n][j];
             }
+        }
+    }
+    __syncthreads();
+    const int kvh = work.h / P.tiles, row0 = (work.h - kvh * P.tiles) * S::kRows;
+    const long long part = 2ll * kWarps * cta;
+    const int rows = min(P.group - row0, S::kRows);
+#pragma unroll 4
+    for (int u = threadIdx.x; u < S::kRows * (DP / 4); u += kThreads) {
+        const int row = u / (DP / 4), col = u % (DP / 4) * 4;
+        if (row >= rows || col >= D) continue;
+        float M = -INFINITY, L = 0.0f;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const uint32_t a[4] = {bits_of(x[0][0][c]), bits_of(x[0][1][c]), bits_of(x[1][0][c]), bits_of(x[1][1][c])};
+        for (int w = 0; w < kWarps; ++w) M = fmaxf(M, ml[w][row][0]);
+        float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-                for (int n = 0; n < NT; ++n) mma16816<__half>(o[i * 4 + c][n], a, p[b][n][0], p[b][n][1]);
-            }
+        for (int w = 0; w < kWarps; ++w) {
+            const float f = ex2(ml[w][row][0] - (M == -INFINITY ? 0.0f : M));
+            const float4 y = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(smem + w * kSlots * kSlotBytes) + row * S::kSumPitch + col);
+            L += ml[w][row][1] * f;
+            sum.x += y.x * f; sum.y += y.y * f; sum.z += y.z * f; sum.w += y.w * f;
+        }
+        if (whole) {
+            const float inv = Src::kQuant ? inverse(M, L) * P.out_scale : inverse(M, L);
+            uint16_t* to = P.out + work.s * P.o_stride[0] + (kvh * P.group + row0 + row) * P.o_stride[1] + col;
+            *reinterpret_cast<uint2*>(to) = make_uint2(Half16<T>::pack(sum.x * inv, sum.y * inv), Half16<T>::pack(sum.z * inv, sum.w * inv));
+        } else {
+            *reinterpret_cast<float4*>(P.part_o + (part * P.rows + row) * D + col) = sum;
+            if (col == 0) *reinterpret_cast<float2*>(P.part_ml + (part * P.rows + row) * 2) = make_float2(M, L);
+        }
+    }
+    if (threadIdx.x == 0 && from_start) {
+        const int item = work.s * heads + work.h;
+        if (whole) {
+            if (P.join_by_item) P.joins[item] = make_int4(-1, 0, 0, 0);
+        } else {
+            const int by = line.last_worker(work.units, work.n);
+            P.joins[P.join_by_item ? item : worker] = make_int4(item, static_cast<int>(part), by, line.ends_merged(work.units, work.n, by) ? 3 : 1);
         }
     }
 }
 
 // kAligned: the page size is a multiple of 16, so that 16 rows from a multiple of 16 on lie in one page and share an address
-template <typename Src, typename T, int DP, int NT, bool kAligned, bool kWindow>
-__device__ __forceinline__ void attend_pages(const DecodeParams& P) {
+template <typename T, int DP, int NT, bool kAligned, bool kWindow>
+__device__ __forceinline__ void attend_rows(const DecodeParams& P) {
+    using Src = Rows16;
     using S = Shape<Src, DP, NT>;
-    using C = std::conditional_t<Src::kQuant, __half, T>;        // type of the products: 4-bit values times their scales are exact in fp16
-    constexpr int kSlotBytes = S::kSlotBytes;
-    static_assert(kAligned || !Src::kQuant, "");
+    constexpr int kSlotBytes = S::kSlotBytes, kSlots = S::kSlots;
     extern __shared__ __align__(128) uint8_t smem[];
     float* slab = reinterpret_cast<float*>(smem + kWarps * kSlots * kSlotBytes);
-    Control<NT>* ctl = reinterpret_cast<Control<NT>*>(slab + kWarps * S::kRows * S::kSlabPitch);
+    auto* ctl = reinterpret_cast<Control<S>*>(slab + kWarps * S::kRows * S::kSlabPitch);
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-    const int heads = P.cache.kv_heads * P.tiles;
     const int D = P.cache.head_dim;
 
-    // ------------------------------------------------ this warp's piece of the line
-    // Every warp for itself, without a barrier: slots and units before each lane's run of sequences, then the places where its piece
-    // begins and ends.
-    const bool staged = P.cache.seqs <= kLengths;        // all warps write the same lengths there, each reads its own
-    const int run = (P.cache.seqs + 31) / 32, s0 = min(P.cache.seqs, lane * run), s1 = min(P.cache.seqs, s0 + run);
-    int slots_here = 0, units_here = 0;
-    bool empty = false;
-    for (int s = s0; s < s1; ++s) {
-        const int len = keys_of(P.cache, s), n = extent_of<S::kKeys, kWindow>(P, len).n;
-        if (staged) ctl->lengths[s] = len;
-        slots_here += n * heads;
-        units_here += n > 0 ? (n * kSlotUnits + kItemUnits) * heads : 0;
-        empty = empty || n == 0;
-    }
-    __syncwarp();
-    auto length = [&](int s) { return staged ? ctl->lengths[s] : keys_of(P.cache, s); };
-    int slots_to = slots_here, units_to = units_here;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int x = __shfl_up_sync(0xffffffffu, slots_to, o), y = __shfl_up_sync(0xffffffffu, units_to, o);
-        if (lane >= o) {
-            slots_to += x;
-            units_to += y;
-        }
-    }
-    const Share line(__shfl_sync(0xffffffffu, units_to, 31), static_cast<int>(gridDim.x));
-    const int cta = blockIdx.x, worker = cta * kWarps + warp;
-    // sequences without keys: zeros
-    if (__any_sync(0xffffffffu, empty)) {
-        for (int s = worker; s < P.cache.seqs; s += gridDim.x * kWarps) {
-            if (length(s) > 0) continue;
-            const int per_head = D / 8;
-            for (int i = lane; i < P.cache.kv_heads * P.group * per_head; i += 32) {
-                const int hq = i / per_head, c = i - hq * per_head;
-                *reinterpret_cast<uint4*>(P.out + s * P.o_stride[0] + hq * P.o_stride[1] + c * 8) = make_uint4(0, 0, 0, 0);
-            }
-            if (P.join_by_item) {
-                for (int h = lane; h < heads; h += 32) P.joins[s * heads + h] = make_int4(-1, 0, 0, 0);
-            }
-        }
-    }
-    if (!P.join_by_item && lane == 0) P.joins[worker] = make_int4(-1, 0, 0, 0);
-    if (line.total == 0 || cta >= line.ctas) return;
-
-    // The place of the first slot that begins at `unit` or behind it, and the slots of the line before it.  A lane whose run holds the unit
-    // finds the sequence, all lanes the rest.
-    Place<S::kKeys, kWindow> work;
-    int item_first = 0;                  // units of the line before the item that holds the unit, and behind it
-    int item_behind = 0;
-    auto find = [&](int unit) {
-        const bool here = unit >= units_to - units_here && unit < units_to;
-        int s = s0, slots = slots_to - slots_here, units = units_to - units_here;
-        if (here) {
-            for (;; ++s) {
-                const int n = extent_of<S::kKeys, kWindow>(P, length(s)).n, more = n > 0 ? (n * kSlotUnits + kItemUnits) * heads : 0;
-                if (unit < units + more) break;
-                slots += n * heads;
-                units += more;
-            }
-        }
-        const int from = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
-        s = __shfl_sync(0xffffffffu, s, from);
-        slots = __shfl_sync(0xffffffffu, slots, from);
-        units = __shfl_sync(0xffffffffu, units, from);
-        work.s = s;
-        work.len = length(s);
-        work.set_extent(P);
-        const int item = work.n * kSlotUnits + kItemUnits;
-        work.h = (unit - units) / item;
-        work.units = item_first = units + work.h * item;
-        item_behind = item_first + item;
-        const int in = unit - item_first;
-        work.ci = in <= kItemUnits ? 0 : (in - kItemUnits + kSlotUnits - 1) / kSlotUnits;
-        const int before = slots + work.h * work.n + work.ci;
-        if (work.ci == work.n) {         // behind the item's last slot
-            work.ci = work.n - 1;
-            work.step = 1;
-            work.next(P, ctl->lengths);
-        }
-        return before;
-    };
-    const int cta_first = line.cta_begin(cta), cta_behind = line.cta_begin(cta + 1);
-    const int unit_first = line.begin(cta, warp), unit_behind = line.begin(cta, warp + 1);
-    int slots = 0;
-    bool merged = false, whole_item = false;
-    if (unit_first < unit_behind) {
-        if (unit_behind < line.total) slots = find(unit_behind);
-        else slots = __shfl_sync(0xffffffffu, slots_to, 31);
-        slots -= find(unit_first);
-        work.step = 1;
-        // A CTA inside one item adds its warps' sums up itself, and deals its slots to them in turn: neighbours are read together.
-        merged = cta_first >= item_first && cta_behind <= item_behind;
-    } else {                             // one warp's line
-        find(cta_first);
-        merged = cta_behind <= item_behind;
-    }
-    if (merged) {
-        auto slot_of = [&](int unit) {
-            const int in = unit - item_first;
-            return in <= kItemUnits ? 0 : min(work.n, (in - kItemUnits + kSlotUnits - 1) / kSlotUnits);
-        };
-        const int first = slot_of(cta_first), behind = slot_of(cta_behind);
-        whole_item = first == 0 && behind == work.n;
-        slots = max(0, (behind - first - warp + kWarps - 1) / kWarps);
-        work.ci = first + warp;
-        work.step = kWarps;
-    }
-    Place<S::kKeys, kWindow> load = work;
+    Piece<Src, S, kWindow> piece;
+    if (!piece.find(P, ctl->lengths, warp, lane)) return;
+    auto& work = piece.work;
+    const auto& line = piece.line;
+    const int slots = piece.slots, cta = blockIdx.x, worker = cta * kWarps + warp;
+    const bool merged = piece.merged, whole_item = piece.whole_item;
+    auto load = work;
 
     // ------------------------------------------------ loads
     const uint32_t ring = smem_u32(smem) + warp * kSlots * kSlotBytes;
     const int lane_row = lane / S::kLanesRow, lane_col = lane % S::kLanesRow;
-    const bool lane_in = lane_col * 8 < D;       // (Rows16)
+    const bool lane_in = lane_col * 8 < D;
     constexpr int kPlaces = kAligned ? 1 : S::kOwn;
     int left = slots;                    // that the loads have still to enter
     int page_id[kPlaces];                // of this lane's rows of the next slot to load
@@ -525,8 +541,7 @@ __device__ __forceinline__ void attend_pages(const DecodeParams& P) {
             const bool in = own_seen(o, key);
             const bool known = static_cast<unsigned>(page_id[o]) < static_cast<unsigned>(P.cache.num_pages);
             if (in && known) {
-                const unsigned row = key % P.cache.page_size;
-                row_at[o] = page_id[o] * P.cache.page_stride + (Src::kQuant ? row / 16 : row) * P.cache.row_stride +
+                row_at[o] = page_id[o] * P.cache.page_stride + (key % P.cache.page_size) * P.cache.row_stride +
                             load.h / P.tiles * P.cache.head_stride;
             }
             const uint32_t gone = __ballot_sync(0xffffffffu, in && !known);
@@ -538,27 +553,6 @@ __device__ __forceinline__ void attend_pages(const DecodeParams& P) {
         --left;
         if (left > 0) load.next(P, ctl->lengths);
         fetch_ids();
-    };
-    const int groups = (D + 31) / 32;    // of 32 values in a row (Nvfp4)
-    const long long lane_off4 = lane_row * 16 * groups + lane_col * 16;
-    auto copy_tiles = [&](const uint8_t* base, uint32_t dst) {
-        constexpr int kTileCopies = 16 / S::kRowsIter, kScaleLanes = DP / 16;       // copies of a tile's codes; lanes that copy its scales
-        const uint8_t* src = base;
-        bool in = false;
-#pragma unroll
-        for (int i = 0; i < S::kCopies; ++i) {
-            if (i % kTileCopies == 0) {
-                const long long off = __shfl_sync(0xffffffffu, row_at[0], i / kTileCopies);
-                in = off >= 0 && lane_col < groups;
-                src = in ? base + off + lane_off4 : base;
-            }
-            cp_async16(dst + code_at<DP>(i * S::kRowsIter + lane_row, lane_col), src, in ? 16 : 0);
-            if (in) src += S::kRowsIter * 16 * groups;
-        }
-        const long long off = __shfl_sync(0xffffffffu, row_at[0], lane / kScaleLanes);
-        const int c = lane % kScaleLanes;
-        in = off >= 0 && c < 2 * groups;
-        cp_async16(dst + S::kKeys * (DP / 2) + lane * 16, in ? base + off + 256 * groups + c * 16 : base, in ? 16 : 0);
     };
     auto copy_rows = [&](const uint16_t* base, uint32_t dst) {
         if constexpr (kAligned) {
@@ -596,7 +590,7 @@ __device__ __forceinline__ void attend_pages(const DecodeParams& P) {
     // byte offsets of a lane's row in a 16-row fragment, for the four positions of a 16-column step in 128 bytes: K (and V) as A
     // operand; the columns behind them are a constant further on
     uint32_t k_off[4], v_off[4];
-    if constexpr (!Src::kQuant) {
+    {
         const int kr = (lane & 7) + ((lane >> 3) & 1) * 8, kc = lane >> 4;          // matrices: keys 0-7, 8-15, then 8 columns on
         const int vr = (lane & 7) + (lane >> 4) * 8, vc = (lane >> 3) & 1;          // transposed: columns 0-7, 8-15, then 8 keys on
 #pragma unroll
@@ -608,12 +602,12 @@ __device__ __forceinline__ void attend_pages(const DecodeParams& P) {
     // queries as the B operand: a lane's two pairs of a 16-column step, zero past the group and past head_dim
     uint32_t qf[S::kQueriesStay ? DP / 16 : 1][NT][2], q_ahead[S::kQueriesAhead ? DP / 16 : 1][NT][2];
     const uint16_t* q_row[NT];           // null: no such query head
-    auto aim_queries = [&](const Place<S::kKeys, kWindow>& at) {
+    auto aim_queries = [&](const decltype(piece.work)& at) {
         const int kvh = at.h / P.tiles, row0 = (at.h - kvh * P.tiles) * S::kRows;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             const int r = row0 + t * 8 + (lane >> 2);
-            q_row[t] = r < P.group ? P.q + at.s * P.q_stride[0] + (kvh * P.group + r) * P.q_stride[1] + (Src::kQuant ? 0 : (lane & 3) * 2) : nullptr;
+            q_row[t] = r < P.group ? P.q + at.s * P.q_stride[0] + (kvh * P.group + r) * P.q_stride[1] + (lane & 3) * 2 : nullptr;
         }
     };
     auto read_queries = [&](int kk, uint32_t (&f)[NT][2]) {
@@ -621,45 +615,13 @@ __device__ __forceinline__ void attend_pages(const DecodeParams& P) {
         for (int t = 0; t < NT; ++t) {
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                const int c = Src::kQuant ? query_column<DP>(kk, lane & 3) + j * 2 : kk * 16 + j * 8;
+                const int c = kk * 16 + j * 8;
                 f[t][j] = q_row[t] != nullptr && c < D ? __ldg(reinterpret_cast<const uint32_t*>(q_row[t] + c)) : 0u;
             }
         }
     };
     float o[DP / 16][NT][4];             // O^T: columns of head_dim by query heads
     float m[NT][2], l[NT][2];            // reference and sum of the lane's two query heads of a tile; l over the lane's keys only
-    float scale2[NT][2];                 // of the lane's two query heads of a tile
-    // Nvfp4: queries as fp16 for the product with values that are.  fp16 ones are taken as they are; bf16 ones are divided by the power of two of
-    // their head's largest, which moves into the scale (a query 2^-24 of the largest and below is rounded to a multiple of 2^-24 of it).
-    auto convert_queries = [&]() {
-        if constexpr (Src::kQuant && std::is_same<T, __nv_bfloat16>::value) {
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                uint32_t top = 0;
-#pragma unroll
-                for (int kk = 0; kk < DP / 16; ++kk)
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) top = max(top, max(qf[kk][t][j] & 0x7fffu, (qf[kk][t][j] >> 16) & 0x7fffu));
-                top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const int e = min(max(static_cast<int>(top >> 7), 1), 253);          // exponent field; 2^(127 - e) and its inverse are normal
-                const float down = __uint_as_float((254u - e) << 23);
-#pragma unroll
-                for (int kk = 0; kk < DP / 16; ++kk)
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const float2 x = Half16<T>::unpack(qf[kk][t][j]);
-                        qf[kk][t][j] = Half16<__half>::pack(x.x * down, x.y * down);
-                    }
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    scale2[t][j] = P.scale2 * __uint_as_float(static_cast<uint32_t>(__shfl_sync(0xffffffffu, e, ((lane & 3) * 2 + j) * 4)) << 23);
-                }
-            }
-        }
-    };
-#pragma unroll
-    for (int t = 0; t < NT; ++t) scale2[t][0] = scale2[t][1] = P.scale2;
     auto clear = [&]() {
 #pragma unroll
         for (int i = 0; i < DP / 16; ++i)
@@ -690,10 +652,9 @@ __device__ __forceinline__ void attend_pages(const DecodeParams& P) {
 #pragma unroll
                 for (int kk = 0; kk < DP / 16; ++kk) read_queries(kk, qf[kk]);
             }
-            convert_queries();
         }
     };
-    auto ask_queries = [&](const Place<S::kKeys, kWindow>& at) {
+    auto ask_queries = [&](const decltype(piece.work)& at) {
         if constexpr (S::kQueriesAhead) {
             aim_queries(at);
 #pragma unroll
@@ -703,7 +664,7 @@ __device__ __forceinline__ void attend_pages(const DecodeParams& P) {
 
     auto ask_next = [&]() {              // the queries of the item behind `work`
         if constexpr (S::kQueriesAhead) {
-            Place<S::kKeys, kWindow> then = work;
+            auto then = work;
             then.ci = then.n - 1;
             then.next(P, ctl->lengths);
             ask_queries(then);
@@ -739,9 +700,6 @@ __device__ __forceinline__ void attend_pages(const DecodeParams& P) {
                         for (int b = 0; b < S::kChains; ++b) odd[b][n][j] = 0.0f;
                     }
                 }
-                if constexpr (Src::kQuant) {
-                    scores4<DP, NT>(sc, smem + (at - smem_u32(smem)), S::kKeys, groups, lane, qf);
-                } else
 #pragma unroll
                 for (int kk = 0; kk < DP / 16; ++kk) {
                     uint32_t f[NT][2];
@@ -786,7 +744,7 @@ __device__ __forceinline__ void attend_pages(const DecodeParams& P) {
                             const int key = b * 16 + (lane >> 2) + (j >> 1) * 8;
                             const bool seen = key < valid && ((absent >> (kAligned ? b : key)) & 1) == 0 && !(kWindow && key >= hidden && key < shown);
 #pragma unroll
-                            for (int n = 0; n < NT; ++n) sc[b][n][j] = seen ? sc[b][n][j] * (Src::kQuant ? scale2[n][j & 1] : P.scale2) : -INFINITY;
+                            for (int n = 0; n < NT; ++n) sc[b][n][j] = seen ? sc[b][n][j] * P.scale2 : -INFINITY;
                         }
                 } else {
 #pragma unroll
@@ -794,7 +752,7 @@ __device__ __forceinline__ void attend_pages(const DecodeParams& P) {
 #pragma unroll
                         for (int n = 0; n < NT; ++n)
 #pragma unroll
-                            for (int j = 0; j < 4; ++j) sc[b][n][j] *= Src::kQuant ? scale2[n][j & 1] : P.scale2;
+                            for (int j = 0; j < 4; ++j) sc[b][n][j] *= P.scale2;
                 }
                 bool raise = false;
 #pragma unroll
@@ -829,7 +787,7 @@ __device__ __forceinline__ void attend_pages(const DecodeParams& P) {
                 // its B operand
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    const float b0 = (m[n][0] == -INFINITY ? 0.0f : m[n][0]) - Half16<C>::kLift, b1 = (m[n][1] == -INFINITY ? 0.0f : m[n][1]) - Half16<C>::kLift;
+                    const float b0 = (m[n][0] == -INFINITY ? 0.0f : m[n][0]) - Half16<T>::kLift, b1 = (m[n][1] == -INFINITY ? 0.0f : m[n][1]) - Half16<T>::kLift;
 #pragma unroll
                     for (int b = 0; b < S::kKeys / 16; ++b) {
                         float w[4];
@@ -837,24 +795,12 @@ __device__ __forceinline__ void attend_pages(const DecodeParams& P) {
                         for (int j = 0; j < 4; ++j) w[j] = ex2(sc[b][n][j] - (j & 1 ? b1 : b0));
                         l[n][0] += w[0] + w[2];
                         l[n][1] += w[1] + w[3];
-                        p[b][n][0] = transpose8x8(Half16<C>::pack(w[0], w[1]));
-                        p[b][n][1] = transpose8x8(Half16<C>::pack(w[2], w[3]));
+                        p[b][n][0] = transpose8x8(Half16<T>::pack(w[0], w[1]));
+                        p[b][n][1] = transpose8x8(Half16<T>::pack(w[2], w[3]));
                     }
                 }
             } else {
                 // ---- O^T += V^T P^T
-                if constexpr (Src::kQuant) {
-                    uint8_t* slot_at = smem + (at - smem_u32(smem));
-                    if (valid < S::kKeys || some_hidden) {       // a scale that is NaN would pass a weight of 0: none for keys that are not seen
-                        for (int key = lane; key < S::kKeys; key += 32) {
-                            if (key < valid && !(kWindow && key >= hidden && key < shown)) continue;
-                            uint16_t* of = reinterpret_cast<uint16_t*>(slot_at + S::kKeys * (DP / 2) + key / 16 * DP) + key % 16 * groups;
-                            for (int c = 0; c < groups; ++c) of[c] = 0;
-                        }
-                        __syncwarp();
-                    }
-                    values4<DP, NT>(o, slot_at, S::kKeys, groups, lane, p);
-                } else
 #pragma unroll
                 for (int i = 0; i < DP / 16; ++i) {
 #pragma unroll
@@ -874,9 +820,7 @@ __device__ __forceinline__ void attend_pages(const DecodeParams& P) {
         }
         if (t < uses) {
             if ((t & 1) == 0) enter_slot();
-            const void* from = (t & 1) == 0 ? P.cache.k_pages : P.cache.v_pages;
-            if constexpr (Src::kQuant) copy_tiles(static_cast<const uint8_t*>(from), at);
-            else copy_rows(static_cast<const uint16_t*>(from), at);
+            copy_rows(static_cast<const uint16_t*>((t & 1) == 0 ? P.cache.k_pages : P.cache.v_pages), at);
         }
         cp_async_commit();
         slot = slot == kSlots - 1 ? 0 : slot + 1;
@@ -893,65 +837,8 @@ __device__ __forceinline__ void attend_pages(const DecodeParams& P) {
             work.ci += work.step;
             continue;
         }
-        // ------------------------------------------------ the warp's sums -> the output, or a part of it
-        const bool whole = first_ci == 0 && item_done;
-        const int kvh = work.h / P.tiles, row0 = (work.h - kvh * P.tiles) * S::kRows;
-        const long long part = 2ll * worker + parts;
-        float f[NT][2];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-#pragma unroll
-                for (int x = 4; x < 32; x <<= 1) l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], x);
-                f[n][j] = whole ? inverse(m[n][j], l[n][j]) : 1.0f;
-                if (Src::kQuant && whole) f[n][j] *= P.out_scale;
-                const int row = n * 8 + (lane & 3) * 2 + j;
-                if (!whole && lane < 4 && row < P.rows) {
-                    *reinterpret_cast<float2*>(P.part_ml + (part * P.rows + row) * 2) = make_float2(m[n][j], l[n][j]);
-                }
-            }
-        }
         float* own = slab + warp * S::kRows * S::kSlabPitch;
-        constexpr int kQuads = S::kSlab / 4;
-#pragma unroll
-        for (int x = 0; x < DP / S::kSlab; ++x) {
-#pragma unroll
-            for (int i = 0; i < S::kSlab / 16; ++i) {
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        own[(n * 8 + (lane & 3) * 2 + (j & 1)) * S::kSlabPitch + S::slab_column(i, lane, j)] =
-                            o[x * (S::kSlab / 16) + i][n][j] * f[n][j & 1];
-                    }
-                }
-            }
-            __syncwarp();
-            for (int u = lane; u < min(P.group - row0, S::kRows) * kQuads; u += 32) {
-                const int row = u / kQuads, col = S::column_of_slab(x, u % kQuads * 4);
-                if (col >= D) continue;
-                const float4 y = *reinterpret_cast<const float4*>(own + row * S::kSlabPitch + u % kQuads * 4);
-                if (whole) {
-                    uint16_t* to = P.out + work.s * P.o_stride[0] + (kvh * P.group + row0 + row) * P.o_stride[1] + col;
-                    *reinterpret_cast<uint2*>(to) = make_uint2(Half16<T>::pack(y.x, y.y), Half16<T>::pack(y.z, y.w));
-                } else {
-                    *reinterpret_cast<float4*>(P.part_o + (part * P.rows + row) * D + col) = y;
-                }
-            }
-            __syncwarp();
-        }
-        if (lane == 0 && first_ci == 0) {
-            const int item = work.s * heads + work.h;
-            if (whole) {
-                if (P.join_by_item) P.joins[item] = make_int4(-1, 0, 0, 0);
-            } else {                     // it begins here and ends with a later warp
-                const int by = line.last_worker(work.units, work.n);
-                P.joins[P.join_by_item ? item : worker] =
-                    make_int4(item, static_cast<int>(part), by, by / kWarps != cta && line.ends_merged(work.units, work.n, by) ? 2 : 0);
-            }
-        }
-        if (!whole) ++parts;
+        if (!store_item<Src, T, S, DP, NT>(P, work, line, own, cta, worker, lane, parts, first_ci == 0, item_done, o, m, l)) ++parts;
         if (!last) {
             work.next(P, ctl->lengths);
             first_ci = 0;
@@ -961,63 +848,7 @@ __device__ __forceinline__ void attend_pages(const DecodeParams& P) {
     }
     cp_async_wait<0>();
     if (!merged) return;
-    // ------------------------------------------------ the CTA's sums, each warp's where its ring was
-    float* sums = reinterpret_cast<float*>(smem + warp * kSlots * kSlotBytes);
-    __syncwarp();
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-#pragma unroll
-            for (int x = 4; x < 32; x <<= 1) l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], x);
-            if (lane < 4) *reinterpret_cast<float2*>(ctl->ml[warp][n * 8 + lane * 2 + j]) = make_float2(m[n][j], l[n][j]);
-        }
-#pragma unroll
-        for (int i = 0; i < DP / 16; ++i) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                sums[(n * 8 + (lane & 3) * 2 + (j & 1)) * S::kSumPitch + S::column(i, lane, j)] = o[i][n][j];
-            }
-        }
-    }
-    __syncthreads();
-    const bool whole = whole_item;
-    const int kvh = work.h / P.tiles, row0 = (work.h - kvh * P.tiles) * S::kRows;
-    const long long part = 2ll * kWarps * cta;
-    const int rows = min(P.group - row0, S::kRows);
-#pragma unroll 4
-    for (int u = threadIdx.x; u < S::kRows * (DP / 4); u += kThreads) {
-        const int row = u / (DP / 4), col = u % (DP / 4) * 4;
-        if (row >= rows || col >= D) continue;
-        float M = -INFINITY, L = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) M = fmaxf(M, ctl->ml[w][row][0]);
-        float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-            const float f = ex2(ctl->ml[w][row][0] - (M == -INFINITY ? 0.0f : M));
-            const float4 y = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(smem + w * kSlots * kSlotBytes) + row * S::kSumPitch + col);
-            L += ctl->ml[w][row][1] * f;
-            sum.x += y.x * f; sum.y += y.y * f; sum.z += y.z * f; sum.w += y.w * f;
-        }
-        if (whole) {
-            const float inv = Src::kQuant ? inverse(M, L) * P.out_scale : inverse(M, L);
-            uint16_t* to = P.out + work.s * P.o_stride[0] + (kvh * P.group + row0 + row) * P.o_stride[1] + col;
-            *reinterpret_cast<uint2*>(to) = make_uint2(Half16<T>::pack(sum.x * inv, sum.y * inv), Half16<T>::pack(sum.z * inv, sum.w * inv));
-        } else {
-            *reinterpret_cast<float4*>(P.part_o + (part * P.rows + row) * D + col) = sum;
-            if (col == 0) *reinterpret_cast<float2*>(P.part_ml + (part * P.rows + row) * 2) = make_float2(M, L);
-        }
-    }
-    if (threadIdx.x == 0 && first_ci == 0) {
-        const int item = work.s * heads + work.h;
-        if (whole) {
-            if (P.join_by_item) P.joins[item] = make_int4(-1, 0, 0, 0);
-        } else {
-            const int by = line.last_worker(work.units, work.n);
-            P.joins[P.join_by_item ? item : worker] = make_int4(item, static_cast<int>(part), by, line.ends_merged(work.units, work.n, by) ? 3 : 1);
-        }
-    }
+    merge_cta<Src, T, S, DP, NT>(P, work, line, smem, ctl->ml, cta, warp, lane, first_ci == 0, whole_item, o, m, l);
 }
 
 // Where an item begins that ends with another worker, its parts are joined.  Workers are warps; a CTA that lies inside the item has
@@ -1125,20 +956,26 @@ DecodeScratch decode_scratch(int ctas, int rows, int head_dim) {
 // ------------------------------------------------------------------------------------------------ launches
 using Kernel = void (*)(DecodeParams);
 
-template <typename Src, int DP, int NT, Kernel kernel>
-int launch_decode(const DecodeParams& P, int ctas, cudaStream_t stream) {
-    constexpr int smem = smem_bytes<Src, DP, NT>();
-    static_assert(Shape<Src, DP, NT>::kCtas * (smem + 1024) <= 228 * 1024, "shared memory of an SM");
+// Once per device: dynamic shared memory, and the whole of an SM's for shared memory (all_shared).  An SM that runs the joins of a call with a
+// smaller share keeps it until it is idle, and takes fewer of the next call's CTAs; one that came to run a fourth then began 20 us late.
+template <Kernel kernel>
+bool configure(int smem, bool all_shared) {
     static std::atomic<uint64_t> configured{0};
     int dev = 0;
     cudaGetDevice(&dev);
     const uint64_t bit = 1ull << (dev & 63);
-    if (!(configured.load(std::memory_order_relaxed) & bit)) {
-        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
-            return TPB200_ERR_CUDA;
-        }
-        configured.fetch_or(bit, std::memory_order_relaxed);
-    }
+    if (configured.load(std::memory_order_relaxed) & bit) return true;
+    if (smem > 0 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return false;
+    if (all_shared && cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared) != cudaSuccess) return false;
+    configured.fetch_or(bit, std::memory_order_relaxed);
+    return true;
+}
+
+template <typename Src, int DP, int NT, Kernel kernel>
+int launch_decode(const DecodeParams& P, int ctas, cudaStream_t stream) {
+    constexpr int smem = smem_bytes<Src, DP, NT>();
+    static_assert(Shape<Src, DP, NT>::kCtas * (smem + 1024) <= 228 * 1024, "shared memory of an SM");
+    if (!configure<kernel>(smem, Src::kQuant)) return TPB200_ERR_CUDA;
     cudaLaunchAttribute attr;
     const cudaLaunchConfig_t cfg = paged_config(static_cast<unsigned>(ctas), kThreads, smem, &attr, stream);
     return cudaLaunchKernelEx(&cfg, kernel, P) == cudaSuccess ? TPB200_OK : TPB200_ERR_CUDA;
@@ -1157,7 +994,7 @@ struct DecodeCall {
 };
 
 // The checks of a call and its parameters, P->cache being set; group_rows: query heads that go through together
-int prepare_decode(const DecodeCall& a, int group_rows, int slot_keys, int ctas, DecodeParams* out) {
+int prepare_decode(const DecodeCall& a, int group_rows, int slot_keys, int item_units, int ctas, DecodeParams* out) {
     DecodeParams& P = *out;
     TPB_REQUIRE(a.q && a.out, TPB200_ERR_NULL);
     TPB_REQUIRE((a.flags & ~TPB200_FLAG_PDL) == 0, TPB200_ERR_ENUM);
@@ -1187,7 +1024,7 @@ int prepare_decode(const DecodeCall& a, int group_rows, int slot_keys, int ctas,
     const int positions = P.cache.page_size * P.cache.table_width;
     const long long most = (static_cast<long long>(positions) + slot_keys - 1) / slot_keys;
     P.items = static_cast<long long>(P.cache.kv_heads) * P.tiles * P.cache.seqs;
-    TPB_REQUIRE(P.items <= 0x7fffffff && (most * kSlotUnits + kItemUnits) * P.items <= 0x7fffffff, TPB200_ERR_SHAPE);
+    TPB_REQUIRE(P.items <= 0x7fffffff && (most * kSlotUnits + item_units) * P.items <= 0x7fffffff, TPB200_ERR_SHAPE);
     P.window = a.window > 0 ? std::min(a.window, positions) : positions;
     P.sinks = a.window > 0 ? std::min(a.sinks, positions) : 0;
     P.out_scale = 1.0f;
@@ -1205,15 +1042,15 @@ int prepare_decode(const DecodeCall& a, int group_rows, int slot_keys, int ctas,
     return TPB200_OK;
 }
 
-// The second kernel, given for many parts of an item and for few.  Its launch hides behind the first, which it waits for.  Where items are
-// few they have many parts each (eight lanes of eight loads), else few (two of four, so that the whole launch is resident at once).
-int launch_join(const DecodeParams& P, Kernel many_parts, Kernel few_parts, int ctas, cudaStream_t stream) {
-    const bool few = P.items * 8 < static_cast<long long>(ctas) * kWarps;
-    const int quads = kJoinThreads / (few ? 8 : 2);
+// The second kernel, given for items of a hundred parts, of many and of few.  Its launch hides behind the first, which it waits for.  Where items are
+// few they have many parts each (eight lanes of eight loads, or 32), else few (two of four, so that the whole launch is resident at once).
+int launch_join(const DecodeParams& P, Kernel most_parts, Kernel many_parts, Kernel few_parts, int ctas, cudaStream_t stream) {
+    const bool few = P.items * 8 < static_cast<long long>(ctas) * kWarps, fewest = most_parts != nullptr && P.items * 32 < ctas;
+    const int quads = kJoinThreads / (fewest ? 32 : (few ? 8 : 2));
     cudaLaunchAttribute attr;
     cudaLaunchConfig_t cfg = paged_config(static_cast<unsigned>(P.join_by_item ? P.items : ctas * kWarps - 1), kJoinThreads, 0, &attr, stream);
     cfg.gridDim.y = static_cast<unsigned>((P.rows * P.cache.head_dim / 4 + quads - 1) / quads);
-    return cudaLaunchKernelEx(&cfg, few ? many_parts : few_parts, P) == cudaSuccess ? TPB200_OK : TPB200_ERR_CUDA;
+    return cudaLaunchKernelEx(&cfg, fewest ? most_parts : (few ? many_parts : few_parts), P) == cudaSuccess ? TPB200_OK : TPB200_ERR_CUDA;
 }
 
 }  // namespace

@@ -758,7 +758,7 @@ def packed_attention(q, k, v, cu, scale, out=None, causal=True, cu_keys=None, wi
     offsets are read on the device: a captured call follows them; ones outside the tensors are clamped.
     window (causal only): of these keys a query sees the last `window`, its own among them, and its sequence's first `sinks`; the tiles in
     between are not read."""
-    w, s = _window("packed_attention", window, sinks)
+    w, s = (0, 0) if window is None and sinks == 0 else _window("packed_attention", window, sinks)
     if w == 0:
         done = (_lib._native or _lib.native()).packed_attention(q, k, v, cu, scale, out, bool(causal), cu_keys, _flags.value)
     elif not causal:
@@ -815,7 +815,7 @@ def paged_attention(q, k_pages, v_pages, table, lengths, scale, out=None, worksp
     them.  Positions without a page in the pool, or beyond the table, are left out and reported by tpb200_device_error().
     window: the token sees the last `window` keys, its own among them, and the first `sinks`; pages that hold none of these are not read
     and need not be in the table."""
-    w, s = _window("paged_attention", window, sinks)
+    w, s = (0, 0) if window is None and sinks == 0 else _window("paged_attention", window, sinks)
     if w == 0:
         done = (_lib._native or _lib.native()).paged_attention(q, k_pages, v_pages, table, lengths, scale, out, workspace, _flags.value)
     else:
@@ -954,7 +954,7 @@ def paged_attention_nvfp4(q, k_pages, v_pages, table, lengths, scale, out=None, 
     """`paged_attention` on a cache of 4-bit pages (`nvfp4_page_shape`): q / out [S, Hq, D] bf16 or fp16.  Keys are k_scale times what their codes and
     scales stand for, values v_scale times that (powers of two).  The cached values enter the products as they are held, in fp16, which holds
     them exactly; weights are rounded to fp16, sums are fp32, outputs are rounded once."""
-    w, s = _window("paged_attention_nvfp4", window, sinks)
+    w, s = (0, 0) if window is None and sinks == 0 else _window("paged_attention_nvfp4", window, sinks)
     done = (_lib._native or _lib.native()).paged_attention_nvfp4(q, k_pages, v_pages, table, lengths, scale, out, workspace, w, s, k_scale,
                                                                  v_scale, _flags.value)
     if done is not None:
