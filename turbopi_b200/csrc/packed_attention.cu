@@ -55,6 +55,7 @@ namespace tpb {
 namespace {
 
 constexpr int kTile = 128;               // rows of a query tile, keys of a key tile
+constexpr int kHalf = kTile / 2;         // keys of a request where a window may leave out keys between two of them
 constexpr int kBlockBytes = kTile * 128; // 128 rows x 64 columns of 16 bits
 constexpr long long kWait = 200000000LL; // about 0.1 s: the bound of each wait
 constexpr float kRaise = 8.0f;
@@ -318,25 +319,31 @@ __global__ void __launch_bounds__(Layout<DP, R>::kThreads, Layout<DP, R>::kCtas)
         tiles[x] = (x < R && last >= first) ? (row_limit(P, nq, nk, last) + kTile - 1) / kTile : 0;
     }
     if (!L::kOwn) tiles[1] = 0;
-    // With a window, the key tiles between those of the sinks and the first one that the first row's window reaches are left out: tile j of the
-    // CTA is key tile real(j).  Those from left_begin to left_end hold pairs hidden by the window, kBadTiles at most: the last one of the sinks, and
-    // where the windows of 256 rows begin.
-    int skip = 0, sink_tiles = 0, left_begin = 0, left_end = 0;
+    // With a window, the keys between those of the sinks (whole halves of a tile) and the first one that the first row's window reaches are left out:
+    // the CTA's keys are numbered without these `gap` keys, and so are the rows' limits.  Whatever is left between the sinks and a row's window is one
+    // range for each row.  Tiles from left_begin to left_end hold pairs of it, kBadTiles at most: the windows of 256 rows begin within
+    // 256 keys, behind at most 64 of the sinks' last half.
+    int gap = 0, sink_keys = 0, left_begin = 0, left_end = 0;
+    const int first_limit = row_limit(P, nq, nk, token0);
     if (kWindow) {
-        const int first = row_limit(P, nq, nk, token0), last = row_limit(P, nq, nk, min(token0 + tokens_cta, nq) - 1);
-        sink_tiles = static_cast<int>((static_cast<unsigned>(P.sinks) + kTile - 1) / kTile);
-        skip = max(0, max(0, first - P.window) / kTile - sink_tiles);
-        const int behind = last - P.window;              // of the keys that some row does not see, but for the sinks
+        const int last = row_limit(P, nq, nk, min(token0 + tokens_cta, nq) - 1);
+        sink_keys = static_cast<int>(min((static_cast<unsigned>(P.sinks) + kHalf - 1) / kHalf * kHalf, 0x7fffff00u));
+        const int reach = max(0, first_limit - P.window);        // the first row's first key in its window
+        gap = reach > sink_keys ? reach - sink_keys : 0;
+        const int behind = last - gap - P.window;        // of the keys that some row does not see, but for the sinks
         if (behind > P.sinks) {
-            left_begin = min(P.sinks / kTile, first / kTile - skip);
-            left_end = max(sink_tiles, (behind + kTile - 1) / kTile - skip);
+            left_begin = min(P.sinks, first_limit - gap) / kTile;
+            left_end = (behind + kTile - 1) / kTile;
         }
 #pragma unroll
-        for (int x = 0; x < 2; ++x) tiles[x] = max(0, tiles[x] - skip);
+        for (int x = 0; x < 2; ++x) {
+            const int first = token0 + x * tokens_tile, end = min(first + tokens_tile, nq) - 1;
+            if (tiles[x] > 0) tiles[x] = (row_limit(P, nq, nk, end) - gap + kTile - 1) / kTile;
+        }
     }
-    auto real = [&](int j) { return kWindow && j >= sink_tiles ? j + skip : j; };
+    auto real = [&](int key) { return kWindow && key >= sink_keys ? key + gap : key; };      // of its sequence
     const int n_tiles = max(tiles[0], tiles[1]);
-    const int first_masked = row_limit(P, nq, nk, token0) / kTile - skip;      // tiles from here on hold masked pairs: kBadTiles at most
+    const int first_masked = (first_limit - gap) / kTile;                // tiles from here on hold masked pairs: kBadTiles at most
     const int right_begin = kWindow ? max(first_masked, left_end) : first_masked;
     // the places of tiles with masked pairs in v_landed and bad
     auto looked_over = [&](int j) { return j >= first_masked || (kWindow && j >= left_begin && j < left_end); };
@@ -371,8 +378,10 @@ __global__ void __launch_bounds__(Layout<DP, R>::kThreads, Layout<DP, R>::kCtas)
                         uint64_t* bar = values && looked_over(j) ? &ctl->v_landed[place(j)] : &ctl->full[slot];
                         mbar_expect_tx(bar, L::kUnitBytes);
                         for (int b = 0; b < L::kUnitBlocks; ++b) {
-                            tma_load_3d(ring + slot * L::kUnitBytes + b * kBlockBytes, map, (h * L::kUnitBlocks + b) * 64, kv_head,
-                                        k0 + real(j) * kTile, bar);
+                            uint8_t* to = ring + slot * L::kUnitBytes + b * kBlockBytes;
+                            const int column = (h * L::kUnitBlocks + b) * 64;
+                            tma_load_3d(to, map, column, kv_head, k0 + real(j * kTile), bar);
+                            if (kWindow) tma_load_3d(to + kBlockBytes / 2, map, column, kv_head, k0 + real(j * kTile + kHalf), bar);
                         }
                     }
                     return true;
@@ -536,7 +545,7 @@ __global__ void __launch_bounds__(Layout<DP, R>::kThreads, Layout<DP, R>::kCtas)
                 const int u0 = v_unit(j);
                 bool ok = wait_warp(&ctl->v_landed[place(j)], 0);
                 for (int r = (warp - 2) * 32 + lane; r < kTile && ok; r += 64) {
-                    const bool there = real(j) * kTile + r < nk;
+                    const bool there = real(j * kTile + r) < nk;
                     bool bad = false;
                     for (int h = 0; h < L::kHalves; ++h) {
                         for (int b = 0; b < L::kUnitBlocks; ++b) {
@@ -591,10 +600,10 @@ __global__ void __launch_bounds__(Layout<DP, R>::kThreads, Layout<DP, R>::kCtas)
         const uint32_t s_at = lanes + x * kTile, p_at = lanes + L::kColP + x * L::kStepP, o_at = lanes + L::kColO + (L::kOwn ? x * DP : 0);
         const int my_tile = L::kOwn ? x : 0;
         const int token = token0 + my_tile * tokens_tile + (row >> P.pack_shift);
-        const int limit = row_limit(P, nq, nk, token);
-        const int lowest = row_limit(P, nq, nk, token0 + my_tile * tokens_tile);     // of the tile's rows that exist
+        const int limit = token < nq ? row_limit(P, nq, nk, token) - gap : 0;
+        const int lowest = row_limit(P, nq, nk, token0 + my_tile * tokens_tile) - gap;       // of the tile's rows that exist
         // of the tile's rows that exist: behind the last key that the window hides from one
-        const int behind = kWindow ? row_limit(P, nq, nk, min(token0 + (my_tile + 1) * tokens_tile, nq) - 1) - P.window : 0;
+        const int behind = kWindow ? row_limit(P, nq, nk, min(token0 + (my_tile + 1) * tokens_tile, nq) - 1) - gap - P.window : 0;
         float ref = -INFINITY, l = 0.0f;
         float l_ref = -INFINITY;         // the reference that l is relative to (one row tile: the groups share ref)
         bool ok = true;
@@ -603,7 +612,7 @@ __global__ void __launch_bounds__(Layout<DP, R>::kThreads, Layout<DP, R>::kCtas)
             const int j = key_tile(e);
             if (!wait_warp(&ctl->s_ready[x], (e >> 1) & 1)) { ok = false; break; }
             tc::fence_after_thread_sync();
-            const int key0 = real(j) * kTile;
+            const int key0 = j * kTile;
             const bool masked = key0 + kTile > lowest || (kWindow && key0 < behind && key0 + kTile > P.sinks);
             const int lim = limit - key0;
             uint32_t s[kTile];
@@ -729,10 +738,10 @@ __global__ void __launch_bounds__(Layout<DP, R>::kThreads, Layout<DP, R>::kCtas)
                 }
                 if (any_bad && token < nq) {             // what was taken out of V, for the rows that see it
                     for (int i = 0; i < (kWindow ? 2 : 1) * kBadTiles * kTile; ++i) {
-                        const int key = real(tile_at(i / kTile)) * kTile + i % kTile;
+                        const int key = tile_at(i / kTile) * kTile + i % kTile;
                         if (!((ctl->bad[i >> 7][(i >> 5) & 3] >> (i & 31)) & 1) || key >= limit) continue;
                         if (kWindow && key >= P.sinks && key < limit - P.window) continue;
-                        const uint16_t* from = P.v_rows + static_cast<long long>(k0 + key) * P.v_stride[0] +
+                        const uint16_t* from = P.v_rows + static_cast<long long>(k0 + real(key)) * P.v_stride[0] +
                                                head_group / P.groups_per_kv * P.v_stride[1];
 #pragma unroll
                         for (int n = 0; n < 32; ++n) {
@@ -880,8 +889,9 @@ int attend(const tpb200_packed_attention_args* a, int window, int sinks, tpb200_
     const int rows_tokens = kTile / pack;
     if (!rows_map(&P.q, a->q, a->head_dim, a->q_heads, a->q_stride[1], a->q_tokens, a->q_stride[0], pack, rows_tokens)) return TPB200_ERR_SHAPE;
     if (a->k_tokens > 0) {
-        if (!rows_map(&P.k, a->k, a->head_dim, a->kv_heads, a->k_stride[1], a->k_tokens, a->k_stride[0], 1, kTile) ||
-            !rows_map(&P.v, a->v, a->head_dim, a->kv_heads, a->v_stride[1], a->k_tokens, a->v_stride[0], 1, kTile)) {
+        const int keys_box = hides ? kHalf : kTile;
+        if (!rows_map(&P.k, a->k, a->head_dim, a->kv_heads, a->k_stride[1], a->k_tokens, a->k_stride[0], 1, keys_box) ||
+            !rows_map(&P.v, a->v, a->head_dim, a->kv_heads, a->v_stride[1], a->k_tokens, a->v_stride[0], 1, keys_box)) {
             return TPB200_ERR_SHAPE;
         }
     }
