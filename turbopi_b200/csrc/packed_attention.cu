@@ -900,7 +900,7 @@ int attend(const tpb200_packed_attention_args* a, int window, int sinks, tpb200_
     // 24 sequences of 100 / 8 of 1536, 16 heads of 64: 13.5 us with one, 18.1 with two / 91.6, 92.6; 16 heads of 128: 21.0, 25.2 / 129, 118.
     // Batches of sequences alike; not measured where lengths differ much or queries are few beside the keys.
     const long long keys = hides ? std::min<long long>(a->k_tokens, (static_cast<long long>(window) + P.sinks) * a->seqs) : a->k_tokens;
-    const bool two = DP <= 128 && keys > (DP == 64 ? 1000ll : 200ll) * a->seqs;
+    const bool two = DP <= 128 && keys > (DP == 64 || hides ? 1000ll : 200ll) * a->seqs;
     // no more tiles than whole ones and a ragged one per sequence
     const long long tiles = static_cast<long long>(a->q_tokens) / (rows_tokens * (two ? 2 : 1)) + std::min(a->seqs, a->q_tokens);
     const long long blocks = tiles * P.head_groups;

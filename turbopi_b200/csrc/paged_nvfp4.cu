@@ -6,14 +6,17 @@
 //
 // Both are bound by HBM for prompts and by the chain offsets -> length -> page id -> row for a decode step.
 #include <algorithm>
+#include <type_traits>
 
 #include "paged.cuh"
 
 namespace tpb {
 namespace {
 
-constexpr int kThreads = 256;            // of a block at most
-constexpr int kAppendLoads = 2;          // tokens whose unit a thread has in flight
+constexpr int kAppendThreads = 256;      // of a block at most
+constexpr int kPairThreads = 256, kPairBlocks = 4;
+constexpr int kReadThreads = 256;
+constexpr int kAppendLoads = 1;          // tokens whose unit a thread has in flight
 constexpr int kAppendTokens = 4;         // of a block at most
 constexpr int kReadLoads = 4;
 constexpr int kReadTokens = 16;
@@ -68,47 +71,185 @@ struct AppendParams {
     float k_inv, v_inv;                  // 1 / k_scale, 1 / v_scale
 };
 
-// x * c - y * s and x * c + y * s, each operation rounded: the sums that elementary operations give, whatever else is compiled around them
-__device__ __forceinline__ float turn_first(float x, float y, float c, float s) { return __fsub_rn(__fmul_rn(x, c), __fmul_rn(y, s)); }
-__device__ __forceinline__ float turn_second(float x, float y, float c, float s) { return __fadd_rn(__fmul_rn(x, c), __fmul_rn(y, s)); }
+// Two floats an instruction, each result rounded by itself
+__device__ __forceinline__ uint64_t two(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 one_by_one(uint64_t p) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ uint64_t unpack2(uint32_t w) {
+    const float2 f = Half16<T>::unpack(w);
+    return two(f.x, f.y);
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(uint64_t p) {
+    const float2 f = one_by_one(p);
+    return Half16<T>::pack(f.x, f.y);
+}
 
-// 16 values -> a scale and 16 codes.  The quotient is x times the rounded inverse of s, off by 2^-22 at most for |x / s| <= 6.  Ties are common (s has four
-// bits, x eight or eleven) and have to stay ties: the sum with 128 rounds the quotient to a multiple of 2^-17 or 2^-16.  A quotient that is no tie is 2^-13 from one
-// at least, since x differs from a tie times s, which the type of x holds, by a step of that type.
-__device__ __forceinline__ void quantise16(const float (&x)[16], float inv, uint2& codes, uint8_t& scale) {
-    float top = 0.0f, odd = 0.0f;
+// 16 values of a type as eight words -> a scale and 16 codes.  The quotient is x times the rounded inverse of s, off by 2^-22 at most for |x / s| <= 6.
+// Ties are common (s has four bits, x eight or eleven) and have to stay ties: the sum with 128 rounds the quotient to a multiple of 2^-17 or 2^-16.
+// A quotient that is no tie is 2^-13 from one at least, since x differs from a tie times s, which the type of x holds, by a step of that type.
+// (Powers of two in `inv` change nothing of this; past 6 the conversion saturates.)
+template <typename T>
+__device__ __forceinline__ void quantise16(const uint32_t (&x)[8], float inv, uint2& codes, uint32_t& scale) {
+    constexpr uint32_t kInf = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+    uint32_t both = 0;                   // the largest size in the low halves and in the high ones: sizes are ordered as their bits are
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        top = fmaxf(top, fabsf(x[i]));
-        odd = fmaf(x[i], 0.0f, odd);     // NaN from the first infinity or NaN on
-    }
+    for (int i = 0; i < 8; ++i) both = __vmaxu2(both, x[i] & 0x7fff7fffu);
+    const uint32_t top = max(both & 0xffffu, both >> 16);
     codes = make_uint2(0, 0);
-    if (odd != 0.0f || isnan(odd)) {
-        scale = 0x7f;                    // NaN
-        return;
-    }
-    scale = encode_e4m3(__fdiv_rn(top * inv, 6.0f));
+    scale = 0x7f;                        // NaN
+    if (top >= kInf) return;
+    scale = encode_e4m3(__fdiv_rn(Half16<T>::unpack(top).x * inv, 6.0f));
     if (scale == 0) return;
-    const float r = __frcp_rn(decode_e4m3(scale));
-    uint32_t w[2] = {0, 0};
+    const float inverse = __frcp_rn(decode_e4m3(static_cast<uint8_t>(scale))) * inv;
+    const uint64_t f = two(inverse, inverse), up = two(128.0f, 128.0f), down = two(-128.0f, -128.0f);
+    uint32_t w[2];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        float y[2];
+    for (int i = 0; i < 2; ++i) {
+        float y[8];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            // (x * inv is exact: a power of two.  Past 6 the conversion saturates.)
-            y[j] = __fmul_rn(__fmul_rn(x[2 * i + j], inv), r);
-            y[j] = __fsub_rn(__fadd_rn(y[j], 128.0f), 128.0f);
+        for (int j = 0; j < 4; ++j) {
+            const float2 q = one_by_one(add2(fma2(unpack2<T>(x[i * 4 + j]), f, up), down));
+            y[2 * j] = q.x;
+            y[2 * j + 1] = q.y;
         }
-        w[i >> 2] |= encode_e2m1x2(y[0], y[1]) << ((i & 3) * 8);
+        asm("{\n .reg .b8 a, b, c, d;\n cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n"
+            " cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n mov.b32 %0, {a, b, c, d};\n}\n"
+            : "=r"(w[i]) : "f"(y[0]), "f"(y[1]), "f"(y[2]), "f"(y[3]), "f"(y[4]), "f"(y[5]), "f"(y[6]), "f"(y[7]));
     }
     codes = make_uint2(w[0], w[1]);
 }
 
-// A unit of the queries is V values and the V values half a row further on, V = 8 where half a row is a multiple of 8, else 4; a unit of
-// the keys or values is a block of 16, for keys with the 16 values half a row away beside it.  A thread keeps its unit for all tokens of the block.
+// Turns V values and the V values half a row further on: x c - y s and y c + x s in fp32, each operation rounded, as elementary operations give
+// them whatever else is compiled around them, then rounded to the type
 template <typename T, int V>
-__global__ void __launch_bounds__(kThreads, 3) append_nvfp4_kernel(const __grid_constant__ AppendParams P) {
+__device__ __forceinline__ void turn_pair(Vec<V>& a, Vec<V>& b, const AppendParams& P, int pos, int at) {
+    float c[V], s[V];
+    const size_t e = static_cast<size_t>(pos) * (P.cache.head_dim / 2) + at;
+    load_table<V>(P.cos, P.rope_dtype, e, c);
+    load_table<V>(P.sin, P.rope_dtype, e, s);
+#pragma unroll
+    for (int j = 0; j < V / 2; ++j) {
+        const uint64_t x = unpack2<T>(a.w[j]), y = unpack2<T>(b.w[j]), c2 = two(c[2 * j], c[2 * j + 1]), s2 = two(s[2 * j], s[2 * j + 1]);
+        a.w[j] = pack2<T>(fma2(mul2(y, s2), two(-1.0f, -1.0f), mul2(x, c2)));
+        b.w[j] = pack2<T>(add2(mul2(y, c2), mul2(x, s2)));
+    }
+}
+
+// Head sizes that are multiples of 32.  A unit of the queries is 8 values and the 8 values half a row further on; of the keys and values two blocks of
+// 16, half a row apart for keys that are turned, else side by side.  A thread keeps its unit for all tokens of the block, and has 64 bytes on their way:
+// two tokens of the queries, or one of the keys or values.
+template <typename T>
+__global__ void __launch_bounds__(kPairThreads, kPairBlocks) append_pairs_kernel(const __grid_constant__ AppendParams P) {
+    __shared__ int seq[kAppendTokens];
+    __shared__ int position[kAppendTokens];
+    __shared__ long long row_at[kAppendTokens];
+    pdl_wait_prior_grids();
+    pdl_launch_dependents();
+    const int t0 = blockIdx.x * P.tokens_per_block;
+    const int count = min(P.tokens_per_block, P.tokens - t0);
+    const int per_token = P.units_q + 2 * P.units_kv;
+    const int D = P.cache.head_dim, half = D / 2, per_row = half / 8, groups = D / 32;
+    bool placed = false;
+    for (int base = 0; base < per_token; base += blockDim.x) {
+        const int u = base + threadIdx.x;
+        const bool mine = u < per_token;
+        const int kind = u < P.units_q ? 0 : (u < P.units_q + P.units_kv ? 1 : 2);       // queries, keys, values
+        const int r = u - (kind == 0 ? 0 : (kind == 1 ? P.units_q : P.units_q + P.units_kv));
+        const int head = kind == 0 ? r / per_row : r / groups, in = kind == 0 ? r - head * per_row : r - head * groups;
+        const bool turn = P.rope_positions > 0 && kind < 2;
+        const int at = kind == 0 ? in * 8 : (turn ? in * 16 : in * 32), at2 = turn ? at + half : at + 16;        // first columns of the two blocks
+        const long long* st = kind == 0 ? P.q_stride : (kind == 1 ? P.k_stride : P.v_stride);
+        const long long step = st[0];
+        const uint16_t* src = (kind == 0 ? P.q : (kind == 1 ? P.k : P.v)) + t0 * step + head * st[1] + at;
+        const int apart = at2 - at;
+        const int tokens = kind == 0 ? 2 : 1;
+        Vec<8> a, b, a2, b2;             // of the queries: a, b of a token, a2, b2 of the next; else the first and second halves of two blocks
+        auto load = [&](int first) {
+            const uint16_t* row = src + first * step;
+            if (!mine || first >= count) return;
+            a = load_vec<8>(row);
+            b = load_vec<8>(row + apart);
+            row += kind == 0 ? step : 8;
+            if (kind == 0 && first + 1 >= count) return;
+            a2 = load_vec<8>(row);
+            b2 = load_vec<8>(row + apart);
+        };
+        load(0);
+        if (!placed) {                   // the tokens' rows, behind the first loads
+            placed = true;
+            place_tokens<true, kAppendTokens>(P.cache, P.cu, t0, count, P.rope_positions, seq, position, row_at);
+        }
+        for (int first = 0; mine && first < count; first += tokens) {
+            if (kind == 0) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    if (first + i >= count || row_at[first + i] < 0) continue;
+                    Vec<8>&x = i == 0 ? a : a2, &y = i == 0 ? b : b2;
+                    turn_pair<T, 8>(x, y, P, position[first + i], at);
+                    uint16_t* to = P.q_out + (t0 + first + i) * P.o_stride[0] + head * P.o_stride[1] + at;
+                    store_vec<8>(to, x);
+                    store_vec<8>(to + half, y);
+                }
+            } else if (row_at[first] >= 0) {
+                const int pos = position[first];
+                if (turn) {
+                    turn_pair<T, 8>(a, b, P, pos, at);
+                    turn_pair<T, 8>(a2, b2, P, pos, at + 8);
+                }
+                uint8_t* tile = static_cast<uint8_t*>(kind == 1 ? P.cache.k_pages : P.cache.v_pages) + row_at[first] + head * P.cache.head_stride;
+                const float inv = kind == 1 ? P.k_inv : P.v_inv;
+                uint8_t* codes_at = tile + (pos & 15) * 16 * groups;
+                uint8_t* scales_at = tile + 256 * groups + (pos & 15) * 2 * groups;
+                const uint32_t x[8] = {a.w[0], a.w[1], a.w[2], a.w[3], a2.w[0], a2.w[1], a2.w[2], a2.w[3]};
+                const uint32_t y[8] = {b.w[0], b.w[1], b.w[2], b.w[3], b2.w[0], b2.w[1], b2.w[2], b2.w[3]};
+                uint2 codes, codes2;
+                uint32_t scale, scale2;
+                quantise16<T>(x, inv, codes, scale);
+                quantise16<T>(y, inv, codes2, scale2);
+                if (turn) {
+                    *reinterpret_cast<uint2*>(codes_at + at / 2) = codes;
+                    *reinterpret_cast<uint2*>(codes_at + at2 / 2) = codes2;
+                    scales_at[at / 16] = static_cast<uint8_t>(scale);
+                    scales_at[at2 / 16] = static_cast<uint8_t>(scale2);
+                } else {
+                    *reinterpret_cast<uint4*>(codes_at + at / 2) = make_uint4(codes.x, codes.y, codes2.x, codes2.y);
+                    *reinterpret_cast<uint16_t*>(scales_at + at / 16) = static_cast<uint16_t>(scale | scale2 << 8);
+                }
+            }
+            load(first + tokens);
+        }
+    }
+}
+
+// Other head sizes.  A unit of the queries is V values and the V values half a row further on, V = 8 where half a row is a multiple of 8, else 4; a unit of
+// the keys or values is a block of 16, for keys that are turned with the 16 values half a row away beside it.  A thread keeps its unit for all tokens of the
+// block.
+template <typename T, int V>
+__global__ void __launch_bounds__(kAppendThreads, 4) append_blocks_kernel(const __grid_constant__ AppendParams P) {
     __shared__ int seq[kAppendTokens];
     __shared__ int position[kAppendTokens];
     __shared__ long long row_at[kAppendTokens];
@@ -126,11 +267,11 @@ __global__ void __launch_bounds__(kThreads, 3) append_nvfp4_kernel(const __grid_
         const int kind = u < P.units_q ? 0 : (u < P.units_q + P.units_kv ? 1 : 2);       // queries, keys, values
         const int r = u - (kind == 0 ? 0 : (kind == 1 ? P.units_q : P.units_q + P.units_kv));
         const int head = kind == 0 ? r / per_row : r / (2 * groups), in = kind == 0 ? r - head * per_row : r - head * 2 * groups;
+        const bool turn = P.rope_positions > 0 && kind < 2;
         const int at = kind == 0 ? in * V : in * 16;     // first column; the partners of column c stand at c + half or c - half
         const long long* st = kind == 0 ? P.q_stride : (kind == 1 ? P.k_stride : P.v_stride);
         const long long step = st[0];
         const uint16_t* src = (kind == 0 ? P.q : (kind == 1 ? P.k : P.v)) + t0 * step + head * st[1];
-        const bool turn = P.rope_positions > 0 && kind < 2;
         for (int first = 0; first < count; first += kAppendLoads) {
             Vec<V> x[kAppendLoads][kVecs], y[kAppendLoads][kVecs];
 #pragma unroll
@@ -157,52 +298,29 @@ __global__ void __launch_bounds__(kThreads, 3) append_nvfp4_kernel(const __grid_
                 if (row < 0) continue;
                 const int pos = position[first + i];
                 if (kind == 0) {
-                    float c[V], s[V];
-                    const size_t e = static_cast<size_t>(pos) * half + at;
-                    load_table<V>(P.cos, P.rope_dtype, e, c);
-                    load_table<V>(P.sin, P.rope_dtype, e, s);
-                    Vec<V> a, b;
-#pragma unroll
-                    for (int j = 0; j < V / 2; ++j) {    // in fp32, rounded once
-                        const float2 p = Half16<T>::unpack(x[i][0].w[j]), q = Half16<T>::unpack(y[i][0].w[j]);
-                        a.w[j] = Half16<T>::pack(turn_first(p.x, q.x, c[2 * j], s[2 * j]), turn_first(p.y, q.y, c[2 * j + 1], s[2 * j + 1]));
-                        b.w[j] = Half16<T>::pack(turn_second(q.x, p.x, c[2 * j], s[2 * j]), turn_second(q.y, p.y, c[2 * j + 1], s[2 * j + 1]));
-                    }
+                    turn_pair<T, V>(x[i][0], y[i][0], P, pos, at);
                     uint16_t* to = P.q_out + (t0 + first + i) * P.o_stride[0] + head * P.o_stride[1] + at;
-                    store_vec<V>(to, a);
-                    store_vec<V>(to + half, b);
+                    store_vec<V>(to, x[i][0]);
+                    store_vec<V>(to + half, y[i][0]);
                     continue;
                 }
-                float f[16];
+                if (turn) {
 #pragma unroll
-                for (int n = 0; n < kVecs; ++n) {
-                    const int col = at + n * V;
-                    if (turn && col < D) {
-                        float c[V], s[V];
-                        const bool low = col < half;
-                        const size_t e = static_cast<size_t>(pos) * half + (low ? col : col - half);
-                        load_table<V>(P.cos, P.rope_dtype, e, c);
-                        load_table<V>(P.sin, P.rope_dtype, e, s);
-#pragma unroll
-                        for (int j = 0; j < V / 2; ++j) {
-                            const float2 p = Half16<T>::unpack(x[i][n].w[j]), q = Half16<T>::unpack(y[i][n].w[j]);
-                            const float s0 = low ? -s[2 * j] : s[2 * j], s1 = low ? -s[2 * j + 1] : s[2 * j + 1];
-                            x[i][n].w[j] = Half16<T>::pack(turn_second(p.x, q.x, c[2 * j], s0), turn_second(p.y, q.y, c[2 * j + 1], s1));
-                        }
-                    }
-#pragma unroll
-                    for (int j = 0; j < V / 2; ++j) {
-                        const float2 p = Half16<T>::unpack(x[i][n].w[j]);
-                        f[n * V + 2 * j] = p.x;
-                        f[n * V + 2 * j + 1] = p.y;
+                    for (int n = 0; n < kVecs; ++n) {
+                        const int c = at + n * V;
+                        if (c < half) turn_pair<T, V>(x[i][n], y[i][n], P, pos, c);
+                        else if (c < D) turn_pair<T, V>(y[i][n], x[i][n], P, pos, c - half);
                     }
                 }
-                uint2 codes;
-                uint8_t scale;
-                quantise16(f, kind == 1 ? P.k_inv : P.v_inv, codes, scale);
                 uint8_t* tile = static_cast<uint8_t*>(kind == 1 ? P.cache.k_pages : P.cache.v_pages) + row + head * P.cache.head_stride;
-                *reinterpret_cast<uint2*>(tile + (pos & 15) * 16 * groups + in * 8) = codes;
-                tile[256 * groups + (pos & 15) * 2 * groups + in] = scale;
+                const float inv = kind == 1 ? P.k_inv : P.v_inv;
+                uint8_t* codes_at = tile + (pos & 15) * 16 * groups;
+                uint8_t* scales_at = tile + 256 * groups + (pos & 15) * 2 * groups;
+                uint2 codes;
+                uint32_t scale;
+                quantise16<T>(reinterpret_cast<const uint32_t(&)[8]>(x[i]), inv, codes, scale);
+                *reinterpret_cast<uint2*>(codes_at + in * 8) = codes;
+                scales_at[in] = static_cast<uint8_t>(scale);
             }
         }
     }
@@ -215,13 +333,14 @@ struct ReadParams {
     long long k_stride[2], v_stride[2];
     const int* cu;
     int tokens, tokens_per_block;
-    int units;                           // of eight values, per token of keys, and of values
+    int units;                           // per token of keys, and of values
     float k_scale, v_scale;
 };
 
-// A thread has eight columns of a head's keys or values (16 bytes to write, whole warps write whole lines) of every kLanes-th token of the block.
-template <typename T, bool kTiles>
-__global__ void __launch_bounds__(kThreads) read_kernel(const __grid_constant__ ReadParams P) {
+// A thread has a unit, 16 columns of a head's keys or values (8 of 16-bit pages), of every kLanes-th token of the block.  kWide: the rows it writes begin
+// on 32 bytes, and a unit leaves in one store.
+template <typename T, bool kTiles, bool kWide>
+__global__ void __launch_bounds__(kReadThreads) read_kernel(const __grid_constant__ ReadParams P) {
     __shared__ int seq[kReadTokens];
     __shared__ int position[kReadTokens];
     __shared__ long long row_at[kReadTokens];
@@ -230,59 +349,71 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const __grid_constant__ 
     const int t0 = blockIdx.x * P.tokens_per_block;
     const int count = min(P.tokens_per_block, P.tokens - t0);
     place_tokens<kTiles, kReadTokens>(P.cache, P.cu, t0, count, 0, seq, position, row_at);
-    const int D = P.cache.head_dim, per_row = D / 8, groups = (D + 31) / 32;
+    constexpr int kColumns = kTiles ? 16 : 8;
+    const int D = P.cache.head_dim, per_row = (D + kColumns - 1) / kColumns, groups = (D + 31) / 32;
     const int all = 2 * P.units, lanes = max(1, static_cast<int>(blockDim.x) / all), lane = all <= static_cast<int>(blockDim.x) ? threadIdx.x / all : 0;
     if (lane >= lanes) return;
     for (int u = threadIdx.x - lane * all; u < all; u += blockDim.x) {
         const bool keys = u < P.units;
         const int r = keys ? u : u - P.units, head = r / per_row, in = r - head * per_row;
-        const uint8_t* pages = static_cast<const uint8_t*>(keys ? P.cache.k_pages : P.cache.v_pages);
+        const uint8_t* from = static_cast<const uint8_t*>(keys ? P.cache.k_pages : P.cache.v_pages) + head * P.cache.head_stride * (kTiles ? 1 : 2);
         const long long* st = keys ? P.k_stride : P.v_stride;
-        uint16_t* to = (keys ? P.k : P.v) + t0 * st[0] + head * st[1] + in * 8;
+        const long long step = lanes * st[0];
+        uint16_t* to = (keys ? P.k : P.v) + (t0 + lane) * st[0] + head * st[1] + in * kColumns;
         const float factor = keys ? P.k_scale : P.v_scale;
+        const bool whole = kWide || in * kColumns + kColumns <= D;       // of 16 columns the last 8 may be past the head's
         for (int first = lane; first < count; first += lanes * kReadLoads) {
             uint4 x[kReadLoads];
-            uint32_t scale[kReadLoads];
+            long long row[kReadLoads];
 #pragma unroll
             for (int i = 0; i < kReadLoads; ++i) {
                 const int t = first + i * lanes;
                 x[i] = make_uint4(0, 0, 0, 0);
-                scale[i] = 0;
-                if (t >= count || row_at[t] < 0) continue;
+                row[i] = t < count ? row_at[t] : -2;
+                if (row[i] < 0) continue;
                 if constexpr (kTiles) {
-                    const uint8_t* tile = pages + row_at[t] + head * P.cache.head_stride;
-                    const int row = position[t] & 15;
-                    x[i].x = __ldg(reinterpret_cast<const uint32_t*>(tile + row * 16 * groups + in * 4));
-                    scale[i] = __ldg(tile + 256 * groups + row * 2 * groups + in / 2);
+                    const uint8_t* tile = from + row[i];
+                    const int line = (position[t] & 15) * 2 * groups;
+                    const uint2 codes = __ldg(reinterpret_cast<const uint2*>(tile + line * 8 + in * 8));
+                    x[i] = make_uint4(codes.x, codes.y, __ldg(tile + 256 * groups + line + in), 0);
                 } else {
-                    x[i] = __ldg(reinterpret_cast<const uint4*>(pages + 2 * (row_at[t] + head * P.cache.head_stride + in * 8)));
+                    x[i] = __ldg(reinterpret_cast<const uint4*>(from + 2 * row[i] + in * 16));
                 }
             }
 #pragma unroll
-            for (int i = 0; i < kReadLoads; ++i) {
-                const int t = first + i * lanes;
-                if (t >= count || row_at[t] == -2) continue;
+            for (int i = 0; i < kReadLoads; ++i, to += step) {
+                if (row[i] == -2) continue;
                 if constexpr (kTiles) {
-                    __half2 h[4];
-                    uint32_t w[4];
-                    decode_e2m1x8(x[i].x, h);
-                    const float s = decode_e4m3(static_cast<uint8_t>(scale[i])) * factor;
+                    const float s = decode_e4m3(static_cast<uint8_t>(x[i].z)) * factor;
+                    uint32_t w[8];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {        // exact but for an overflow of fp16 or a factor's underflow
-                        const float2 f = __half22float2(h[j]);
-                        w[j] = Half16<T>::pack(f.x * s, f.y * s);
+                    for (int half = 0; half < 2; ++half) {
+                        __half2 h[4];
+                        decode_e2m1x8(half == 0 ? x[i].x : x[i].y, h);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {    // exact but for an overflow of fp16 or a factor's underflow
+                            const float2 f = __half22float2(h[j]);
+                            w[half * 4 + j] = Half16<T>::pack(f.x * s, f.y * s);
+                        }
                     }
-                    x[i] = make_uint4(w[0], w[1], w[2], w[3]);
+                    if constexpr (kWide) {
+                        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+                                     "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
+                    } else {
+                        *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+                        if (whole) *reinterpret_cast<uint4*>(to + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+                    }
+                } else {
+                    *reinterpret_cast<uint4*>(to) = x[i];
                 }
-                *reinterpret_cast<uint4*>(to + t * st[0]) = x[i];
             }
         }
     }
 }
 
-// a block's threads for `units` a token: as few passes over them as kThreads allows, and those even
-int threads_for(long long units) {
-    const long long passes = (units + kThreads - 1) / kThreads;
+// a block's threads for `units` a token: as few passes over them as `most` threads allow, and those even
+int threads_for(long long units, int most) {
+    const long long passes = (units + most - 1) / most;
     return static_cast<int>(((units + passes - 1) / passes + 31) / 32 * 32);
 }
 
@@ -325,16 +456,18 @@ int read_rows(const PagedView& cache, int dtype, bool tiles, float k_scale, floa
     P.tokens = a->tokens;
     P.k_scale = k_scale;
     P.v_scale = v_scale;
-    const long long units = static_cast<long long>(cache.head_dim / 8) * cache.kv_heads;
+    const long long units = static_cast<long long>(tiles ? (cache.head_dim + 15) / 16 : cache.head_dim / 8) * cache.kv_heads;
     TPB_REQUIRE(units <= (1 << 24), TPB200_ERR_SHAPE);
     P.units = static_cast<int>(units);
-    const int threads = 2 * units <= kThreads ? kThreads : threads_for(2 * units), lanes = std::max(1, static_cast<int>(threads / (2 * units)));
+    const int threads = 2 * units <= kReadThreads ? kReadThreads : threads_for(2 * units, kReadThreads), lanes = std::max(1, static_cast<int>(threads / (2 * units)));
     // a block's look-up serves up to a tile of tokens, fewer where that would leave SMs without a block, but at least one for each lane
     P.tokens_per_block = std::max(std::min(lanes, kReadTokens), std::min(kReadTokens, a->tokens / 592));
     cudaLaunchAttribute attr;
     const cudaLaunchConfig_t cfg = paged_config(static_cast<unsigned>((a->tokens - 1) / P.tokens_per_block + 1), threads, 0, &attr, stream);
-    const bool bf = a->dtype == TPB200_BF16;
-    const auto kernel = tiles ? (bf ? read_kernel<__nv_bfloat16, true> : read_kernel<__half, true>) : read_kernel<__half, false>;
+    bool wide = cache.head_dim % 16 == 0 && (reinterpret_cast<uintptr_t>(a->k) | reinterpret_cast<uintptr_t>(a->v)) % 32 == 0;
+    for (const long long st : {P.k_stride[0], P.k_stride[1], P.v_stride[0], P.v_stride[1]}) wide = wide && st % 16 == 0;
+    auto pick = [&](auto type) { return wide ? read_kernel<decltype(type), true, true> : read_kernel<decltype(type), true, false>; };
+    const auto kernel = !tiles ? read_kernel<__half, false, false> : (a->dtype == TPB200_BF16 ? pick(__nv_bfloat16()) : pick(__half()));
     return cudaLaunchKernelEx(&cfg, kernel, P) == cudaSuccess ? TPB200_OK : TPB200_ERR_CUDA;
 }
 
@@ -416,7 +549,7 @@ extern "C" int tpb200_paged_append_nvfp4(const tpb200_paged_append_nvfp4_args* a
     P.k_inv = 1.0f / a->cache.k_scale;
     P.v_inv = 1.0f / a->cache.v_scale;
     const int half = D / 2, V = half % 8 == 0 ? 8 : 4;
-    const long long units_q = a->q != nullptr ? static_cast<long long>(half / V) * a->q_heads : 0, units_kv = 2ll * ((D + 31) / 32) * H;
+    const long long units_q = a->q != nullptr ? static_cast<long long>(half / V) * a->q_heads : 0, units_kv = (D % 32 == 0 ? 1ll : 2ll) * ((D + 31) / 32) * H;
     TPB_REQUIRE(units_q + 2 * units_kv <= (1 << 24), TPB200_ERR_SHAPE);
     P.units_q = static_cast<int>(units_q);
     P.units_kv = static_cast<int>(units_kv);
@@ -424,9 +557,14 @@ extern "C" int tpb200_paged_append_nvfp4(const tpb200_paged_append_nvfp4_args* a
     P.tokens_per_block = std::max(1, std::min(kAppendTokens, a->tokens / 444));
     const unsigned blocks = static_cast<unsigned>((a->tokens - 1) / P.tokens_per_block + 1);
     const bool bf = a->dtype == TPB200_BF16;
-    const auto kernel = bf ? (V == 8 ? append_nvfp4_kernel<__nv_bfloat16, 8> : append_nvfp4_kernel<__nv_bfloat16, 4>)
-                           : (V == 8 ? append_nvfp4_kernel<__half, 8> : append_nvfp4_kernel<__half, 4>);
+    const bool pairs = D % 32 == 0;
+    auto pick = [&](auto type) {
+        using T = decltype(type);
+        return pairs ? append_pairs_kernel<T> : (V == 8 ? append_blocks_kernel<T, 8> : append_blocks_kernel<T, 4>);
+    };
+    const auto kernel = bf ? pick(__nv_bfloat16()) : pick(__half());
     cudaLaunchAttribute attr;
-    const cudaLaunchConfig_t cfg = paged_config(blocks, threads_for(units_q + 2 * units_kv), 0, &attr, reinterpret_cast<cudaStream_t>(stream));
+    const cudaLaunchConfig_t cfg = paged_config(blocks, threads_for(units_q + 2 * units_kv, pairs ? kPairThreads : kAppendThreads), 0, &attr,
+                                                reinterpret_cast<cudaStream_t>(stream));
     return cudaLaunchKernelEx(&cfg, kernel, P) == cudaSuccess ? TPB200_OK : TPB200_ERR_CUDA;
 }
