@@ -101,6 +101,7 @@ def _check_append(device, lens, new, hq, hk, D, page, dtype, rope=None, k_scale=
         assert got is None
     else:
         assert got is kw["q_out"] and bool((got[T:] == 9).all())
+        assert torch.equal(got[:T], _turned(q[:T], cos[pos], sin[pos]))         # no operation fused with another
         want = rotate(q[:T], cos[pos], sin[pos])
         big = q[:T].double().abs().sum(-1, keepdim=True)
         assert bool(((got[:T].double() - want).abs() <= HALF_STEP[dtype] * want.abs() + 2.0 ** -22 * big + 2.0 ** -24).all())

@@ -155,7 +155,9 @@ __device__ __forceinline__ void turn_pair(Vec<V>& a, Vec<V>& b, const AppendPara
     for (int j = 0; j < V / 2; ++j) {
         const uint64_t x = unpack2<T>(a.w[j]), y = unpack2<T>(b.w[j]), c2 = two(c[2 * j], c[2 * j + 1]), s2 = two(s[2 * j], s[2 * j + 1]);
         a.w[j] = pack2<T>(fma2(mul2(y, s2), two(-1.0f, -1.0f), mul2(x, c2)));
-        b.w[j] = pack2<T>(add2(mul2(y, c2), mul2(x, s2)));
+        // (a packed sum of packed products would become a product and a fused sum)
+        const float2 p = one_by_one(mul2(y, c2)), q = one_by_one(mul2(x, s2));
+        b.w[j] = Half16<T>::pack(__fadd_rn(p.x, q.x), __fadd_rn(p.y, q.y));
     }
 }
 
