@@ -193,7 +193,7 @@ def test_python_refusals(monkeypatch):
         with pytest.raises(TurboPiError):
             append(**kw)
     for kw in (dict(head_dim=60), dict(head_dim=96), dict(tokens=-1), dict(tokens=1.5), dict(dtype=torch.float32), dict(out=(g["k"],)),
-               dict(out=(g["k"], g["k"][:2])), dict(out=(f32, f32)), dict(out=7 * (g["k"],)), dict(out=(None, g["k"])), dict(cu=g["cu"][:1]), dict(tokens=2 ** 31)):
+               dict(out=(g["k"], g["k"][:2])), dict(out=(f32, f32)), dict(out=7 * (g["k"],)), dict(out=(None, g["k"])), dict(out=5), dict(head_dim=64.0), dict(cu=g["cu"][:1]), dict(tokens=2 ** 31)):
         with pytest.raises(TurboPiError):
             read(**kw)
     for kw in (dict(q=f32), dict(q=g["k"][:1, 0]), dict(q=_claims(torch.zeros(1, 3, 64, dtype=torch.bfloat16))), dict(q=_claims(torch.zeros(2, 4, 64, dtype=torch.bfloat16))),

@@ -14,8 +14,6 @@
 namespace tpb {
 namespace {
 
-constexpr int kWarps = 4;
-constexpr int kThreads = kWarps * 32;
 constexpr int kSlotUnits = 2;            // what a slot costs; an item besides, for queries, sums and the output: Src::kItemUnits
 constexpr float kLowest = -FLT_MAX;      // the least reference of a row with a key
 
@@ -28,6 +26,7 @@ struct DecodeParams {
     int tiles;                           // tiles of query heads per key head
     int rows;                            // rows of a tile that are used at most
     long long items;                     // (sequence, tile of query heads)
+    int workers, warps;                  // warps of the grid, and of a CTA
     int join_by_item;                    // joins[] has a place per item, else one per worker
     float scale2;                        // scale * log2 e, times the factor of the keys' scales
     float out_scale;                     // factor of the values' scales (Nvfp4)
@@ -56,6 +55,7 @@ struct Shape {
     static constexpr int kSlotBytes = Src::kQuant ? 2 * kKeys * (DP / 2 + DP / 16) : kKeys * DP * 2;     // tiles of keys and of values; rows of keys, or of values
     static constexpr int kSlots = 3;                        // of a warp's ring
     static constexpr int kCtas = Src::kQuant && DP < 256 ? 3 : 2;       // on an SM
+    static constexpr int kWarps = 4, kThreads = kWarps * 32;
     static constexpr int kLengths = 1024;                   // lengths kept in shared memory; with more sequences they are read where they lie
     static constexpr int kLanesRow = Src::kQuant ? DP / 32 : DP / 8;        // lanes that copy a row
     static constexpr int kRowsIter = 32 / kLanesRow;        // rows a warp copies at a time
@@ -86,7 +86,7 @@ struct Shape {
 template <typename S>
 struct Control {
     int lengths[S::kLengths];
-    float ml[kWarps][S::kRows][2];
+    float ml[S::kWarps][S::kRows][2];
 };
 
 // 4-bit tiles: sums pass through the slot whose tiles were used last
@@ -94,7 +94,7 @@ template <typename Src, int DP, int NT>
 constexpr int smem_bytes() {
     using S = Shape<Src, DP, NT>;
     static_assert(!Src::kQuant || S::kRows * S::kSlabPitch * 4 <= S::kSlotBytes, "");
-    return kWarps * S::kSlots * S::kSlotBytes + (Src::kQuant ? 0 : kWarps * S::kRows * S::kSlabPitch * 4) + static_cast<int>(sizeof(Control<S>));
+    return S::kWarps * S::kSlots * S::kSlotBytes + (Src::kQuant ? 0 : S::kWarps * S::kRows * S::kSlabPitch * 4) + static_cast<int>(sizeof(Control<S>));
 }
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
@@ -187,7 +187,7 @@ struct Place {
 // The line cut into pieces of equal cost, over the CTAs and a CTA's over its warps, the first ones of each getting a unit more.  A
 // slot belongs to the piece in which its first unit lies, behind the item's own; pieces are two units at least, so a warp between the
 // first and the last of an item always has a slot of it.  A line shorter than that for four warps is one warp's.
-template <int kItemUnits>
+template <int kItemUnits, int kWarps>
 struct Share {
     int total, ctas, each, more;         // `more` CTAs of each + 1 units, the others of each
     __device__ __forceinline__ void cut(int units, int grid) {
@@ -223,7 +223,8 @@ struct Share {
 template <typename Src, typename S, bool kWindow>
 struct Piece {
     Place<Src, S::kKeys, S::kLengths, kWindow> work;
-    Share<Src::kItemUnits> line;
+    Share<Src::kItemUnits, S::kWarps> line;
+    static constexpr int kWarps = S::kWarps;
     int slots;
     bool merged, whole_item;             // the CTA lies inside one item; it is the whole of it
 
@@ -398,7 +399,7 @@ __device__ __forceinline__ bool store_item(const DecodeParams& P, const Work& wo
         } else {                     // it begins here and ends with a later warp
             const int by = line.last_worker(work.units, work.n);
             P.joins[P.join_by_item ? item : worker] =
-                make_int4(item, static_cast<int>(part), by, by / kWarps != cta && line.ends_merged(work.units, work.n, by) ? 2 : 0);
+                make_int4(item, static_cast<int>(part), by, by / S::kWarps != cta && line.ends_merged(work.units, work.n, by) ? 2 : 0);
         }
     }
     return whole;
@@ -406,9 +407,9 @@ __device__ __forceinline__ bool store_item(const DecodeParams& P, const Work& wo
 
 // The sums of a CTA inside one item, each warp's where its ring was
 template <typename Src, typename T, typename S, int DP, int NT, typename Work, typename Line>
-__device__ __forceinline__ void merge_cta(const DecodeParams& P, const Work& work, const Line& line, uint8_t* smem, float (&ml)[kWarps][S::kRows][2], int cta,
+__device__ __forceinline__ void merge_cta(const DecodeParams& P, const Work& work, const Line& line, uint8_t* smem, float (&ml)[S::kWarps][S::kRows][2], int cta,
                                           int warp, int lane, bool from_start, bool whole, const float (&o)[DP / 16][NT][4], const float (&m)[NT][2], float (&l)[NT][2]) {
-    constexpr int kSlotBytes = S::kSlotBytes, kSlots = S::kSlots;
+    constexpr int kSlotBytes = S::kSlotBytes, kSlots = S::kSlots, kWarps = S::kWarps;
     const int heads = P.cache.kv_heads * P.tiles, D = P.cache.head_dim, worker = cta * kWarps;
     float* sums = reinterpret_cast<float*>(smem + warp * kSlots * kSlotBytes);
     __syncwarp();
@@ -433,7 +434,7 @@ __device__ __forceinline__ void merge_cta(const DecodeParams& P, const Work& wor
     const long long part = 2ll * kWarps * cta;
     const int rows = min(P.group - row0, S::kRows);
 #pragma unroll 4
-    for (int u = threadIdx.x; u < S::kRows * (DP / 4); u += kThreads) {
+    for (int u = threadIdx.x; u < S::kRows * (DP / 4); u += S::kThreads) {
         const int row = u / (DP / 4), col = u % (DP / 4) * 4;
         if (row >= rows || col >= D) continue;
         float M = -INFINITY, L = 0.0f;
@@ -472,7 +473,7 @@ template <typename T, int DP, int NT, bool kAligned, bool kWindow>
 __device__ __forceinline__ void attend_rows(const DecodeParams& P) {
     using Src = Rows16;
     using S = Shape<Src, DP, NT>;
-    constexpr int kSlotBytes = S::kSlotBytes, kSlots = S::kSlots;
+    constexpr int kSlotBytes = S::kSlotBytes, kSlots = S::kSlots, kWarps = S::kWarps;
     extern __shared__ __align__(128) uint8_t smem[];
     float* slab = reinterpret_cast<float*>(smem + kWarps * kSlots * kSlotBytes);
     auto* ctl = reinterpret_cast<Control<S>*>(slab + kWarps * S::kRows * S::kSlabPitch);
@@ -852,6 +853,7 @@ constexpr int kJoinThreads = 128;
 
 template <typename Src, typename T, int kLanes, int kLoads>
 __device__ __forceinline__ void join_parts(const DecodeParams& P) {
+    const int kWarps = Src::kQuant ? P.warps : 4;
     constexpr int kQuads = kJoinThreads / kLanes;
     __shared__ float4 sums[kLanes][kQuads];
     __shared__ float2 mls[kLanes][kQuads];
@@ -935,9 +937,8 @@ int decode_ctas(int per_sm) {
 // places for joins: an item's where the items are fewer than the workers, else a worker's
 struct DecodeScratch { size_t part_ml, part_o, bytes; };
 
-DecodeScratch decode_scratch(int ctas, int rows, int head_dim) {
+DecodeScratch decode_scratch(size_t workers, int rows, int head_dim) {
     DecodeScratch d;
-    const size_t workers = static_cast<size_t>(ctas) * kWarps;
     d.part_ml = workers * sizeof(int4);
     d.part_o = d.part_ml + 2 * workers * rows * 2 * sizeof(float);
     d.part_o = (d.part_o + 255) / 256 * 256;
@@ -970,7 +971,7 @@ int launch_decode(const DecodeParams& P, int ctas, cudaStream_t stream) {
     static_assert(Shape<Src, DP, NT>::kCtas * (smem + 1024) <= 228 * 1024, "shared memory of an SM");
     if (!configure<kernel>(smem, Src::kQuant)) return TPB200_ERR_CUDA;
     cudaLaunchAttribute attr;
-    const cudaLaunchConfig_t cfg = paged_config(static_cast<unsigned>(ctas), kThreads, smem, &attr, stream);
+    const cudaLaunchConfig_t cfg = paged_config(static_cast<unsigned>(ctas), Shape<Src, DP, NT>::kThreads, smem, &attr, stream);
     return cudaLaunchKernelEx(&cfg, kernel, P) == cudaSuccess ? TPB200_OK : TPB200_ERR_CUDA;
 }
 
@@ -987,7 +988,7 @@ struct DecodeCall {
 };
 
 // The checks of a call and its parameters, P->cache being set; group_rows: query heads that go through together
-int prepare_decode(const DecodeCall& a, int group_rows, int slot_keys, int item_units, int ctas, DecodeParams* out) {
+int prepare_decode(const DecodeCall& a, int group_rows, int slot_keys, int item_units, int ctas, int warps, DecodeParams* out) {
     DecodeParams& P = *out;
     TPB_REQUIRE(a.q && a.out, TPB200_ERR_NULL);
     TPB_REQUIRE((a.flags & ~TPB200_FLAG_PDL) == 0, TPB200_ERR_ENUM);
@@ -1022,14 +1023,16 @@ int prepare_decode(const DecodeCall& a, int group_rows, int slot_keys, int item_
     P.sinks = a.window > 0 ? std::min(a.sinks, positions) : 0;
     P.out_scale = 1.0f;
     TPB_REQUIRE(ctas >= 2, TPB200_ERR_CUDA);
-    const DecodeScratch d = decode_scratch(ctas, P.rows, P.cache.head_dim);
+    P.workers = ctas * warps;
+    P.warps = warps;
+    const DecodeScratch d = decode_scratch(P.workers, P.rows, P.cache.head_dim);
     TPB_REQUIRE(a.workspace != nullptr && a.workspace_bytes >= d.bytes, TPB200_ERR_WORKSPACE);
     TPB_REQUIRE(tpb_aligned16(a.workspace), TPB200_ERR_ALIGN);
     uint8_t* ws = static_cast<uint8_t*>(a.workspace);
     P.joins = reinterpret_cast<int4*>(ws);
     P.part_ml = reinterpret_cast<float*>(ws + d.part_ml);
     P.part_o = reinterpret_cast<float*>(ws + d.part_o);
-    P.join_by_item = P.items < static_cast<long long>(ctas) * kWarps;
+    P.join_by_item = P.items < P.workers;
     P.q = static_cast<const uint16_t*>(a.q);
     P.out = static_cast<uint16_t*>(a.out);
     return TPB200_OK;
@@ -1038,10 +1041,10 @@ int prepare_decode(const DecodeCall& a, int group_rows, int slot_keys, int item_
 // The second kernel, given for items of a hundred parts, of many and of few.  Its launch hides behind the first, which it waits for.  Where items are
 // few they have many parts each (eight lanes of eight loads, or 32), else few (two of four, so that the whole launch is resident at once).
 int launch_join(const DecodeParams& P, Kernel most_parts, Kernel many_parts, Kernel few_parts, int ctas, cudaStream_t stream) {
-    const bool few = P.items * 8 < static_cast<long long>(ctas) * kWarps, fewest = most_parts != nullptr && P.items * 32 < ctas;
+    const bool few = P.items * 8 < P.workers, fewest = most_parts != nullptr && P.items * 32 < ctas;
     const int quads = kJoinThreads / (fewest ? 32 : (few ? 8 : 2));
     cudaLaunchAttribute attr;
-    cudaLaunchConfig_t cfg = paged_config(static_cast<unsigned>(P.join_by_item ? P.items : ctas * kWarps - 1), kJoinThreads, 0, &attr, stream);
+    cudaLaunchConfig_t cfg = paged_config(static_cast<unsigned>(P.join_by_item ? P.items : P.workers - 1), kJoinThreads, 0, &attr, stream);
     cfg.gridDim.y = static_cast<unsigned>((P.rows * P.cache.head_dim / 4 + quads - 1) / quads);
     return cudaLaunchKernelEx(&cfg, fewest ? most_parts : (few ? many_parts : few_parts), P) == cudaSuccess ? TPB200_OK : TPB200_ERR_CUDA;
 }

@@ -1028,20 +1028,28 @@ def paged_append_nvfp4(k, v, k_pages, v_pages, table, cu, lengths, q=None, cos=N
     return q_out
 
 
-def _read_rows(what, view, heads, D, dtype, cu, tokens, out, device):
+def _two_rows(what, out):
+    """out of paged_read: (k, v), or (None, None)."""
+    try:
+        k, v = (None, None) if out is None else out
+    except (TypeError, ValueError):
+        raise TurboPiError(f"{what}: out is a pair of tensors") from None
+    if out is not None and not (torch.is_tensor(k) and torch.is_tensor(v)):
+        raise TurboPiError(f"{what}: out is a pair of tensors")
+    return k, v
+
+
+def _read_rows(what, view, heads, D, dtype, cu, tokens, k, v, device):
     """The rest of paged_read and paged_read_nvfp4."""
     if cu.dtype != torch.int32 or cu.dim() != 1 or cu.numel() != view.seqs + 1 or not cu.is_contiguous():
         raise TurboPiError(f"{what}: cu must be contiguous int32 [sequences + 1]")
     try:
         tokens = operator.index(tokens)
-        k, v = (None, None) if out is None else out
-    except (TypeError, ValueError):
-        raise TurboPiError(f"{what}: tokens is the number of rows, out a pair of tensors") from None
+    except TypeError:
+        tokens = -1
     if tokens < 0:
-        raise TurboPiError(f"{what}: tokens is the number of rows, out a pair of tensors")
+        raise TurboPiError(f"{what}: tokens is the number of rows")
     _counts(what, tokens)
-    if out is not None and not (torch.is_tensor(k) and torch.is_tensor(v)):
-        raise TurboPiError(f"{what}: tokens is the number of rows, out a pair of tensors")
     _cuda(cu, k, v)
     k, v = _new_rows(what, "k", k, tokens, heads, D, dtype, device), _new_rows(what, "v", v, tokens, heads, D, dtype, device)
     return k, v, _lib.PagedRows(k=_ptr(k), v=_ptr(v), dtype=_HALF[dtype], k_stride=_strides(k), v_stride=_strides(v), cu=_ptr(cu),
@@ -1052,13 +1060,12 @@ def paged_read(k_pages, v_pages, table, cu, lengths, tokens, out=None):
     """(k, v) [tokens, Hk, D] of the pages' type: tokens of a cache one sequence behind the other, as `packed_attention` takes them (cu is
     then its cu_keys).  Sequence s gives rows [cu[s], cu[s + 1]) its last cu[s + 1] - cu[s] positions, up to lengths[s] - 1.  Rows behind
     cu[S] are left as they are; a row without a page gets zeros and is reported by tpb200_device_error().  out: (k, v) to write."""
-    k, v = (None, None) if out is None or len(out) != 2 else out
-    done = (_lib._native or _lib.native()).paged_read(k_pages, v_pages, table, cu, lengths, tokens, k, v, _flags.value) \
-        if out is None or len(out) == 2 else None
+    k, v = _two_rows("paged_read", out)
+    done = (_lib._native or _lib.native()).paged_read(k_pages, v_pages, table, cu, lengths, tokens, k, v, _flags.value)
     if done is not None:
         return _result(done, "tpb200_paged_read")
     view = _paged_view("paged_read", k_pages, v_pages, table, lengths)
-    k, v, rows = _read_rows("paged_read", view, view.kv_heads, view.head_dim, k_pages.dtype, cu, tokens, out, k_pages.device)
+    k, v, rows = _read_rows("paged_read", view, view.kv_heads, view.head_dim, k_pages.dtype, cu, tokens, k, v, k_pages.device)
     _one_device("paged_read", k_pages, cu, k, v)
     _lib.check(_run(k_pages, _lib.load().tpb200_paged_read, view, rows), "tpb200_paged_read")
     return k, v
@@ -1067,15 +1074,19 @@ def paged_read(k_pages, v_pages, table, cu, lengths, tokens, out=None):
 def paged_read_nvfp4(k_pages, v_pages, table, cu, lengths, head_dim, tokens, dtype=torch.bfloat16, out=None, k_scale=1.0, v_scale=1.0):
     """`paged_read` out of 4-bit pages: the values that are held, in bf16 or fp16, which hold them exactly unless k_scale or v_scale
     takes them out of the type's range."""
-    k, v = (None, None) if out is None or len(out) != 2 else out
+    k, v = _two_rows("paged_read_nvfp4", out)
     done = (_lib._native or _lib.native()).paged_read_nvfp4(k_pages, v_pages, table, cu, lengths, head_dim, tokens, dtype, k, v, k_scale,
-                                                            v_scale, _flags.value) if out is None or len(out) == 2 else None
+                                                            v_scale, _flags.value)
     if done is not None:
         return _result(done, "tpb200_paged_read_nvfp4")
     if dtype not in _HALF:
         raise TurboPiError("paged_read_nvfp4: bf16 or fp16")
+    try:
+        head_dim = operator.index(head_dim)
+    except TypeError:
+        raise TurboPiError("paged_read_nvfp4: head_dim must be a multiple of 8 up to 256") from None
     view = _nvfp4_view("paged_read_nvfp4", k_pages, v_pages, table, lengths, head_dim, k_scale, v_scale)
-    k, v, rows = _read_rows("paged_read_nvfp4", view, view.kv_heads, head_dim, dtype, cu, tokens, out, k_pages.device)
+    k, v, rows = _read_rows("paged_read_nvfp4", view, view.kv_heads, head_dim, dtype, cu, tokens, k, v, k_pages.device)
     _one_device("paged_read_nvfp4", k_pages, cu, k, v)
     _lib.check(_run(k_pages, _lib.load().tpb200_paged_read_nvfp4, view, rows), "tpb200_paged_read_nvfp4")
     return k, v
