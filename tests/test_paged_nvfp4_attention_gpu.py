@@ -182,6 +182,17 @@ def test_factors_and_large_queries(cuda_device, dtype):
         p.check(out, 1e-30)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_scales_and_queries_of_nothing(cuda_device, dtype):
+    """A scale of zero, the least one, queries of zero and subnormal ones: the mean of what is seen, under masks too."""
+    p = _Problem([300, 17, 1000, 1], 8, 2, 64, 16, dtype, cuda_device, seed=11)
+    p.q[0] = 0
+    p.q[1] *= torch.finfo(dtype).smallest_normal / 8
+    for scale in (0.0, 1e-38, -1e-38, 1e-42, 0.1, -0.1):
+        p.check(p.run(scale), scale)
+        p.check(p.run(scale, window=20, sinks=3), scale, 20, 3)
+
+
 def test_values_that_are_not_numbers(cuda_device):
     """A block of values with a NaN scale that is visible reaches its 16 columns, in its head and sequence alone; keys their whole head."""
     p = _Problem([300, 200], 4, 2, 128, 16, torch.bfloat16, cuda_device, seed=4)

@@ -425,8 +425,13 @@ bool read_rows(const at::Tensor& pages, int64_t heads, int64_t D, at::ScalarType
         (k.has_value() && (!rows(*k, dev, tokens, heads, D, type) || !rows(*v, dev, tokens, heads, D, type)))) {
         return false;
     }
-    for (int i = 0; i < 2; ++i) {
-        y[i] = k.has_value() ? *(i == 0 ? k : v) : at::empty({tokens, heads, D}, pages.options().dtype(type));
+    if (k.has_value()) {
+        y[0] = *k;
+        y[1] = *v;
+    } else {                                              // one allocation for both
+        const at::Tensor both = at::empty({2, tokens, heads, D}, pages.options().dtype(type));
+        y[0] = both.select(0, 0);
+        y[1] = both.select(0, 1);
     }
     a.k = y[0].data_ptr();
     a.v = y[1].data_ptr();

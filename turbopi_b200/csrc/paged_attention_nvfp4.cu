@@ -209,7 +209,8 @@ __device__ __forceinline__ void attend_tiles(const DecodeParams& P) {
     int unknown = slots;                 // slots from there on
     int page_id = -1;                    // of this lane's tile of the look-up that begins at `next`
     int known = 0, at = 0;               // slots of the look-up the loads take their tiles from, and which one is next
-    long long tile_at = -1;              // this lane's tile of it: byte offset, -1: not there, or no key of it is seen
+    long long tile_at = 0;               // this lane's tile of it: byte offset
+    uint32_t here = 0;                   // tiles of it that are there and have a key that is seen; the others are not read
     uint32_t gone = 0;                   // tiles of it with a key that is seen, and without a page in the pool
     uint32_t absent = 0;                 // the same of the slots in the ring, four bits each
     auto ahead = [&]() { return min(unknown, min(kAhead, (next.n - next.ci + next.step - 1) / next.step)); };
@@ -239,10 +240,11 @@ __device__ __forceinline__ void attend_tiles(const DecodeParams& P) {
     auto look_up = [&]() {               // the tiles from `next` on; page ids of those behind them are asked for
         int key = 0;
         const bool in = own_tile(key), there = in && static_cast<unsigned>(page_id) < static_cast<unsigned>(P.cache.num_pages);
-        tile_at = -1;
+        tile_at = 0;
         if (there) {
             tile_at = page_id * P.cache.page_stride + key % P.cache.page_size / 16 * P.cache.row_stride + next.h / P.tiles * P.cache.head_stride;
         }
+        here = __ballot_sync(0xffffffffu, there);
         gone = __ballot_sync(0xffffffffu, in && !there);
         if (gone != 0) record_error(kErrPagedIndex);
         if (next.ci == 0) ask_queries(next);
@@ -268,31 +270,30 @@ __device__ __forceinline__ void attend_tiles(const DecodeParams& P) {
         const uint32_t to = smem_u32(ring) + slot * S::kSlotBytes;
         constexpr int kIters = kCodes / 512, kTileIters = kIters / kBlocks;
         static_assert(S::kRowsIter * kTileIters == 16, "");
+        const uint32_t there = here >> (at * kBlocks);
         const uint8_t *k = k_pages, *v = v_pages;
-        bool in = false;
+        int bytes = 0;
 #pragma unroll
         for (int i = 0; i < kIters; ++i) {
             if (i % kTileIters == 0) {
                 const long long off = __shfl_sync(0xffffffffu, tile_at, at * kBlocks + i / kTileIters);
-                in = off >= 0 && (kFull || lane_col < groups);
-                k = k_pages + (in ? off + from_lane : 0);
-                v = v_pages + (in ? off + from_lane : 0);
+                bytes = (there >> (i / kTileIters)) & 1 && (kFull || lane_col < groups) ? 16 : 0;
+                k = k_pages + off + (kFull || bytes > 0 ? from_lane : 0);
+                v = v_pages + off + (kFull || bytes > 0 ? from_lane : 0);
             }
             // rows further on by kRowsIter stand in the same place of a later line: code_at repeats every eight rows
             const uint32_t row_at = S::kRowsIter % 8 == 0 ? to_lane + i * 512 : code_at<DP>(i * S::kRowsIter + lane_row, lane_col);
-            cp_async16(to + row_at, k, in ? 16 : 0);
-            cp_async16(to + kCodes + row_at, v, in ? 16 : 0);
-            if (in) {
-                k += step;
-                v += step;
-            }
+            const int on = i % kTileIters * (kFull || bytes > 0 ? step : 0);
+            cp_async16(to + row_at, k + on, bytes);
+            cp_async16(to + kCodes + row_at, v + on, bytes);
         }
 #pragma unroll
         for (int i = 0; i < kScaleCopies; ++i) {         // lanes 0 to 15: of keys
-            const long long off = __shfl_sync(0xffffffffu, tile_at, at * kBlocks + i * (256 / DP) + scale_tile);
-            in = off >= 0 && (kFull || scale_chunk < 2 * groups);
-            const uint8_t* from = lane < 16 ? k_pages : v_pages;
-            cp_async16(to + 2 * kCodes + (lane >> 4) * kScales + i * 256 + (lane & 15) * 16, in ? from + off + 256 * groups + scale_chunk * 16 : from, in ? 16 : 0);
+            const int tile = i * (256 / DP) + scale_tile;
+            const long long off = __shfl_sync(0xffffffffu, tile_at, at * kBlocks + tile);
+            const bool in = (there >> tile) & 1 && (kFull || scale_chunk < 2 * groups);
+            cp_async16(to + 2 * kCodes + (lane >> 4) * kScales + i * 256 + (lane & 15) * 16,
+                       (lane < 16 ? k_pages : v_pages) + off + (kFull || in ? 256 * groups + scale_chunk * 16 : 0), in ? 16 : 0);
         }
         absent = (absent & ~(15u << (4 * slot))) | ((gone >> (at * kBlocks)) & ((1u << kBlocks) - 1)) << (4 * slot);
         ++at;
@@ -328,7 +329,16 @@ __device__ __forceinline__ void attend_tiles(const DecodeParams& P) {
                 qf[kk][t][0] = x.x;
                 qf[kk][t][1] = x.y;
             }
-            scale2[t][0] = scale2[t][1] = P.scale2;
+            if (P.scale2 < 0.0f) {       // the sign goes into the queries: scores are compared before they are scaled
+#pragma unroll
+                for (int kk = 0; kk < DP / 16; ++kk) {
+                    qf[kk][t][0] ^= 0x80008000u;
+                    qf[kk][t][1] ^= 0x80008000u;
+                }
+            }
+            constexpr float kLeast = 1.1754944e-38f;     // no scale at all would lose the mask
+            const float size = fmaxf(fabsf(P.scale2), kLeast);
+            scale2[t][0] = scale2[t][1] = size;
             if constexpr (std::is_same<T, __nv_bfloat16>::value) {
                 // fp16 queries are taken as they are; bf16 ones are divided by the power of two of their head's largest, which moves into the scale (a
                 // query 2^-15 of the largest and below is rounded to a multiple of 2^-24 of it)
@@ -350,7 +360,8 @@ __device__ __forceinline__ void attend_tiles(const DecodeParams& P) {
                     }
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    scale2[t][j] = P.scale2 * __uint_as_float(static_cast<uint32_t>(__shfl_sync(0xffffffffu, e, ((lane & 3) * 2 + j) * 4)) << 23);
+                    const uint32_t power = static_cast<uint32_t>(__shfl_sync(0xffffffffu, e, ((lane & 3) * 2 + j) * 4)) << 23;
+                    scale2[t][j] = fmaxf(size * __uint_as_float(power), kLeast);
                 }
             }
         }
@@ -386,12 +397,6 @@ __device__ __forceinline__ void attend_tiles(const DecodeParams& P) {
         // stay below 2^8), so the maximum crosses the lanes hardly ever.  A slot with a key that is seen has a finite reference, whatever the
         // score: one of -infinity at the end means that there was no key.
         float lowest = kLowest;
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int b = 0; b < kBlocks; ++b)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) sc[b][n][j] *= scale2[n][j & 1];
         if (edge || off != 0) {
             bool any = false;
 #pragma unroll
@@ -419,12 +424,14 @@ __device__ __forceinline__ void attend_tiles(const DecodeParams& P) {
         bool raise = false;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            top[n][0] = top[n][1] = lowest;
+            top[n][0] = top[n][1] = -INFINITY;
 #pragma unroll
             for (int b = 0; b < kBlocks; ++b) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) top[n][j & 1] = fmaxf(top[n][j & 1], sc[b][n][j]);
             }
+#pragma unroll
+            for (int j = 0; j < 2; ++j) top[n][j] = fmaxf(top[n][j] * scale2[n][j], lowest);
             raise = raise || top[n][0] > m[n][0] + 8.0f || top[n][1] > m[n][1] + 8.0f;
         }
         if (__any_sync(0xffffffffu, raise)) {
@@ -455,7 +462,7 @@ __device__ __forceinline__ void attend_tiles(const DecodeParams& P) {
             for (int b = 0; b < kBlocks; ++b) {
                 float w[4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) w[j] = ex2(sc[b][n][j] - (j & 1 ? b1 : b0));
+                for (int j = 0; j < 4; ++j) w[j] = ex2(fmaf(sc[b][n][j], scale2[n][j & 1], j & 1 ? -b1 : -b0));
                 l[n][0] += w[0] + w[2];
                 l[n][1] += w[1] + w[3];
                 p[b][n][0] = transpose8x8(Half16<__half>::pack(w[0], w[1]));
