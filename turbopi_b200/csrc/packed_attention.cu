@@ -40,6 +40,10 @@
 // sequences of 100 tokens gain 7 %, those of 1 to 1200 lose 6 %); pairs of CTAs on one product (cta_group::2, M = 256: 2.47 ms, the single
 // sequence 250 us, each hand-over crosses the cluster).
 //
+// Sliding windows (kWindow): tiles without a visible pair are not visited.  One sequence of 8191 tokens, 8 on 1 heads of 256, window 1024, four sinks: 85.8 us
+// (all keys: 197), 9 tiles a CTA for 8.03 of visible pairs; 512 CTAs of 21 us, 5 of them look-up, first loads and output, in four waves.  24 ragged sequences of 1 to 1200, 16 on 4 heads
+// of 64, window 200: 25.9; four long ones, 32 on 8 of 128, window 1500: 280, 0.55 of the measured bf16 burst rate.  With whole tiles left out instead of keys: 93, 27.8, 291.
+//
 // What may stand in masked places does not matter: scores are selected, not biased.  Rows of V behind a sequence's end are zeroed in
 // shared memory, and in tiles that hold masked pairs V is searched for infinities and NaN (weight 0 times those would be NaN): they are
 // taken out and added to the rows that do see them at the end.
@@ -898,7 +902,8 @@ int attend(const tpb200_packed_attention_args* a, int window, int sinks, tpb200_
     // Up to head size 128, two row tiles per CTA where sequences are long (each unit of K and V serves both), else one, and two CTAs on an
     // SM: half the rows to fill up, and one's loads and output beside the other's products.  The border is where the two meet on average:
     // 24 sequences of 100 / 8 of 1536, 16 heads of 64: 13.5 us with one, 18.1 with two / 91.6, 92.6; 16 heads of 128: 21.0, 25.2 / 129, 118.
-    // Batches of sequences alike; not measured where lengths differ much or queries are few beside the keys.
+    // Batches of sequences alike; not measured where lengths differ much or queries are few beside the keys.  With a window its keys count, and the border for
+    // heads of 128 is 1000: windows of 200 / 400 / 800 / 1500, 4000 tokens, 32 on 8 heads, 95 / 106 / 138 / 194 us with one, 97 / 121 / 149 / 187 with two.
     const long long keys = hides ? std::min<long long>(a->k_tokens, (static_cast<long long>(window) + P.sinks) * a->seqs) : a->k_tokens;
     const bool two = DP <= 128 && keys > (DP == 64 || hides ? 1000ll : 200ll) * a->seqs;
     // no more tiles than whole ones and a ragged one per sequence

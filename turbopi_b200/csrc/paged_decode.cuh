@@ -45,6 +45,7 @@ struct Rows16 {
 };
 struct Nvfp4 {
     static constexpr bool kQuant = true;
+    // 96 ragged sequences 40.3 us, with 4: 42.7, 2: 52.5, 8: 41; the windows of 64 like ones 39.1, 37.9, -, 40.1
     static constexpr int kItemUnits = 6;
 };
 

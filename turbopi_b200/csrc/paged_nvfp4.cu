@@ -4,7 +4,9 @@
 //            s = e4m3(max |x| / 6), code = e2m1(x / s).  Queries are rotated beside them.  One launch.
 //   read     rows of the last tokens of each sequence, one sequence behind the other: values out of 4 bits, or copies out of 16.
 //
-// Both are bound by HBM for prompts and by the chain offsets -> length -> page id -> row for a decode step.
+// A decode step is the chain offsets -> length -> page id -> row.  Prompts, calls in a CUDA graph: 14.4 k tokens of six sequences, 32 on 8 heads of 128, turned and
+// written (312 MB) 68 us = 4.6 TB/s: what a block waits for (its look-up, then each token's loads) and 70 instructions for 16 values; keys and values alone 26.  The
+// same tokens into 16 bits (354 MB): 63.  25 k tokens of 8 heads of 128 read back (132 MB) 26.6 us = 5.0 TB/s, 0.76 of the measured copy rate.
 #include <algorithm>
 #include <type_traits>
 
