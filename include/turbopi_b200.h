@@ -498,8 +498,8 @@ typedef struct {
 int tpb200_paged_append(const tpb200_paged_append_args* args, tpb200_stream_t stream);
 
 /* One layer of a paged cache held in 4 bits (NVFP4).  With G = ceil(head_dim / 32), a page has page_size / 16 tiles for each key head, a tile of 16
- * tokens is 288 G bytes: 16 rows of 16 G bytes of E2M1 codes (value 2 i in the low half of byte i, 2 i + 1 in the high half, zeros behind
- * head_dim), then 16 rows of 2 G E4M3 scales, one for every 16 values.  A key is k_scale * scale * code, a value v_scale * scale * code; k_scale and
+ * tokens is 288 G bytes: 16 rows of 16 G bytes of E2M1 codes (value 2 i in the low half of byte i, 2 i + 1 in the high half), then 16 rows of
+ * 2 G E4M3 scales, one for every 16 values; codes and scales of values behind head_dim are zeros.  A key is k_scale * scale * code, a value v_scale * scale * code; k_scale and
  * v_scale are powers of two from 2^-63 to 2^64.  scale * code is exact in fp16 and bf16.  page_size is a multiple of 16; the strides are in bytes,
  * multiples of 16: from page to page, from head to head, from tile to tile.  Table and lengths as in tpb200_paged_cache. */
 typedef struct {
