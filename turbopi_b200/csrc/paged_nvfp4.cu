@@ -5,7 +5,7 @@
 //   read     rows of the last tokens of each sequence, one sequence behind the other: values out of 4 bits, or copies out of 16.
 //
 // A decode step is the chain offsets -> length -> page id -> row.  Prompts, calls in a CUDA graph: 14.4 k tokens of six sequences, 32 on 8 heads of 128, turned and
-// written (312 MB) 68 us = 4.6 TB/s: what a block waits for (its look-up, then each token's loads) and 70 instructions for 16 values; keys and values alone 26.  The
+// written (312 MB) 66 us = 4.7 TB/s: what a block waits for (its look-up, then each token's loads) and 70 instructions for 16 values; keys and values alone 26.  The
 // same tokens into 16 bits (354 MB): 63.  25 k tokens of 8 heads of 128 read back (132 MB) 26.6 us = 5.0 TB/s, 0.76 of the measured copy rate.
 #include <algorithm>
 #include <type_traits>
@@ -19,7 +19,7 @@ constexpr int kAppendThreads = 256;      // of a block at most
 constexpr int kPairThreads = 256, kPairBlocks = 4;
 constexpr int kReadThreads = 256;
 constexpr int kAppendLoads = 1;          // tokens whose unit a thread has in flight
-constexpr int kAppendTokens = 4;         // of a block at most
+constexpr int kAppendTokens = 6;         // of a block at most
 constexpr int kReadLoads = 4;
 constexpr int kReadTokens = 16;
 
@@ -557,11 +557,12 @@ extern "C" int tpb200_paged_append_nvfp4(const tpb200_paged_append_nvfp4_args* a
     TPB_REQUIRE(units_q + 2 * units_kv <= (1 << 24), TPB200_ERR_SHAPE);
     P.units_q = static_cast<int>(units_q);
     P.units_kv = static_cast<int>(units_kv);
-    // four tokens share a block's look-up, fewer where that would leave SMs without a block
-    P.tokens_per_block = std::max(1, std::min(kAppendTokens, a->tokens / 444));
+    // Six tokens share a block's look-up, of other head sizes four, fewer where that would leave SMs without a block (the prompts of six sequences 66 us, with four
+    // 68, eight 73; heads of 72, 4800 tokens, 37 with four, 46 with six)
+    const bool pairs = D % 32 == 0;
+    P.tokens_per_block = std::max(1, std::min(pairs ? kAppendTokens : kAppendTokens - 2, a->tokens / 444));
     const unsigned blocks = static_cast<unsigned>((a->tokens - 1) / P.tokens_per_block + 1);
     const bool bf = a->dtype == TPB200_BF16;
-    const bool pairs = D % 32 == 0;
     auto pick = [&](auto type) {
         using T = decltype(type);
         return pairs ? append_pairs_kernel<T> : (V == 8 ? append_blocks_kernel<T, 8> : append_blocks_kernel<T, 4>);
