@@ -542,7 +542,8 @@ typedef struct {
 int tpb200_paged_append_nvfp4(const tpb200_paged_append_nvfp4_args* args, tpb200_stream_t stream);
 
 /* Tokens out of a cache, one sequence behind the other, as packed attention takes them: rows [cu[s], cu[s + 1]) of k and v get sequence s's last
- * cu[s + 1] - cu[s] positions, the last one lengths[s] - 1.  Rows behind cu[seqs] are left alone; a row without a place (501) gets zeros.  The 16-bit form
+ * cu[s + 1] - cu[s] positions, the last one lengths[s] - 1.  Rows behind cu[seqs] are left alone; a row without a place (501) gets zeros; offsets past
+ * `tokens` name rows that are not there (501, the others are read).  The 16-bit form
  * copies, the 4-bit one gives the values that are held, in `dtype`, exactly where k_scale or v_scale does not take them out of its range. */
 typedef struct {
     void* k; void* v; int dtype;

@@ -352,6 +352,7 @@ __global__ void __launch_bounds__(kReadThreads) read_kernel(const __grid_constan
     pdl_launch_dependents();
     const int t0 = blockIdx.x * P.tokens_per_block;
     const int count = min(P.tokens_per_block, P.tokens - t0);
+    const int named = blockIdx.x == 0 && threadIdx.x == 0 ? P.cu[P.cache.seqs] : 0;       // rows that the offsets name
     place_tokens<kTiles, kReadTokens>(P.cache, P.cu, t0, count, 0, seq, position, row_at);
     constexpr int kColumns = kTiles ? 16 : 8;
     const int D = P.cache.head_dim, per_row = (D + kColumns - 1) / kColumns, groups = (D + 31) / 32;
@@ -413,6 +414,8 @@ __global__ void __launch_bounds__(kReadThreads) read_kernel(const __grid_constan
             }
         }
     }
+    // A captured call whose offsets have grown: what a caller goes on to use lacks tokens
+    if (named > P.tokens) record_error(kErrPagedIndex);
 }
 
 // a block's threads for `units` a token: as few passes over them as `most` threads allow, and those even

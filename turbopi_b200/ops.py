@@ -1059,7 +1059,9 @@ def _read_rows(what, view, heads, D, dtype, cu, tokens, k, v, device):
 def paged_read(k_pages, v_pages, table, cu, lengths, tokens, out=None):
     """(k, v) [tokens, Hk, D] of the pages' type: tokens of a cache one sequence behind the other, as `packed_attention` takes them (cu is
     then its cu_keys).  Sequence s gives rows [cu[s], cu[s + 1]) its last cu[s + 1] - cu[s] positions, up to lengths[s] - 1.  Rows behind
-    cu[S] are left as they are; a row without a page gets zeros and is reported by tpb200_device_error().  out: (k, v) to write."""
+    cu[S] are left as they are; a row without a page gets zeros and is reported by tpb200_device_error().  out: (k, v) to write.
+    A captured call follows table, cu and lengths within its `tokens` rows; a cu[S] beyond them is reported, and the rows there are read:
+    capture it with as many rows as the sequences may come to hold."""
     k, v = _two_rows("paged_read", out)
     done = (_lib._native or _lib.native()).paged_read(k_pages, v_pages, table, cu, lengths, tokens, k, v, _flags.value)
     if done is not None:

@@ -317,7 +317,9 @@ class PagedCache:
 
     def read(self, layer, batch, dtype=torch.bfloat16, out=None):
         """(k, v) [batch.keys, kv_heads, head_dim]: all tokens of the batch's sequences, one sequence behind the other (offsets: batch.cu_keys),
-        by ops.paged_read or paged_read_nvfp4.  dtype: of rows read out of 4 bits, else the pages' own.  out: (k, v) to write."""
+        by ops.paged_read or paged_read_nvfp4.  dtype: of rows read out of 4 bits, else the pages' own.  out: (k, v) to write.
+        The number of rows is the host's: a captured call keeps that of its capture.  Replayed for a batch that has grown since (extend with
+        out=) it lacks the last tokens, which tpb200_device_error() reports; capture ops.paged_read with room for them instead."""
         self._current(batch)
         if self.nvfp4:
             return ops.paged_read_nvfp4(*self.layer(layer), batch.table, batch.cu_keys, batch.lengths, self.head_dim, batch.keys, dtype=dtype,
@@ -326,7 +328,8 @@ class PagedCache:
 
     def prompt_attention(self, layer, batch, q, scale, out=None, window=None, sinks=0):
         """Causal attention of the batch's new tokens, q [batch.tokens, heads, head_dim], over all tokens of their sequences (or a window), new
-        and cached, as the cache holds them: `read`, then ops.packed_attention.  Append the new tokens first."""
+        and cached, as the cache holds them: `read`, then ops.packed_attention.  Append the new tokens first.  A captured call holds for as many
+        keys as its capture had, as `read` does; `attention` follows its batch."""
         if q.shape[0] != batch.tokens:
             raise TurboPiError(f"PagedCache: {q.shape[0]} rows for {batch.tokens} new tokens")
         k, v = self.read(layer, batch, dtype=q.dtype)
