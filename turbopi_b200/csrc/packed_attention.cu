@@ -167,6 +167,10 @@ __device__ __forceinline__ void tmem_ld_wait_for(uint32_t* r) {
                  :
                  : "memory");
 }
+__device__ __forceinline__ void tmem_st_x8(uint32_t addr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
+                 "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
+}
 __device__ __forceinline__ void tmem_st_done() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -685,23 +689,51 @@ __global__ void __launch_bounds__(Layout<DP, R>::kThreads, Layout<DP, R>::kCtas)
             // P = 2^(scale2 S - m), its row sum (before rounding), rounded pairs into the columns S was in
             const uint64_t scale = pair(P.scale2, P.scale2), minus = pair(Half16<T>::kLift - base, Half16<T>::kLift - base);
             uint64_t sum[2] = {pair(0.0f, 0.0f), pair(0.0f, 0.0f)};
+            if (__builtin_expect(__reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(base))) > __float_as_uint(kFar), 0)) {
+                // scores rounded as their reference was; the other rows' stay what they are.  (In local memory, a few at a time: in place the other
+                // branch kept fewer registers, and the ragged prompts took 27.3 us.)
+                float y[kTile];
+                const float up = Half16<T>::kLift - base;
 #pragma unroll
-            for (int c = 0; c < kTile / 2; c += 32) {
-                uint32_t p[32];
-#pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    float a, b;
-                    unpair(fma2(pair(__uint_as_float(s[2 * (c + i)]), __uint_as_float(s[2 * (c + i) + 1])), scale, minus), a, b);
-                    a = ex2(a);
-                    b = ex2(b);
-                    sum[i & 1] = add2(sum[i & 1], pair(a, b));
-                    p[i] = Half16<T>::pack(a, b);
+                for (int i = 0; i < kTile; ++i) {
+                    const float z = __uint_as_float(s[i]);
+                    y[i] = fabsf(base) > kFar ? __fadd_rn(__fmul_rn(z, P.scale2), up) : fmaf(z, P.scale2, up);
                 }
-                tmem_st_x32(p_at + c, p);
-                tmem_st_done();
-                tc::fence_before_thread_sync();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&ctl->p_ready[x][c / 32]);
+#pragma unroll 1
+                for (int c = 0; c < kTile / 2; c += 8) {
+                    uint32_t p[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const float a = ex2(y[2 * (c + i)]), b = ex2(y[2 * (c + i) + 1]);
+                        sum[i & 1] = add2(sum[i & 1], pair(a, b));
+                        p[i] = Half16<T>::pack(a, b);
+                    }
+                    tmem_st_x8(p_at + c, p);
+                    tmem_st_done();
+                    if (c % 32 != 24) continue;
+                    tc::fence_before_thread_sync();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&ctl->p_ready[x][c / 32]);
+                }
+            } else {
+#pragma unroll
+                for (int c = 0; c < kTile / 2; c += 32) {
+                    uint32_t p[32];
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        float a, b;
+                        unpair(fma2(pair(__uint_as_float(s[2 * (c + i)]), __uint_as_float(s[2 * (c + i) + 1])), scale, minus), a, b);
+                        a = ex2(a);
+                        b = ex2(b);
+                        sum[i & 1] = add2(sum[i & 1], pair(a, b));
+                        p[i] = Half16<T>::pack(a, b);
+                    }
+                    tmem_st_x32(p_at + c, p);
+                    tmem_st_done();
+                    tc::fence_before_thread_sync();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&ctl->p_ready[x][c / 32]);
+                }
             }
             float a, b;
             unpair(add2(sum[0], sum[1]), a, b);

@@ -384,6 +384,7 @@ __device__ __forceinline__ void attend_tiles(const DecodeParams& P) {
 
     const Lane<DP, kFull> of(lane, groups);
     int parts = 0;                       // partial results this warp has left
+    bool far = false;                    // a reference whose rounding error is no small part of one
     const int first_ci = work.ci;
     bool from_start = first_ci == 0;
     if (slots > 0) ask_ids();
@@ -467,17 +468,35 @@ __device__ __forceinline__ void attend_tiles(const DecodeParams& P) {
                     m[n][j] = now;
                 }
             }
+            far = false;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) far = far || fabsf(m[n][0]) > kFar || fabsf(m[n][1]) > kFar;
+            far = __any_sync(0xffffffffu, far);
         }
         // ---- weights, rounded to fp16 for the second product (their sum is that of the unrounded ones), transposed into its B operand
         uint32_t p[kBlocks][NT][2];
+        auto exponents = [&](auto of_score) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const float up[2] = {Half16<__half>::kLift - (m[n][0] == -INFINITY ? 0.0f : m[n][0]), Half16<__half>::kLift - (m[n][1] == -INFINITY ? 0.0f : m[n][1])};
+#pragma unroll
+                for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) sc[b][n][j] = of_score(sc[b][n][j], scale2[n][j & 1], up[j & 1], m[n][j & 1]);
+            }
+        };
+        if (__builtin_expect(far, 0)) {  // scores rounded as their reference was; the other heads' stay what they are
+            exponents([](float x, float f, float up, float ref) { return fabsf(ref) > kFar ? __fadd_rn(__fmul_rn(x, f), up) : fmaf(x, f, up); });
+        } else {
+            exponents([](float x, float f, float up, float) { return fmaf(x, f, up); });
+        }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            const float b0 = (m[n][0] == -INFINITY ? 0.0f : m[n][0]) - Half16<__half>::kLift, b1 = (m[n][1] == -INFINITY ? 0.0f : m[n][1]) - Half16<__half>::kLift;
 #pragma unroll
             for (int b = 0; b < kBlocks; ++b) {
                 float w[4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) w[j] = ex2(fmaf(sc[b][n][j], scale2[n][j & 1], j & 1 ? -b1 : -b0));
+                for (int j = 0; j < 4; ++j) w[j] = ex2(sc[b][n][j]);
                 l[n][0] += w[0] + w[2];
                 l[n][1] += w[1] + w[3];
                 p[b][n][0] = transpose8x8(Half16<__half>::pack(w[0], w[1]));
