@@ -352,8 +352,8 @@ __device__ __forceinline__ void attend_tiles(const DecodeParams& P) {
                 }
             }
             constexpr float kLeast = 1.1754944e-38f;     // no scale at all would lose the mask
-            const float size = fmaxf(fabsf(P.scale2), kLeast);
-            scale2[t][0] = scale2[t][1] = size;
+            const float size = fabsf(P.scale2);
+            scale2[t][0] = scale2[t][1] = fmaxf(size, kLeast);
             if constexpr (std::is_same<T, __nv_bfloat16>::value) {
                 // fp16 queries are taken as they are; bf16 ones are divided by the power of two of their head's largest, which moves into the scale (a
                 // query 2^-15 of the largest and below is rounded to a multiple of 2^-24 of it)
@@ -376,7 +376,9 @@ __device__ __forceinline__ void attend_tiles(const DecodeParams& P) {
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     const uint32_t power = static_cast<uint32_t>(__shfl_sync(0xffffffffu, e, ((lane & 3) * 2 + j) * 4)) << 23;
-                    scale2[t][j] = fmaxf(size * __uint_as_float(power), kLeast);
+                    // a product past fp32 would make NaN of scores of 0; with the largest number in its place scores that are not 0 are still 2^90 and
+                    // more apart, as they would be
+                    scale2[t][j] = fminf(fmaxf(size * __uint_as_float(power), kLeast), FLT_MAX);
                 }
             }
         }
