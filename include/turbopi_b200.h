@@ -501,7 +501,8 @@ int tpb200_paged_append(const tpb200_paged_append_args* args, tpb200_stream_t st
  * tokens is 288 G bytes: 16 rows of 16 G bytes of E2M1 codes (value 2 i in the low half of byte i, 2 i + 1 in the high half), then 16 rows of
  * 2 G E4M3 scales, one for every 16 values; codes and scales of values behind head_dim are zeros.  A key is k_scale * scale * code, a value v_scale * scale * code; k_scale and
  * v_scale are powers of two from 2^-63 to 2^64.  scale * code is exact in fp16 and bf16.  page_size is a multiple of 16; the strides are in bytes,
- * multiples of 16: from page to page, from head to head, from tile to tile.  Table and lengths as in tpb200_paged_cache. */
+ * multiples of 16: from page to page, from head to head, from tile to tile.  Table and lengths as in tpb200_paged_cache.  Calls that write refuse tiles
+ * that share bytes (the values' tiles may lie between the keys'), and rows that they read or write between a pool's first and last byte. */
 typedef struct {
     void* k_pages; void* v_pages;
     long long page_stride, head_stride, tile_stride;

@@ -224,6 +224,46 @@ static inline int paged_view_nvfp4(const tpb200_paged_nvfp4_cache& c, PagedView*
     return TPB200_OK;
 }
 
+// bytes from the first to behind the last of a cache's keys, and of its values
+static inline long long pool_bytes(const PagedView& c, long long row_bytes, int rows, int element) {
+    return ((c.num_pages - 1) * c.page_stride + (rows - 1) * c.row_stride + (c.kv_heads - 1) * c.head_stride) * element + row_bytes;
+}
+static inline long long nvfp4_tile_bytes(const PagedView& c) { return 288ll * ((c.head_dim + 31) / 32); }
+static inline long long nvfp4_pool_bytes(const PagedView& c) { return pool_bytes(c, nvfp4_tile_bytes(c), c.page_size / 16, 1); }
+// whether rows reach into what lies between a pool's first and last byte
+static inline bool rows_in_pools(const RowSet& rows, const PagedView& c, long long bytes) {
+    for (const void* pages : {c.k_pages, c.v_pages}) {
+        const long long at = static_cast<long long>(reinterpret_cast<uintptr_t>(pages));
+        if (2 * rows.end() > at && at + bytes > 2 * rows.at) return true;
+    }
+    return false;
+}
+// Whether a tile of the keys shares bytes with one of the values (which may lie between the keys' pages, heads or tiles), or two of either do.  Dimensions whose
+// strides reach over the ones below them, as those of any tensor do, have one place or two near a distance to look at; others count as meeting.
+static inline bool nvfp4_tiles_meet(const PagedView& c) {
+    const long long tile = nvfp4_tile_bytes(c);
+    struct { long long stride; int n; } dim[3] = {{c.page_stride, c.num_pages}, {c.head_stride, c.kv_heads}, {c.row_stride, c.page_size / 16}};
+    std::sort(dim, dim + 3, [](const auto& a, const auto& b) { return a.stride > b.stride; });       // of one: 0, and the last
+    long long reach[4] = {0, 0, 0, tile};            // bytes of the dimensions from i on
+    for (int i = 2; i >= 0; --i) {
+        reach[i] = reach[i + 1] + (dim[i].n - 1) * dim[i].stride;
+        if (dim[i].n > 1 && dim[i].stride < reach[i + 1]) return true;
+    }
+    long long d = static_cast<long long>(reinterpret_cast<uintptr_t>(c.v_pages)) - static_cast<long long>(reinterpret_cast<uintptr_t>(c.k_pages));
+    if (d < 0) d = -d;
+    auto near = [&](auto&& self, int i, long long off) -> bool {       // whether places `off` apart but for the dimensions before i may share bytes
+        if (off <= -reach[i] || off >= reach[i]) return false;
+        if (i == 3) return true;
+        if (dim[i].n == 1) return self(self, i + 1, off);
+        const long long s = dim[i].stride, t = off / s - (off % s < 0);             // rounded down
+        for (const long long x : {t, t + 1}) {
+            if (x > -dim[i].n && x < dim[i].n && self(self, i + 1, off - x * s)) return true;
+        }
+        return false;
+    };
+    return near(near, 0, d);
+}
+
 // These kernels wait for the launch before them ahead of everything they read or write, so they are always launched as dependents
 // (TPB200_FLAG_PDL or not): their CTAs start while it drains.  They let the next launch in behind that wait, not before it: what was
 // enqueued ahead of one of them is complete when a launch behind it starts, as behind any launch without the flag.

@@ -588,7 +588,8 @@ extern "C" int tpb200_paged_attention_nvfp4(const tpb200_paged_attention_nvfp4_a
     if (st != TPB200_OK) return st;
     TPB_REQUIRE(a->dtype == TPB200_BF16 || a->dtype == TPB200_F16, TPB200_ERR_ENUM);
     TPB_REQUIRE(a->window >= 0 && a->sinks >= 0 && (a->window > 0 || a->sinks == 0), TPB200_ERR_SHAPE);
-    const DecodeCall call = {a->q, a->out, a->q_stride, a->o_stride, a->q_heads, a->scale, a->workspace, a->workspace_bytes, a->flags, a->window, a->sinks};
+    const DecodeCall call = {a->q, a->out, a->q_stride, a->o_stride, a->q_heads, a->scale, a->workspace, a->workspace_bytes, a->flags, a->window, a->sinks,
+                             nvfp4_pool_bytes(P.cache)};
     const int D = P.cache.head_dim, group = a->q_heads / P.cache.kv_heads, rows = decode_rows4(group, D);
     const int ctas = decode_ctas(ctas_per_sm4(D));
     const int ready = prepare_decode(call, rows, D <= 64 ? kKeysOf<64> : (D <= 128 ? kKeysOf<128> : kKeysOf<256>), Nvfp4::kItemUnits, ctas, warps4(D), &P);

@@ -986,6 +986,7 @@ struct DecodeCall {
     void* workspace;
     size_t workspace_bytes;
     int flags, window, sinks;            // window 0: all keys
+    long long pool_bytes = 0;            // of the pages, which the output must not reach into; 0: not asked
 };
 
 // The checks of a call and its parameters, P->cache being set; group_rows: query heads that go through together
@@ -1012,6 +1013,8 @@ int prepare_decode(const DecodeCall& a, int group_rows, int slot_keys, int item_
     if (P.cache.seqs == 0) return TPB200_OK;
     TPB_REQUIRE(output_fits(RowSet(a.out, o_stride, P.cache.seqs, a.q_heads, P.cache.head_dim),
                             RowSet(a.q, q_stride, P.cache.seqs, a.q_heads, P.cache.head_dim)), TPB200_ERR_SHAPE);
+    TPB_REQUIRE(a.pool_bytes == 0 || !rows_in_pools(RowSet(a.out, o_stride, P.cache.seqs, a.q_heads, P.cache.head_dim), P.cache, a.pool_bytes),
+                TPB200_ERR_SHAPE);
     P.group = a.q_heads / P.cache.kv_heads;
     P.tiles = (P.group + group_rows - 1) / group_rows;
     P.rows = std::min(P.group, group_rows);

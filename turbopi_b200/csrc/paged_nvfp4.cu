@@ -424,11 +424,6 @@ int threads_for(long long units, int most) {
     return static_cast<int>(((units + passes - 1) / passes + 31) / 32 * 32);
 }
 
-// bytes from the first to behind the last of a cache's pages
-long long pool_bytes(const PagedView& c, long long row_bytes, int rows, int element) {
-    return ((c.num_pages - 1) * c.page_stride + (rows - 1) * c.row_stride + (c.kv_heads - 1) * c.head_stride) * element + row_bytes;
-}
-
 int read_rows(const PagedView& cache, int dtype, bool tiles, float k_scale, float v_scale, const tpb200_paged_rows* a, cudaStream_t stream) {
     TPB_REQUIRE(a->tokens >= 0, TPB200_ERR_SHAPE);
     TPB_REQUIRE((a->flags & ~TPB200_FLAG_PDL) == 0 && (a->dtype == TPB200_BF16 || a->dtype == TPB200_F16) && (tiles || a->dtype == dtype), TPB200_ERR_ENUM);
@@ -449,14 +444,8 @@ int read_rows(const PagedView& cache, int dtype, bool tiles, float k_scale, floa
     // rows that meet one another, or the pages that other threads read
     const RowSet k(a->k, P.k_stride, a->tokens, cache.kv_heads, cache.head_dim), v(a->v, P.v_stride, a->tokens, cache.kv_heads, cache.head_dim);
     TPB_REQUIRE(!rows_cross(k) && !rows_cross(v) && !rows_meet(k, v), TPB200_ERR_SHAPE);
-    const long long bytes = tiles ? pool_bytes(cache, 288ll * ((cache.head_dim + 31) / 32), cache.page_size / 16, 1)
-                                  : pool_bytes(cache, 2ll * cache.head_dim, cache.page_size, 2);
-    for (const RowSet& rows : {k, v}) {
-        for (const void* pages : {cache.k_pages, cache.v_pages}) {
-            const long long at = static_cast<long long>(reinterpret_cast<uintptr_t>(pages));
-            TPB_REQUIRE(2 * rows.end() <= at || at + bytes <= 2 * rows.at, TPB200_ERR_SHAPE);
-        }
-    }
+    const long long bytes = tiles ? nvfp4_pool_bytes(cache) : pool_bytes(cache, 2ll * cache.head_dim, cache.page_size, 2);
+    TPB_REQUIRE(!rows_in_pools(k, cache, bytes) && !rows_in_pools(v, cache, bytes), TPB200_ERR_SHAPE);
     P.k = static_cast<uint16_t*>(a->k);
     P.v = static_cast<uint16_t*>(a->v);
     P.cu = a->cu;
@@ -535,13 +524,16 @@ extern "C" int tpb200_paged_append_nvfp4(const tpb200_paged_append_nvfp4_args* a
         P.o_stride[i] = a->o_stride[i];
     }
     if (a->tokens == 0 || P.cache.seqs == 0) return TPB200_OK;
-    TPB_REQUIRE(a->cache.k_pages != a->cache.v_pages, TPB200_ERR_SHAPE);
+    // tiles that are written twice, and rows in the pages that other threads write
+    TPB_REQUIRE(!nvfp4_tiles_meet(P.cache), TPB200_ERR_SHAPE);
     const int D = P.cache.head_dim, H = P.cache.kv_heads;
+    const long long bytes = nvfp4_pool_bytes(P.cache);
+    const RowSet k_rows(a->k, a->k_stride, a->tokens, H, D), v_rows(a->v, a->v_stride, a->tokens, H, D);
+    TPB_REQUIRE(!rows_in_pools(k_rows, P.cache, bytes) && !rows_in_pools(v_rows, P.cache, bytes), TPB200_ERR_SHAPE);
     if (a->q != nullptr) {               // other threads read what lies there
-        const RowSet out(a->q_out, a->o_stride, a->tokens, a->q_heads, D);
-        TPB_REQUIRE(output_fits(out, RowSet(a->q, a->q_stride, a->tokens, a->q_heads, D)), TPB200_ERR_SHAPE);
-        TPB_REQUIRE(!rows_meet(out, RowSet(a->k, a->k_stride, a->tokens, H, D)) && !rows_meet(out, RowSet(a->v, a->v_stride, a->tokens, H, D)),
-                    TPB200_ERR_SHAPE);
+        const RowSet in(a->q, a->q_stride, a->tokens, a->q_heads, D), out(a->q_out, a->o_stride, a->tokens, a->q_heads, D);
+        TPB_REQUIRE(output_fits(out, in) && !rows_meet(out, k_rows) && !rows_meet(out, v_rows), TPB200_ERR_SHAPE);
+        TPB_REQUIRE(!rows_in_pools(in, P.cache, bytes) && !rows_in_pools(out, P.cache, bytes), TPB200_ERR_SHAPE);
     }
     P.k = static_cast<const uint16_t*>(a->k);
     P.v = static_cast<const uint16_t*>(a->v);

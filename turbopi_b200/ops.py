@@ -987,8 +987,8 @@ def paged_attention_nvfp4(q, k_pages, v_pages, table, lengths, scale, out=None, 
 def paged_append_nvfp4(k, v, k_pages, v_pages, table, cu, lengths, q=None, cos=None, sin=None, q_out=None, k_scale=1.0, v_scale=1.0):
     """`paged_append` into 4-bit pages (`nvfp4_page_shape`): k, v [T, Hk, D] and q [T, Hq, D] in bf16 or fp16.  Keys are rotated and rounded
     to their type, then 16 values at a time, over k_scale or v_scale (powers of two), get the scale max / 6, rounded to E4M3, and the codes
-    nearest to them (ties to the even code; past 448 * 6 they saturate; below 2^-10 * 6 the 16 become zeros).  An infinity or a NaN makes
-    its 16 values NaN."""
+    nearest to them (ties to the even code; past 448 * 6 they saturate; up to 2^-10 * 6 the 16 become zeros).  An infinity or a NaN makes
+    its 16 values NaN.  Rows must not lie in the pages, nor tiles share bytes; the values' may lie between the keys'."""
     done = (_lib._native or _lib.native()).paged_append_nvfp4(k, v, k_pages, v_pages, table, cu, lengths, q, cos, sin, q_out, k_scale,
                                                               v_scale, _flags.value)
     if done is not None:
