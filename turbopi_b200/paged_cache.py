@@ -271,7 +271,10 @@ class PagedCache:
             out.table.copy_(table)
             out.lengths.copy_(lengths)
             out.cu.copy_(offsets)
-            out.cu_keys.copy_(key_offsets)
+            if out.cu_keys is None:
+                out.cu_keys = key_offsets
+            else:
+                out.cu_keys.copy_(key_offsets)
             out.tokens, out._stale, out._late, out._layers = sum(new), None, None, set()
         out.keys = sum(self._seqs[seq][1] for seq in seqs)
         out._new = {seq: (self._seqs[seq][1] - n, self._seqs[seq][1]) for seq, n in zip(seqs, new)}
