@@ -45,7 +45,8 @@ struct Rows16 {
 };
 struct Nvfp4 {
     static constexpr bool kQuant = true;
-    // 96 ragged sequences 40.3 us, with 4: 42.7, 2: 52.5, 8: 41; the windows of 64 like ones 39.1, 37.9, -, 40.1
+    // With 2, 4, 5, 6, 7: 96 ragged sequences 47.7, 40.0, 39.4, 36.8, 36.4 us (heads of 128), windows of 64 sequences 38.9, 38.3, 39.0, 39.4, 39.0 (of 64),
+    // five long ones 35.4, 34.6, 34.6, 34.6, 34.6 (of 256): medians, the first two of which move by 1 us from run to run
     static constexpr int kItemUnits = 6;
 };
 
@@ -190,6 +191,8 @@ struct Place {
 // first and the last of an item always has a slot of it.  A line shorter than that for four warps is one warp's.
 template <int kItemUnits, int kWarps>
 struct Share {
+    // a CTA has at least as many units; one inside an item has a slot of it, since the item's own units are fewer
+    static_assert(kItemUnits < kWarps * kSlotUnits, "a CTA inside an item leaves a part");
     int total, ctas, each, more;         // `more` CTAs of each + 1 units, the others of each
     __device__ __forceinline__ void cut(int units, int grid) {
         total = units;
