@@ -90,8 +90,6 @@ template <int DP, int NT, int kBlocks, bool kFull>
 __device__ __forceinline__ void scores4(float (&sc)[kBlocks][NT][4], uint32_t slot, const Lane<DP, kFull>& of, const uint32_t (&qf)[DP / 16][NT][2]) {
     constexpr int kRuns = DP == 256 ? 2 : 1;             // of 32 values, or of 16 (DP = 64), that a lane has of a row
     constexpr int kWords = DP == 64 ? 2 : 4;
-    // two chains of products where a block would leave one alone
-    float odd[kBlocks == 1 ? NT : 1][4] = {};
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b) {
 #pragma unroll
@@ -131,16 +129,10 @@ __device__ __forceinline__ void scores4(float (&sc)[kBlocks][NT][4], uint32_t sl
                     const uint32_t a[4] = {bits_of(x[0][2 * j]), bits_of(x[1][2 * j]), bits_of(x[0][2 * j + 1]), bits_of(x[1][2 * j + 1])};
                     const int kk = run * 8 + i * 2 + j;
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) mma16816<__half>(kBlocks == 1 && j == 1 ? odd[kBlocks == 1 ? n : 0] : sc[b][n], a, qf[kk][n][0], qf[kk][n][1]);
+                    for (int n = 0; n < NT; ++n) mma16816<__half>(sc[b][n], a, qf[kk][n][0], qf[kk][n][1]);
                 }
             }
         }
-    }
-    if constexpr (kBlocks == 1) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) sc[0][n][j] += odd[n][j];
     }
 }
 
@@ -194,7 +186,7 @@ __device__ __forceinline__ void values4(float (&o)[DP / 16][NT][4], uint32_t slo
     }
 }
 
-// One pass over a warp's piece of the line: per slot (16, 32 or 64 keys, their tiles and those of their values) the scores, the running reference and
+// One pass over a warp's piece of the line: per slot (32 or 64 keys, their tiles and those of their values) the scores, the running reference and
 // sum of a softmax, and the product with the values.  Two slots are on their way while a third is worked on.  Page ids are looked up for up
 // to 32 tiles at a time, a lane each, and asked for that long before they are needed.
 template <typename T, int DP, int NT, bool kFull>
@@ -203,7 +195,7 @@ __device__ __forceinline__ void attend_tiles(const DecodeParams& P) {
     using S = Shape<Src, DP, NT>;
     constexpr int kSlots = S::kSlots, kWarps = S::kWarps, kCodes = kCodesOf<DP>, kScales = kScalesOf<DP>;
     constexpr int kKeys = S::kKeys, kBlocks = kKeys / 16, kAhead = 32 / kBlocks;       // slots of a look-up
-    static_assert(S::kSlotBytes == 2 * (kCodes + kScales) && kBlocks <= 4 && kSlots <= 8, "");
+    static_assert(S::kSlotBytes == 2 * (kCodes + kScales) && (kBlocks == 2 || kBlocks == 4) && kSlots <= 8, "");
     extern __shared__ __align__(128) uint8_t smem[];
     auto* ctl = reinterpret_cast<Control<S>*>(smem + kWarps * kSlots * S::kSlotBytes);
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
