@@ -46,7 +46,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attention_join_kernel(cons
 // 4096, 4 key heads of 128, 80 MB: groups of 8 21 us, of 16 28, of 32 47)
 int decode_rows(int group) { return group <= 8 ? 8 : 16; }
 
-constexpr int kCtasPerSm = Shape<Rows16, 64, 1>::kCtas, kWarps = Shape<Rows16, 64, 1>::kWarps;
+constexpr int kCtasPerSm = Shape<Rows16, 64, 1>::kCtas;
 
 template <typename T, int DP, bool kWindow>
 int launch_rows(const DecodeParams& P, int ctas, cudaStream_t stream) {
@@ -75,7 +75,7 @@ int attend(const tpb200_paged_attention_args* a, int window, int sinks, cudaStre
     const DecodeCall call = {a->q, a->out, a->q_stride, a->o_stride, a->q_heads, a->scale, a->workspace, a->workspace_bytes, a->flags, window, sinks};
     const int group = a->q_heads / P.cache.kv_heads, slot_keys = P.cache.head_dim <= 64 ? 64 : (P.cache.head_dim <= 128 ? 32 : 16);
     const int ctas = decode_ctas(kCtasPerSm);
-    const int ready = prepare_decode(call, decode_rows(group), slot_keys, Rows16::kItemUnits, ctas, kWarps, &P);
+    const int ready = prepare_decode(call, decode_rows(group), slot_keys, Rows16::kItemUnits, ctas, &P);
     if (ready != TPB200_OK || P.cache.seqs == 0) return ready;
     const bool bf = a->cache.dtype == TPB200_BF16;
     // a window that no sequence of the table passes hides nothing
@@ -98,7 +98,7 @@ extern "C" size_t tpb200_paged_attention_workspace_size(int q_heads, int kv_head
     const int ctas = tpb::decode_ctas(tpb::kCtasPerSm);
     if (ctas < 1) return 0;
     const int group = q_heads / kv_heads;
-    return tpb::decode_scratch(static_cast<size_t>(ctas) * tpb::kWarps, std::min(group, tpb::decode_rows(group)), head_dim).bytes;
+    return tpb::decode_scratch(static_cast<size_t>(ctas) * tpb::kCtaWarps, std::min(group, tpb::decode_rows(group)), head_dim).bytes;
 }
 
 extern "C" int tpb200_paged_attention(const tpb200_paged_attention_args* a, tpb200_stream_t stream) {

@@ -553,10 +553,9 @@ int join_tiles(const DecodeParams& P, int ctas, cudaStream_t stream) {
     if (!configure<most>(0, true) || !configure<many>(0, true) || !configure<few>(0, true)) return TPB200_ERR_CUDA;
     return launch_join(P, most, many, few, ctas, stream);
 }
-// warps of a CTA, and CTAs of an SM: the same for one tile of query heads and for two
-int warps4(int head_dim) { return head_dim > 128 ? Shape<Nvfp4, 256, 1>::kWarps : Shape<Nvfp4, 128, 1>::kWarps; }
+// CTAs of an SM: the same for one tile of query heads and for two
 int ctas_per_sm4(int head_dim) { return head_dim > 128 ? Shape<Nvfp4, 256, 1>::kCtas : Shape<Nvfp4, 128, 1>::kCtas; }
-static_assert(Shape<Nvfp4, 64, 1>::kWarps == Shape<Nvfp4, 128, 1>::kWarps && Shape<Nvfp4, 64, 1>::kCtas == Shape<Nvfp4, 128, 1>::kCtas, "");
+static_assert(Shape<Nvfp4, 64, 1>::kCtas == Shape<Nvfp4, 128, 1>::kCtas, "");
 
 }  // namespace
 
@@ -569,7 +568,7 @@ extern "C" size_t tpb200_paged_attention_nvfp4_workspace_size(int q_heads, int k
     if (q_heads < 1 || kv_heads < 1 || q_heads % kv_heads != 0 || head_dim < 8 || head_dim > 256) return 0;
     const int group = q_heads / kv_heads, rows = std::min(group, decode_rows4(group, head_dim));
     const int ctas = decode_ctas(ctas_per_sm4(head_dim));
-    return ctas < 1 ? 0 : decode_scratch(static_cast<size_t>(ctas) * warps4(head_dim), rows, head_dim).bytes;
+    return ctas < 1 ? 0 : decode_scratch(static_cast<size_t>(ctas) * kCtaWarps, rows, head_dim).bytes;
 }
 
 extern "C" int tpb200_paged_attention_nvfp4(const tpb200_paged_attention_nvfp4_args* a, tpb200_stream_t stream) {
@@ -584,7 +583,7 @@ extern "C" int tpb200_paged_attention_nvfp4(const tpb200_paged_attention_nvfp4_a
                              nvfp4_pool_bytes(P.cache)};
     const int D = P.cache.head_dim, group = a->q_heads / P.cache.kv_heads, rows = decode_rows4(group, D);
     const int ctas = decode_ctas(ctas_per_sm4(D));
-    const int ready = prepare_decode(call, rows, D <= 64 ? kKeysOf<64> : (D <= 128 ? kKeysOf<128> : kKeysOf<256>), Nvfp4::kItemUnits, ctas, warps4(D), &P);
+    const int ready = prepare_decode(call, rows, D <= 64 ? kKeysOf<64> : (D <= 128 ? kKeysOf<128> : kKeysOf<256>), Nvfp4::kItemUnits, ctas, &P);
     if (ready != TPB200_OK || P.cache.seqs == 0) return ready;
     P.scale2 *= a->cache.k_scale;
     TPB_REQUIRE(std::isfinite(P.scale2), TPB200_ERR_SHAPE);

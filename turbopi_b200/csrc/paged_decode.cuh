@@ -14,6 +14,7 @@
 namespace tpb {
 namespace {
 
+constexpr int kCtaWarps = 4;
 constexpr int kSlotUnits = 2;            // what a slot costs; an item besides, for queries, sums and the output: Src::kItemUnits
 constexpr float kLowest = -FLT_MAX;      // the least reference of a row with a key
 
@@ -26,7 +27,7 @@ struct DecodeParams {
     int tiles;                           // tiles of query heads per key head
     int rows;                            // rows of a tile that are used at most
     long long items;                     // (sequence, tile of query heads)
-    int workers, warps;                  // warps of the grid, and of a CTA
+    int workers;                         // warps of the grid
     int join_by_item;                    // joins[] has a place per item, else one per worker
     float scale2;                        // scale * log2 e, times the factor of the keys' scales
     float out_scale;                     // factor of the values' scales (Nvfp4)
@@ -57,7 +58,7 @@ struct Shape {
     static constexpr int kSlotBytes = Src::kQuant ? 2 * kKeys * (DP / 2 + DP / 16) : kKeys * DP * 2;     // tiles of keys and of values; rows of keys, or of values
     static constexpr int kSlots = 3;                        // of a warp's ring
     static constexpr int kCtas = Src::kQuant && DP < 256 ? 3 : 2;       // on an SM
-    static constexpr int kWarps = 4, kThreads = kWarps * 32;
+    static constexpr int kWarps = kCtaWarps, kThreads = kWarps * 32;
     static constexpr int kLengths = 1024;                   // lengths kept in shared memory; with more sequences they are read where they lie
     static constexpr int kLanesRow = Src::kQuant ? DP / 32 : DP / 8;        // lanes that copy a row
     static constexpr int kRowsIter = 32 / kLanesRow;        // rows a warp copies at a time
@@ -857,7 +858,7 @@ constexpr int kJoinThreads = 128;
 
 template <typename Src, typename T, int kLanes, int kLoads>
 __device__ __forceinline__ void join_parts(const DecodeParams& P) {
-    const int kWarps = Src::kQuant ? P.warps : 4;
+    constexpr int kWarps = kCtaWarps;
     constexpr int kQuads = kJoinThreads / kLanes;
     __shared__ float4 sums[kLanes][kQuads];
     __shared__ float2 mls[kLanes][kQuads];
@@ -993,7 +994,7 @@ struct DecodeCall {
 };
 
 // The checks of a call and its parameters, P->cache being set; group_rows: query heads that go through together
-int prepare_decode(const DecodeCall& a, int group_rows, int slot_keys, int item_units, int ctas, int warps, DecodeParams* out) {
+int prepare_decode(const DecodeCall& a, int group_rows, int slot_keys, int item_units, int ctas, DecodeParams* out) {
     DecodeParams& P = *out;
     TPB_REQUIRE(a.q && a.out, TPB200_ERR_NULL);
     TPB_REQUIRE((a.flags & ~TPB200_FLAG_PDL) == 0, TPB200_ERR_ENUM);
@@ -1030,8 +1031,7 @@ int prepare_decode(const DecodeCall& a, int group_rows, int slot_keys, int item_
     P.sinks = a.window > 0 ? std::min(a.sinks, positions) : 0;
     P.out_scale = 1.0f;
     TPB_REQUIRE(ctas >= 2, TPB200_ERR_CUDA);
-    P.workers = ctas * warps;
-    P.warps = warps;
+    P.workers = ctas * kCtaWarps;
     const DecodeScratch d = decode_scratch(P.workers, P.rows, P.cache.head_dim);
     TPB_REQUIRE(a.workspace != nullptr && a.workspace_bytes >= d.bytes, TPB200_ERR_WORKSPACE);
     TPB_REQUIRE(tpb_aligned16(a.workspace), TPB200_ERR_ALIGN);
