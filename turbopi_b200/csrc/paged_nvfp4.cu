@@ -18,7 +18,6 @@ namespace {
 constexpr int kAppendThreads = 256;      // of a block at most
 constexpr int kPairThreads = 256, kPairBlocks = 4;
 constexpr int kReadThreads = 256;
-constexpr int kAppendLoads = 1;          // tokens whose unit a thread has in flight
 constexpr int kAppendTokens = 6;         // of a block at most
 constexpr int kReadLoads = 4;
 constexpr int kReadTokens = 16;
@@ -276,56 +275,50 @@ __global__ void __launch_bounds__(kAppendThreads, 4) append_blocks_kernel(const 
         const long long* st = kind == 0 ? P.q_stride : (kind == 1 ? P.k_stride : P.v_stride);
         const long long step = st[0];
         const uint16_t* src = (kind == 0 ? P.q : (kind == 1 ? P.k : P.v)) + t0 * step + head * st[1];
-        for (int first = 0; first < count; first += kAppendLoads) {
-            Vec<V> x[kAppendLoads][kVecs], y[kAppendLoads][kVecs];
-#pragma unroll
-            for (int i = 0; i < kAppendLoads; ++i) {
-                if (!mine || first + i >= count) continue;
-                const uint16_t* row = src + (first + i) * step;
+        for (int t = 0; t < count; ++t) {
+            Vec<V> x[kVecs], y[kVecs];
+            if (mine) {
+                const uint16_t* row = src + t * step;
 #pragma unroll
                 for (int n = 0; n < kVecs; ++n) {
                     const int c = at + n * V;
-                    x[i][n] = y[i][n] = Vec<V>{};
+                    x[n] = y[n] = Vec<V>{};
                     if ((kind == 0 && n > 0) || c >= D) continue;
-                    x[i][n] = load_vec<V>(row + c);
-                    if (turn) y[i][n] = load_vec<V>(row + (c < half ? c + half : c - half));
+                    x[n] = load_vec<V>(row + c);
+                    if (turn) y[n] = load_vec<V>(row + (c < half ? c + half : c - half));
                 }
             }
             if (!placed) {               // the tokens' rows, behind the first loads
                 placed = true;
                 place_tokens<true, kAppendTokens>(P.cache, P.cu, t0, count, P.rope_positions, seq, position, row_at);
             }
-#pragma unroll
-            for (int i = 0; i < kAppendLoads; ++i) {
-                if (!mine || first + i >= count) continue;
-                const long long row = row_at[first + i];
-                if (row < 0) continue;
-                const int pos = position[first + i];
-                if (kind == 0) {
-                    turn_pair<T, V>(x[i][0], y[i][0], P, pos, at);
-                    uint16_t* to = P.q_out + (t0 + first + i) * P.o_stride[0] + head * P.o_stride[1] + at;
-                    store_vec<V>(to, x[i][0]);
-                    store_vec<V>(to + half, y[i][0]);
-                    continue;
-                }
-                if (turn) {
-#pragma unroll
-                    for (int n = 0; n < kVecs; ++n) {
-                        const int c = at + n * V;
-                        if (c < half) turn_pair<T, V>(x[i][n], y[i][n], P, pos, c);
-                        else if (c < D) turn_pair<T, V>(y[i][n], x[i][n], P, pos, c - half);
-                    }
-                }
-                uint8_t* tile = static_cast<uint8_t*>(kind == 1 ? P.cache.k_pages : P.cache.v_pages) + row + head * P.cache.head_stride;
-                const float inv = kind == 1 ? P.k_inv : P.v_inv;
-                uint8_t* codes_at = tile + (pos & 15) * 16 * groups;
-                uint8_t* scales_at = tile + 256 * groups + (pos & 15) * 2 * groups;
-                uint2 codes;
-                uint32_t scale;
-                quantise16<T>(reinterpret_cast<const uint32_t(&)[8]>(x[i]), inv, codes, scale);
-                *reinterpret_cast<uint2*>(codes_at + in * 8) = codes;
-                scales_at[in] = static_cast<uint8_t>(scale);
+            const long long row = row_at[t];
+            if (!mine || row < 0) continue;
+            const int pos = position[t];
+            if (kind == 0) {
+                turn_pair<T, V>(x[0], y[0], P, pos, at);
+                uint16_t* to = P.q_out + (t0 + t) * P.o_stride[0] + head * P.o_stride[1] + at;
+                store_vec<V>(to, x[0]);
+                store_vec<V>(to + half, y[0]);
+                continue;
             }
+            if (turn) {
+#pragma unroll
+                for (int n = 0; n < kVecs; ++n) {
+                    const int c = at + n * V;
+                    if (c < half) turn_pair<T, V>(x[n], y[n], P, pos, c);
+                    else if (c < D) turn_pair<T, V>(y[n], x[n], P, pos, c - half);
+                }
+            }
+            uint8_t* tile = static_cast<uint8_t*>(kind == 1 ? P.cache.k_pages : P.cache.v_pages) + row + head * P.cache.head_stride;
+            const float inv = kind == 1 ? P.k_inv : P.v_inv;
+            uint8_t* codes_at = tile + (pos & 15) * 16 * groups;
+            uint8_t* scales_at = tile + 256 * groups + (pos & 15) * 2 * groups;
+            uint2 codes;
+            uint32_t scale;
+            quantise16<T>(reinterpret_cast<const uint32_t(&)[8]>(x), inv, codes, scale);
+            *reinterpret_cast<uint2*>(codes_at + in * 8) = codes;
+            scales_at[in] = static_cast<uint8_t>(scale);
         }
     }
 }
