@@ -109,10 +109,11 @@ __device__ __forceinline__ uint32_t pack2(uint64_t p) {
     return Half16<T>::pack(f.x, f.y);
 }
 
-// 16 values of a type as eight words -> a scale and 16 codes.  The quotient is x times the rounded inverse of s, off by 2^-22 at most for |x / s| <= 6.
-// Ties are common (s has four bits, x eight or eleven) and have to stay ties: the sum with 128 rounds the quotient to a multiple of 2^-17 or 2^-16.
-// A quotient that is no tie is 2^-13 from one at least, since x differs from a tie times s, which the type of x holds, by a step of that type.
-// (Powers of two in `inv` change nothing of this; past 6 the conversion saturates.)
+// 16 values of a type as eight words -> a scale and 16 codes.  The quotient is x times the rounded inverse of s, off by |x / s| 2^-24: less than 2^-21 up to
+// 6 (s may have been rounded down, so that quotients pass 6; there the conversion saturates).
+// Ties are common (s has four bits, x eight or eleven) and have to stay ties: the sum with 128 rounds the quotient to a multiple of 2^-17 or 2^-16, half a
+// step of which, 2^-18, is more than that error.  A quotient that is no tie is 2^-13 from one at least, since x differs from a tie times s, which the type
+// of x holds, by a step of that type.  (Powers of two in `inv` change nothing of this.)
 template <typename T>
 __device__ __forceinline__ void quantise16(const uint32_t (&x)[8], float inv, uint2& codes, uint32_t& scale) {
     constexpr uint32_t kInf = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
