@@ -936,6 +936,8 @@ int attend(const tpb200_packed_attention_args* a, int window, int sinks, tpb200_
     // 24 sequences of 100 / 8 of 1536, 16 heads of 64: 13.5 us with one, 18.1 with two / 91.6, 92.6; 16 heads of 128: 21.0, 25.2 / 129, 118.
     // Batches of sequences alike; not measured where lengths differ much or queries are few beside the keys.  With a window its keys count, and the border for
     // heads of 128 is 1000: windows of 200 / 400 / 800 / 1500, 4000 tokens, 32 on 8 heads, 95 / 106 / 138 / 194 us with one, 97 / 121 / 149 / 187 with two.
+    // That holds for windows shorter than the prompts.  Longer ones, which hide nothing, take that border too: 24 prompts of 200 / 400 / 600 / 1000 tokens, 32
+    // on 8 heads of 128, 52 / 101 / 160 / 327 us with a window of 4096, 51 / 100 / 157 / 305 without one; heads of 64 and 256 1 to 5 % more.
     const long long keys = hides ? std::min<long long>(a->k_tokens, (static_cast<long long>(window) + P.sinks) * a->seqs) : a->k_tokens;
     const bool two = DP <= 128 && keys > (DP == 64 || hides ? 1000ll : 200ll) * a->seqs;
     // no more tiles than whole ones and a ragged one per sequence
