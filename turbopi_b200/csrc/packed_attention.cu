@@ -40,9 +40,9 @@
 // sequences of 100 tokens gain 7 %, those of 1 to 1200 lose 6 %); pairs of CTAs on one product (cta_group::2, M = 256: 2.47 ms, the single
 // sequence 250 us, each hand-over crosses the cluster).
 //
-// Sliding windows (kWindow): tiles without a visible pair are not visited.  One sequence of 8191 tokens, 8 on 1 heads of 256, window 1024, four sinks: 85.8 us
+// Sliding windows (kWindow): tiles without a visible pair are not visited.  One sequence of 8191 tokens, 8 on 1 heads of 256, window 1024, four sinks: 86.4 us
 // (all keys: 197), 9 tiles a CTA for 8.03 of visible pairs; 512 CTAs of 21 us, 5 of them look-up, first loads and output, in four waves.  24 ragged sequences of 1 to 1200, 16 on 4 heads
-// of 64, window 200: 25.9; four long ones, 32 on 8 of 128, window 1500: 280, 0.55 of the measured bf16 burst rate.  With whole tiles left out instead of keys: 93, 27.8, 291.
+// of 64, window 200: 26.1; four long ones, 32 on 8 of 128, window 1500: 281, 0.55 of the measured bf16 burst rate.  With whole tiles left out instead of keys: 93, 27.8, 291.
 //
 // What may stand in masked places does not matter: scores are selected, not biased.  Rows of V behind a sequence's end are zeroed in
 // shared memory, and in tiles that hold masked pairs V is searched for infinities and NaN (weight 0 times those would be NaN): they are

@@ -49,7 +49,7 @@ struct Half16<__half> {
 // Weights 2^(scale S - m), the product fused into the sum, are off by the rounding of their reference m, the product of the largest score.  It cancels out
 // with their sum, but from 2^24 on it may be a factor of two, which fp16 weights have no room for, and from 2^31 on all of them may be infinite, or zeros.
 // Past this size (a quarter of a power of two) scores are rounded first, as the reference is, so that the largest weight is what it should be.  Asking costs
-// short prompts most: 24 of 1 to 1200 tokens, 16 on 4 heads of 64, 25.9 -> 26.5 us; others up to 1 %.
+// short prompts most: 24 of 1 to 1200 tokens, 16 on 4 heads of 64, 26.0 -> 26.3 us; others up to 1 %.
 constexpr float kFar = 4194304.0f;       // 2^22
 
 // V values of a 16-bit type

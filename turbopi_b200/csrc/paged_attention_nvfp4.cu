@@ -12,8 +12,8 @@
 //
 // Inside a piece (two lengths of one long sequence compared): heads of 256 470 warp instructions for 16 keys, 5.8 TB/s = 0.89 of the measured copy rate; of 128 574 for
 // 32, 5.3; of 64 667 for 64, 4.8.  Around it: 2.3 us until a warp knows its piece, 2 until its first slot is there, warps of an SM that end up to a third
-// apart, 4-5 us for the second kernel.  Calls in a CUDA graph: 96 sequences of 1 to 8192, 32 on 8 of 128, bf16 (111 MB) 35.7 us = 3.1 TB/s; 5 of 60 to 131 k, 8 on 1 of 256,
-// fp16 (124 MB) 33.9 = 3.7; 64 of up to 12,000 under a window of 2048, 16 on 16 of 64 (116 MB) 38.1 = 3.1; one of 762 keys 10.6.  (On 16 bits the first would
+// apart, 4-5 us for the second kernel.  Calls in a CUDA graph: 96 sequences of 1 to 8192, 32 on 8 of 128, bf16 (111 MB) 35.3 us = 3.1 TB/s; 5 of 60 to 131 k, 8 on 1 of 256,
+// fp16 (124 MB) 34.2 = 3.6; 64 of up to 12,000 under a window of 2048, 16 on 16 of 64 (116 MB) 38.6 = 3.0; one of 762 keys 10.5.  (On 16 bits the first would
 // have 394 MB to read.)
 #include "paged_decode.cuh"
 
@@ -532,7 +532,8 @@ __global__ void __launch_bounds__(kJoinThreads) paged_attention_nvfp4_join_kerne
 }
 
 // query heads that go through together: eight, or sixteen where a group has more and their sums leave registers for the rest (head sizes up to 128);
-// larger groups read the cache again, mostly out of L2
+// larger groups read the cache again, mostly out of L2.  38 MB of sequences of 8192, one key head, groups of 8 / 16: heads of 64 17 / 22 us, of 128 17 / 25, of 256
+// 18.5 / 25.  Two tiles of heads of 128 have 56 to 168 bytes of spills at the 168 registers that three CTAs an SM leave; with two CTAs they were not timed.
 int decode_rows4(int group, int head_dim) { return group <= 8 || head_dim > 128 ? 8 : 16; }
 
 template <typename T, int DP, int NT>

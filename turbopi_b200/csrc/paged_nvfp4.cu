@@ -5,8 +5,9 @@
 //   read     rows of the last tokens of each sequence, one sequence behind the other: values out of 4 bits, or copies out of 16.
 //
 // A decode step is the chain offsets -> length -> page id -> row.  Prompts, calls in a CUDA graph: 14.4 k tokens of six sequences, 32 on 8 heads of 128, turned and
-// written (312 MB) 66 us = 4.7 TB/s: what a block waits for (its look-up, then each token's loads) and 70 instructions for 16 values; keys and values alone 26.  The
-// same tokens into 16 bits (354 MB): 63.  25 k tokens of 8 heads of 128 read back (132 MB) 26.6 us = 5.0 TB/s, 0.76 of the measured copy rate.
+// written (312 MB) 66 us = 4.7 TB/s: what a block waits for (its look-up, then each token's loads) and 70 instructions for 16 values; keys and values alone 30 (floor 12.6), not turned
+// 19.6 (11.5).  The same tokens into 16 bits (354 MB): 63.  25 k tokens of 8 heads of 128 read back (132 MB) 26.2 us = 5.0 TB/s, 0.77 of the measured copy rate;
+// out of 16 bits (206 MB) 39 = 5.3.
 #include <algorithm>
 #include <type_traits>
 

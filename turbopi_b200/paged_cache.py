@@ -17,7 +17,7 @@ same pages); the bytes are moved by `ops.copy_pages`, written by `ops.paged_appe
         out = cache.attention(l, batch, q, scale)
 
 dtype="nvfp4" holds keys and values in 4 bits (`ops.nvfp4_page_shape`): 18 bytes for 32 values instead of 64, the same calls.  A prompt behind tokens
-that are cached attends through `cache.prompt_attention`, which reads them back (`cache.read`) for `ops.packed_attention`; window= and sinks=
+that are cached attends through `cache.prompt_attention`, which reads them all back (`cache.read`) for `ops.packed_attention`; window= and sinks=
 restrict either attention to a sliding window and the first tokens.
 
 A batch holds for its cache until one of its sequences is freed, truncated or had a shared page copied, or pages have moved (compact);
@@ -331,7 +331,7 @@ class PagedCache:
 
     def prompt_attention(self, layer, batch, q, scale, out=None, window=None, sinks=0):
         """Causal attention of the batch's new tokens, q [batch.tokens, heads, head_dim], over all tokens of their sequences (or a window), new
-        and cached, as the cache holds them: `read`, then ops.packed_attention.  Append the new tokens first.  A captured call holds for as many
+        and cached, as the cache holds them: `read`, then ops.packed_attention.  All tokens are read, whatever the window.  Append the new tokens first.  A captured call holds for as many
         keys as its capture had, as `read` does; `attention` follows its batch."""
         if q.shape[0] != batch.tokens:
             raise TurboPiError(f"PagedCache: {q.shape[0]} rows for {batch.tokens} new tokens")
