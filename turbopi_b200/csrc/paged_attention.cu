@@ -31,9 +31,10 @@ namespace {
 
 template <typename T, int DP, int NT, bool kAligned, bool kWindow>
 __global__ void __launch_bounds__(Shape<Rows16, DP, NT>::kThreads, Shape<Rows16, DP, NT>::kCtas) paged_attention_kernel(const __grid_constant__ DecodeParams P) {
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), D = P.cache.head_dim;
     pdl_wait_prior_grids();
     pdl_launch_dependents();
-    attend_rows<T, DP, NT, kAligned, kWindow>(P);
+    attend_rows<T, DP, NT, kAligned, kWindow>(P, warp, D);
 }
 template <typename T, int kLanes, int kLoads>
 __global__ void __launch_bounds__(kJoinThreads) paged_attention_join_kernel(const __grid_constant__ DecodeParams P) {

@@ -18,6 +18,7 @@ constexpr int kCtaWarps = 4;
 constexpr int kSlotUnits = 2;            // what a slot costs; an item besides, for queries, sums and the output: Src::kItemUnits
 constexpr float kLowest = -FLT_MAX;      // the least reference of a row with a key
 
+// What only the host or some calls read stands last: a small call of one that reads all from the front takes 0.05-0.1 us less
 struct DecodeParams {
     PagedView cache;
     const uint16_t* q;
@@ -26,15 +27,15 @@ struct DecodeParams {
     int group;                           // query heads per key head
     int tiles;                           // tiles of query heads per key head
     int rows;                            // rows of a tile that are used at most
-    long long items;                     // (sequence, tile of query heads)
-    int workers;                         // warps of the grid
     int join_by_item;                    // joins[] has a place per item, else one per worker
     float scale2;                        // scale * log2 e, times the factor of the keys' scales
-    float out_scale;                     // factor of the values' scales (Nvfp4)
-    int window, sinks;                   // keys that are seen: the last `window` and the first `sinks` (kWindow)
     float* part_o;                       // [2 * workers][rows][head_dim]
     float* part_ml;                      // [2 * workers][rows][2]
     int4* joins;                         // (item or -1, its first part, its last worker, 1: first CTA merged | 2: last CTA merged)
+    long long items;                     // (sequence, tile of query heads)
+    int workers;                         // warps of the grid
+    float out_scale;                     // factor of the values' scales (Nvfp4)
+    int window, sinks;                   // keys that are seen: the last `window` and the first `sinks` (kWindow)
 };
 
 // What a cache holds.  Rows16: rows of head_dim 16-bit values, strides in elements.  Nvfp4: tiles of 16 tokens of one head, strides in bytes
@@ -473,17 +474,17 @@ __device__ __forceinline__ void merge_cta(const DecodeParams& P, const Work& wor
     }
 }
 
-// kAligned: the page size is a multiple of 16, so that 16 rows from a multiple of 16 on lie in one page and share an address
+// kAligned: the page size is a multiple of 16, so that 16 rows from a multiple of 16 on lie in one page and share an address.  The warp and D are what its
+// kernel has found out ahead of its wait for the launch before.
 template <typename T, int DP, int NT, bool kAligned, bool kWindow>
-__device__ __forceinline__ void attend_rows(const DecodeParams& P) {
+__device__ __forceinline__ void attend_rows(const DecodeParams& P, int warp, int D) {
     using Src = Rows16;
     using S = Shape<Src, DP, NT>;
     constexpr int kSlotBytes = S::kSlotBytes, kSlots = S::kSlots, kWarps = S::kWarps;
     extern __shared__ __align__(128) uint8_t smem[];
     float* slab = reinterpret_cast<float*>(smem + kWarps * kSlots * kSlotBytes);
     auto* ctl = reinterpret_cast<Control<S>*>(slab + kWarps * S::kRows * S::kSlabPitch);
-    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-    const int D = P.cache.head_dim;
+    const int lane = threadIdx.x & 31;
 
     Piece<Src, S, kWindow> piece;
     if (!piece.find(P, ctl->lengths, warp, lane)) return;
